@@ -567,6 +567,83 @@ int nmtgan_disc_fold_bn(const float* conv_b, const float* gamma, const float* be
 int nmtgan_clip_values(float* w, int64_t n, float lo, float hi, void* w_op, int op_dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Operators of teacher-forced training and of prompts / single tokens over a packed key buffer.  Nothing in the reference
+ * corresponds to them one to one: its attention is dot_product_attention over padded batches (common_attention.py:294-331),
+ * its loss materialises the logits (model.py:804-820), its clipping is by value (share_function.py:413-441).
+ *
+ * Span attention: query row i sees the keys lo[i] <= j < hi[i] of the key rows (lo, hi are cut to [0, N]); causal,
+ * document, prefix and padding masks of packed or padded batches are all spans, and rows may share or repeat them.
+ *   r = scale q_i.k_j;  s = cap > 0 ? cap tanh(r / cap) : r;  s -= slopes[h] |pos[i] - j|;  softmax over the span
+ * q/out [M][heads dh], k/v [N][kv_heads dh] in `dtype`, head-major inside a row, ld* elements from row to row; query head h
+ * reads key head h / (heads / kv_heads).  A row with an empty span gets out = 0, lse = -inf and no gradient.  Rows outside
+ * every span may hold anything, and a NaN or an infinity reaches exactly the rows that see it.
+ * dh: a multiple of 8 up to 128; rows 16-byte aligned; inputs and outputs do not overlap.
+ * nmtgan_attn_span: prompts and training rows.  nmtgan_attn_span_step: few rows over long spans (single tokens): each
+ *   span is cut along its keys.  max_keys is a hint for the cut - the longest span expected - and changes no value beyond
+ *   the order of fp32 sums.
+ * nmtgan_attn_span_grads: bf16 or fp32; `out` and `lse` are nmtgan_attn_span's results for the same arguments; dk and dv
+ *   are written for every key row (0 where nobody looks) and summed over the heads that share a key head.  Each value is
+ *   computed by one workgroup in a fixed order: results repeat bit for bit.
+ */
+typedef struct {
+  int dtype;
+  int M, N, heads, kv_heads, dh;
+  const void* q; int64_t ldq;
+  const void* k; int64_t ldk;
+  const void* v; int64_t ldv;
+  const int32_t* lo; const int32_t* hi;      /* [M] */
+  const int32_t* pos;                        /* [M] place of row i among the keys (for slopes); NULL: hi[i] - 1 */
+  const float* slopes;                       /* [heads] or NULL */
+  float scale, cap;                          /* cap <= 0 is refused unless exactly 0 = no cap */
+  void* out; int64_t ldo;
+  float* lse;                                /* [M][heads] natural log; NULL if not wanted (forward only) */
+} nmtgan_span_args;
+typedef struct {
+  const void* dout; int64_t ld_dout;         /* [M][heads dh] */
+  void* dq; int64_t ld_dq;                   /* [M][heads dh] */
+  void* dk; int64_t ld_dk;                   /* [N][kv_heads dh] */
+  void* dv; int64_t ld_dv;
+} nmtgan_span_grads;
+int nmtgan_attn_span(const nmtgan_span_args* a, void* stream);
+size_t nmtgan_attn_span_step_workspace_bytes(int M, int heads, int kv_heads, int dh, int max_keys);
+int nmtgan_attn_span_step(const nmtgan_span_args* a, int max_keys, void* workspace, size_t workspace_bytes, void* stream);
+size_t nmtgan_attn_span_grads_workspace_bytes(int M, int heads);
+int nmtgan_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Softmax cross entropy of hidden rows h [M][d] against a table w [V][d] (the softmax table of top(), model.py:804-820)
+ * without the logits in memory.  Target distribution: 1 - smoothing on the label, smoothing / (V - 1) on every other entry.
+ *   loss[i] = -sum_j q_j log softmax(h_i w^T)_j (label outside [0, V): 0),  lse[i] = log sum_j exp(h_i . w_j)
+ * nmtgan_linear_xent_grads: bf16 or fp32; grad_row[i] = d(objective)/d(loss[i]) (NULL: 1; a mean over n rows is 1/n), lse of
+ * the forward call; dh [M][d], dw [V][d] in `dtype` are overwritten.  Rows without a label have dh = 0 and add nothing to dw.
+ * d(logits) is formed one piece of the vocabulary at a time in the workspace, rounded once to `dtype`.
+ * d*esize a multiple of 16 bytes, rows 16-byte aligned, workspace 256-byte aligned. */
+typedef struct {
+  int dtype;
+  int M, V, d;
+  const void* h; int64_t ldh;
+  const void* w; int64_t ldw;
+  const int32_t* labels;                     /* [M] */
+  float smoothing;                           /* [0, 1) */
+} nmtgan_xent_args;
+size_t nmtgan_linear_xent_workspace_bytes(const nmtgan_xent_args* a, int grads);
+int nmtgan_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int nmtgan_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh,
+                             void* dw, int64_t ld_dw, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Norm over a list of gradient tensors and clipping by it, ahead of the update kernels:
+ *   norm[0] = sqrt(sum (grad_scale g)^2)     out = g grad_scale min(1, max_norm / norm)
+ * `tensors` is a HOST array read before the call returns; g and out are device pointers aligned to their element, out in
+ * the gradient's type or fp32 (the update kernels read fp32), equal to g for clipping in place.  Squares are summed in
+ * fp64.  A norm that is not finite makes every output NaN.  Outputs may overlap neither each other nor another gradient. */
+typedef struct { const void* g; void* out; int64_t n; int dtype; int out_dtype; } nmtgan_grad_ref;
+size_t nmtgan_global_norm_workspace_bytes(int n_tensors);
+int nmtgan_global_norm(const nmtgan_grad_ref* tensors, int n_tensors, float grad_scale, float* norm, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int nmtgan_clip_global_norm(const nmtgan_grad_ref* tensors, int n_tensors, float max_norm, float grad_scale, float* norm,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Measurement hook (no counterpart in the reference; used by bench.py's roofline leg only).
  * Between start and stop every kernel launch is bracketed by HIP events on its own stream;
  * stop synchronises the device and returns summed milliseconds and launch counts per class:

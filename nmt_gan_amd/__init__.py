@@ -10,7 +10,8 @@ from .share_function import (deal_generated_samples, deal_generated_samples_to_m
                              timing_signal, prepare_gan_dis_data)
 from .model import Model                               # noqa: F401
 from .cnn_discriminator import DisCNN                  # noqa: F401
+from . import ops                                      # noqa: F401  (span attention, cross entropy, norm clipping)
 
 __all__ = ["Model", "DisCNN", "AttrDict", "deal_generated_samples", "deal_generated_samples_to_maxlen",
            "extend_sentence_to_maxlen", "FlushFile",
-           "build_rollout_plan", "split_bounds", "timing_signal", "prepare_gan_dis_data", "lib", "LIB_PATH", "NmtGanError"]
+           "build_rollout_plan", "split_bounds", "timing_signal", "prepare_gan_dis_data", "ops", "lib", "LIB_PATH", "NmtGanError"]

@@ -127,6 +127,26 @@ class RewardPlan(C.Structure):
                 ("conv_table", i32), ("conv_table_max_bytes", i64)]
 
 
+class SpanArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("M", i32), ("N", i32), ("heads", i32), ("kv_heads", i32), ("dh", i32),
+                ("q", vp), ("ldq", i64), ("k", vp), ("ldk", i64), ("v", vp), ("ldv", i64),
+                ("lo", vp), ("hi", vp), ("pos", vp), ("slopes", vp), ("scale", f32), ("cap", f32),
+                ("out", vp), ("ldo", i64), ("lse", vp)]
+
+
+class SpanGrads(C.Structure):
+    _fields_ = [("dout", vp), ("ld_dout", i64), ("dq", vp), ("ld_dq", i64), ("dk", vp), ("ld_dk", i64), ("dv", vp), ("ld_dv", i64)]
+
+
+class XentArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("M", i32), ("V", i32), ("d", i32), ("h", vp), ("ldh", i64), ("w", vp), ("ldw", i64),
+                ("labels", vp), ("smoothing", f32)]
+
+
+class GradRef(C.Structure):
+    _fields_ = [("g", vp), ("out", vp), ("n", i64), ("dtype", i32), ("out_dtype", i32)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "nmtgan_version": (i32, []),
@@ -169,6 +189,17 @@ EXPORTS = {
     "nmtgan_clip_values": (i32, [vp, i64, f32, f32, vp, i32, vp]),
     "nmtgan_sgd_update": (i32, [vp, vp, i64, f32, f32, f32, vp, i32, vp]),
     "nmtgan_adam_update": (i32, [vp, vp, vp, vp, i64, f32, f32, f32, f32, i32, f32, f32, vp, i32, vp]),
+    "nmtgan_attn_span": (i32, [C.POINTER(SpanArgs), vp]),
+    "nmtgan_attn_span_step_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "nmtgan_attn_span_step": (i32, [C.POINTER(SpanArgs), i32, vp, sz, vp]),
+    "nmtgan_attn_span_grads_workspace_bytes": (sz, [i32, i32]),
+    "nmtgan_attn_span_grads": (i32, [C.POINTER(SpanArgs), C.POINTER(SpanGrads), vp, sz, vp]),
+    "nmtgan_linear_xent_workspace_bytes": (sz, [C.POINTER(XentArgs), i32]),
+    "nmtgan_linear_xent": (i32, [C.POINTER(XentArgs), vp, vp, vp, sz, vp]),
+    "nmtgan_linear_xent_grads": (i32, [C.POINTER(XentArgs), vp, vp, vp, i64, vp, i64, vp, sz, vp]),
+    "nmtgan_global_norm_workspace_bytes": (sz, [i32]),
+    "nmtgan_global_norm": (i32, [C.POINTER(GradRef), i32, f32, vp, vp, sz, vp]),
+    "nmtgan_clip_global_norm": (i32, [C.POINTER(GradRef), i32, f32, f32, vp, vp, sz, vp]),
     "nmtgan_profile_classes": (i32, []),
     "nmtgan_profile_start": (i32, []),
     "nmtgan_profile_stop": (i32, [C.POINTER(f64), C.POINTER(i64), i32]),

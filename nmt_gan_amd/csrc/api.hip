@@ -244,4 +244,36 @@ int nmtgan_adam_update(float* w, float* m, float* v, const float* grad, int64_t 
                          (hipStream_t)stream);
 }
 
+int nmtgan_attn_span(const nmtgan_span_args* a, void* stream) { return launch_attn_span(a, (hipStream_t)stream); }
+size_t nmtgan_attn_span_step_workspace_bytes(int M, int heads, int kv_heads, int dh, int max_keys) {
+  return attn_span_step_workspace(M, heads, kv_heads, dh, max_keys);
+}
+int nmtgan_attn_span_step(const nmtgan_span_args* a, int max_keys, void* workspace, size_t workspace_bytes, void* stream) {
+  return launch_attn_span_step(a, max_keys, workspace, workspace_bytes, (hipStream_t)stream);
+}
+size_t nmtgan_attn_span_grads_workspace_bytes(int M, int heads) { return attn_span_grads_workspace(M, heads); }
+int nmtgan_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  return launch_attn_span_grads(a, g, workspace, workspace_bytes, (hipStream_t)stream);
+}
+size_t nmtgan_linear_xent_workspace_bytes(const nmtgan_xent_args* a, int grads) { return linear_xent_workspace(a, grads != 0); }
+int nmtgan_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  return launch_linear_xent(a, loss, lse, workspace, workspace_bytes, (hipStream_t)stream);
+}
+int nmtgan_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh,
+                             void* dw, int64_t ld_dw, void* workspace, size_t workspace_bytes, void* stream) {
+  return launch_linear_xent_grads(a, lse, grad_row, dh, ld_dh, dw, ld_dw, workspace, workspace_bytes, (hipStream_t)stream);
+}
+size_t nmtgan_global_norm_workspace_bytes(int n_tensors) { return global_norm_workspace(n_tensors); }
+int nmtgan_global_norm(const nmtgan_grad_ref* tensors, int n_tensors, float grad_scale, float* norm, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return launch_global_norm(tensors, n_tensors, grad_scale, norm, workspace, workspace_bytes, (hipStream_t)stream);
+}
+int nmtgan_clip_global_norm(const nmtgan_grad_ref* tensors, int n_tensors, float max_norm, float grad_scale, float* norm,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  return launch_clip_global_norm(tensors, n_tensors, max_norm, grad_scale, norm, workspace, workspace_bytes,
+                                 (hipStream_t)stream);
+}
+
 }  // extern "C"

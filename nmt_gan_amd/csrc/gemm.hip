@@ -72,8 +72,11 @@ struct GemmParams {
   // instead of the product - add[(add_blk[r / a_group] * add_rows + add_row0 + r % a_group) * N + n] is added to the
   // accumulator before scale / shift / ReLU / max
   const float* add; const int32_t* add_blk; int add_rows; int add_row0;
+  // cross-entropy epilogues (xent.hip)
+  XentEpilogue x;
 };
 constexpr int EPI_STATS = 100;                  // internal: never a value of nmtgan_gemm_args.epilogue
+constexpr int EPI_XSTAT = 102, EPI_XGRAD = 103; // internal: vocabulary cross entropy, forward and d(logits)
 constexpr int EPI_CONVADD = 101;                // internal: CONVMAX + additive term, chosen when nmtgan_gemm_args.add is set
 
 // acc[I0 + i][J0 + j] += A-fragment i x B-fragment j for one k-half of a k-tile (MT x NT 16x16 tiles).  Consecutive
@@ -133,12 +136,100 @@ __device__ __forceinline__ int64_t a_row_offset(const GemmParams& p, int r) {
                          : (int64_t)r * p.lda_b;
 }
 
+// Cross-entropy epilogues.  The product runs transposed like the STATS form: C rows = vocabulary entries, C columns =
+// hidden rows, so one hidden row's 64 logits of a wave tile sit in 16 registers of each of four lanes.
+// XSTAT: stats[vtile][row] = (max, sum exp(z - max)) over the entries of a 64-entry tile that exist, and with smoothing
+// their plain sum in zsum[vtile][row].
+template <int MT>
+__device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
+  const int fc = lane & 15, fq = lane >> 4;
+#pragma unroll
+  for (int ip = 0; ip < MT / 4; ++ip) {
+    const int mb = m0 + 64 * ip;
+    if (mb >= p.M) continue;
+    const bool whole = mb + 64 <= p.M;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = n0 + j * 16 + fc;
+      float mx = -INFINITY, zs = 0.f;
+#pragma unroll
+      for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!whole && m0 + i * 16 + 4 * fq + e >= p.M) acc[i][j][e] = -INFINITY;
+          mx = fmaxf(mx, acc[i][j][e]);
+        }
+      mx = groups4_max(mx);
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((acc[i][j][e] - mu) * 1.44269504088896341f);
+      sum = groups4_sum(sum);
+      if (p.x.zsum) {
+#pragma unroll
+        for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (whole || m0 + i * 16 + 4 * fq + e < p.M) zs += acc[i][j][e];
+        zs = groups4_sum(zs);
+      }
+      if (fq == 0 && row < p.N) {
+        const int64_t at = (int64_t)((m0 >> 6) + ip) * p.N + row;
+        p.stats[at] = make_float2(mx, sum);
+        if (p.x.zsum) p.x.zsum[at] = zs;
+      }
+    }
+  }
+}
+
+// XGRAD: d(logit) = g (exp(z - lse) - low - high [entry == label]) in the operand type, entry-major (gt, K = rows of the
+// weight gradient's product) and row-major (g, K = entries of the hidden gradient's); entries and rows that pad either
+// K to whole k-tiles are written as zeros
+template <typename OpT, int MT>
+__device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
+  const int fc = lane & 15, fq = lane >> 4;
+  const XentEpilogue& x = p.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = n0 + j * 16 + fc;
+    if (row >= x.rows_padded) continue;
+    float gr = 0.f, ls = 0.f;
+    int label = -1;
+    if (row < p.N) {
+      label = x.labels[row];
+      if (label < 0 || label >= x.vocab) label = -1;
+      gr = label < 0 ? 0.f : (x.grad_row ? x.grad_row[row] : 1.f);
+      ls = x.lse[row];
+      label -= x.first;                            // entry inside this piece of the vocabulary
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int mb = m0 + i * 16 + 4 * fq;
+      if (mb >= x.piece_padded) continue;
+      OpT* out = reinterpret_cast<OpT*>(x.g) + (int64_t)row * x.piece_padded + mb;
+      OpT* outt = reinterpret_cast<OpT*>(x.gt) + (int64_t)mb * x.rows_padded + row;
+      float d[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float pe = __builtin_amdgcn_exp2f((acc[i][j][e] - ls) * 1.44269504088896341f) - x.low;
+        d[e] = gr == 0.f || mb + e >= p.M ? 0.f : gr * (mb + e == label ? pe - x.high : pe);
+        if (mb + e < p.M) OpTraits<OpT>::store(outt + (int64_t)e * x.rows_padded, d[e]);
+      }
+      if (row < p.N) VecIO<OpT, 4>::store(out, d);
+    }
+  }
+}
+
 // Epilogue of one wave's (16 MT) x 64 tile.  16x16 C layout: col = lane & 15, row = 4 * (lane >> 4) + reg
 // ev: optional LDS copy of the wave's 64 per-column epilogue values ([64] bias, or [64] scale + [64] shift),
 // staged by LDS-DMA so that no compiler-visible vector load sits next to the hand-counted DMA stream
 template <typename OpT, int EPI, int MT = 4>
 __device__ __forceinline__ void epilogue(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane,
                                          const float* ev = nullptr) {
+  if constexpr (EPI == EPI_XSTAT) { epilogue_xstat<MT>(p, acc, m0, n0, lane); return; }
+  if constexpr (EPI == EPI_XGRAD) { epilogue_xgrad<OpT, MT>(p, acc, m0, n0, lane); return; }
   const int fc = lane & 15, fq = lane >> 4;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -1721,6 +1812,28 @@ int launch_gemm_stats(int op_dtype, const void* W, int V, const void* X, int row
 bool gemm_stats_supported(int op_dtype, int V, int K) {
   const int es = dtype_size(op_dtype);
   return V % 64 == 0 && V <= 65536 && (K * es) % BKB == 0 && (K * es) / BKB >= 4;   // <= 1024 vocabulary tiles
+}
+
+// z^T = W[entries,K] . H[rows,K]^T with one of the cross-entropy epilogues; N of the product covers the padding rows of
+// the transposed gradient (rows_padded) through the last tile
+int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
+                     int K, float2* stats, const XentEpilogue& x, hipStream_t st) {
+  const int es = dtype_size(op_dtype);
+  GemmParams p{};
+  p.A = (const char*)W; p.W = (const char*)H;
+  p.M = entries; p.N = rows; p.K = K;
+  p.lda_b = ldw * es; p.ldw_b = ldh * es; p.kbytes = K * es;
+  p.k_inner = 1; p.k_step = BKB; p.k_jump = BKB;
+  p.stats = stats;
+  p.x = x;
+  if (!grad) {
+    NMTGAN_DISPATCH_OP(op_dtype, OpT, return (dispatch<OpT, EPI_XSTAT>(p, st)));
+  } else if (op_dtype == NMTGAN_BF16) {
+    return dispatch<bf16_t, EPI_XGRAD>(p, st);
+  } else {
+    return dispatch<float, EPI_XGRAD>(p, st);
+  }
+  return 0;
 }
 
 static int launch_gemm_impl(const nmtgan_gemm_args* a, hipStream_t st);

@@ -5,6 +5,17 @@
 
 namespace nmtgan {
 
+// operands of the cross-entropy epilogues of the GEMM (xent.hip); `first` .. first + entries is the piece of the
+// vocabulary the product covers, the gradient images are padded to whole k-tiles (64 entries / 64 rows)
+struct XentEpilogue {
+  const int32_t* labels; const float* grad_row; const float* lse;
+  float* zsum;                                   // forward, label smoothing only
+  void* g; void* gt;                             // [rows][piece_padded], [entries][rows_padded]
+  int vocab, first, piece_padded, rows_padded;
+  float low, high;
+};
+int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
+                     int K, float2* stats, const XentEpilogue& x, hipStream_t st);
 int launch_gemm(const nmtgan_gemm_args* a, hipStream_t st);
 // n independent problems of one epilogue kind (CONVMAX - with or without the additive term - or LINEAR with one fp32 or
 // op-dtype output) in one persistent launch per 24 problems; min_tiles > 0 leaves problems of at least that many 256x128 tiles to
@@ -42,6 +53,19 @@ int launch_attn_rows(const nmtgan_attn_args* a, hipStream_t st);
 int launch_sample_rows(const nmtgan_sample_args* a, hipStream_t st);
 int launch_attn_group(const nmtgan_attn_group_args* a, hipStream_t st);
 int launch_transpose_v(const void* v, void* vt, int nblk, int L, int Lp, int d, int esize, hipStream_t st);
+int launch_attn_span(const nmtgan_span_args* a, hipStream_t st);
+size_t attn_span_step_workspace(int M, int heads, int kv_heads, int dh, int max_keys);
+int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, size_t ws_bytes, hipStream_t st);
+size_t attn_span_grads_workspace(int M, int heads);
+int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g, void* ws, size_t ws_bytes, hipStream_t st);
+size_t linear_xent_workspace(const nmtgan_xent_args* a, bool grads);
+int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void* ws, size_t ws_bytes, hipStream_t st);
+int launch_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh,
+                             void* dw, int64_t ld_dw, void* ws, size_t ws_bytes, hipStream_t st);
+size_t global_norm_workspace(int n_tensors);
+int launch_global_norm(const nmtgan_grad_ref* t, int n, float grad_scale, float* norm, void* ws, size_t ws_bytes, hipStream_t st);
+int launch_clip_global_norm(const nmtgan_grad_ref* t, int n, float max_norm, float grad_scale, float* norm, void* ws,
+                            size_t ws_bytes, hipStream_t st);
 
 // rollout token bookkeeping (model.py:242-243, 250-252)
 int launch_init_rollouts(const int32_t* y, const int32_t* row_b, const int32_t* row_g, int n_rows, int T,
