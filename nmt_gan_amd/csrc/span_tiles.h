@@ -1,0 +1,439 @@
+// Span attention: query row i attends to the keys lo[i] <= j < hi[i] of one packed key buffer.  Causal, document, prefix
+// and padding masks of a packed (or padded) batch are all spans, so one kernel family serves teacher-forced training on
+// packed sentences, prompts, and single tokens over a long cache.
+//
+//   r = scale q_i . k_j          t = tanh(r / cap), s = cap t   (s = r without a cap)
+//   s -= slope_h |pos_i - j|     p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij)       out_i = sum_j p_ij v_j
+//   dp = dout_i . v_j   delta_i = dout_i . out_i   dr = p (dp - delta_i) (1 - t^2) scale
+//   dq_i = sum_j dr k_j    dk_j = sum_i dr q_i    dv_j = sum_i p dout_i   (sums over the heads that share a key head too)
+//
+// The tile kernels (span_fwd.hip, span_grad.hip) multiply whole tiles on the matrix cores and give the pairs outside the
+// spans the weight zero.  A NaN or an infinity in such a row would still come through (0 x NaN), so a wave that ends with
+// a value that is not finite does those rows again with the row functions below: one row by one wave in plain fp32
+// arithmetic over visible (row, key) pairs only.
+#pragma once
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace nmtgan {
+
+constexpr int SPAN_MAX_DH = 128;
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.69314718055994531f;
+
+struct SpanParams {
+  const void* q; const void* k; const void* v;
+  int64_t ldq, ldk, ldv, ldo;
+  const int32_t* lo; const int32_t* hi; const int32_t* pos;
+  const float* slopes;
+  void* out; float* lse;
+  int M, N, heads, kv_heads, dh;
+  float scale, cap;
+  // gradients
+  const void* dout; int64_t ld_do;
+  void* dq; void* dk; void* dv;
+  int64_t ld_dq, ld_dk, ld_dv;
+  float* delta;                                  // [M][heads]
+  int4* hull;                                    // [ceil(M / 32)] of 32 rows: keys seen by any row [x, y), by every row [z, w)
+};
+
+__device__ __forceinline__ float span_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
+// span of row i, cut to the key buffer; an empty one is (0, 0)
+__device__ __forceinline__ int2 span_of(const SpanParams& p, int i) {
+  const int a = max(p.lo[i], 0), b = min(p.hi[i], p.N);
+  return b > a ? make_int2(a, b) : make_int2(0, 0);
+}
+__device__ __forceinline__ int pos_of(const SpanParams& p, int i) { return p.pos ? p.pos[i] : p.hi[i] - 1; }
+
+// score of a raw product and the factor d(score)/d(product)
+__device__ __forceinline__ float span_score(const SpanParams& p, float dot, float slope, int pos, int j, float& turn) {
+  float r = dot * p.scale;
+  turn = p.scale;
+  if (p.cap > 0.f) {
+    const float t = tanhf(r / p.cap);
+    r = p.cap * t;
+    turn = (1.f - t * t) * p.scale;
+  }
+  if (p.slopes) r -= slope * fabsf((float)(pos - j));
+  return r;
+}
+
+// dot product of dh elements at `row` with the fp32 vector x (LDS, the same address in every lane)
+template <typename T>
+__device__ __forceinline__ float dot_row(const T* row, const float* x, int dh) {
+  float s = 0.f;
+  for (int c = 0; c < dh; c += 8) {
+    float a[8];
+    VecIO<T, 8>::load(row + c, a);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(a[e], x[c + e], s);
+  }
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ void stage_row(const T* row, float* x, int dh, int lane) {
+  for (int c = lane; c < dh; c += 64) x[c] = OpTraits<T>::load(row + c);
+}
+
+template <typename T>
+__device__ void span_fwd_row(const SpanParams& p, int i, int h, float* x, int lane) {
+  const int dh = p.dh, kvh = h / (p.heads / p.kv_heads);
+  const T* K = (const T*)p.k + kvh * dh;
+  const T* V = (const T*)p.v + kvh * dh;
+  stage_row((const T*)p.q + i * p.ldq + h * dh, x, dh, lane);
+  __builtin_amdgcn_wave_barrier();
+  const int2 sp = span_of(p, i);
+  const int pos = pos_of(p, i);
+  const float slope = p.slopes ? p.slopes[h] : 0.f;
+  float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
+  for (int j0 = sp.x; j0 < sp.y; j0 += 64) {
+    const int j = j0 + lane;
+    float s = -INFINITY, turn;
+    if (j < sp.y) s = span_score(p, dot_row(K + j * p.ldk, x, dh), slope, pos, j, turn);
+    const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
+    const float pe = j < sp.y ? span_exp(s - mu) : 0.f, f = span_exp(m - mu);
+    l = l * f + wave_sum(pe);
+    acc[0] *= f;
+    acc[1] *= f;
+    m = mn;
+    const int n = min(64, sp.y - j0);
+    for (int t = 0; t < n; ++t) {
+      const float pt = __shfl(pe, t, 64);
+      const T* row = V + (j0 + t) * p.ldv;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < dh) acc[u] = fmaf(pt, OpTraits<T>::load(row + lane + 64 * u), acc[u]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;               // NaN stays NaN
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 64 * u < dh) OpTraits<T>::store((T*)p.out + i * p.ldo + h * dh + lane + 64 * u, l == 0.f ? 0.f : acc[u] * inv);
+  if (p.lse && lane == 0) p.lse[(int64_t)i * p.heads + h] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + logf(l);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// p_ij and dr_ij of lane's pair; x = q row, y = dout row
+template <typename T>
+__device__ __forceinline__ void span_pair(const SpanParams& p, const T* krow, const T* vrow, const float* x, const float* y,
+                                          float lse, float delta, float slope, int pos, int j, float& pe, float& dr) {
+  float turn;
+  const float s = span_score(p, dot_row(krow, x, p.dh), slope, pos, j, turn);
+  pe = lse == -INFINITY ? 0.f : span_exp(s - lse);
+  dr = pe * (dot_row(vrow, y, p.dh) - delta) * turn;
+}
+
+template <typename T>
+__device__ void span_dq_row(const SpanParams& p, int i, int h, float* x, float* y, int lane) {
+  const int dh = p.dh, kvh = h / (p.heads / p.kv_heads);
+  const T* K = (const T*)p.k + kvh * dh;
+  const T* V = (const T*)p.v + kvh * dh;
+  stage_row((const T*)p.q + i * p.ldq + h * dh, x, dh, lane);
+  stage_row((const T*)p.dout + i * p.ld_do + h * dh, y, dh, lane);
+  __builtin_amdgcn_wave_barrier();
+  const int2 sp = span_of(p, i);
+  const int pos = pos_of(p, i);
+  const float slope = p.slopes ? p.slopes[h] : 0.f;
+  const float lse = p.lse[(int64_t)i * p.heads + h], delta = p.delta[(int64_t)i * p.heads + h];
+  float acc[2] = {0.f, 0.f};
+  for (int j0 = sp.x; j0 < sp.y; j0 += 64) {
+    const int j = j0 + lane;
+    float pe = 0.f, dr = 0.f;
+    if (j < sp.y) span_pair(p, K + j * p.ldk, V + j * p.ldv, x, y, lse, delta, slope, pos, j, pe, dr);
+    const int n = min(64, sp.y - j0);
+    for (int t = 0; t < n; ++t) {
+      const float d = __shfl(dr, t, 64);
+      const T* row = K + (j0 + t) * p.ldk;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < dh) acc[u] = fmaf(d, OpTraits<T>::load(row + lane + 64 * u), acc[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 64 * u < dh) OpTraits<T>::store((T*)p.dq + i * p.ld_dq + h * dh + lane + 64 * u, acc[u]);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// key j of key head kvh: x = k row, y = v row; walks the query rows that see it, head by head of the group
+template <typename T>
+__device__ void span_dkv_key(const SpanParams& p, int j, int kvh, float* x, float* y, int lane) {
+  const int dh = p.dh, g = p.heads / p.kv_heads;
+  stage_row((const T*)p.k + j * p.ldk + kvh * dh, x, dh, lane);
+  stage_row((const T*)p.v + j * p.ldv + kvh * dh, y, dh, lane);
+  __builtin_amdgcn_wave_barrier();
+  float ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
+  const int nh = (p.M + 31) / 32;
+  for (int b = 0; 2 * b < nh; ++b) {
+    int4 hl = p.hull[2 * b];
+    if (2 * b + 1 < nh) { const int4 o = p.hull[2 * b + 1]; hl = make_int4(min(hl.x, o.x), max(hl.y, o.y), 0, 0); }
+    if (j < hl.x || j >= hl.y) continue;
+    const int i = b * 64 + lane;
+    int2 sp = make_int2(0, 0);
+    int pos = 0;
+    if (i < p.M) { sp = span_of(p, i); pos = pos_of(p, i); }
+    const bool on = j >= sp.x && j < sp.y;
+    const unsigned long long mask = __ballot(on);
+    if (mask == 0) continue;
+    for (int h = kvh * g; h < (kvh + 1) * g; ++h) {
+      const T* Q = (const T*)p.q + h * dh;
+      const T* D = (const T*)p.dout + h * dh;
+      float pe = 0.f, dr = 0.f;
+      if (on)
+        span_pair(p, Q + i * p.ldq, D + i * p.ld_do, x, y, p.lse[(int64_t)i * p.heads + h],
+                  p.delta[(int64_t)i * p.heads + h], p.slopes ? p.slopes[h] : 0.f, pos, j, pe, dr);
+      for (unsigned long long left = mask; left; left &= left - 1) {
+        const int t = __builtin_ctzll(left);
+        const float pt = __shfl(pe, t, 64), dt = __shfl(dr, t, 64);
+        const int64_t r = b * 64 + t;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (lane + 64 * u < dh) {
+            av[u] = fmaf(pt, OpTraits<T>::load(D + r * p.ld_do + lane + 64 * u), av[u]);
+            ak[u] = fmaf(dt, OpTraits<T>::load(Q + r * p.ldq + lane + 64 * u), ak[u]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 64 * u < dh) {
+      OpTraits<T>::store((T*)p.dk + j * p.ld_dk + kvh * dh + lane + 64 * u, ak[u]);
+      OpTraits<T>::store((T*)p.dv + j * p.ld_dv + kvh * dh + lane + 64 * u, av[u]);
+    }
+  __builtin_amdgcn_wave_barrier();
+}
+
+#define NMTGAN_DISPATCH_GRAD(dt, T, ...)                                          \
+  do {                                                                            \
+    if ((dt) == NMTGAN_BF16) { using T = ::nmtgan::bf16_t; __VA_ARGS__; }         \
+    else { using T = float; __VA_ARGS__; }                                        \
+  } while (0)
+
+// ------------------------------------------------------------------------------------------ tiles on the matrix cores
+// A wave owns 32 query rows (32 key rows in the dk/dv kernel) and walks the other side in tiles staged through LDS.
+// Scores come transposed, S^T = K Q^T (32x32 products: lane & 31 = the wave's own row, 16 registers = rows of the tile), so
+//   * a softmax row lives in the registers of two lanes (l, l ^ 32): its maximum and sum need one lane swap each;
+//   * the same registers are the B operand of the second product (out^T = V^T P^T, dq^T = K^T dS^T, dv^T = dO^T P,
+//     dk^T = Q^T dS) as they stand: which of a step's 16 tile rows sits in which k slot is free as long as A agrees, and A
+//     is read in that order (ds_read_b64_tr_b16 turns 4 rows x 16 columns of the 16-bit tile; fp32 reads words).
+// Rows of a tile are 16-byte chunks, XOR-swizzled so that 16 lanes that read one chunk of 16 rows hit 64 banks.
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_p;
+
+template <typename T, int DP> struct Geo {
+  static constexpr int RB = DP * (int)sizeof(T), CH = RB / 16, STEPS = RB / 32, DB = DP / 32;
+  static constexpr int RPL = RB >= 256 ? 1 : 256 / RB, MASK = CH < 16 ? CH - 1 : 15;
+  __device__ static __forceinline__ int swz(int row, int chunk) { return row * RB + ((chunk ^ ((row / RPL) & MASK)) << 4); }
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16_t mma_rows(const uint4& a, const uint4& b, f32x16_t c) {
+  if constexpr (sizeof(T) == 2) {
+    return mfma16<T>(a, b, c);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  }
+}
+// s += tile rows [32 kb, +32) . own rows
+template <typename T, int DP>
+__device__ __forceinline__ f32x16_t score_block(const unsigned char* tile, int kb, const uint4 (&own)[Geo<T, DP>::STEPS], int lane) {
+  using G = Geo<T, DP>;
+  f32x16_t c;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) c[r] = 0.f;
+#pragma unroll
+  for (int s = 0; s < G::STEPS; ++s) {
+    const uint4 a = *reinterpret_cast<const uint4*>(tile + G::swz(32 * kb + (lane & 31), 2 * s + (lane >> 5)));
+    c = mma_rows<T>(a, own[s], c);
+  }
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ unsigned pack_pair(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(T, bf16_t)) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{a, b}), b2));
+  } else {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{a, b}), f16x2_t));
+  }
+}
+// acc^T[dh][own] += (tile^T)[dh][rows 32 kb ..] . x, x = a score block's registers
+template <typename T, int DP>
+__device__ __forceinline__ void accum_block(const unsigned char* tile, int kb, const f32x16_t& x, f32x16_t (&acc)[Geo<T, DP>::DB],
+                                            int lane) {
+  using G = Geo<T, DP>;
+  const int hl = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint4 b = make_uint4(pack_pair<T>(x[8 * t], x[8 * t + 1]), pack_pair<T>(x[8 * t + 2], x[8 * t + 3]),
+                                 pack_pair<T>(x[8 * t + 4], x[8 * t + 5]), pack_pair<T>(x[8 * t + 6], x[8 * t + 7]));
+      const int row = 32 * kb + 16 * t + 4 * hl + ((lane & 15) >> 2);
+#pragma unroll
+      for (int db = 0; db < G::DB; ++db) {
+        const int col = 32 * db + (lane & 16) + 4 * (lane & 3);
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4_p)(tile + G::swz(row, col >> 3) + 2 * (col & 7)));
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4_p)(tile + G::swz(row + 8, col >> 3) + 2 * (col & 7)));
+        const uint2 u = __builtin_bit_cast(uint2, lo), v = __builtin_bit_cast(uint2, hi);
+        acc[db] = mfma16<T>(make_uint4(u.x, u.y, v.x, v.y), b, acc[db]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 32 * kb + 8 * (r >> 2) + 4 * hl + (r & 3);
+#pragma unroll
+      for (int db = 0; db < G::DB; ++db) {
+        const int col = 32 * db + (lane & 31);
+        const float a = *reinterpret_cast<const float*>(tile + G::swz(row, col >> 2) + 4 * (col & 3));
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[r], acc[db], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// rows [row0, row0 + R) of a [*][ld] matrix on their way to LDS through registers; rows from `end` on and columns from dh
+// on are zeros
+template <typename T, int DP, int R, int NT> struct Stage {
+  using G = Geo<T, DP>;
+  static constexpr int N = R * G::CH / NT;
+  static_assert(R * G::CH % NT == 0, "whole chunks per thread");
+  uint4 x[N];
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int end, int dh, int tid) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int idx = tid + u * NT, row = row0 + idx / G::CH, c = idx % G::CH;
+      const bool ok = row < end && c * (16 / (int)sizeof(T)) < dh;
+      x[u] = ok ? *reinterpret_cast<const uint4*>(base + (int64_t)row * ld + c * (16 / (int)sizeof(T))) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* tile, int tid) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int idx = tid + u * NT;
+      *reinterpret_cast<uint4*>(tile + G::swz(idx / G::CH, idx % G::CH)) = x[u];
+    }
+  }
+};
+// own row as the B operand of score_block
+template <typename T, int DP>
+__device__ __forceinline__ void load_own(const T* row, bool ok, int dh, int lane, uint4 (&own)[Geo<T, DP>::STEPS]) {
+#pragma unroll
+  for (int s = 0; s < Geo<T, DP>::STEPS; ++s) {
+    const int c = (2 * s + (lane >> 5)) * (16 / (int)sizeof(T));
+    own[s] = ok && c < dh ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+  }
+}
+// transposed accumulators of the wave's own rows -> memory
+template <typename T, int DP>
+__device__ __forceinline__ void store_own(T* row, const f32x16_t (&acc)[Geo<T, DP>::DB], float f, int dh, int lane) {
+#pragma unroll
+  for (int db = 0; db < Geo<T, DP>::DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * db + 8 * g + 4 * (lane >> 5);
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = acc[db][4 * g + e] * f;
+      if (col < dh) VecIO<T, 4>::store(row + col, x);
+    }
+}
+template <int DB>
+__device__ __forceinline__ bool all_finite(const f32x16_t (&acc)[DB]) {
+  float z = 0.f;                                  // x * 0 is 0 for every finite x and NaN for the others
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z = fmaf(acc[db][r], 0.f, z);
+  return z == 0.f;
+}
+template <int DB>
+__device__ __forceinline__ void clear(f32x16_t (&acc)[DB]) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+}
+__device__ __forceinline__ float both_halves_max(float v) {
+  const u32x2_t b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float both_halves_sum(float v) {
+  const u32x2_t b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// tanh to about 2^-23 absolute: exp2 and a reciprocal for the 16-bit types, the library function for fp32
+template <typename T>
+__device__ __forceinline__ float span_tanh(float x) {
+  if constexpr (sizeof(T) == 4) return tanhf(x);
+  else return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * LOG2E)));
+}
+// score of a raw product in units of log 2, and 1 - t^2
+template <typename T>
+__device__ __forceinline__ float score2(const SpanParams& p, float dot, float inv_cap, float slope, int pos, int j, float& turn) {
+  float r = dot * p.scale;
+  turn = 1.f;
+  if (p.cap > 0.f) {
+    const float t = span_tanh<T>(r * inv_cap);
+    r = p.cap * t;
+    turn = fmaf(-t, t, 1.f);
+  }
+  r -= slope * fabsf((float)(pos - j));
+  return r * LOG2E;
+}
+
+struct WaveSpan { int lo, hi, all_lo, all_hi; };   // hull of a wave's spans; keys all of its rows see
+__device__ __forceinline__ WaveSpan wave_span(int2 sp) {
+  int a = sp.y > sp.x ? sp.x : 0x7fffffff, b = sp.y, c = sp.x, d = sp.y;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    a = min(a, __shfl_xor(a, o, 64));
+    b = max(b, __shfl_xor(b, o, 64));
+    c = max(c, __shfl_xor(c, o, 64));
+    d = min(d, __shfl_xor(d, o, 64));
+  }
+  return WaveSpan{__builtin_amdgcn_readfirstlane(a), __builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(c),
+                  __builtin_amdgcn_readfirstlane(d)};
+}
+// hull over the workgroup's waves
+template <int NW>
+__device__ __forceinline__ int2 block_span(const WaveSpan& ws, int (*red)[2], int w) {
+  if constexpr (NW == 1) return make_int2(ws.lo, ws.hi);
+  if ((threadIdx.x & 63) == 0) { red[w][0] = ws.lo; red[w][1] = ws.hi; }
+  __syncthreads();
+  int a = 0x7fffffff, b = 0;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) { a = min(a, red[k][0]); b = max(b, red[k][1]); }
+  return make_int2(a, b);
+}
+
+
+// dynamic LDS beyond 64 KiB has to be asked for once per device and kernel
+template <typename F>
+static inline int raise_lds(F* kernel, size_t bytes, const char* what) {
+  if (bytes <= 64 * 1024) return 0;
+  NMTGAN_REQUIRE(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
+                     hipSuccess, "%s: cannot raise the dynamic LDS limit", what);
+  return 0;
+}
+// Waves of 32 rows that a launch has in all: below two per SIMD every wave is a workgroup of its own (32-row tiles, more
+// workgroups to spread); above, four waves share the tiles they stage.
+constexpr int64_t SPAN_FEW_WAVES = 2048;
+
+int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st);
+int span_dq_tiles(int dtype, const SpanParams& p, hipStream_t st);
+int span_dkv_tiles(int dtype, const SpanParams& p, hipStream_t st);
+
+}  // namespace nmtgan
