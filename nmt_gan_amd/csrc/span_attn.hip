@@ -49,61 +49,186 @@ __global__ __launch_bounds__(256) void span_prep_kernel(SpanParams p) {
 }
 
 // ------------------------------------------------------------------------------------------ single tokens
-// One query row per workgroup and key head, `splits` workgroups along the span; every wave takes every fourth block of
-// keys.  part[row][head][split] = (acc[dh], m, l), joined in split order by span_join_kernel.
+// One query row and one key head with up to GT of its query heads per workgroup, `splits` workgroups along the span.  A key
+// row is read once, as 16-byte chunks by LPK neighbouring lanes, so a wave reads 64 / LPK keys per instruction and STEP_U
+// such groups of K and of V are in flight while the previous ones are used.  Every lane group keeps a softmax of its own
+// (no exchange inside the loop but the LPK-lane sum of a dot product); groups, waves and splits are joined at the end in a
+// fixed order.  The arithmetic stays on the vector units: at 8 heads per key head it is what bounds the loop, at 4 or fewer
+// the reads are (48 rows, 8 heads over 2, spans of up to 16384 keys of 64 fp16: see the table of measurements).
+constexpr int STEP_U = 4;
+
+template <int LPK>
+__device__ __forceinline__ float key_sum(float v) {          // over the lanes of one key
+  v = dpp_add<0xB1>(v);
+  v = dpp_add<0x4E>(v);
+  if constexpr (LPK >= 8) v = dpp_add<0x141>(v);
+  if constexpr (LPK >= 16) v = dpp_add<0x140>(v);
+  if constexpr (LPK >= 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)));
+}
+// over the lanes that hold the same chunk of different keys (rotations by 8 and 4 inside 16 lanes, then across)
+template <int LPK>
+__device__ __forceinline__ float chunk_sum(float v) {
+  if constexpr (LPK <= 8) v = dpp_add<0x128>(v);
+  if constexpr (LPK <= 4) v = dpp_add<0x124>(v);
+  if constexpr (LPK <= 16) return groups4_sum(v);
+  else return both_halves_sum(v);
+}
+template <int LPK>
+__device__ __forceinline__ float chunk_max(float v) {
+  if constexpr (LPK <= 8) v = dpp_max<0x128>(v);
+  if constexpr (LPK <= 4) v = dpp_max<0x124>(v);
+  if constexpr (LPK <= 16) return groups4_max(v);
+  else return both_halves_max(v);
+}
 template <typename T>
-__global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits, float* part) {
-  __shared__ float xs[4][SPAN_MAX_DH];
-  __shared__ float ms[4], ls[4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int i = blockIdx.x / splits, z = blockIdx.x % splits, h = blockIdx.y, dh = p.dh;
-  const int kvh = h / (p.heads / p.kv_heads);
-  const int2 sp = span_of(p, i);
-  const int pos = pos_of(p, i), len = sp.y - sp.x;
-  const int j0 = sp.x + (int)((int64_t)len * z / splits), j1 = sp.x + (int)((int64_t)len * (z + 1) / splits);
-  const float slope = p.slopes ? p.slopes[h] : 0.f;
-  const T* K = (const T*)p.k + kvh * dh;
-  const T* V = (const T*)p.v + kvh * dh;
-  stage_row((const T*)p.q + i * p.ldq + h * dh, xs[w], dh, lane);
-  __builtin_amdgcn_wave_barrier();
-  float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
-  for (int b = j0 + 64 * w; b < j1; b += 256) {
-    const int j = b + lane;
-    float s = -INFINITY, turn;
-    if (j < j1) s = span_score(p, dot_row(K + j * p.ldk, xs[w], dh), slope, pos, j, turn);
-    const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
-    const float pe = j < j1 ? span_exp(s - mu) : 0.f, f = span_exp(m - mu);
-    l = l * f + wave_sum(pe);
-    m = mn;
-    acc[0] *= f;
-    acc[1] *= f;
-    const int n = min(64, j1 - b);
-    for (int t = 0; t < n; ++t) {
-      const float pt = __shfl(pe, t, 64);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < dh) acc[u] = fmaf(pt, OpTraits<T>::load(V + (b + t) * p.ldv + lane + 64 * u), acc[u]);
-    }
-  }
-  __syncthreads();
-  if (lane == 0) { ms[w] = m; ls[w] = l; }
-  __syncthreads();
-  const float mt = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), mu = mt == -INFINITY ? 0.f : mt;
-  const float f = span_exp(m - mu);
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (lane + 64 * u < dh) xs[w][lane + 64 * u] = acc[u] * f;
-  __syncthreads();
-  float* o = part + (((int64_t)i * p.heads + h) * splits + z) * (dh + 2);
-  for (int c = threadIdx.x; c < dh; c += 256) o[c] = (xs[0][c] + xs[1][c]) + (xs[2][c] + xs[3][c]);
-  if (threadIdx.x == 0) {
-    float lt = 0.f;
-    for (int k = 0; k < 4; ++k) lt += ls[k] * span_exp(ms[k] - mu);
-    o[dh] = mu;
-    o[dh + 1] = lt;
+__device__ __forceinline__ void unpack_chunk(const uint4& r, float (&f)[16 / (int)sizeof(T)]) {
+  if constexpr (sizeof(T) == 2) {
+    unpack8<T>(r, f);
+  } else {
+    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
   }
 }
 
+template <typename T, int DP, int GT, bool EXTRA>
+__global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits, int groups, float* part) {
+  constexpr int EPC = 16 / (int)sizeof(T), LPK = DP / EPC, KPW = 64 / LPK, KB = STEP_U * KPW;
+  __shared__ float s_acc[4][GT][DP];
+  __shared__ float s_m[4][GT], s_l[4][GT];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, dh = p.dh, g = p.heads / p.kv_heads;
+  const int i = blockIdx.x / splits, z = blockIdx.x % splits;
+  const int kvh = blockIdx.y / groups, h0 = kvh * g + (blockIdx.y % groups) * GT, ng = min(GT, (kvh + 1) * g - h0);
+  const int c = (lane % LPK) * EPC, kk = lane / LPK;
+  const int2 sp = span_of(p, i);
+  const int64_t len = sp.y - sp.x;
+  const int j0 = sp.x + (int)(len * z / splits), j1 = sp.x + (int)(len * (z + 1) / splits);
+  const bool has = c < dh;
+  const T* K = (const T*)p.k + kvh * dh + c;
+  const T* V = (const T*)p.v + kvh * dh + c;
+  const float f = EXTRA ? 1.f : p.scale * LOG2E;             // products come out in units of log 2
+  float q[GT][EPC], acc[GT][EPC], m[GT], l[GT], slope[GT];
+#pragma unroll
+  for (int u = 0; u < GT; ++u) {
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (has && u < ng) r = *reinterpret_cast<const uint4*>((const T*)p.q + (int64_t)i * p.ldq + (h0 + u) * dh + c);
+    unpack_chunk<T>(r, q[u]);
+    m[u] = -INFINITY;
+    l[u] = slope[u] = 0.f;
+    if (EXTRA && p.slopes && u < ng) slope[u] = p.slopes[h0 + u];
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) {
+      q[u][e] *= f;
+      acc[u][e] = 0.f;
+    }
+  }
+  const int pos = EXTRA ? pos_of(p, i) : 0;
+  const float inv_cap = EXTRA && p.cap > 0.f ? 1.f / p.cap : 0.f;
+
+  uint4 kr[STEP_U], vr[STEP_U];
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < STEP_U; ++u) {
+      const int j = b + u * KPW + kk;
+      const bool ok = has && j < j1;
+      kr[u] = ok ? *reinterpret_cast<const uint4*>(K + (int64_t)j * p.ldk) : make_uint4(0, 0, 0, 0);
+      vr[u] = ok ? *reinterpret_cast<const uint4*>(V + (int64_t)j * p.ldv) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  int b = j0 + KB * w;
+  if (b < j1) fetch(b);
+  for (; b < j1; b += 4 * KB) {
+    uint4 ka[STEP_U], va[STEP_U];
+#pragma unroll
+    for (int u = 0; u < STEP_U; ++u) { ka[u] = kr[u]; va[u] = vr[u]; }
+    if (b + 4 * KB < j1) fetch(b + 4 * KB);
+    float s[STEP_U][GT];
+#pragma unroll
+    for (int u = 0; u < STEP_U; ++u) {
+      float x[EPC];
+      unpack_chunk<T>(ka[u], x);
+      const int j = b + u * KPW + kk;
+#pragma unroll
+      for (int t = 0; t < GT; ++t) {
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) d = fmaf(x[e], q[t][e], d);
+        d = key_sum<LPK>(d);
+        float turn;
+        if constexpr (EXTRA) d = score2<T>(p, d, inv_cap, slope[t], pos, j, turn);
+        s[u][t] = j < j1 ? d : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < GT; ++t) {
+      float mx = s[0][t];
+#pragma unroll
+      for (int u = 1; u < STEP_U; ++u) mx = fmaxf(mx, s[u][t]);
+      const float mn = fmaxf(m[t], mx), mu = mn == -INFINITY ? 0.f : mn;
+      if (__any(mn > m[t])) {
+        const float r = __builtin_amdgcn_exp2f(m[t] - mu);
+        l[t] *= r;
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) acc[t][e] *= r;
+        m[t] = mn;
+      }
+#pragma unroll
+      for (int u = 0; u < STEP_U; ++u) {
+        s[u][t] = __builtin_amdgcn_exp2f(s[u][t] - mu);
+        l[t] += s[u][t];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < STEP_U; ++u) {
+      float x[EPC];
+      unpack_chunk<T>(va[u], x);
+#pragma unroll
+      for (int t = 0; t < GT; ++t)
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) acc[t][e] = fmaf(s[u][t], x[e], acc[t][e]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < GT; ++t) {
+    const float mt = chunk_max<LPK>(m[t]), mu = mt == -INFINITY ? 0.f : mt, r = __builtin_amdgcn_exp2f(m[t] - mu);
+    const float lt = chunk_sum<LPK>(l[t] * r);
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) {
+      const float a = chunk_sum<LPK>(acc[t][e] * r);
+      if (kk == 0) s_acc[w][t][c + e] = a;
+    }
+    if (lane == 0) { s_m[w][t] = mt; s_l[w][t] = lt; }
+  }
+  __syncthreads();
+  for (int t = w; t < ng; t += 4) {                          // a wave per head joins the four
+    const float mt = fmaxf(fmaxf(s_m[0][t], s_m[1][t]), fmaxf(s_m[2][t], s_m[3][t])), mu = mt == -INFINITY ? 0.f : mt;
+    float r[4], lt = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      r[k] = __builtin_amdgcn_exp2f(s_m[k][t] - mu);
+      lt += s_l[k][t] * r[k];
+    }
+    const int64_t at = (int64_t)i * p.heads + h0 + t;
+    for (int k = lane; k < dh; k += 64) {
+      const float a = (s_acc[0][t][k] * r[0] + s_acc[1][t][k] * r[1]) + (s_acc[2][t][k] * r[2] + s_acc[3][t][k] * r[3]);
+      if (splits == 1) OpTraits<T>::store((T*)p.out + (int64_t)i * p.ldo + (h0 + t) * dh + k, lt == 0.f ? 0.f : a / lt);
+      else part[(at * splits + z) * (dh + 2) + k] = a;
+    }
+    if (lane == 0) {
+      if (splits > 1) {
+        part[(at * splits + z) * (dh + 2) + dh] = mt;
+        part[(at * splits + z) * (dh + 2) + dh + 1] = lt;
+      } else if (p.lse) {
+        p.lse[at] = lt == 0.f ? -INFINITY : mt * LN2 + logf(lt);
+      }
+    }
+  }
+}
+
+// one wave per (row, head): the splits' parts, in order
 template <typename T>
 __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, int splits, const float* part) {
   const int lane = threadIdx.x & 63;
@@ -111,25 +236,17 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, int splits
   if (t >= (int64_t)p.M * p.heads) return;
   const int i = (int)(t / p.heads), h = (int)(t % p.heads), dh = p.dh;
   const float* o = part + t * splits * (dh + 2);
-  float m = -INFINITY;
-  for (int z = 0; z < splits; ++z)
-    if (o[z * (dh + 2) + dh + 1] != 0.f) m = fmaxf(m, o[z * (dh + 2) + dh]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[2] = {0.f, 0.f};
-  for (int z = 0; z < splits; ++z) {
-    const float* q = o + z * (dh + 2);
-    if (q[dh + 1] == 0.f) continue;
-    const float f = span_exp(q[dh] - mu);
-    l += q[dh + 1] * f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < dh) acc[u] += q[lane + 64 * u] * f;
+  // splits <= 64: lane z holds split z's maximum and sum
+  const float mz = lane < splits ? o[lane * (dh + 2) + dh] : -INFINITY, lz = lane < splits ? o[lane * (dh + 2) + dh + 1] : 0.f;
+  const float m = wave_max(mz), mu = m == -INFINITY ? 0.f : m, rz = __builtin_amdgcn_exp2f(mz - mu);
+  const float l = wave_sum(lz * rz);
+  for (int c0 = 0; c0 < dh; c0 += 64) {                      // every lane stays in the loop: it answers the exchange
+    const int c = min(c0 + lane, dh - 1);
+    float acc = 0.f;
+    for (int z = 0; z < splits; ++z) acc = fmaf(o[z * (dh + 2) + c], __shfl(rz, z, 64), acc);
+    if (c0 + lane < dh) OpTraits<T>::store((T*)p.out + (int64_t)i * p.ldo + h * dh + c, l == 0.f ? 0.f : acc / l);
   }
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (lane + 64 * u < dh)
-      OpTraits<T>::store((T*)p.out + i * p.ldo + h * dh + lane + 64 * u, l == 0.f ? 0.f : acc[u] / l);
-  if (p.lse && lane == 0) p.lse[t] = l == 0.f ? -INFINITY : mu + logf(l);
+  if (p.lse && lane == 0) p.lse[t] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -172,16 +289,38 @@ int launch_attn_span(const nmtgan_span_args* a, hipStream_t st) {
   return span_fwd_tiles(a->dtype, p, st);
 }
 
-// Workgroups along a span: enough to fill the chip, none with less than 256 keys.  max_keys is a hint (the split is
-// made of the true length on the device), so a wrong one costs time only.
+// Workgroups along a span: enough to fill the chip four workgroups deep, none with less than 512 keys, and none but one
+// below 1024 keys - the second launch that joins them costs more than the walk.  max_keys is a hint (the cut is made of the
+// true length on the device), so a wrong one costs time only.
 static int span_splits(int M, int kv_heads, int max_keys) {
+  if (max_keys <= 1024) return 1;
   const int64_t groups = std::max<int64_t>(1, (int64_t)M * kv_heads);
   const int64_t fill = (1024 + groups - 1) / groups;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(fill, 64), (max_keys + 255) / 256));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(fill, 64), (max_keys + 511) / 512));
 }
 size_t attn_span_step_workspace(int M, int heads, int kv_heads, int dh, int max_keys) {
   if (M <= 0 || heads <= 0 || kv_heads <= 0 || dh <= 0) return 0;
-  return (size_t)M * heads * span_splits(M, kv_heads, max_keys) * (dh + 2) * sizeof(float);
+  const int splits = span_splits(M, kv_heads, max_keys);
+  return splits == 1 ? 0 : (size_t)M * heads * splits * (dh + 2) * sizeof(float);
+}
+template <typename T, int DP, int GT>
+static int launch_step(const SpanParams& p, int splits, float* part, hipStream_t st) {
+  const int groups = (p.heads / p.kv_heads + GT - 1) / GT;
+  const dim3 grid((unsigned)(p.M * splits), p.kv_heads * groups);
+  if (p.cap > 0.f || p.slopes)
+    hipLaunchKernelGGL((span_step_kernel<T, DP, GT, true>), grid, dim3(256), 0, st, p, splits, groups, part);
+  else
+    hipLaunchKernelGGL((span_step_kernel<T, DP, GT, false>), grid, dim3(256), 0, st, p, splits, groups, part);
+  NMTGAN_CHECK_LAUNCH("attn_span_step");
+  return 0;
+}
+template <typename T, int DP>
+static int choose_step(const SpanParams& p, int splits, float* part, hipStream_t st) {
+  const int g = p.heads / p.kv_heads;
+  if (g == 1) return launch_step<T, DP, 1>(p, splits, part, st);
+  if (g == 2) return launch_step<T, DP, 2>(p, splits, part, st);
+  if (g <= 4) return launch_step<T, DP, 4>(p, splits, part, st);
+  return launch_step<T, DP, 8>(p, splits, part, st);
 }
 int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, size_t ws_bytes, hipStream_t st) {
   prof::Scope prof_scope(prof::OTHER, st);
@@ -190,13 +329,15 @@ int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, siz
   NMTGAN_REQUIRE(max_keys >= 0, "attn_span_step: max_keys=%d", max_keys);
   if (p.M == 0) return 0;
   const size_t need = attn_span_step_workspace(p.M, p.heads, p.kv_heads, p.dh, max_keys);
-  NMTGAN_REQUIRE(ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0, "attn_span_step: workspace of %zu bytes needed, %zu given",
-                 need, ws_bytes);
+  NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0),
+                 "attn_span_step: workspace of %zu bytes needed, %zu given", need, ws_bytes);
   const int splits = span_splits(p.M, p.kv_heads, max_keys);
   NMTGAN_REQUIRE((int64_t)p.M * splits < (1LL << 31), "attn_span_step: too many rows");
   NMTGAN_DISPATCH_OP(a->dtype, T, {
-    hipLaunchKernelGGL(span_step_kernel<T>, dim3(p.M * splits, p.heads), dim3(256), 0, st, p, splits, (float*)ws);
-    NMTGAN_CHECK_LAUNCH("attn_span_step");
+    if (p.dh <= 32) NMTGAN_TRY((choose_step<T, 32>(p, splits, (float*)ws, st)));
+    else if (p.dh <= 64) NMTGAN_TRY((choose_step<T, 64>(p, splits, (float*)ws, st)));
+    else NMTGAN_TRY((choose_step<T, 128>(p, splits, (float*)ws, st)));
+    if (splits == 1) return 0;
     hipLaunchKernelGGL(span_join_kernel<T>, dim3((unsigned)(((int64_t)p.M * p.heads + 3) / 4)), dim3(256), 0, st, p, splits,
                        (const float*)ws);
   });

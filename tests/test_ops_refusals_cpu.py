@@ -36,8 +36,8 @@ def test_span_refusals(kw, part):
 
 def test_span_null_arguments_and_workspaces():
     _refused(L.lib.nmtgan_attn_span(None, None), "null")
-    _refused(L.lib.nmtgan_attn_span_step(C.byref(_span()), 4, P, 16, None), "workspace")
-    _refused(L.lib.nmtgan_attn_span_step(C.byref(_span()), 4, None, 1 << 30, None), "workspace")
+    _refused(L.lib.nmtgan_attn_span_step(C.byref(_span()), 4000, P, 16, None), "workspace")
+    _refused(L.lib.nmtgan_attn_span_step(C.byref(_span()), 4000, None, 1 << 30, None), "workspace")
     _refused(L.lib.nmtgan_attn_span_step(C.byref(_span()), -1, P, 1 << 30, None), "max_keys")
     assert L.lib.nmtgan_attn_span(C.byref(_span(M=0, q=None, lo=None, hi=None, out=None)), None) == 0      # nothing to do
     assert L.lib.nmtgan_attn_span_step_workspace_bytes(0, 2, 2, 64, 100) == 0
