@@ -17,6 +17,8 @@ from . import _lib as L
 from ._lib import lib
 
 _CODE = {torch.bfloat16: L.NMTGAN_BF16, torch.float16: L.NMTGAN_F16, torch.float32: L.NMTGAN_F32}
+_SIZE = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4}
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the hipStream_t of torch.cuda.current_stream(index)
 
 
 def _fail(what, text):
@@ -24,19 +26,22 @@ def _fail(what, text):
 
 
 def _rows(what, name, t, width, device, dtype):
-    """Row stride of a [rows, width] matrix whose rows are contiguous and 16-byte aligned."""
-    if t.dim() != 2 or t.shape[1] != width:
-        _fail(what, "%s must be [rows, %d], is %s" % (name, width, tuple(t.shape)))
+    """(address, row stride) of a [rows, width] matrix whose rows are contiguous and 16-byte aligned."""
+    shape, at = t.shape, t.data_ptr()
+    if len(shape) != 2 or shape[1] != width:
+        _fail(what, "%s must be [rows, %d], is %s" % (name, width, tuple(shape)))
     if t.dtype != dtype or t.device != device:
         _fail(what, "%s is %s on %s, expected %s on %s" % (name, t.dtype, t.device, dtype, device))
-    step = t.stride(0) if t.shape[0] > 1 else width
-    if (width > 1 and t.stride(1) != 1) or step < width or step * t.element_size() % 16 or t.data_ptr() % 16:
+    step, one = t.stride()
+    if shape[0] < 2:
+        step = width
+    if (one != 1 and width > 1) or step < width or step * _SIZE[dtype] % 16 or at % 16:
         _fail(what, "%s needs contiguous rows that start at 16-byte boundaries" % name)
-    return step
+    return at, step
 
 
 def _vector(what, name, t, n, device, dtype):
-    if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or t.device != device or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or t.dtype != dtype or t.device != device or (n > 1 and t.stride(0) != 1):
         _fail(what, "%s must be a contiguous %s vector of %d on %s" % (name, dtype, n, device))
     return t.data_ptr()
 
@@ -60,11 +65,12 @@ def _gpu(what, t):
 
 def _run(what, device, fn, *args):
     """Calls an entry point on the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc:
         L.check(rc, what)
 
@@ -89,18 +95,11 @@ def _span(what, q, k, v, lo, hi, heads, kv_heads, scale, cap, slopes, pos):
     m, n = q.shape[0], k.shape[0]
     if m >= 1 << 31 or n >= 1 << 31 or v.shape[0] != n:
         _fail(what, "k has %d rows, v %d" % (n, v.shape[0]))
-    a = L.SpanArgs()
-    a.dtype, a.M, a.N, a.heads, a.kv_heads, a.dh = _CODE[dt], m, n, heads, kv_heads, dh
-    a.ldq, a.q = _rows(what, "q", q, heads * dh, dev, dt), q.data_ptr()
-    a.ldk, a.k = _rows(what, "k", k, kv_heads * dh, dev, dt), k.data_ptr()
-    a.ldv, a.v = _rows(what, "v", v, kv_heads * dh, dev, dt), v.data_ptr()
-    a.lo = _vector(what, "lo", lo, m, dev, torch.int32)
-    a.hi = _vector(what, "hi", hi, m, dev, torch.int32)
-    if pos is not None:
-        a.pos = _vector(what, "pos", pos, m, dev, torch.int32)
-    if slopes is not None:
-        a.slopes = _vector(what, "slopes", slopes, heads, dev, torch.float32)
-    a.scale, a.cap = scale, cap
+    a = L.SpanArgs(_CODE[dt], m, n, heads, kv_heads, dh, *_rows(what, "q", q, heads * dh, dev, dt),
+                   *_rows(what, "k", k, kv_heads * dh, dev, dt), *_rows(what, "v", v, kv_heads * dh, dev, dt),
+                   _vector(what, "lo", lo, m, dev, torch.int32), _vector(what, "hi", hi, m, dev, torch.int32),
+                   None if pos is None else _vector(what, "pos", pos, m, dev, torch.int32),
+                   None if slopes is None else _vector(what, "slopes", slopes, heads, dev, torch.float32), scale, cap)
     return a, dev, dt
 
 
@@ -113,7 +112,8 @@ def attn_span(q, k, v, lo, hi, *, heads, kv_heads=None, scale=1.0, cap=0.0, slop
     a, dev, dt = _span("attn_span", q, k, v, lo, hi, heads, kv_heads, scale, cap, slopes, pos)
     out = _target("attn_span", "out", out, a.M, q.shape[1], dev, dt)
     lse = torch.empty(a.M, heads, device=dev, dtype=torch.float32)
-    a.ldo, a.out, a.lse = _rows("attn_span", "out", out, q.shape[1], dev, dt), out.data_ptr(), lse.data_ptr()
+    a.out, a.ldo = _rows("attn_span", "out", out, q.shape[1], dev, dt)
+    a.lse = lse.data_ptr()
     _run("attn_span", dev, lib.nmtgan_attn_span, C.byref(a))
     return out, lse
 
@@ -125,10 +125,10 @@ def attn_span_step(q, k, v, lo, hi, *, heads, max_keys, kv_heads=None, scale=1.0
     if not 0 <= max_keys < 1 << 31:
         _fail("attn_span_step", "max_keys=%r" % max_keys)
     out = _target("attn_span_step", "out", out, a.M, q.shape[1], dev, dt)
-    a.ldo, a.out = _rows("attn_span_step", "out", out, q.shape[1], dev, dt), out.data_ptr()
+    a.out, a.ldo = _rows("attn_span_step", "out", out, q.shape[1], dev, dt)
     n = lib.nmtgan_attn_span_step_workspace_bytes(a.M, heads, a.kv_heads, a.dh, max_keys)
-    ws = _scratch(n, dev)
-    _run("attn_span_step", dev, lib.nmtgan_attn_span_step, C.byref(a), max_keys, ws.data_ptr(), n)
+    ws = _scratch(n, dev) if n else None
+    _run("attn_span_step", dev, lib.nmtgan_attn_span_step, C.byref(a), max_keys, L.ptr(ws), n)
     return out
 
 
@@ -148,12 +148,10 @@ def attn_span_grads(dout, q, k, v, out, lse, lo, hi, *, heads, kv_heads=None, sc
     dq = _target(what, "dq", dq, a.M, wq, dev, dt)
     dk = _target(what, "dk", dk, a.N, wk, dev, dt)
     dv = _target(what, "dv", dv, a.N, wk, dev, dt)
-    a.ldo, a.out, a.lse = _rows(what, "out", out, wq, dev, dt), out.data_ptr(), lse.data_ptr()
-    g = L.SpanGrads()
-    g.ld_dout, g.dout = _rows(what, "dout", dout, wq, dev, dt), dout.data_ptr()
-    g.ld_dq, g.dq = _rows(what, "dq", dq, wq, dev, dt), dq.data_ptr()
-    g.ld_dk, g.dk = _rows(what, "dk", dk, wk, dev, dt), dk.data_ptr()
-    g.ld_dv, g.dv = _rows(what, "dv", dv, wk, dev, dt), dv.data_ptr()
+    a.out, a.ldo = _rows(what, "out", out, wq, dev, dt)
+    a.lse = lse.data_ptr()
+    g = L.SpanGrads(*_rows(what, "dout", dout, wq, dev, dt), *_rows(what, "dq", dq, wq, dev, dt),
+                    *_rows(what, "dk", dk, wk, dev, dt), *_rows(what, "dv", dv, wk, dev, dt))
     n = lib.nmtgan_attn_span_grads_workspace_bytes(a.M, heads)
     ws = _scratch(n, dev)
     _run(what, dev, lib.nmtgan_attn_span_grads, C.byref(a), C.byref(g), ws.data_ptr(), n)
@@ -169,11 +167,9 @@ def _xent(what, h, w, labels, smoothing):
         _fail(what, "smoothing must be in [0, 1), and 0 for a vocabulary of one")
     if h.shape[1] * h.element_size() % 16 or max(h.shape[0], w.shape[0], w.shape[1]) >= 1 << 31:
         _fail(what, "a row of h must be a multiple of 16 bytes")
-    a = L.XentArgs()
-    a.dtype, a.M, a.V, a.d = _CODE[dt], h.shape[0], w.shape[0], h.shape[1]
-    a.ldh, a.h = _rows(what, "h", h, a.d, dev, dt), h.data_ptr()
-    a.ldw, a.w = _rows(what, "w", w, a.d, dev, dt), w.data_ptr()
-    a.labels, a.smoothing = _vector(what, "labels", labels, a.M, dev, torch.int32), smoothing
+    m, v, d = h.shape[0], w.shape[0], h.shape[1]
+    a = L.XentArgs(_CODE[dt], m, v, d, *_rows(what, "h", h, d, dev, dt), *_rows(what, "w", w, d, dev, dt),
+                   _vector(what, "labels", labels, m, dev, torch.int32), smoothing)
     return a, dev, dt
 
 
@@ -196,12 +192,12 @@ def linear_xent_grads(h, w, labels, lse, grad_row=None, *, smoothing=0.0, dh=Non
         _fail(what, "bfloat16 or float32 (float16 gradients would underflow without loss scaling)")
     dh = _target(what, "dh", dh, a.M, a.d, dev, dt)
     dw = _target(what, "dw", dw, a.V, a.d, dev, dt)
-    ld_dh, ld_dw = _rows(what, "dh", dh, a.d, dev, dt), _rows(what, "dw", dw, a.d, dev, dt)
+    dh_at, dw_at = _rows(what, "dh", dh, a.d, dev, dt), _rows(what, "dw", dw, a.d, dev, dt)
     ls = _vector(what, "lse", lse, a.M, dev, torch.float32)
     g = None if grad_row is None else _vector(what, "grad_row", grad_row, a.M, dev, torch.float32)
     n = lib.nmtgan_linear_xent_workspace_bytes(C.byref(a), 1)
     ws = _scratch(n, dev)
-    _run(what, dev, lib.nmtgan_linear_xent_grads, C.byref(a), ls, g, dh.data_ptr(), ld_dh, dw.data_ptr(), ld_dw, ws.data_ptr(), n)
+    _run(what, dev, lib.nmtgan_linear_xent_grads, C.byref(a), ls, g, *dh_at, *dw_at, ws.data_ptr(), n)
     return dh, dw
 
 
