@@ -39,6 +39,8 @@ using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_p;
 
 constexpr int BKB = 128;                        // k-tile width in bytes
 constexpr int GROUP_M = 16;
@@ -74,9 +76,12 @@ struct GemmParams {
   const float* add; const int32_t* add_blk; int add_rows; int add_row0;
   // cross-entropy epilogues (xent.hip)
   XentEpilogue x;
+  // EPI_KPART (K-major operands, split_k slices of kt_slice k-tiles each): last k row and last 8-column chunk of A and W
+  int kt_slice, ka_last, kw_last, m_last, n_last;
 };
 constexpr int EPI_STATS = 100;                  // internal: never a value of nmtgan_gemm_args.epilogue
 constexpr int EPI_XSTAT = 102, EPI_XGRAD = 103; // internal: vocabulary cross entropy, forward and d(logits)
+constexpr int EPI_KPART = 104;                  // internal: fp32 partials of A[K][M]^T . W[K][N], both operands K-major
 constexpr int EPI_CONVADD = 101;                // internal: CONVMAX + additive term, chosen when nmtgan_gemm_args.add is set
 
 // acc[I0 + i][J0 + j] += A-fragment i x B-fragment j for one k-half of a k-tile (MT x NT 16x16 tiles).  Consecutive
@@ -184,40 +189,76 @@ __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)
   }
 }
 
-// XGRAD: d(logit) = g (exp(z - lse) - low - high [entry == label]) in the operand type, entry-major (gt, K = rows of the
-// weight gradient's product) and row-major (g, K = entries of the hidden gradient's); entries and rows that pad either
-// K to whole k-tiles are written as zeros
+// XGRAD: acc <- the part of d(logit) that differs from entry to entry, coef (exp(z - lse) - high [entry == label]), zero
+// where no row or entry is (the images are padded to whole k-tiles) - the constant -coef low is added in fp32 to the sums it
+// ends up in, where its rounding to 16 bits would add up.
+template <int MT>
+__device__ __forceinline__ void xgrad_values(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int lane, const float (&coef)[4],
+                                             const float (&lse2)[4], const int (&label)[4]) {
+  const int fq = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[i][j][e] = coef[j] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[j]));
+    if (__any(coef[j] == 0.f)) {                   // rows without a label: 0 whatever their logits are
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = coef[j] == 0.f ? 0.f : acc[i][j][e];
+    }
+    const int at = label[j] - m0;                  // few wave tiles hold the label of one of their columns
+    if (__any(at >= 0 && at < 16 * MT)) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at == 16 * i + 4 * fq + e) acc[i][j][e] -= coef[j] * p.x.high;
+    }
+  }
+  if (m0 + 16 * MT > p.M) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (m0 + 16 * i + 4 * fq + e >= p.M) acc[i][j][e] = 0.f;
+  }
+}
+// ... and its images: entry-major gt (rows contiguous) and, if asked for, row-major g
 template <typename OpT, int MT>
 __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
   const int fc = lane & 15, fq = lane >> 4;
   const XentEpilogue& x = p.x;
+  float coef[4], lse2[4];
+  int label[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = min(n0 + j * 16 + fc, x.rows_padded - 1);
+    coef[j] = x.coef[row];
+    lse2[j] = x.lse2[row];
+    label[j] = x.label[row] - x.first;
+  }
+  xgrad_values<MT>(p, acc, m0, lane, coef, lse2, label);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int row = n0 + j * 16 + fc;
     if (row >= x.rows_padded) continue;
-    float gr = 0.f, ls = 0.f;
-    int label = -1;
-    if (row < p.N) {
-      label = x.labels[row];
-      if (label < 0 || label >= x.vocab) label = -1;
-      gr = label < 0 ? 0.f : (x.grad_row ? x.grad_row[row] : 1.f);
-      ls = x.lse[row];
-      label -= x.first;                            // entry inside this piece of the vocabulary
-    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int mb = m0 + i * 16 + 4 * fq;
       if (mb >= x.piece_padded) continue;
-      OpT* out = reinterpret_cast<OpT*>(x.g) + (int64_t)row * x.piece_padded + mb;
       OpT* outt = reinterpret_cast<OpT*>(x.gt) + (int64_t)mb * x.rows_padded + row;
       float d[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float pe = __builtin_amdgcn_exp2f((acc[i][j][e] - ls) * 1.44269504088896341f) - x.low;
-        d[e] = gr == 0.f || mb + e >= p.M ? 0.f : gr * (mb + e == label ? pe - x.high : pe);
-        if (mb + e < p.M) OpTraits<OpT>::store(outt + (int64_t)e * x.rows_padded, d[e]);
+        d[e] = acc[i][j][e];
+        OpTraits<OpT>::store(outt + (int64_t)e * x.rows_padded, d[e]);
       }
-      if (row < p.N) VecIO<OpT, 4>::store(out, d);
+      if (x.g && row < p.N) VecIO<OpT, 4>::store(reinterpret_cast<OpT*>(x.g) + (int64_t)row * x.piece_padded + mb, d);
     }
   }
 }
@@ -699,7 +740,7 @@ static int launch_pipe(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = (p.M + PBM - 1) / PBM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + PBM - 1) / PBM;
   p.ntn = (p.N + PBN - 1) / PBN;
   p.group_m = 2;                                 // tile order knob (L2 sharing of A panels vs Wt tiles); 1-4 measured best
   if (const char* e = getenv("NMTGAN_GEMM_GM")) p.group_m = atoi(e);
@@ -935,19 +976,29 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave >> 2, wc = wave & 3;
-  const int nwg = p.ntm * p.ntn;
+  // KM (EPI_KPART): both operands are K-major, A[K][M] and W[K][N].  A staging unit then holds 64 k rows of its 128 columns
+  // (256 bytes each), a fragment is two ds_read_b64_tr_b16 (4 k x 16 columns turned per 16 lanes), and column pair P of 16
+  // sits at P ^ ((k & 3) | (k >> 1 & 4)): the 16 rows one read touches spread over all banks.
+  constexpr bool KM = EPI == EPI_KPART;
+  const int nwg = p.ntm * p.ntn * (KM ? p.split_k : 1);
   const int G = gridDim.x;
-  const int nkt = p.kbytes / BKB;                // >= 4 (launch guarantees it)
+  const int nkt = KM ? p.kt_slice : p.kbytes / BKB;      // >= 4 (launch guarantees it)
   const int my_tiles = (nwg - (int)blockIdx.x + G - 1) / G;
 
   auto tile_of = [&](int L, int& tm, int& tn) {
     const int xcd = L & 7, q = nwg >> 3, r = nwg & 7;
-    const int idx = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (L >> 3);
+    int idx = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (L >> 3);
+    int slice = 0;
+    if constexpr (KM) {
+      slice = idx / (p.ntm * p.ntn);
+      idx -= slice * (p.ntm * p.ntn);
+    }
     const int group_size = p.group_m * p.ntn;
     const int first_m = (idx / group_size) * p.group_m;
     const int gsz = min(p.ntm - first_m, p.group_m);
     tm = first_m + (idx % group_size) % gsz;
     tn = (idx % group_size) / gsz;
+    return slice;
   };
   const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_ptr_t)smem);
 
@@ -957,12 +1008,22 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   using U2 = std::integral_constant<int, 2>;
   using U3 = std::integral_constant<int, 3>;
   const char* src[4][2];
+  int krow[4][2];                                // KM: k row of the lane's chunk ...
+  unsigned kcol[4];                              // ... and its byte offset inside the row
   int kin[4];                                    // position of unit u inside its run of k_inner k-tiles
   auto point = [&](auto U, int ord) {            // unit U's sources at k-tile 0 of the block's tile `ord`
     constexpr int u = decltype(U)::value;
     kin[u] = 0;
     int tm, tn;
-    tile_of((int)blockIdx.x + ord * G, tm, tn);
+    const int slice = tile_of((int)blockIdx.x + ord * G, tm, tn);
+    if constexpr (KM) {
+      const int pair = ((lane & 15) >> 1) ^ ((lane >> 4) | ((wave & 2) << 1)), col = 16 * pair + 8 * (lane & 1);
+      kcol[u] = 2u * (unsigned)(u < 2 ? min(tm * QBM + (col >> 6) * 128 + u * 64 + (col & 63), p.m_last)
+                                      : min(tn * QBN + (col >> 5) * 64 + (u - 2) * 32 + (col & 31), p.n_last));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) krow[u][j] = slice * nkt * 64 + 4 * (wave + 8 * j) + (lane >> 4);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int rho = 8 * (wave + 8 * j) + (lane >> 3);
@@ -979,6 +1040,17 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   auto issue = [&](auto U, int parity) {         // next k-tile of unit U into the stage of that parity
     constexpr int u = decltype(U)::value;
     const unsigned dst = lds_base + parity * QSTAGE + u * QUNIT + wave * 1024;
+    if constexpr (KM) {
+      const char* base = u < 2 ? p.A : p.W;
+      const unsigned ld = (unsigned)(u < 2 ? p.lda_b : p.ldw_b);
+      const int last = u < 2 ? p.ka_last : p.kw_last;    // rows the operand has; those behind meet zeros of the other
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        glds16_s((unsigned)min(krow[u][j], last) * ld + kcol[u], base, dst + j * 8 * 1024);
+        krow[u][j] += 64;
+      }
+      return;
+    }
     glds16_m0(src[u][0], dst);
     glds16_m0(src[u][1], dst + 8 * 1024);
     kin[u] += 1;
@@ -1006,19 +1078,24 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   // per-column epilogue values of the wave's 64 columns, LDS-DMA'd at the start of the tile's last k-step:
   // they ride the same in-order vmcnt stream as the tile DMAs and the epilogue needs no vector load (which
   // the compiler would wait vmcnt(0) for, draining the prefetch of the next tile)
-  constexpr int QEV = 2 * QSTAGE + 8 * 2048;
-  const float* ev = reinterpret_cast<const float*>(smem + QEV + wave * 512);
+  constexpr int QEV = 2 * QSTAGE + 8 * 2048, QEVW = EPI == EPI_XGRAD ? 1024 : 512;
+  const float* ev = reinterpret_cast<const float*>(smem + QEV + wave * QEVW);
   const bool use_ev = (EPI == NMTGAN_EPI_LINEAR && p.bias != nullptr) || EPI == NMTGAN_EPI_CONVMAX;
   auto stage_ev = [&](int ord) {
     int tm, tn;
     tile_of((int)blockIdx.x + ord * G, tm, tn);
     const int n = min(tn * QBN + wc * 64 + lane, p.N - 1);
-    const unsigned dst = lds_base + QEV + wave * 512;
+    const unsigned dst = lds_base + QEV + wave * QEVW;
     if constexpr (EPI == NMTGAN_EPI_LINEAR) {
       if (p.bias) glds4(p.bias + n, dst);
     } else if constexpr (EPI == NMTGAN_EPI_CONVMAX) {
       glds4(p.scale + n, dst);
       glds4(p.shift + n, dst + 256);
+    } else if constexpr (EPI == EPI_XGRAD) {
+      const int r = min(tn * QBN + wc * 64 + lane, p.x.rows_padded - 1);
+      glds4(p.x.coef + r, dst);
+      glds4(p.x.lse2 + r, dst + 256);
+      glds4(p.x.label + r, dst + 512);
     }
   };
 
@@ -1032,7 +1109,22 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     asm volatile("" ::: "memory");         \
     __builtin_amdgcn_sched_barrier(0);     \
   } while (0)
+  const int kf = ((lane & 15) >> 2) | ((fq & 1) << 2);
+  const int k_rd = (8 * fq + ((lane & 15) >> 2)) * 256 + (lane & 3) * 8;
+  auto turned = [&](const unsigned char* unit, int kh, int pair) -> uint4 {
+    const unsigned char* q = unit + kh * 32 * 256 + k_rd + ((pair ^ kf) << 5);
+    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_p)q));
+    const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_p)(q + 4 * 256)));
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
   auto read_a = [&](const unsigned char* base, int h) {
+    if constexpr (KM) {
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fa[kh][i] = turned(base + h * QUNIT, kh, wr * 4 + i);
+      return;
+    }
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
@@ -1040,6 +1132,13 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
         fa[kh][i] = *reinterpret_cast<const uint4*>(base + h * QUNIT + a_rd + i * 16 * BKB + pc[kh]);
   };
   auto read_b = [&](const unsigned char* base, int h, uint4 (&fb)[2][2]) {
+    if constexpr (KM) {
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) fb[kh][j] = turned(base + (2 + h) * QUNIT, kh, wc * 2 + j);
+      return;
+    }
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
@@ -1127,12 +1226,34 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     kstep(M1{}, has_next);
     kstep(M2{}, has_next);
     int tm, tn;
-    tile_of((int)blockIdx.x + t * G, tm, tn);
+    const int slice = tile_of((int)blockIdx.x + t * G, tm, tn);
     const int m0 = tm * QBM + wr * 128, n0 = tn * QBN + wc * 64;
     bool wide = false;
     if constexpr (EPI == NMTGAN_EPI_LINEAR) wide = p.wide_ok && n0 < p.N;
     if constexpr (EPI == EPI_STATS) {
       epilogue_stats<8>(p, acc, m0, n0, lane);
+    } else if constexpr (EPI == EPI_XGRAD) {
+      float coef[4], lse2[4];
+      int label[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        coef[j] = ev[j * 16 + fc];
+        lse2[j] = ev[64 + j * 16 + fc];
+        label[j] = __float_as_int(ev[128 + j * 16 + fc]) - p.x.first;
+      }
+      xgrad_values<8>(p, acc, m0, lane, coef, lse2, label);
+      if (n0 < p.x.rows_padded) {
+        GemmParams v{};                            // whole 64-column rows of gt; rows_padded and piece_padded bound them
+        v.M = p.x.piece_padded; v.N = p.x.rows_padded; v.wide_ok = 2; v.n_seg = 1;
+        v.out[0] = p.x.gt; v.ldo[0] = p.x.rows_padded; v.seg_scale[0] = 1.f;
+        epilogue_wide<OpT, 8>(v, acc, m0, n0, lane, scr, sizeof(OpT) == 4, 0, n0);
+      }
+    } else if constexpr (KM) {
+      GemmParams v{};
+      v.M = p.M; v.N = p.N; v.n_seg = 1; v.out_f32[0] = 1; v.ldo[0] = p.N; v.seg_scale[0] = 1.f;
+      v.out[0] = p.split_part + (int64_t)slice * p.M * p.N;
+      if (p.wide_ok && n0 < p.N) epilogue_wide<OpT, 8>(v, acc, m0, n0, lane, scr, true, 0, n0);
+      else if (!p.wide_ok) epilogue<OpT, NMTGAN_EPI_LINEAR, 8>(v, acc, m0, n0, lane);
     } else if (wide) {
       const int seg = (p.n_seg > 1) ? n0 / p.seg_width : 0;
       const int omode = pick3(p.out_f32, seg);
@@ -1154,7 +1275,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
 
 template <typename OpT, int EPI>
 static int launch_p8(GemmParams p, hipStream_t st) {
-  constexpr int smem = 2 * QSTAGE + 8 * 2048 + 8 * 512;   // 128 KiB of staging + per-wave epilogue scratch + vectors
+  constexpr int smem = 2 * QSTAGE + 8 * 2048 + 8 * (EPI == EPI_XGRAD ? 1024 : 512);   // 128 KiB of staging + per-wave epilogue scratch + vectors
   static bool attr_done = false;
   if (!attr_done) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_p8_kernel<OpT, EPI>),
@@ -1162,12 +1283,12 @@ static int launch_p8(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = (p.M + QBM - 1) / QBM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + QBM - 1) / QBM;
   p.ntn = (p.N + QBN - 1) / QBN;
   // tile groups of 2 row tiles (4 are as fast); the logits GEMM (rows = vocabulary) takes 8: an XCD then keeps 2 MiB
   // of the table in its L2 and sweeps the activations twice instead of eight times - same time, a third of the
   // fetches past the L2
-  p.group_m = EPI == EPI_STATS ? 8 : 2;
+  p.group_m = EPI == EPI_STATS || EPI == EPI_XSTAT || EPI == EPI_XGRAD ? 8 : 2;
   if (const char* e = getenv("NMTGAN_GEMM_GM")) p.group_m = atoi(e);
   if constexpr (EPI == NMTGAN_EPI_LINEAR) {
     const int es = sizeof(OpT);
@@ -1179,7 +1300,8 @@ static int launch_p8(GemmParams p, hipStream_t st) {
     p.wide_ok = ok ? 2 : 0;
     if (const char* e = getenv("NMTGAN_GEMM_WIDE")) p.wide_ok = p.wide_ok ? atoi(e) : 0;
   }
-  const int nwg = p.ntm * p.ntn;
+  if constexpr (EPI == EPI_KPART) p.wide_ok = p.N % 64 == 0;
+  const int nwg = p.ntm * p.ntn * (EPI == EPI_KPART ? p.split_k : 1);
   const int grid = persistent_grid(nwg);
   hipLaunchKernelGGL((gemm_p8_kernel<OpT, EPI>), dim3(grid), dim3(512), smem, st, p);
   NMTGAN_CHECK_LAUNCH("gemm_p8");
@@ -1572,7 +1694,7 @@ static int launch_glds(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = (p.M + BM - 1) / BM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + BM - 1) / BM;
   p.ntn = (p.N + BN - 1) / BN;
   const int slices = (EPI == NMTGAN_EPI_LINEAR && p.split_k > 1) ? p.split_k : 1;
   if (slices == 1) p.split_k = 0;
@@ -1619,7 +1741,7 @@ static int launch_generic(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = (p.M + GBM - 1) / GBM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + GBM - 1) / GBM;
   p.ntn = (p.N + GBN - 1) / GBN;
   hipLaunchKernelGGL((gemm_kernel<OpT, EPI>), dim3(p.ntm * p.ntn), dim3(256), 4 * GTILE, st, p);
   NMTGAN_CHECK_LAUNCH("gemm");
@@ -1814,8 +1936,8 @@ bool gemm_stats_supported(int op_dtype, int V, int K) {
   return V % 64 == 0 && V <= 65536 && (K * es) % BKB == 0 && (K * es) / BKB >= 4;   // <= 1024 vocabulary tiles
 }
 
-// z^T = W[entries,K] . H[rows,K]^T with one of the cross-entropy epilogues; N of the product covers the padding rows of
-// the transposed gradient (rows_padded) through the last tile
+// z^T = W[entries,K] . H[rows,K]^T with one of the cross-entropy epilogues; the last tiles reach over the padding of the
+// gradient's images (both extents are at most a tile beyond the product's)
 int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
                      int K, float2* stats, const XentEpilogue& x, hipStream_t st) {
   const int es = dtype_size(op_dtype);
@@ -1831,9 +1953,30 @@ int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int en
   } else if (op_dtype == NMTGAN_BF16) {
     return dispatch<bf16_t, EPI_XGRAD>(p, st);
   } else {
-    return dispatch<float, EPI_XGRAD>(p, st);
+    // the fp32 form needs the row-major image too, which only the scalar epilogue writes
+    if (p.kbytes % BKB == 0) return launch_glds<float, EPI_XGRAD, 128, 128>(p, st);
+    return launch_generic<float, EPI_XGRAD>(p, st);
   }
   return 0;
+}
+
+// part[z][M][N] (fp32) = sum over k rows [64 z kt_slice, 64 (z + 1) kt_slice) of A[k][m] W[k][n], 16-bit operands; rows of A
+// from ka on and of W from kw on are not read, and one of the two holds zeros where the other ends.  lda, ldw in elements
+// (multiples of 8, at least M resp. N rounded up to 8); both matrices below 4 GiB.
+int launch_gemm_kmajor(int op_dtype, const void* A, int64_t lda, int ka, const void* W, int64_t ldw, int kw, int M, int N,
+                       int slices, int kt_slice, float* part, hipStream_t st) {
+  NMTGAN_REQUIRE(op_dtype == NMTGAN_BF16, "gemm_kmajor: bf16 operands");
+  NMTGAN_REQUIRE(A && W && part && M > 0 && N > 0 && ka > 0 && kw > 0 && slices > 0 && kt_slice >= 4 && lda % 8 == 0 && ldw % 8 == 0 &&
+                     lda >= (M + 7) / 8 * 8 && ldw >= (N + 7) / 8 * 8 && (int64_t)ka * lda < (1LL << 31) && (int64_t)kw * ldw < (1LL << 31),
+                 "gemm_kmajor: bad arguments");
+  GemmParams p{};
+  p.A = (const char*)A; p.W = (const char*)W;
+  p.M = M; p.N = N;
+  p.lda_b = lda * 2; p.ldw_b = ldw * 2;
+  p.split_k = slices; p.split_part = part; p.kt_slice = kt_slice;
+  p.ka_last = ka - 1; p.kw_last = kw - 1;
+  p.m_last = (M + 7) / 8 * 8 - 8; p.n_last = (N + 7) / 8 * 8 - 8;
+  return launch_p8<bf16_t, EPI_KPART>(p, st);
 }
 
 static int launch_gemm_impl(const nmtgan_gemm_args* a, hipStream_t st);

@@ -6,16 +6,19 @@
 namespace nmtgan {
 
 // operands of the cross-entropy epilogues of the GEMM (xent.hip); `first` .. first + entries is the piece of the
-// vocabulary the product covers, the gradient images are padded to whole k-tiles (64 entries / 64 rows)
+// vocabulary the product covers, the images of d(logits) are padded with zeros to whole k-tiles
 struct XentEpilogue {
-  const int32_t* labels; const float* grad_row; const float* lse;
   float* zsum;                                   // forward, label smoothing only
-  void* g; void* gt;                             // [rows][piece_padded], [entries][rows_padded]
-  int vocab, first, piece_padded, rows_padded;
-  float low, high;
+  // per hidden row, [rows_padded]: gradient of its loss (0 without a label), lse / ln 2, label (-1 without)
+  const float* coef; const float* lse2; const int32_t* label;
+  void* g; void* gt;                             // [rows][piece_padded] (may be null), [piece_padded][rows_padded]
+  int first, piece_padded, rows_padded;
+  float high;
 };
 int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
                      int K, float2* stats, const XentEpilogue& x, hipStream_t st);
+int launch_gemm_kmajor(int op_dtype, const void* A, int64_t lda, int ka, const void* W, int64_t ldw, int kw, int M, int N,
+                       int slices, int kt_slice, float* part, hipStream_t st);
 int launch_gemm(const nmtgan_gemm_args* a, hipStream_t st);
 // n independent problems of one epilogue kind (CONVMAX - with or without the additive term - or LINEAR with one fp32 or
 // op-dtype output) in one persistent launch per 24 problems; min_tiles > 0 leaves problems of at least that many 256x128 tiles to

@@ -8,9 +8,10 @@
 // Forward: one product on the matrix cores whose epilogue leaves (max, sum exp) per 64 entries and row (gemm.hip), joined
 // in tile order by xent_finish_kernel, which also forms the label's own logit from the operands.
 // Gradient, per piece of the vocabulary: the product again (2 M V d operations are cheaper at d <= 1024 than 8 bytes of
-// fp32 logit written and read), its epilogue writes dz in the operand type; two products with that image give the piece's
-// rows of dw and a partial of dh.  dz is rounded once to the operand type - the matrix cores take no more - like every
-// activation gradient of this library; lse, loss and all sums are fp32.
+// fp32 logit written and read), its epilogue writes dz in the operand type, entry-major; two products with that image give
+// the piece's rows of dw (K = rows) and partials of dh (K = entries, both operands turned on their way out of LDS).  dz is
+// rounded once to the operand type - the matrix cores take no more - like every activation gradient of this library; lse,
+// loss and all sums are fp32.
 #include <math.h>
 
 #include <algorithm>
@@ -107,14 +108,84 @@ __global__ __launch_bounds__(256) void xent_transpose_kernel(const T* in, int64_
   }
 }
 
-// dh = sum of the partials in order, rounded once
+// per-row operands of the d(logits) epilogue, padded: coef = gradient of the row's loss (0 without a label), lse / ln 2, label
+__global__ __launch_bounds__(256) void xent_rows_kernel(const int32_t* labels, const float* grad_row, const float* lse, int M,
+                                                        int Mp, int V, float* coef, float* lse2, int32_t* label) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= Mp) return;
+  const bool used = r < M && labels[r] >= 0 && labels[r] < V;
+  coef[r] = used ? (grad_row ? grad_row[r] : 1.f) : 0.f;
+  lse2[r] = r < M ? lse[r] * 1.44269504088896341f : 0.f;
+  label[r] = used ? labels[r] : -1;
+}
+
+// Column sums behind label smoothing, whose constant -coef_r low of every d(logit) is kept out of the 16-bit images:
+// dh_r -= coef_r low sum_j w_j, dw_j -= low sum_r coef_r h_r.  part[block][d] = sums over a block's rows (weighted if coef
+// is given), added in block order by xent_colsum_finish_kernel.
+constexpr int COLSUM_BLOCKS = 256;
 template <typename T>
-__global__ __launch_bounds__(256) void xent_dh_kernel(const float* part, int n_part, int M, int d, T* dh, int64_t ld) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)M * d;
-  if (i >= n) return;
+__global__ __launch_bounds__(256) void xent_colsum_kernel(const T* x, int64_t ld, int R, int C, const float* coef, float* part) {
+  __shared__ float red[4][64];
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int r0 = (int)((int64_t)R * blockIdx.x / COLSUM_BLOCKS), r1 = (int)((int64_t)R * (blockIdx.x + 1) / COLSUM_BLOCKS);
+  for (int c0 = 0; c0 < C; c0 += 512) {            // 64 lanes x 8 columns, four rows at a time
+    const int c = c0 + 8 * tx;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < C)
+      for (int r = r0 + ty; r < r1; r += 4) {
+        const float f = coef ? coef[r] : 1.f;
+        if (f == 0.f) continue;
+#pragma unroll
+        for (int h = 0; h < 8; h += 16 / (int)sizeof(T)) {
+          if (c + h >= C) break;
+          float v[16 / (int)sizeof(T)];
+          VecIO<T, 16 / (int)sizeof(T)>::load(x + (int64_t)r * ld + c + h, v);
+#pragma unroll
+          for (int e = 0; e < 16 / (int)sizeof(T); ++e) s[h + e] = fmaf(f, v[e], s[h + e]);
+        }
+      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      __syncthreads();
+      red[ty][tx] = s[e];
+      __syncthreads();
+      if (ty == 0 && c + e < C) part[(int64_t)blockIdx.x * C + c + e] = (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
+    }
+  }
+}
+__global__ __launch_bounds__(256) void xent_colsum_finish_kernel(const float* part, int C, float f, float* out) {
+  __shared__ float red[4][64];
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, c = blockIdx.x * 64 + tx;
   float s = 0.f;
-  for (int k = 0; k < n_part; ++k) s += part[k * n + i];
-  OpTraits<T>::store(dh + (i / d) * ld + i % d, s);
+  if (c < C)
+    for (int k = ty; k < COLSUM_BLOCKS; k += 4) s += part[(int64_t)k * C + c];
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < C) out[c] = f * ((red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]));
+}
+
+// dh = sum of the partials in order (+ the smoothing constant's part), rounded once
+template <typename T>
+__global__ __launch_bounds__(256) void xent_dh_kernel(const float* part, int n_part, int M, int d, const float* coef,
+                                                      const float* wsum, T* dh, int64_t ld) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = (int64_t)M * d;      // d % 4 == 0
+  if (i >= n) return;
+  const int64_t r = i / d;
+  const int c = (int)(i % d);
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < n_part; ++k) {
+    float v[4];
+    VecIO<float, 4>::load(part + k * n + i, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += v[e];
+  }
+  const float f = coef[r];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (wsum) s[e] = fmaf(f, wsum[c + e], s[e]);
+    if (f == 0.f) s[e] = 0.f;
+  }
+  VecIO<T, 4>::store(dh + r * ld + c, s);
 }
 
 template <typename T>
@@ -142,28 +213,46 @@ static int check_xent(const nmtgan_xent_args* a, const char* what) {
 static int pad64(int n) { return (n + 63) / 64 * 64; }
 
 struct XentPlan {
-  int rows_padded, piece, piece_padded, n_pieces, slices;      // slices of a piece's entries in the dh product
+  int rows_padded, piece, n_pieces, slices, kt_slice;        // a piece = slices of kt_slice k-tiles of 64 entries
   size_t bytes;
-  void *g, *gt, *wt, *ht; float* part;
+  float *coef, *lse2, *part, *colsum, *wsum, *hsum;
+  int32_t* label;
+  void *g, *gt, *wt, *ht;
 };
+// Pieces of the vocabulary: as few as keep a piece's d(logits) inside the 256 MB memory-side cache (the two products read
+// what the epilogue wrote).  Inside a piece the hidden gradient's product is cut along the entries into enough slices to
+// give every CU a tile.
 static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPlan& q) {
   const int es = dtype_size(a->dtype);
+  const bool f32 = a->dtype == NMTGAN_F32;
   q.rows_padded = pad64(a->M);
-  // both images of dz of a piece stay inside the 256 MB memory-side cache
-  const int64_t fit = (192LL << 20) / (2LL * es * q.rows_padded);
+  const int64_t fit = (224LL << 20) / ((f32 ? 2LL : 1LL) * es * q.rows_padded);
   int64_t n = (a->V + fit - 1) / std::max<int64_t>(fit, 1);
   n = std::max<int64_t>(1, std::min<int64_t>(n, (a->V + 1023) / 1024));
-  q.piece = pad64((int)((a->V + n - 1) / n));
+  const int64_t want = (a->V + n - 1) / n, kt = std::max<int64_t>(4, (want + 63) / 64);
+  const int64_t tiles = (int64_t)((a->M + 255) / 256) * (f32 ? (a->d + 127) / 128 : (a->d + 255) / 256);
+  q.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
+  q.kt_slice = (int)((kt + q.slices - 1) / q.slices);
+  q.piece = q.slices * q.kt_slice * 64;
   q.n_pieces = (a->V + q.piece - 1) / q.piece;
-  q.piece_padded = q.piece;
-  const int64_t tiles = (int64_t)((a->M + 255) / 256) * ((a->d + 127) / 128);
-  q.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), q.piece / 512));
   Arena ar(base, cap);
-  q.g = ar.take((size_t)a->M * q.piece_padded * es);
-  q.gt = ar.take((size_t)q.piece_padded * q.rows_padded * es);
-  q.wt = ar.take((size_t)a->d * q.piece_padded * es);
+  q.coef = ar.get<float>(q.rows_padded);
+  q.lse2 = ar.get<float>(q.rows_padded);
+  q.label = ar.get<int32_t>(q.rows_padded);
+  q.gt = ar.take((size_t)q.piece * q.rows_padded * es);
   q.ht = ar.take((size_t)a->d * q.rows_padded * es);
   q.part = ar.get<float>((size_t)q.n_pieces * q.slices * a->M * a->d);
+  q.colsum = q.wsum = q.hsum = nullptr;
+  if (a->smoothing > 0.f) {
+    q.colsum = ar.get<float>((size_t)COLSUM_BLOCKS * a->d);
+    q.wsum = ar.get<float>(a->d);
+    q.hsum = ar.get<float>(a->d);
+  }
+  q.g = q.wt = nullptr;
+  if (f32) {
+    q.g = ar.take((size_t)a->M * q.piece * es);
+    q.wt = ar.take((size_t)a->d * q.piece * es);
+  }
   q.bytes = ar.off;
 }
 size_t linear_xent_workspace(const nmtgan_xent_args* a, bool grads) {
@@ -188,7 +277,6 @@ int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void*
   const int tiles = (a->V + 63) / 64;
   float2* stats = (float2*)ws;
   XentEpilogue x{};
-  x.vocab = a->V;
   if (a->smoothing > 0.f) x.zsum = (float*)((char*)ws + align_up((size_t)tiles * a->M * sizeof(float2), 256));
   NMTGAN_TRY(launch_gemm_xent(a->dtype, false, a->w, a->ldw, a->V, a->h, a->ldh, a->M, a->d, stats, x, st));
   const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f, high = 1.f - a->smoothing - low;
@@ -203,7 +291,7 @@ int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void*
 template <typename T>
 static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh, void* dw,
                         int64_t ld_dw, void* ws, size_t ws_bytes, hipStream_t st) {
-  const int es = sizeof(T);
+  constexpr int es = sizeof(T);
   if (a->M == 0) {
     hipLaunchKernelGGL(xent_zero_rows_kernel<T>, dim3((unsigned)(((int64_t)a->V * a->d + 255) / 256)), dim3(256), 0, st, (T*)dw,
                        ld_dw, a->V, a->d);
@@ -212,50 +300,69 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
   }
   XentPlan q;
   carve_xent(a, (char*)ws, ws_bytes, q);
+  const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f;
+  hipLaunchKernelGGL(xent_rows_kernel, dim3((q.rows_padded + 255) / 256), dim3(256), 0, st, a->labels, grad_row, lse, a->M,
+                     q.rows_padded, a->V, q.coef, q.lse2, q.label);
+  NMTGAN_CHECK_LAUNCH("linear_xent_rows");
   hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3(q.rows_padded / 64, (a->d + 63) / 64), dim3(256), 0, st, (const T*)a->h,
                      a->ldh, a->M, a->d, (T*)q.ht, q.rows_padded, a->labels, a->V);
   NMTGAN_CHECK_LAUNCH("linear_xent_transpose");
+  if (low > 0.f) {
+    hipLaunchKernelGGL(xent_colsum_kernel<T>, dim3(COLSUM_BLOCKS), dim3(256), 0, st, (const T*)a->w, a->ldw, a->V, a->d,
+                       (const float*)nullptr, q.colsum);
+    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
+    hipLaunchKernelGGL(xent_colsum_finish_kernel, dim3((a->d + 63) / 64), dim3(256), 0, st, q.colsum, a->d, -low, q.wsum);
+    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
+    hipLaunchKernelGGL(xent_colsum_kernel<T>, dim3(COLSUM_BLOCKS), dim3(256), 0, st, (const T*)a->h, a->ldh, a->M, a->d, q.coef,
+                       q.colsum);
+    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
+    hipLaunchKernelGGL(xent_colsum_finish_kernel, dim3((a->d + 63) / 64), dim3(256), 0, st, q.colsum, a->d, -low, q.hsum);
+    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
+  }
   XentEpilogue x{};
-  x.labels = a->labels; x.grad_row = grad_row; x.lse = lse; x.g = q.g; x.gt = q.gt; x.vocab = a->V;
+  x.coef = q.coef; x.lse2 = q.lse2; x.label = q.label; x.g = q.g; x.gt = q.gt;
   x.rows_padded = q.rows_padded;
-  x.low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f;
-  x.high = 1.f - a->smoothing - x.low;
+  x.piece_padded = q.piece;
+  x.high = 1.f - a->smoothing - low;
   int n_part = 0;
   for (int v0 = 0; v0 < a->V; v0 += q.piece) {
-    const int n = std::min(q.piece, a->V - v0), np = pad64(n);
+    const int n = std::min(q.piece, a->V - v0);
     x.first = v0;
-    x.piece_padded = np;
     const T* w = (const T*)a->w + (int64_t)v0 * a->ldw;
     NMTGAN_TRY(launch_gemm_xent(a->dtype, true, w, a->ldw, n, a->h, a->ldh, a->M, a->d, nullptr, x, st));
-    hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3(np / 64, (a->d + 63) / 64), dim3(256), 0, st, w, a->ldw, n, a->d, (T*)q.wt,
-                       np, (const int32_t*)nullptr, 0);
-    NMTGAN_CHECK_LAUNCH("linear_xent_transpose");
-    // dh partials: slices of the piece's entries, whole k-tiles each
-    nmtgan_gemm_args g[24];
-    int ng = 0;
-    for (int s = 0; s < q.slices; ++s) {
-      const int k0 = (int)((int64_t)(np / 64) * s / q.slices) * 64, k1 = (int)((int64_t)(np / 64) * (s + 1) / q.slices) * 64;
-      if (k1 == k0) continue;
-      nmtgan_gemm_args& b = g[ng++];
-      b = nmtgan_gemm_args{};
-      b.op_dtype = a->dtype;
-      b.epilogue = NMTGAN_EPI_LINEAR;
-      b.A = (const T*)q.g + k0; b.lda = np;
-      b.Wt = (const T*)q.wt + k0; b.ldw = np;
-      b.M = a->M; b.N = a->d; b.K = k1 - k0;
-      b.n_seg = 1; b.out[0] = q.part + (int64_t)n_part++ * a->M * a->d; b.ldo[0] = a->d; b.out_f32[0] = 1; b.seg_scale[0] = 1.f;
+    float* part = q.part + (int64_t)n_part * a->M * a->d;
+    if constexpr (es == 2) {
+      NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.gt, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice, part,
+                                    st));
+      n_part += q.slices;
+    } else {
+      hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3(q.piece / 64, (a->d + 63) / 64), dim3(256), 0, st, w, a->ldw, n, a->d,
+                         (T*)q.wt, q.piece, (const int32_t*)nullptr, 0);
+      NMTGAN_CHECK_LAUNCH("linear_xent_transpose");
+      nmtgan_gemm_args g[24];
+      for (int s = 0; s < q.slices; ++s) {
+        nmtgan_gemm_args& b = g[s];
+        b = nmtgan_gemm_args{};
+        b.op_dtype = a->dtype;
+        b.epilogue = NMTGAN_EPI_LINEAR;
+        b.A = (const T*)q.g + s * q.kt_slice * 64; b.lda = q.piece;
+        b.Wt = (const T*)q.wt + s * q.kt_slice * 64; b.ldw = q.piece;
+        b.M = a->M; b.N = a->d; b.K = q.kt_slice * 64;
+        b.n_seg = 1; b.out[0] = part + (int64_t)s * a->M * a->d; b.ldo[0] = a->d; b.out_f32[0] = 1; b.seg_scale[0] = 1.f;
+      }
+      NMTGAN_TRY(launch_gemm_group(g, q.slices, st));
+      n_part += q.slices;
     }
-    NMTGAN_TRY(launch_gemm_group(g, ng, st));
     nmtgan_gemm_args b{};
     b.op_dtype = a->dtype;
     b.epilogue = NMTGAN_EPI_LINEAR;
-    b.A = q.gt; b.lda = q.rows_padded; b.Wt = q.ht;
+    b.A = q.gt; b.lda = q.rows_padded; b.Wt = q.ht; b.bias = q.hsum;
     b.M = n; b.N = a->d; b.K = q.rows_padded;
     b.n_seg = 1; b.out[0] = (T*)dw + (int64_t)v0 * ld_dw; b.ldo[0] = ld_dw; b.out_f32[0] = es == 4; b.seg_scale[0] = 1.f;
     NMTGAN_TRY(launch_gemm(&b, st));
   }
-  hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d + 255) / 256)), dim3(256), 0, st, q.part, n_part,
-                     a->M, a->d, (T*)dh, ld_dh);
+  hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, n_part,
+                     a->M, a->d, q.coef, q.wsum, (T*)dh, ld_dh);
   NMTGAN_CHECK_LAUNCH("linear_xent_dh");
   return 0;
 }
