@@ -23,27 +23,41 @@ __global__ __launch_bounds__(256) void span_prep_kernel(SpanParams p) {
       hl.w = min(hl.w, __shfl_xor(hl.w, o, 64));
     }
     if ((lane & 31) == 0 && i < p.M) p.hull[2 * b + (lane >> 5)] = hl;
+    if (b * 64 + (lane & 32) < p.M) {                        // the block of 32 exists: its record is whole
+      int* s = p.spans + (int64_t)(2 * b + (lane >> 5)) * 64 + (lane & 31);
+      s[0] = sp.x;
+      s[32] = sp.y;
+      if (p.slopes) p.posr[(int64_t)(2 * b + (lane >> 5)) * 64 + (lane & 31)] = i < p.M ? pos_of(p, i) : 0;
+    }
   }
-  const int n = min(64, p.M - b * 64) * p.heads, c8 = p.dh / 8;
-  for (int t = threadIdx.x >> 3; t < n; t += 32) {
-    const int64_t i = b * 64 + t / p.heads;
-    const int h = t % p.heads;
-    const T* o = (const T*)p.out + i * p.ldo + h * p.dh;
-    const T* d = (const T*)p.dout + i * p.ld_do + h * p.dh;
-    float s = 0.f;
-    for (int c = threadIdx.x & 7; c < c8; c += 8) {
-      float x[8], y[8];
-      VecIO<T, 8>::load(o + 8 * c, x);
-      VecIO<T, 8>::load(d + 8 * c, y);
+  const int rows = min(64, (p.M - b * 64 + 31) / 32 * 32), c8 = p.dh / 8;
+  for (int t = threadIdx.x >> 3; t < rows * p.heads; t += 32) {
+    const int i = b * 64 + t / p.heads, h = t % p.heads;
+    float s = 0.f, ls = 0.f;
+    if (i < p.M) {
+      const T* o = (const T*)p.out + (int64_t)i * p.ldo + h * p.dh;
+      const T* d = (const T*)p.dout + (int64_t)i * p.ld_do + h * p.dh;
+      for (int c = threadIdx.x & 7; c < c8; c += 8) {
+        float x[8], y[8];
+        VecIO<T, 8>::load(o + 8 * c, x);
+        VecIO<T, 8>::load(d + 8 * c, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+      }
     }
     s = dpp_add<0xB1>(s);
     s = dpp_add<0x4E>(s);
     s = dpp_add<0x141>(s);
     if ((threadIdx.x & 7) == 0) {
-      const int2 sp = span_of(p, (int)i);
-      p.delta[i * p.heads + h] = sp.y > sp.x ? s : 0.f;
+      float* at = delta_at(p, i, h);
+      bool some = false;
+      if (i < p.M) {
+        const int2 sp = span_of(p, i);
+        some = sp.y > sp.x;
+        ls = p.lse[(int64_t)i * p.heads + h];
+      }
+      at[-32] = ls == -INFINITY ? 0.f : ls * LOG2E;
+      at[0] = some ? s : 0.f;
     }
   }
 }
@@ -263,6 +277,7 @@ static int fill_span(const nmtgan_span_args* a, SpanParams& p, const char* what)
                  what, a->dh, SPAN_MAX_DH);
   NMTGAN_REQUIRE(isfinite(a->scale) && isfinite(a->cap) && a->cap >= 0.f, "%s: scale and cap must be finite, cap >= 0", what);
   const int es = dtype_size(a->dtype);
+  NMTGAN_REQUIRE(a->ldq < (1 << 24) && a->ldk < (1 << 24) && a->ldv < (1 << 24), "%s: rows further than 2^24 elements apart", what);
   if (a->M > 0) {
     NMTGAN_REQUIRE(a->q && a->lo && a->hi && a->out, "%s: null pointer", what);
     NMTGAN_REQUIRE(rows_ok(a->q, a->ldq, (int64_t)a->heads * a->dh, es) && rows_ok(a->out, a->ldo, (int64_t)a->heads * a->dh, es),
@@ -345,14 +360,18 @@ int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, siz
   return 0;
 }
 
-static size_t carve_span_grads(int M, int heads, char* base, float** delta, int4** hull) {
-  const size_t a = align_up((size_t)M * heads * sizeof(float), 256);
-  if (base) { *delta = (float*)base; *hull = (int4*)(base + a); }
-  return a + align_up((size_t)((M + 31) / 32) * sizeof(int4), 256);
+static size_t carve_span_grads(int M, int heads, char* base, SpanParams* p) {
+  const size_t nb = ((size_t)M + 31) / 32;
+  const size_t a = align_up(nb * heads * 64 * sizeof(float), 256), b = align_up(nb * sizeof(int4), 256), c = align_up(nb * 64 * sizeof(int), 256);
+  if (p) {
+    p->rec = (float*)base;
+    p->hull = (int4*)(base + a);
+    p->spans = (int*)(base + a + b);
+    p->posr = (int*)(base + a + b + c);
+  }
+  return a + b + 2 * c;
 }
-size_t attn_span_grads_workspace(int M, int heads) {
-  return M > 0 && heads > 0 ? carve_span_grads(M, heads, nullptr, nullptr, nullptr) : 0;
-}
+size_t attn_span_grads_workspace(int M, int heads) { return M > 0 && heads > 0 ? carve_span_grads(M, heads, nullptr, nullptr) : 0; }
 int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g, void* ws, size_t ws_bytes, hipStream_t st) {
   prof::Scope prof_scope(prof::OTHER, st);
   SpanParams p;
@@ -360,6 +379,7 @@ int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
   NMTGAN_REQUIRE(g != nullptr, "attn_span_grads: null gradients");
   NMTGAN_REQUIRE(a->dtype != NMTGAN_F16, "attn_span_grads: bf16 or fp32 (fp16 gradients would underflow without loss scaling)");
   const int es = dtype_size(a->dtype);
+  NMTGAN_REQUIRE(g->ld_dout < (1 << 24), "attn_span_grads: rows further than 2^24 elements apart");
   const int64_t wq = (int64_t)p.heads * p.dh, wk = (int64_t)p.kv_heads * p.dh;
   if (p.M > 0) {
     NMTGAN_REQUIRE(p.lse && g->dout && g->dq, "attn_span_grads: null pointer");
@@ -374,7 +394,7 @@ int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
   const size_t need = attn_span_grads_workspace(p.M, p.heads);
   NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0),
                  "attn_span_grads: workspace of %zu bytes needed, %zu given", need, ws_bytes);
-  if (p.M > 0) carve_span_grads(p.M, p.heads, (char*)ws, &p.delta, &p.hull);
+  if (p.M > 0) carve_span_grads(p.M, p.heads, (char*)ws, &p);
   p.dout = g->dout; p.ld_do = g->ld_dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
   p.ld_dq = g->ld_dq; p.ld_dk = g->ld_dk; p.ld_dv = g->ld_dv;
   if (p.M > 0) {

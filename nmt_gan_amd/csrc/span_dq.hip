@@ -1,4 +1,6 @@
 // Span attention, gradient of the queries on tiles (span_tiles.h has the formulas and the layout).
+#include <type_traits>
+
 #include "span_tiles.h"
 
 namespace nmtgan {
@@ -25,9 +27,9 @@ __global__ __launch_bounds__(64 * NW) void span_dq_kernel(SpanParams p) {
   uint4 own[G::STEPS], dout[G::STEPS];
   load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
   load_own<T, DP>((const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh, ok, p.dh, lane, dout);
-  const int64_t at = (int64_t)ic * p.heads + h;
-  const float ls = p.lse[at], lse2 = ls == -INFINITY ? 0.f : ls * LOG2E, sc2 = p.scale * LOG2E;
-  float delta = p.delta[at];
+  float* const at = delta_at(p, ic, h);
+  const float lse2 = at[-32], sc2 = p.scale * LOG2E;
+  float delta = at[0];
   float slope = 0.f, inv_cap = 0.f;
   int pos = 0;
   if constexpr (EXTRA) {
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(64 * NW) void span_dq_kernel(SpanParams p) {
     }
     if (passes == 2 && it == nt) {
       delta = both_halves_sum(sum);
-      if (ok && lane < 32) p.delta[at] = sp.y > sp.x ? delta : 0.f;
+      if (ok && lane < 32) at[0] = sp.y > sp.x ? delta : 0.f;
     }
     if (j0 < ws.hi && j0 + KT > ws.lo) {
       const unsigned char* tk = smem + (it & 1) * TB;
@@ -110,6 +112,141 @@ __global__ __launch_bounds__(64 * NW) void span_dq_kernel(SpanParams p) {
 }
 
 
+template <typename T, int DP, int KW, bool EXTRA>
+__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dq_split_kernel(SpanParams p) {
+  using G = Geo<T, DP>;
+  using D = Dma<T, DP>;
+  constexpr int REGION = 4 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ float s_sum[KW][32], xs[KW][2][SPAN_MAX_DH];
+  __shared__ int bad[32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = blockIdx.x % p.heads, tile = gridDim.x / p.heads - 1 - blockIdx.x / p.heads;
+  const int kvh = h / (p.heads / p.kv_heads);
+  const int i = tile * 32 + (lane & 31), ic = min(i, p.M - 1);
+  const bool ok = i < p.M;
+  const int2 sp = ok ? span_of(p, i) : make_int2(0, 0);
+  const WaveSpan ws = wave_span(sp);
+  const T* K = (const T*)p.k + kvh * p.dh;
+  const T* V = (const T*)p.v + kvh * p.dh;
+  unsigned char* mine = smem + w * REGION;
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)mine);
+  D dk, dv;
+  dk.init(p.ldk, p.dh, lane);
+  dv.init(p.ldv, p.dh, lane);
+  const int nt = ws.hi > ws.lo ? (ws.hi - ws.lo + 31) / 32 : 0;
+  auto issue = [&](int t, int buf) {
+    const int j0 = ws.lo + 32 * t;
+    dk.issue(K, p.ldk, j0, ws.hi - j0, lds + buf * 2 * D::BYTES, lane);
+    dv.issue(V, p.ldv, j0, ws.hi - j0, lds + (buf * 2 + 1) * D::BYTES, lane);
+  };
+  uint4 own[G::STEPS], dout[G::STEPS];
+  load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
+  load_own<T, DP>((const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh, ok, p.dh, lane, dout);
+  float* const at = delta_at(p, ic, h);
+  const float lse2 = at[-32], sc2 = p.scale * LOG2E;
+  float delta = at[0];
+  float slope2 = 0.f;
+  int pos = 0;
+  if constexpr (EXTRA) {
+    if (p.slopes) { slope2 = p.slopes[h] * LOG2E; pos = pos_of(p, ic); }
+  }
+  f32x16_t acc[G::DB];
+  clear(acc);
+  const unsigned len = (unsigned)(sp.y - sp.x);
+  float sum = 0.f;
+  auto walk = [&](auto FIRST) {                   // FIRST: sum p dp only
+    constexpr bool first_pass = decltype(FIRST)::value;
+    if (w < nt) issue(w, 0);
+    if (w + KW < nt) issue(w + KW, 1);
+    int buf = 0;
+    for (int t = w; t < nt; t += KW, buf ^= 1) {
+      const int j0 = ws.lo + 32 * t;
+      if (t + KW < nt) wait_dma<2 * D::NI>();
+      else wait_dma<0>();
+      if (__any(sp.x < j0 + 32 && sp.y > j0)) {
+        const unsigned char* tk = mine + buf * 2 * D::BYTES;
+        f32x16_t s = score_block<T, DP>(tk, 0, own, lane), turn;
+        f32x16_t d = score_block<T, DP>(tk + D::BYTES, 0, dout, lane);
+        const int first = j0 + 4 * (lane >> 5);
+        if constexpr (EXTRA) {
+          if (p.cap > 0.f) {
+            cap_scores<T, true>(s, turn, p.scale, p.cap);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              s[r] *= sc2;
+              turn[r] = 1.f;
+            }
+          }
+          if (p.slopes) {
+            const float away = (float)(pos - first);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[r]);
+          }
+        }
+        const bool whole = j0 >= ws.all_lo && j0 + 32 <= ws.all_hi;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float pe = __builtin_amdgcn_exp2f(EXTRA ? s[r] - lse2 : fmaf(s[r], sc2, -lse2));
+          float ds = pe * (first_pass ? d[r] : d[r] - delta);
+          if (EXTRA && !first_pass) ds *= turn[r];
+          s[r] = ds;
+        }
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = (unsigned)(first - sp.x + 8 * (r >> 2) + (r & 3)) < len ? s[r] : 0.f;
+        }
+        if constexpr (first_pass) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += s[r];
+        } else {
+          accum_block<T, DP>(tk, 0, s, acc, lane);
+        }
+      }
+      if (t + 2 * KW < nt) {
+        wait_lds();
+        issue(t + 2 * KW, buf);
+      }
+    }
+  };
+  if (nt * 32 <= SPAN_SHORT) {
+    walk(std::integral_constant<bool, true>{});
+    sum = both_halves_sum(sum);
+    if (lane < 32) s_sum[w][lane] = sum;
+    __syncthreads();
+    delta = s_sum[0][lane & 31];
+#pragma unroll
+    for (int k = 1; k < KW; ++k) delta += s_sum[k][lane & 31];
+    if (ok && tid < 32) at[0] = sp.y > sp.x ? delta : 0.f;
+  }
+  walk(std::integral_constant<bool, false>{});
+  if (tid < 32) bad[tid] = 0;
+  join_write<DP>(reinterpret_cast<float*>(mine), acc, 1.f, lane);
+  __syncthreads();
+  float4 tot[JN];
+#pragma unroll
+  for (int u = 0; u < JN; ++u) {
+    const int idx = tid + u * NT, row = idx / (DP / 4), c4 = idx % (DP / 4), r = tile * 32 + row;
+    tot[u] = join_read<DP, KW>(reinterpret_cast<const float*>(smem), REGION / 4, row, c4);
+    if (r >= p.M) continue;
+    const int2 span = span_of(p, r);
+    if (span.y <= span.x) tot[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    else if (!finite4(tot[u])) bad[row] = 1;
+  }
+  __threadfence_block();                          // delta is read again by rows that are done one by one
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < JN; ++u) {
+    const int idx = tid + u * NT, row = idx / (DP / 4), col = idx % (DP / 4) * 4, r = tile * 32 + row;
+    if (r >= p.M || col >= p.dh || bad[row]) continue;
+    const float x[4] = {tot[u].x * p.scale, tot[u].y * p.scale, tot[u].z * p.scale, tot[u].w * p.scale};
+    VecIO<T, 4>::store((T*)p.dq + (int64_t)r * p.ld_dq + h * p.dh + col, x);
+  }
+  for (int row = w; row < 32; row += KW)
+    if (bad[row]) span_dq_row<T>(p, tile * 32 + row, h, xs[w][0], xs[w][1], lane);
+}
+
 template <typename T, int DP, int NW>
 static int launch_dq(const SpanParams& p, hipStream_t st) {
   constexpr int RT = NW == 1 || Geo<T, DP>::RB > 128 ? 32 : 64;
@@ -128,8 +265,23 @@ static int launch_dq(const SpanParams& p, hipStream_t st) {
   return 0;
 }
 template <typename T, int DP>
+static int launch_dq_split(const SpanParams& p, hipStream_t st) {
+  constexpr int KW = Geo<T, DP>::RB > 256 ? 2 : 4;
+  constexpr size_t smem = (size_t)KW * 4 * Dma<T, DP>::BYTES;
+  const int64_t grid = ((int64_t)p.M + 31) / 32 * p.heads;
+  if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
+    NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, true>, smem, "attn_span_dq"));
+    hipLaunchKernelGGL((span_dq_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+  } else {
+    NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, false>, smem, "attn_span_dq"));
+    hipLaunchKernelGGL((span_dq_split_kernel<T, DP, KW, false>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+  }
+  NMTGAN_CHECK_LAUNCH("attn_span_dq");
+  return 0;
+}
+template <typename T, int DP>
 static int choose_dq(const SpanParams& p, hipStream_t st) {
-  return ((int64_t)p.M + 31) / 32 * p.heads <= SPAN_FEW_WAVES ? launch_dq<T, DP, 1>(p, st) : launch_dq<T, DP, 4>(p, st);
+  return ((int64_t)p.M + 31) / 32 * p.heads <= SPAN_FEW ? launch_dq_split<T, DP>(p, st) : launch_dq<T, DP, 4>(p, st);
 }
 int span_dq_tiles(int dtype, const SpanParams& p, hipStream_t st) {
   NMTGAN_DISPATCH_GRAD(dtype, T, {

@@ -135,6 +135,156 @@ __global__ __launch_bounds__(64 * NW) void span_fwd_kernel(SpanParams p) {
 }
 
 
+template <typename T, int DP, int KW, bool EXTRA>
+__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_fwd_split_kernel(SpanParams p) {
+  using G = Geo<T, DP>;
+  using D = Dma<T, DP>;
+  constexpr int REGION = 4 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // a wave's K, V tiles, twice
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ float s_m[KW][32], s_l[KW][32], xs[KW][SPAN_MAX_DH];
+  __shared__ int bad[32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = blockIdx.x % p.heads, tile = gridDim.x / p.heads - 1 - blockIdx.x / p.heads;
+  const int kvh = h / (p.heads / p.kv_heads);
+  const int i = tile * 32 + (lane & 31), ic = min(i, p.M - 1);
+  const bool ok = i < p.M;
+  const int2 sp = ok ? span_of(p, i) : make_int2(0, 0);
+  const WaveSpan ws = wave_span(sp);
+  const T* K = (const T*)p.k + kvh * p.dh;
+  const T* V = (const T*)p.v + kvh * p.dh;
+  unsigned char* mine = smem + w * REGION;
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)mine);
+  D dk, dv;
+  dk.init(p.ldk, p.dh, lane);
+  dv.init(p.ldv, p.dh, lane);
+  const int nt = ws.hi > ws.lo ? (ws.hi - ws.lo + 31) / 32 : 0;
+  auto issue = [&](int t, int buf) {
+    const int j0 = ws.lo + 32 * t;
+    dk.issue(K, p.ldk, j0, ws.hi - j0, lds + buf * 2 * D::BYTES, lane);
+    dv.issue(V, p.ldv, j0, ws.hi - j0, lds + (buf * 2 + 1) * D::BYTES, lane);
+  };
+  uint4 own[G::STEPS];
+  load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
+  if (w < nt) issue(w, 0);
+  if (w + KW < nt) issue(w + KW, 1);
+  const float sc2 = p.scale * LOG2E;
+  float slope2 = 0.f;
+  int pos = 0;
+  if constexpr (EXTRA) {
+    if (p.slopes) { slope2 = p.slopes[h] * LOG2E; pos = pos_of(p, ic); }
+  }
+  f32x16_t acc[G::DB];
+  clear(acc);
+  float m = -INFINITY, l = 0.f;
+  const unsigned len = (unsigned)(sp.y - sp.x);
+
+  int buf = 0;
+  for (int t = w; t < nt; t += KW, buf ^= 1) {
+    const int j0 = ws.lo + 32 * t;
+    if (t + KW < nt) wait_dma<2 * D::NI>();
+    else wait_dma<0>();
+    if (__any(sp.x < j0 + 32 && sp.y > j0)) {
+      const unsigned char* tk = mine + buf * 2 * D::BYTES;
+      f32x16_t s = score_block<T, DP>(tk, 0, own, lane);
+      const int first = j0 + 4 * (lane >> 5);
+      if constexpr (EXTRA) {
+        if (p.cap > 0.f) {
+          cap_scores<T, false>(s, s, p.scale, p.cap);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= sc2;
+        }
+        if (p.slopes) {
+          const float away = (float)(pos - first);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[r]);
+        }
+      }
+      const bool flip = !EXTRA && sc2 < 0.f;      // the largest score is the smallest product
+      if (!(j0 >= ws.all_lo && j0 + 32 <= ws.all_hi)) {
+        const float out = flip ? INFINITY : -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (unsigned)(first - sp.x + 8 * (r >> 2) + (r & 3)) < len ? s[r] : out;
+      }
+      float mx = flip ? INFINITY : -INFINITY;
+      if (flip) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fminf(mx, s[r]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      }
+      mx = both_halves_max(EXTRA ? mx : (isinf(mx) ? -INFINITY : mx * sc2));
+      const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
+      if (__any(mn > m)) {
+        const float c = __builtin_amdgcn_exp2f(m - mu);
+        l *= c;
+#pragma unroll
+        for (int db = 0; db < G::DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= c;
+        m = mn;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(EXTRA ? s[r] - mu : fmaf(s[r], sc2, -mu));
+        l += s[r];
+      }
+      accum_block<T, DP>(tk + D::BYTES, 0, s, acc, lane);
+    }
+    if (t + 2 * KW < nt) {
+      wait_lds();
+      issue(t + 2 * KW, buf);
+    }
+  }
+  l = both_halves_sum(l);
+  if (lane < 32) { s_m[w][lane] = m; s_l[w][lane] = l; }
+  if (tid < 32) bad[tid] = 0;
+  __syncthreads();
+  float mt = s_m[0][lane & 31];
+#pragma unroll
+  for (int k = 1; k < KW; ++k) mt = fmaxf(mt, s_m[k][lane & 31]);
+  const float mu = mt == -INFINITY ? 0.f : mt;
+  join_write<DP>(reinterpret_cast<float*>(mine), acc, __builtin_amdgcn_exp2f(m - mu), lane);
+  __syncthreads();
+  float4 sum[JN];
+  float inv[JN];
+#pragma unroll
+  for (int u = 0; u < JN; ++u) {
+    const int idx = tid + u * NT, row = idx / (DP / 4), c4 = idx % (DP / 4), r = tile * 32 + row;
+    float mr = s_m[0][row], lr = 0.f;
+#pragma unroll
+    for (int k = 1; k < KW; ++k) mr = fmaxf(mr, s_m[k][row]);
+    const float mur = mr == -INFINITY ? 0.f : mr;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) lr += s_l[k][row] * __builtin_amdgcn_exp2f(s_m[k][row] - mur);
+    sum[u] = join_read<DP, KW>(reinterpret_cast<const float*>(smem), REGION / 4, row, c4);
+    inv[u] = 0.f;
+    if (r >= p.M) continue;
+    const int2 span = span_of(p, r);
+    if (span.y > span.x) {
+      inv[u] = lr == 0.f ? 0.f : 1.f / lr;
+      if (!(finite4(sum[u]) && lr < INFINITY)) bad[row] = 1;
+    } else {
+      sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      lr = 0.f;
+    }
+    if (p.lse && c4 == 0) p.lse[(int64_t)r * p.heads + h] = lr == 0.f ? -INFINITY : mur * LN2 + logf(lr);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < JN; ++u) {
+    const int idx = tid + u * NT, row = idx / (DP / 4), col = idx % (DP / 4) * 4, r = tile * 32 + row;
+    if (r >= p.M || col >= p.dh || bad[row]) continue;
+    const float x[4] = {sum[u].x * inv[u], sum[u].y * inv[u], sum[u].z * inv[u], sum[u].w * inv[u]};
+    VecIO<T, 4>::store((T*)p.out + (int64_t)r * p.ldo + h * p.dh + col, x);
+  }
+  // a product of a zero probability with an infinity or NaN of a row this row does not see: such rows are done again one
+  // by one (as are rows that are not finite by right)
+  for (int row = w; row < 32; row += KW)
+    if (bad[row]) span_fwd_row<T>(p, tile * 32 + row, h, xs[w], lane);
+}
+
 template <typename T, int DP, int NW>
 static int launch_fwd(const SpanParams& p, hipStream_t st) {
   constexpr int RT = NW == 1 || Geo<T, DP>::RB > 128 ? 32 : 64;
@@ -153,8 +303,23 @@ static int launch_fwd(const SpanParams& p, hipStream_t st) {
   return 0;
 }
 template <typename T, int DP>
+static int launch_fwd_split(const SpanParams& p, hipStream_t st) {
+  constexpr int KW = Geo<T, DP>::RB > 256 ? 2 : 4;
+  constexpr size_t smem = (size_t)KW * 4 * Dma<T, DP>::BYTES;
+  const int64_t grid = ((int64_t)p.M + 31) / 32 * p.heads;
+  if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
+    NMTGAN_TRY(raise_lds(&span_fwd_split_kernel<T, DP, KW, true>, smem, "attn_span"));
+    hipLaunchKernelGGL((span_fwd_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+  } else {
+    NMTGAN_TRY(raise_lds(&span_fwd_split_kernel<T, DP, KW, false>, smem, "attn_span"));
+    hipLaunchKernelGGL((span_fwd_split_kernel<T, DP, KW, false>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+  }
+  NMTGAN_CHECK_LAUNCH("attn_span");
+  return 0;
+}
+template <typename T, int DP>
 static int choose_fwd(const SpanParams& p, hipStream_t st) {
-  return ((int64_t)p.M + 31) / 32 * p.heads <= SPAN_FEW_WAVES ? launch_fwd<T, DP, 1>(p, st) : launch_fwd<T, DP, 4>(p, st);
+  return ((int64_t)p.M + 31) / 32 * p.heads <= SPAN_FEW ? launch_fwd_split<T, DP>(p, st) : launch_fwd<T, DP, 4>(p, st);
 }
 int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st) {
   NMTGAN_DISPATCH_OP(dtype, T, {

@@ -36,7 +36,8 @@ struct SpanParams {
   const void* dout; int64_t ld_do;
   void* dq; void* dk; void* dv;
   int64_t ld_dq, ld_dk, ld_dv;
-  float* delta;                                  // [M][heads]
+  // per head and 32 rows: [lse / ln 2 x 32][delta x 32]; per 32 rows: [lo x 32][hi x 32] and [pos x 32][unused x 32]
+  float* rec; int* spans; int* posr;
   int4* hull;                                    // [ceil(M / 32)] of 32 rows: keys seen by any row [x, y), by every row [z, w)
 };
 
@@ -46,6 +47,9 @@ __device__ __forceinline__ float span_exp(float x) { return __builtin_amdgcn_exp
 __device__ __forceinline__ int2 span_of(const SpanParams& p, int i) {
   const int a = max(p.lo[i], 0), b = min(p.hi[i], p.N);
   return b > a ? make_int2(a, b) : make_int2(0, 0);
+}
+__device__ __forceinline__ float* delta_at(const SpanParams& p, int i, int h) {
+  return p.rec + (((int64_t)h * ((p.M + 31) / 32) + (i >> 5)) * 64 + 32 + (i & 31));
 }
 __device__ __forceinline__ int pos_of(const SpanParams& p, int i) { return p.pos ? p.pos[i] : p.hi[i] - 1; }
 
@@ -138,7 +142,7 @@ __device__ void span_dq_row(const SpanParams& p, int i, int h, float* x, float* 
   const int2 sp = span_of(p, i);
   const int pos = pos_of(p, i);
   const float slope = p.slopes ? p.slopes[h] : 0.f;
-  const float lse = p.lse[(int64_t)i * p.heads + h], delta = p.delta[(int64_t)i * p.heads + h];
+  const float lse = p.lse[(int64_t)i * p.heads + h], delta = *delta_at(p, i, h);
   float acc[2] = {0.f, 0.f};
   for (int j0 = sp.x; j0 < sp.y; j0 += 64) {
     const int j = j0 + lane;
@@ -185,7 +189,7 @@ __device__ void span_dkv_key(const SpanParams& p, int j, int kvh, float* x, floa
       float pe = 0.f, dr = 0.f;
       if (on)
         span_pair(p, Q + i * p.ldq, D + i * p.ld_do, x, y, p.lse[(int64_t)i * p.heads + h],
-                  p.delta[(int64_t)i * p.heads + h], p.slopes ? p.slopes[h] : 0.f, pos, j, pe, dr);
+                  *delta_at(p, i, h), p.slopes ? p.slopes[h] : 0.f, pos, j, pe, dr);
       for (unsigned long long left = mask; left; left &= left - 1) {
         const int t = __builtin_ctzll(left);
         const float pt = __shfl(pe, t, 64), dt = __shfl(dr, t, 64);
@@ -420,17 +424,131 @@ __device__ __forceinline__ int2 block_span(const WaveSpan& ws, int (*red)[2], in
 }
 
 
+// ------------------------------------------------------------------------------------------ split form
+// The KW waves of a workgroup share their own 32 rows and take every KW-th 32-row tile of the other side, each into LDS of
+// its own by DMA two tiles ahead - no barrier inside the walk - and are joined at the end.
+// Scalar base + one 32-bit lane offset per swizzle period; chunks behind dh and rows behind the last repeat a valid one
+// (they meet zeros of the own rows or weights of zero).
+// a pointer / offset that is the same in every lane, in scalar registers
+__device__ __forceinline__ const char* scalar_ptr(const void* p) {
+  const uint64_t a = (uint64_t)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+  return (const char*)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ void dma16(unsigned voff, const void* sbase, unsigned lds_dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(voff), "s"(sbase), "s"(lds_dst)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(unsigned voff, const void* base, unsigned dst) {
+  const char* sbase = scalar_ptr(base);
+  const unsigned lds_dst = __builtin_amdgcn_readfirstlane(dst);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+               :
+               : "v"(voff), "s"(sbase), "s"(lds_dst)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_dma() {       // at most N newer transfers may be in flight
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+template <typename T, int DP> struct Dma {
+  using G = Geo<T, DP>;
+  static constexpr int RPI = 64 / G::CH, NI = 32 / RPI;      // rows per instruction, instructions per 32 rows
+  static constexpr int PERIOD = (G::MASK + 1) * G::RPL / RPI, NV = PERIOD < 1 ? 1 : PERIOD;
+  static constexpr int BYTES = 32 * G::RB;
+  unsigned chunk[NV];
+  unsigned ldb;
+  __device__ __forceinline__ void init(int64_t ld, int dh, int lane) {
+    ldb = (unsigned)(ld * (int64_t)sizeof(T));
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int row = v * RPI + lane / G::CH, c = (lane % G::CH) ^ ((row / G::RPL) & G::MASK);
+      chunk[v] = 16u * (unsigned)min(c, dh * (int)sizeof(T) / 16 - 1);
+    }
+  }
+  // rows row0 .. row0 + 31 of `base`, row0 + left the first that is not there (left >= 1)
+  __device__ __forceinline__ void issue(const T* base, int64_t ld, int row0, int left, unsigned dst, int lane) const {
+    const char* b = scalar_ptr(reinterpret_cast<const char*>(base) + (int64_t)row0 * ld * (int64_t)sizeof(T));
+    dst = __builtin_amdgcn_readfirstlane(dst);
+    const unsigned step = __builtin_amdgcn_readfirstlane(ldb);
+    const unsigned own = (unsigned)(lane / G::CH);
+    if (left >= 32) {
+#pragma unroll
+      for (int u = 0; u < NI; ++u) dma16(own * ldb + chunk[u % NV], b + (uint64_t)(u * RPI) * step, dst + u * 1024);
+    } else {
+#pragma unroll
+      for (int u = 0; u < NI; ++u) dma16(min(own + u * RPI, (unsigned)left - 1u) * ldb + chunk[u % NV], b, dst + u * 1024);
+    }
+  }
+};
+
+// tanh and distance terms of a score block in place, in units of log 2: s = raw products -> scores (s, d hold 16 rows of
+// the tile at 8 (r >> 2) + (r & 3) from `first`); turn = 1 - t^2 where wanted
+template <typename T, bool TURN>
+__device__ __forceinline__ void cap_scores(f32x16_t& s, f32x16_t& turn, float scale, float cap) {
+  if constexpr (sizeof(T) == 4) {
+    const float inv = scale / cap, c2 = cap * LOG2E;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float t = tanhf(s[r] * inv);
+      s[r] = c2 * t;
+      if constexpr (TURN) turn[r] = fmaf(-t, t, 1.f);
+    }
+  } else {
+    // t = 1 - 2 d, d = 1 / (1 + exp(2 r / cap)); 1 - t^2 = 4 d (1 - d)
+    const float a = scale / cap * 2.f * LOG2E, c2 = cap * LOG2E, c4 = -2.f * c2;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float d = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * a));
+      s[r] = fmaf(d, c4, c2);
+      if constexpr (TURN) turn[r] = 4.f * fmaf(-d, d, d);
+    }
+  }
+}
+
+// sums the KW waves' transposed accumulators (32 own rows x DP, each wave's in LDS at region w) and hands the result to
+// put(row, col, x[4]) in whole rows; bad[row] is set where a sum is not finite
+template <int DP> __device__ __forceinline__ int join_at(int row, int c4) { return row * DP + ((c4 ^ (row & (DP / 4 - 1))) << 2); }
+template <int DP>
+__device__ __forceinline__ void join_write(float* region, const f32x16_t (&acc)[DP / 32], float f, int lane) {
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c4 = 8 * db + 2 * g + (lane >> 5);
+      *reinterpret_cast<float4*>(region + join_at<DP>(lane & 31, c4)) =
+          make_float4(acc[db][4 * g] * f, acc[db][4 * g + 1] * f, acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f);
+    }
+}
+template <int DP, int KW>
+__device__ __forceinline__ float4 join_read(const float* region, int stride, int row, int c4) {
+  float4 s = *reinterpret_cast<const float4*>(region + join_at<DP>(row, c4));
+#pragma unroll
+  for (int k = 1; k < KW; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(region + k * stride + join_at<DP>(row, c4));
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  return s;
+}
+__device__ __forceinline__ bool finite4(const float4& v) {
+  return fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f))) == 0.f;
+}
+
 // dynamic LDS beyond 64 KiB has to be asked for once per device and kernel
 template <typename F>
 static inline int raise_lds(F* kernel, size_t bytes, const char* what) {
-  if (bytes <= 64 * 1024) return 0;
+  if (bytes <= 48 * 1024) return 0;             // (the static part comes on top)
   NMTGAN_REQUIRE(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
                      hipSuccess, "%s: cannot raise the dynamic LDS limit", what);
   return 0;
 }
-// Waves of 32 rows that a launch has in all: below two per SIMD every wave is a workgroup of its own (32-row tiles, more
-// workgroups to spread); above, four waves share the tiles they stage.
-constexpr int64_t SPAN_FEW_WAVES = 2048;
+// Blocks of 32 rows that a launch has in all: up to SPAN_FEW the waves of a workgroup split the walk of one block (split
+// form); above, four blocks share the tiles they stage.
+constexpr int64_t SPAN_FEW = 2048;
 
 int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st);
 int span_dq_tiles(int dtype, const SpanParams& p, hipStream_t st);
