@@ -3,63 +3,61 @@
 
 namespace nmtgan {
 
-// What the gradient kernels need per row and per 32 rows: delta_i = dout_i . out_i of every head (0 for rows that see
-// nothing, whatever their dout holds) and
-// the hull of the spans of 32 rows.  One workgroup per 64 rows; a row's head products are
-// summed by 8 lanes.
+// What the gradient kernels need per row and per 32 rows: lse and delta_i = dout_i . out_i of every head (0 for rows that see
+// nothing, whatever their dout holds), the spans and their hull.  A workgroup takes 64 rows of one head, 8 lanes a row; the
+// first head's also write what all heads share.
 template <typename T>
 __global__ __launch_bounds__(256) void span_prep_kernel(SpanParams p) {
-  const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  if (w == 0) {
-    const int i = b * 64 + lane;
-    int2 sp = make_int2(0, 0);
-    if (i < p.M) sp = span_of(p, i);
-    int4 hl = make_int4(sp.y > sp.x ? sp.x : 0x7fffffff, sp.y, sp.x, sp.y);
+  const int h = blockIdx.x % p.heads, b = blockIdx.x / p.heads, lane = threadIdx.x & 63, w = threadIdx.x >> 6, c8 = p.dh / 8;
+  float s[2], ls[2];
+  bool some[2];
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-      hl.x = min(hl.x, __shfl_xor(hl.x, o, 64));
-      hl.y = max(hl.y, __shfl_xor(hl.y, o, 64));
-      hl.z = max(hl.z, __shfl_xor(hl.z, o, 64));
-      hl.w = min(hl.w, __shfl_xor(hl.w, o, 64));
-    }
-    if ((lane & 31) == 0 && i < p.M) p.hull[2 * b + (lane >> 5)] = hl;
-    if (b * 64 + (lane & 32) < p.M) {                        // the block of 32 exists: its record is whole
-      int* s = p.spans + (int64_t)(2 * b + (lane >> 5)) * 64 + (lane & 31);
-      s[0] = sp.x;
-      s[32] = sp.y;
-      if (p.slopes) p.posr[(int64_t)(2 * b + (lane >> 5)) * 64 + (lane & 31)] = i < p.M ? pos_of(p, i) : 0;
+  for (int u = 0; u < 2; ++u) {
+    const int i = b * 64 + 32 * u + (threadIdx.x >> 3), ic = min(i, p.M - 1);
+    const T* o = (const T*)p.out + (int64_t)ic * p.ldo + h * p.dh;
+    const T* d = (const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh;
+    const int2 sp = span_of(p, ic);
+    some[u] = i < p.M && sp.y > sp.x;
+    ls[u] = i < p.M ? p.lse[(int64_t)ic * p.heads + h] : 0.f;
+    s[u] = 0.f;
+    for (int c = threadIdx.x & 7; c < c8; c += 8) {
+      float x[8], y[8];
+      VecIO<T, 8>::load(o + 8 * c, x);
+      VecIO<T, 8>::load(d + 8 * c, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[u] = fmaf(x[e], y[e], s[u]);
     }
   }
-  const int rows = min(64, (p.M - b * 64 + 31) / 32 * 32), c8 = p.dh / 8;
-  for (int t = threadIdx.x >> 3; t < rows * p.heads; t += 32) {
-    const int i = b * 64 + t / p.heads, h = t % p.heads;
-    float s = 0.f, ls = 0.f;
-    if (i < p.M) {
-      const T* o = (const T*)p.out + (int64_t)i * p.ldo + h * p.dh;
-      const T* d = (const T*)p.dout + (int64_t)i * p.ld_do + h * p.dh;
-      for (int c = threadIdx.x & 7; c < c8; c += 8) {
-        float x[8], y[8];
-        VecIO<T, 8>::load(o + 8 * c, x);
-        VecIO<T, 8>::load(d + 8 * c, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
-      }
-    }
-    s = dpp_add<0xB1>(s);
-    s = dpp_add<0x4E>(s);
-    s = dpp_add<0x141>(s);
-    if ((threadIdx.x & 7) == 0) {
+  for (int u = 0; u < 2; ++u) {
+    const int i = b * 64 + 32 * u + (threadIdx.x >> 3);
+    s[u] = dpp_add<0xB1>(s[u]);
+    s[u] = dpp_add<0x4E>(s[u]);
+    s[u] = dpp_add<0x141>(s[u]);
+    if ((threadIdx.x & 7) == 0 && b * 64 + 32 * u < p.M) {       // the block of 32 exists: its record is whole
       float* at = delta_at(p, i, h);
-      bool some = false;
-      if (i < p.M) {
-        const int2 sp = span_of(p, i);
-        some = sp.y > sp.x;
-        ls = p.lse[(int64_t)i * p.heads + h];
-      }
-      at[-32] = ls == -INFINITY ? 0.f : ls * LOG2E;
-      at[0] = some ? s : 0.f;
+      at[-32] = ls[u] == -INFINITY ? 0.f : ls[u] * LOG2E;
+      at[0] = some[u] ? s[u] : 0.f;
     }
   }
+  if (h != 0 || w != 0) return;
+  const int i = b * 64 + lane;
+  int2 sp = make_int2(0, 0);
+  if (i < p.M) sp = span_of(p, i);
+  int4 hl = make_int4(sp.y > sp.x ? sp.x : 0x7fffffff, sp.y, sp.x, sp.y);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    hl.x = min(hl.x, __shfl_xor(hl.x, o, 64));
+    hl.y = max(hl.y, __shfl_xor(hl.y, o, 64));
+    hl.z = max(hl.z, __shfl_xor(hl.z, o, 64));
+    hl.w = min(hl.w, __shfl_xor(hl.w, o, 64));
+  }
+  if (b * 64 + (lane & 32) >= p.M) return;
+  const int64_t blk = 2 * b + (lane >> 5);
+  if ((lane & 31) == 0) p.hull[blk] = hl;
+  p.spans[blk * 64 + (lane & 31)] = sp.x;
+  p.spans[blk * 64 + 32 + (lane & 31)] = sp.y;
+  if (p.slopes) p.posr[blk * 64 + (lane & 31)] = i < p.M ? pos_of(p, i) : 0;
 }
 
 // ------------------------------------------------------------------------------------------ single tokens
@@ -398,7 +396,9 @@ int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
   p.dout = g->dout; p.ld_do = g->ld_dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
   p.ld_dq = g->ld_dq; p.ld_dk = g->ld_dk; p.ld_dv = g->ld_dv;
   if (p.M > 0) {
-    NMTGAN_DISPATCH_GRAD(a->dtype, T, hipLaunchKernelGGL(span_prep_kernel<T>, dim3((p.M + 63) / 64), dim3(256), 0, st, p));
+    const int64_t prep = ((int64_t)p.M + 63) / 64 * p.heads;
+    NMTGAN_REQUIRE(prep < (1LL << 31), "attn_span_grads: too many rows");
+    NMTGAN_DISPATCH_GRAD(a->dtype, T, hipLaunchKernelGGL(span_prep_kernel<T>, dim3((unsigned)prep), dim3(256), 0, st, p));
     NMTGAN_CHECK_LAUNCH("attn_span_prep");
     NMTGAN_TRY(span_dq_tiles(a->dtype, p, st));
   }

@@ -165,16 +165,17 @@ __global__ __launch_bounds__(64 * NW) void span_dkv_kernel(SpanParams p) {
   }
 }
 
+// (128 list entries: two workgroups of head width 64 share a CU's LDS)
+constexpr int SPLIT_LIST = 128;
 template <typename T, int DP, int KW, bool EXTRA>
-__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 64 ? 2 : 1) void span_dkv_split_kernel(SpanParams p) {
+__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dkv_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
   constexpr int STAGE = 2 * D::BYTES + 1024;      // Q, dO and the records of 32 rows
   constexpr int REGION = 2 * STAGE, NT = 64 * KW, JN = 32 * DP / 4 / NT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ __attribute__((aligned(16))) int4 hulls[SPAN_LIST];
-  __shared__ int list[SPAN_LIST], n_list[2], bad[32];
-  __shared__ float xs[KW][2][SPAN_MAX_DH];
+  __shared__ __attribute__((aligned(16))) int4 hulls[SPLIT_LIST];
+  __shared__ int list[SPLIT_LIST], n_list[2], bad[32];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % p.kv_heads, g = p.heads / p.kv_heads;
   const int k0 = blockIdx.x / p.kv_heads * 32, j = k0 + (lane & 31), jc = min(j, p.N - 1);
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 64 ? 2 : 1) void span_dk
     __syncthreads();
     if (w == 0) {
       int n = 0, b = next;
-      for (; b < nb && n + 64 <= SPAN_LIST; b += 64) {
+      for (; b < nb && n + 64 <= SPLIT_LIST; b += 64) {
         bool on = false;
         int4 hl;
         if (b + lane < nb) {
@@ -326,8 +327,9 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 64 ? 2 : 1) void span_dk
     VecIO<T, 4>::store((T*)p.dk + r * p.ld_dk + kvh * p.dh + col, x);
     VecIO<T, 4>::store((T*)p.dv + r * p.ld_dv + kvh * p.dh + col, y);
   }
+  float* xs = reinterpret_cast<float*>(mine);      // (the joined sums have been read)
   for (int row = w; row < 32; row += KW)
-    if (bad[row]) span_dkv_key<T>(p, k0 + row, kvh, xs[w][0], xs[w][1], lane);
+    if (bad[row]) span_dkv_key<T>(p, k0 + row, kvh, xs, xs + SPAN_MAX_DH, lane);
 }
 
 template <typename T, int DP, int NW>
