@@ -113,10 +113,10 @@ __global__ __launch_bounds__(64 * NW) void span_dq_kernel(SpanParams p) {
 
 
 template <typename T, int DP, int KW, bool EXTRA>
-__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dq_split_kernel(SpanParams p) {
+__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_dq_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
-  constexpr int REGION = 4 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;
+  constexpr int REGION = 3 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // two K tiles and one V tile per wave
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_sum[KW][32], xs[KW][2][SPAN_MAX_DH];
   __shared__ int bad[32];
@@ -135,11 +135,8 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
   dk.init(p.ldk, p.dh, lane);
   dv.init(p.ldv, p.dh, lane);
   const int nt = ws.hi > ws.lo ? (ws.hi - ws.lo + 31) / 32 : 0;
-  auto issue = [&](int t, int buf) {
-    const int j0 = ws.lo + 32 * t;
-    dk.issue(K, p.ldk, j0, ws.hi - j0, lds + buf * 2 * D::BYTES, lane);
-    dv.issue(V, p.ldv, j0, ws.hi - j0, lds + (buf * 2 + 1) * D::BYTES, lane);
-  };
+  auto issue_k = [&](int t, int buf) { dk.issue(K, p.ldk, ws.lo + 32 * t, ws.hi - ws.lo - 32 * t, lds + buf * D::BYTES, lane); };
+  auto issue_v = [&](int t) { dv.issue(V, p.ldv, ws.lo + 32 * t, ws.hi - ws.lo - 32 * t, lds + 2 * D::BYTES, lane); };
   uint4 own[G::STEPS], dout[G::STEPS];
   load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
   load_own<T, DP>((const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh, ok, p.dh, lane, dout);
@@ -157,17 +154,24 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
   float sum = 0.f;
   auto walk = [&](auto FIRST) {                   // FIRST: sum p dp only
     constexpr bool first_pass = decltype(FIRST)::value;
-    if (w < nt) issue(w, 0);
-    if (w + KW < nt) issue(w + KW, 1);
+    if (w < nt) {
+      issue_k(w, 0);
+      issue_v(w);
+    }
+    if (w + KW < nt) issue_k(w + KW, 1);
     int buf = 0;
     for (int t = w; t < nt; t += KW, buf ^= 1) {
       const int j0 = ws.lo + 32 * t;
-      if (t + KW < nt) wait_dma<2 * D::NI>();
+      if (t + KW < nt) wait_dma<D::NI>();         // the next K may still be under way
       else wait_dma<0>();
+      const unsigned char* tk = mine + buf * D::BYTES;
+      f32x16_t s = score_block<T, DP>(tk, 0, own, lane), turn;
+      f32x16_t d = score_block<T, DP>(mine + 2 * D::BYTES, 0, dout, lane);
+      if (t + KW < nt) {
+        wait_lds();
+        issue_v(t + KW);
+      }
       if (__any(sp.x < j0 + 32 && sp.y > j0)) {
-        const unsigned char* tk = mine + buf * 2 * D::BYTES;
-        f32x16_t s = score_block<T, DP>(tk, 0, own, lane), turn;
-        f32x16_t d = score_block<T, DP>(tk + D::BYTES, 0, dout, lane);
         const int first = j0 + 4 * (lane >> 5);
         if constexpr (EXTRA) {
           if (p.cap > 0.f) {
@@ -206,7 +210,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
       }
       if (t + 2 * KW < nt) {
         wait_lds();
-        issue(t + 2 * KW, buf);
+        issue_k(t + 2 * KW, buf);
       }
     }
   };
@@ -267,7 +271,7 @@ static int launch_dq(const SpanParams& p, hipStream_t st) {
 template <typename T, int DP>
 static int launch_dq_split(const SpanParams& p, hipStream_t st) {
   constexpr int KW = Geo<T, DP>::RB > 256 ? 2 : 4;
-  constexpr size_t smem = (size_t)KW * 4 * Dma<T, DP>::BYTES;
+  constexpr size_t smem = (size_t)KW * 3 * Dma<T, DP>::BYTES;
   const int64_t grid = ((int64_t)p.M + 31) / 32 * p.heads;
   if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
     NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, true>, smem, "attn_span_dq"));

@@ -89,9 +89,9 @@ __global__ __launch_bounds__(64 * NW) void span_fwd_kernel(SpanParams p) {
       }
       const float f = EXTRA ? 1.f : sc2;
       mx = both_halves_max(EXTRA ? mx : (isinf(mx) ? -INFINITY : mx * f));
-      const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-      if (__any(mn > m)) {
-        const float c = __builtin_amdgcn_exp2f(m - mu);
+      // the reference point follows the maximum only when it falls 2^8 behind: probabilities up to 256 fit every type
+      if (__any(mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx), c = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
         l *= c;
 #pragma unroll
         for (int db = 0; db < G::DB; ++db)
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(64 * NW) void span_fwd_kernel(SpanParams p) {
           for (int r = 0; r < 16; ++r) acc[db][r] *= c;
         m = mn;
       }
+      const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int kb = 0; kb < KT / 32; ++kb) {
 #pragma unroll
@@ -136,10 +137,12 @@ __global__ __launch_bounds__(64 * NW) void span_fwd_kernel(SpanParams p) {
 
 
 template <typename T, int DP, int KW, bool EXTRA>
-__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_fwd_split_kernel(SpanParams p) {
+__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_fwd_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
-  constexpr int REGION = 4 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // a wave's K, V tiles, twice
+  // one K and one V tile per wave: the next K is under way during the softmax and the second product, the next V during
+  // the first product and the softmax, and the small footprint buys waves to hide the rest behind
+  constexpr int REGION = 2 * D::BYTES > 32 * DP * 4 ? 2 * D::BYTES : 32 * DP * 4, NT = 64 * KW, JN = 32 * DP / 4 / NT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_m[KW][32], s_l[KW][32], xs[KW][SPAN_MAX_DH];
   __shared__ int bad[32];
@@ -158,15 +161,14 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_f
   dk.init(p.ldk, p.dh, lane);
   dv.init(p.ldv, p.dh, lane);
   const int nt = ws.hi > ws.lo ? (ws.hi - ws.lo + 31) / 32 : 0;
-  auto issue = [&](int t, int buf) {
-    const int j0 = ws.lo + 32 * t;
-    dk.issue(K, p.ldk, j0, ws.hi - j0, lds + buf * 2 * D::BYTES, lane);
-    dv.issue(V, p.ldv, j0, ws.hi - j0, lds + (buf * 2 + 1) * D::BYTES, lane);
-  };
+  auto issue_k = [&](int t) { dk.issue(K, p.ldk, ws.lo + 32 * t, ws.hi - ws.lo - 32 * t, lds, lane); };
+  auto issue_v = [&](int t) { dv.issue(V, p.ldv, ws.lo + 32 * t, ws.hi - ws.lo - 32 * t, lds + D::BYTES, lane); };
   uint4 own[G::STEPS];
   load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
-  if (w < nt) issue(w, 0);
-  if (w + KW < nt) issue(w + KW, 1);
+  if (w < nt) {
+    issue_k(w);
+    issue_v(w);
+  }
   const float sc2 = p.scale * LOG2E;
   float slope2 = 0.f;
   int pos = 0;
@@ -178,14 +180,17 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_f
   float m = -INFINITY, l = 0.f;
   const unsigned len = (unsigned)(sp.y - sp.x);
 
-  int buf = 0;
-  for (int t = w; t < nt; t += KW, buf ^= 1) {
+  for (int t = w; t < nt; t += KW) {
     const int j0 = ws.lo + 32 * t;
-    if (t + KW < nt) wait_dma<2 * D::NI>();
-    else wait_dma<0>();
-    if (__any(sp.x < j0 + 32 && sp.y > j0)) {
-      const unsigned char* tk = mine + buf * 2 * D::BYTES;
-      f32x16_t s = score_block<T, DP>(tk, 0, own, lane);
+    const bool more = t + KW < nt;
+    wait_dma<D::NI>();                            // V may still be under way
+    f32x16_t s = score_block<T, DP>(mine, 0, own, lane);
+    if (more) {
+      wait_lds();
+      issue_k(t + KW);
+    }
+    const bool met = __any(sp.x < j0 + 32 && sp.y > j0);
+    if (met) {
       const int first = j0 + 4 * (lane >> 5);
       if constexpr (EXTRA) {
         if (p.cap > 0.f) {
@@ -215,9 +220,9 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_f
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
       }
       mx = both_halves_max(EXTRA ? mx : (isinf(mx) ? -INFINITY : mx * sc2));
-      const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-      if (__any(mn > m)) {
-        const float c = __builtin_amdgcn_exp2f(m - mu);
+      // the reference point follows the maximum only when it falls 2^8 behind: probabilities up to 256 fit every type
+      if (__any(mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx), c = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
         l *= c;
 #pragma unroll
         for (int db = 0; db < G::DB; ++db)
@@ -225,16 +230,19 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_f
           for (int r = 0; r < 16; ++r) acc[db][r] *= c;
         m = mn;
       }
+      const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[r] = __builtin_amdgcn_exp2f(EXTRA ? s[r] - mu : fmaf(s[r], sc2, -mu));
         l += s[r];
       }
-      accum_block<T, DP>(tk + D::BYTES, 0, s, acc, lane);
     }
-    if (t + 2 * KW < nt) {
+    if (more) wait_dma<D::NI>();                  // the next K may still be under way
+    else wait_dma<0>();
+    if (met) accum_block<T, DP>(mine + D::BYTES, 0, s, acc, lane);
+    if (more) {
       wait_lds();
-      issue(t + 2 * KW, buf);
+      issue_v(t + KW);
     }
   }
   l = both_halves_sum(l);
@@ -305,7 +313,7 @@ static int launch_fwd(const SpanParams& p, hipStream_t st) {
 template <typename T, int DP>
 static int launch_fwd_split(const SpanParams& p, hipStream_t st) {
   constexpr int KW = Geo<T, DP>::RB > 256 ? 2 : 4;
-  constexpr size_t smem = (size_t)KW * 4 * Dma<T, DP>::BYTES;
+  constexpr size_t smem = (size_t)KW * std::max(2 * Dma<T, DP>::BYTES, 32 * DP * 4);
   const int64_t grid = ((int64_t)p.M + 31) / 32 * p.heads;
   if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
     NMTGAN_TRY(raise_lds(&span_fwd_split_kernel<T, DP, KW, true>, smem, "attn_span"));

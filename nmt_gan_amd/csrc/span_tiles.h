@@ -460,14 +460,14 @@ template <typename T, int DP> struct Dma {
   static constexpr int RPI = 64 / G::CH, NI = 32 / RPI;      // rows per instruction, instructions per 32 rows
   static constexpr int PERIOD = (G::MASK + 1) * G::RPL / RPI, NV = PERIOD < 1 ? 1 : PERIOD;
   static constexpr int BYTES = 32 * G::RB;
-  unsigned chunk[NV];
+  unsigned off[NV];                                // lane's row inside an instruction and its chunk
   unsigned ldb;
   __device__ __forceinline__ void init(int64_t ld, int dh, int lane) {
     ldb = (unsigned)(ld * (int64_t)sizeof(T));
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int row = v * RPI + lane / G::CH, c = (lane % G::CH) ^ ((row / G::RPL) & G::MASK);
-      chunk[v] = 16u * (unsigned)min(c, dh * (int)sizeof(T) / 16 - 1);
+      off[v] = (unsigned)(lane / G::CH) * ldb + 16u * (unsigned)min(c, dh * (int)sizeof(T) / 16 - 1);
     }
   }
   // rows row0 .. row0 + 31 of `base`, row0 + left the first that is not there (left >= 1)
@@ -478,10 +478,10 @@ template <typename T, int DP> struct Dma {
     const unsigned own = (unsigned)(lane / G::CH);
     if (left >= 32) {
 #pragma unroll
-      for (int u = 0; u < NI; ++u) dma16(own * ldb + chunk[u % NV], b + (uint64_t)(u * RPI) * step, dst + u * 1024);
+      for (int u = 0; u < NI; ++u) dma16(off[u % NV], b + (uint64_t)(u * RPI) * step, dst + u * 1024);
     } else {
 #pragma unroll
-      for (int u = 0; u < NI; ++u) dma16(min(own + u * RPI, (unsigned)left - 1u) * ldb + chunk[u % NV], b, dst + u * 1024);
+      for (int u = 0; u < NI; ++u) dma16(off[u % NV] + (min(own + u * RPI, (unsigned)left - 1u) - own) * ldb, b, dst + u * 1024);
     }
   }
 };
