@@ -7,111 +7,6 @@ namespace nmtgan {
 
 // dq.  delta of rows whose workgroup's spans fit in SHORT keys is summed from p dp in a first pass over the same tiles: there
 // p is large, and the rounding of `out` would show in it; long spans average it away and take delta from span_prep_kernel.
-constexpr int SPAN_SHORT = 256;
-template <typename T, int DP, int KT, int NW, bool EXTRA>
-__global__ __launch_bounds__(64 * NW) void span_dq_kernel(SpanParams p) {
-  using G = Geo<T, DP>;
-  constexpr int TB = KT * G::RB, NT = 64 * NW;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ int red[NW][2];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int h = blockIdx.x % p.heads, tiles = gridDim.x / p.heads, tile = tiles - 1 - blockIdx.x / p.heads;
-  const int kvh = h / (p.heads / p.kv_heads);
-  const int i = (tile * NW + w) * 32 + (lane & 31), ic = min(i, p.M - 1);
-  const bool ok = i < p.M;
-  const int2 sp = ok ? span_of(p, i) : make_int2(0, 0);
-  const WaveSpan ws = wave_span(sp);
-  const int2 bs = block_span<NW>(ws, red, w);
-  const T* K = (const T*)p.k + kvh * p.dh;
-  const T* V = (const T*)p.v + kvh * p.dh;
-  uint4 own[G::STEPS], dout[G::STEPS];
-  load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
-  load_own<T, DP>((const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh, ok, p.dh, lane, dout);
-  float* const at = delta_at(p, ic, h);
-  const float lse2 = at[-32], sc2 = p.scale * LOG2E;
-  float delta = at[0];
-  float slope = 0.f, inv_cap = 0.f;
-  int pos = 0;
-  if constexpr (EXTRA) {
-    if (p.slopes) { slope = p.slopes[h]; pos = pos_of(p, ic); }
-    if (p.cap > 0.f) inv_cap = 1.f / p.cap;
-  }
-  f32x16_t acc[G::DB];
-  clear(acc);
-  const unsigned len = (unsigned)(sp.y - sp.x);
-
-  Stage<T, DP, KT, NT> sk, sv;
-  const int nt = bs.y > bs.x ? (bs.y - bs.x + KT - 1) / KT : 0;
-  const int passes = bs.y - bs.x <= SPAN_SHORT ? 2 : 1, total = nt * passes;
-  float sum = 0.f;
-  if (total > 0) {
-    sk.load(K, p.ldk, bs.x, bs.y, p.dh, tid);
-    sv.load(V, p.ldv, bs.x, bs.y, p.dh, tid);
-    sk.store(smem, tid);
-    sv.store(smem + 2 * TB, tid);
-  }
-  __syncthreads();
-  for (int it = 0; it < total; ++it) {
-    const int t = it < nt ? it : it - nt, j0 = bs.x + t * KT;
-    const bool first = passes == 2 && it < nt;
-    if (it + 1 < total) {
-      const int jn = it + 1 == nt ? bs.x : j0 + KT;
-      sk.load(K, p.ldk, jn, bs.y, p.dh, tid);
-      sv.load(V, p.ldv, jn, bs.y, p.dh, tid);
-    }
-    if (passes == 2 && it == nt) {
-      delta = both_halves_sum(sum);
-      if (ok && lane < 32) at[0] = sp.y > sp.x ? delta : 0.f;
-    }
-    if (j0 < ws.hi && j0 + KT > ws.lo) {
-      const unsigned char* tk = smem + (it & 1) * TB;
-      const unsigned char* tv = smem + (2 + (it & 1)) * TB;
-      const bool whole = j0 >= ws.all_lo && j0 + KT <= ws.all_hi;
-#pragma unroll
-      for (int kb = 0; kb < KT / 32; ++kb) {
-        f32x16_t s = score_block<T, DP>(tk, kb, own, lane);
-        f32x16_t d = score_block<T, DP>(tv, kb, dout, lane);
-        const int base = j0 + 32 * kb + 4 * (lane >> 5);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = base + 8 * (r >> 2) + (r & 3);
-          float turn = 1.f, x;
-          if constexpr (EXTRA) x = score2<T>(p, s[r], inv_cap, slope, pos, j, turn) - lse2;
-          else x = fmaf(s[r], sc2, -lse2);
-          float pe = __builtin_amdgcn_exp2f(x), ds = pe * (d[r] - (first ? 0.f : delta));
-          if (EXTRA && !first) ds *= turn;
-          if (!whole) ds = (unsigned)(j - sp.x) < len ? ds : 0.f;
-          s[r] = ds;
-        }
-        if (first) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sum += s[r];
-        } else {
-          accum_block<T, DP>(tk, kb, s, acc, lane);
-        }
-      }
-    }
-    if (it + 1 < total) {
-      sk.store(smem + ((it + 1) & 1) * TB, tid);
-      sv.store(smem + (2 + ((it + 1) & 1)) * TB, tid);
-    }
-    __syncthreads();
-  }
-  const bool some = sp.y > sp.x;
-  const unsigned long long bad = __ballot(some && !all_finite(acc));
-  if (ok && !((bad >> (lane & 31) | bad >> ((lane & 31) + 32)) & 1)) {
-    if (!some) clear(acc);
-    store_own<T, DP>((T*)p.dq + (int64_t)i * p.ld_dq + h * p.dh, acc, p.scale, p.dh, lane);
-  }
-  if (bad) {
-    __threadfence_block();
-    float* x = reinterpret_cast<float*>(smem + 4 * TB) + w * 2 * SPAN_MAX_DH;
-    for (unsigned left = (unsigned)bad | (unsigned)(bad >> 32); left; left &= left - 1)
-      span_dq_row<T>(p, (tile * NW + w) * 32 + __builtin_ctz(left), h, x, x + SPAN_MAX_DH, lane);
-  }
-}
-
-
 template <typename T, int DP, int KW, bool EXTRA>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_dq_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
@@ -119,14 +14,22 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   constexpr int REGION = 3 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // two K tiles and one V tile per wave
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_sum[KW][32], xs[KW][2][SPAN_MAX_DH];
-  __shared__ int bad[32];
+  __shared__ int bad[32], s_hull[KW];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = blockIdx.x % p.heads, tile = gridDim.x / p.heads - 1 - blockIdx.x / p.heads;
+  const int h = blockIdx.x % p.heads, last = gridDim.x / p.heads - 1;
   const int kvh = h / (p.heads / p.kv_heads);
+  int tile = last - (int)(blockIdx.x / p.heads);
+  const bool solo = p.solo && group_is_short<KW>(p, tile / KW * KW, s_hull, w, lane);
+  if (solo) {
+    const int group = tile / KW;                  // (not always its first: workgroups go round the shader engines by index)
+    if (tile % KW != group % KW) return;
+    tile = group * KW + w;
+  }
   const int i = tile * 32 + (lane & 31), ic = min(i, p.M - 1);
   const bool ok = i < p.M;
   const int2 sp = ok ? span_of(p, i) : make_int2(0, 0);
   const WaveSpan ws = wave_span(sp);
+  const int t0 = solo ? 0 : w, dt = solo ? 1 : KW;
   const T* K = (const T*)p.k + kvh * p.dh;
   const T* V = (const T*)p.v + kvh * p.dh;
   unsigned char* mine = smem + w * REGION;
@@ -154,22 +57,22 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   float sum = 0.f;
   auto walk = [&](auto FIRST) {                   // FIRST: sum p dp only
     constexpr bool first_pass = decltype(FIRST)::value;
-    if (w < nt) {
-      issue_k(w, 0);
-      issue_v(w);
+    if (t0 < nt) {
+      issue_k(t0, 0);
+      issue_v(t0);
     }
-    if (w + KW < nt) issue_k(w + KW, 1);
+    if (t0 + dt < nt) issue_k(t0 + dt, 1);
     int buf = 0;
-    for (int t = w; t < nt; t += KW, buf ^= 1) {
+    for (int t = t0; t < nt; t += dt, buf ^= 1) {
       const int j0 = ws.lo + 32 * t;
-      if (t + KW < nt) wait_dma<D::NI>();         // the next K may still be under way
+      if (t + dt < nt) wait_dma<D::NI>();         // the next K may still be under way
       else wait_dma<0>();
       const unsigned char* tk = mine + buf * D::BYTES;
       f32x16_t s = score_block<T, DP>(tk, 0, own, lane), turn;
       f32x16_t d = score_block<T, DP>(mine + 2 * D::BYTES, 0, dout, lane);
-      if (t + KW < nt) {
+      if (t + dt < nt) {
         wait_lds();
-        issue_v(t + KW);
+        issue_v(t + dt);
       }
       if (__any(sp.x < j0 + 32 && sp.y > j0)) {
         const int first = j0 + 4 * (lane >> 5);
@@ -208,23 +111,40 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
           accum_block<T, DP>(tk, 0, s, acc, lane);
         }
       }
-      if (t + 2 * KW < nt) {
+      if (t + 2 * dt < nt) {
         wait_lds();
-        issue_k(t + 2 * KW, buf);
+        issue_k(t + 2 * dt, buf);
       }
     }
   };
   if (nt * 32 <= SPAN_SHORT) {
     walk(std::integral_constant<bool, true>{});
     sum = both_halves_sum(sum);
-    if (lane < 32) s_sum[w][lane] = sum;
-    __syncthreads();
-    delta = s_sum[0][lane & 31];
+    if (solo) {
+      delta = sum;
+    } else {
+      if (lane < 32) s_sum[w][lane] = sum;
+      __syncthreads();
+      delta = s_sum[0][lane & 31];
 #pragma unroll
-    for (int k = 1; k < KW; ++k) delta += s_sum[k][lane & 31];
-    if (ok && tid < 32) at[0] = sp.y > sp.x ? delta : 0.f;
+      for (int k = 1; k < KW; ++k) delta += s_sum[k][lane & 31];
+    }
+    if (ok && lane < 32 && (solo || w == 0)) at[0] = sp.y > sp.x ? delta : 0.f;
   }
   walk(std::integral_constant<bool, false>{});
+  if (solo) {
+    const bool some = sp.y > sp.x;
+    const unsigned long long off = __ballot(some && !all_finite(acc));
+    const unsigned again = (unsigned)off | (unsigned)(off >> 32);
+    if (ok && !(again >> (lane & 31) & 1)) {
+      if (!some) clear(acc);
+      store_own<T, DP>((T*)p.dq + (int64_t)i * p.ld_dq + h * p.dh, acc, p.scale, p.dh, lane);
+    }
+    __threadfence_block();
+    for (unsigned left = again; left; left &= left - 1)
+      span_dq_row<T>(p, tile * 32 + __builtin_ctz(left), h, xs[w][0], xs[w][1], lane);
+    return;
+  }
   if (tid < 32) bad[tid] = 0;
   join_write<DP>(reinterpret_cast<float*>(mine), acc, 1.f, lane);
   __syncthreads();
@@ -251,28 +171,13 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
     if (bad[row]) span_dq_row<T>(p, tile * 32 + row, h, xs[w][0], xs[w][1], lane);
 }
 
-template <typename T, int DP, int NW>
-static int launch_dq(const SpanParams& p, hipStream_t st) {
-  constexpr int RT = NW == 1 || Geo<T, DP>::RB > 128 ? 32 : 64;
-  constexpr size_t smem = (size_t)4 * RT * Geo<T, DP>::RB + NW * 2 * SPAN_MAX_DH * sizeof(float);
-  const int64_t grid = ((int64_t)p.M + 32 * NW - 1) / (32 * NW) * p.heads;
-  NMTGAN_REQUIRE(grid < (1LL << 31), "attn_span_dq: too many rows");
-  // no cap, no slopes: the score is the scaled product itself
-  if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
-    NMTGAN_TRY(raise_lds(&span_dq_kernel<T, DP, RT, NW, true>, smem, "attn_span_dq"));
-    hipLaunchKernelGGL((span_dq_kernel<T, DP, RT, NW, true>), dim3((unsigned)grid), dim3(64 * NW), smem, st, p);
-  } else {
-    NMTGAN_TRY(raise_lds(&span_dq_kernel<T, DP, RT, NW, false>, smem, "attn_span_dq"));
-    hipLaunchKernelGGL((span_dq_kernel<T, DP, RT, NW, false>), dim3((unsigned)grid), dim3(64 * NW), smem, st, p);
-  }
-  NMTGAN_CHECK_LAUNCH("attn_span_dq");
-  return 0;
-}
 template <typename T, int DP>
-static int launch_dq_split(const SpanParams& p, hipStream_t st) {
+static int launch_dq(SpanParams p, hipStream_t st) {
   constexpr int KW = Geo<T, DP>::RB > 256 ? 2 : 4;
   constexpr size_t smem = (size_t)KW * 3 * Dma<T, DP>::BYTES;
-  const int64_t grid = ((int64_t)p.M + 31) / 32 * p.heads;
+  const int64_t grid = ((int64_t)p.M + 32 * KW - 1) / (32 * KW) * KW * p.heads;
+  NMTGAN_REQUIRE(grid < (1LL << 31), "attn_span_dq: too many rows");
+  p.solo = grid > SPAN_FEW;
   if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
     NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, true>, smem, "attn_span_dq"));
     hipLaunchKernelGGL((span_dq_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
@@ -283,15 +188,11 @@ static int launch_dq_split(const SpanParams& p, hipStream_t st) {
   NMTGAN_CHECK_LAUNCH("attn_span_dq");
   return 0;
 }
-template <typename T, int DP>
-static int choose_dq(const SpanParams& p, hipStream_t st) {
-  return ((int64_t)p.M + 31) / 32 * p.heads <= SPAN_FEW ? launch_dq_split<T, DP>(p, st) : launch_dq<T, DP, 4>(p, st);
-}
 int span_dq_tiles(int dtype, const SpanParams& p, hipStream_t st) {
   NMTGAN_DISPATCH_GRAD(dtype, T, {
-    if (p.dh <= 32) return choose_dq<T, 32>(p, st);
-    if (p.dh <= 64) return choose_dq<T, 64>(p, st);
-    return choose_dq<T, 128>(p, st);
+    if (p.dh <= 32) return launch_dq<T, 32>(p, st);
+    if (p.dh <= 64) return launch_dq<T, 64>(p, st);
+    return launch_dq<T, 128>(p, st);
   });
   return 0;
 }

@@ -32,6 +32,7 @@ struct SpanParams {
   void* out; float* lse;
   int M, N, heads, kv_heads, dh;
   float scale, cap;
+  int solo;                                      // a wave may walk a short span alone
   // gradients
   const void* dout; int64_t ld_do;
   void* dq; void* dk; void* dv;
@@ -307,29 +308,6 @@ __device__ __forceinline__ void accum_block(const unsigned char* tile, int kb, c
   }
 }
 
-// rows [row0, row0 + R) of a [*][ld] matrix on their way to LDS through registers; rows from `end` on and columns from dh
-// on are zeros
-template <typename T, int DP, int R, int NT> struct Stage {
-  using G = Geo<T, DP>;
-  static constexpr int N = R * G::CH / NT;
-  static_assert(R * G::CH % NT == 0, "whole chunks per thread");
-  uint4 x[N];
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int end, int dh, int tid) {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int idx = tid + u * NT, row = row0 + idx / G::CH, c = idx % G::CH;
-      const bool ok = row < end && c * (16 / (int)sizeof(T)) < dh;
-      x[u] = ok ? *reinterpret_cast<const uint4*>(base + (int64_t)row * ld + c * (16 / (int)sizeof(T))) : make_uint4(0, 0, 0, 0);
-    }
-  }
-  __device__ __forceinline__ void store(unsigned char* tile, int tid) const {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int idx = tid + u * NT;
-      *reinterpret_cast<uint4*>(tile + G::swz(idx / G::CH, idx % G::CH)) = x[u];
-    }
-  }
-};
 // own row as the B operand of score_block
 template <typename T, int DP>
 __device__ __forceinline__ void load_own(const T* row, bool ok, int dh, int lane, uint4 (&own)[Geo<T, DP>::STEPS]) {
@@ -411,22 +389,26 @@ __device__ __forceinline__ WaveSpan wave_span(int2 sp) {
   return WaveSpan{__builtin_amdgcn_readfirstlane(a), __builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(c),
                   __builtin_amdgcn_readfirstlane(d)};
 }
-// hull over the workgroup's waves
-template <int NW>
-__device__ __forceinline__ int2 block_span(const WaveSpan& ws, int (*red)[2], int w) {
-  if constexpr (NW == 1) return make_int2(ws.lo, ws.hi);
-  if ((threadIdx.x & 63) == 0) { red[w][0] = ws.lo; red[w][1] = ws.hi; }
+constexpr int SPAN_SHORT = 256;
+// whether the spans of none of KW consecutive blocks of 32 rows reach over more than SPAN_SHORT keys
+template <int KW>
+__device__ __forceinline__ bool group_is_short(const SpanParams& p, int first, int* hull, int w, int lane) {
+  const int i = (first + w) * 32 + (lane & 31);
+  const WaveSpan ws = wave_span(i < p.M ? span_of(p, i) : make_int2(0, 0));
+  if (lane == 0) hull[w] = ws.hi > ws.lo ? ws.hi - ws.lo : 0;
   __syncthreads();
-  int a = 0x7fffffff, b = 0;
+  int n = 0;
 #pragma unroll
-  for (int k = 0; k < NW; ++k) { a = min(a, red[k][0]); b = max(b, red[k][1]); }
-  return make_int2(a, b);
+  for (int k = 0; k < KW; ++k) n = max(n, hull[k]);
+  return __builtin_amdgcn_readfirstlane(n) <= SPAN_SHORT;
 }
-
 
 // ------------------------------------------------------------------------------------------ split form
 // The KW waves of a workgroup share their own 32 rows and take every KW-th 32-row tile of the other side, each into LDS of
-// its own by DMA two tiles ahead - no barrier inside the walk - and are joined at the end.
+// its own by DMA ahead of its use - no barrier inside the walk - and are joined at the end.  Where a launch has workgroups
+// enough without that (more than SPAN_FEW blocks of 32 rows) and the spans of KW neighbouring blocks are short, one
+// workgroup takes all KW, a wave each ("solo"), and the others leave: sentences of at most 50 tokens would give each of
+// four waves less than a tile.
 // Scalar base + one 32-bit lane offset per swizzle period; chunks behind dh and rows behind the last repeat a valid one
 // (they meet zeros of the own rows or weights of zero).
 // a pointer / offset that is the same in every lane, in scalar registers
@@ -546,8 +528,7 @@ static inline int raise_lds(F* kernel, size_t bytes, const char* what) {
                      hipSuccess, "%s: cannot raise the dynamic LDS limit", what);
   return 0;
 }
-// Blocks of 32 rows that a launch has in all: up to SPAN_FEW the waves of a workgroup split the walk of one block (split
-// form); above, four blocks share the tiles they stage.
+// Blocks of 32 rows (times heads) from which waves may walk alone: two workgroups of four waves on every SIMD.
 constexpr int64_t SPAN_FEW = 2048;
 
 int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st);

@@ -78,6 +78,19 @@ def test_span_documents(cuda, op, rows, longest, kind, heads, kv_heads, dh, cap,
     _span_case(cuda, _ops(), TYPES[op], lo, hi, rows, heads, kv_heads, dh, cap, bias, seed=rows)
 
 
+@pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("heads,kv_heads,dh,longest,kind,cap,bias", [
+    (64, 64, 64, 50, "causal", 0.0, False), (64, 64, 8, 50, "prefix", 3.0, True), (72, 72, 128, 30, "document", 0.0, True),
+    (128, 64, 32, 40, "causal", 0.0, False), (64, 64, 16, 600, "causal", 0.0, False)])
+def test_span_many_blocks(cuda, op, heads, kv_heads, dh, longest, kind, cap, bias):
+    """Launches with so many blocks of rows that waves walk short spans alone; a long document among them does not."""
+    lo, hi = _documents(1100, longest, kind, heads + dh)
+    if longest < 100:
+        lo, hi = lo[:700] + [700] * 400, hi[:700] + [700 + i + 1 for i in range(400)]
+        hi = [min(h, 700) if i < 700 else h for i, h in enumerate(hi)]
+    _span_case(cuda, _ops(), TYPES[op], lo, hi, 1100, heads, kv_heads, dh, cap, bias, seed=dh)
+
+
 @pytest.mark.parametrize("op", ["bf16", "fp32"])
 @pytest.mark.parametrize("m,n", [(1, 1), (1, 200), (200, 1), (3, 0), (0, 5), (77, 500), (500, 77), (1025, 1300)])
 def test_span_shapes_and_cross_attention(cuda, op, m, n):
@@ -132,44 +145,46 @@ def test_span_outputs_given_and_rows_behind(cuda, op):
 
 @pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf")])
-def test_span_unseen_rows_may_hold_anything(cuda, op, poison):
+@pytest.mark.parametrize("heads,m", [(2, 200), (64, 1100)])
+def test_span_unseen_rows_may_hold_anything(cuda, op, poison, heads, m):
     """Padding rows between documents (seen by nobody) and query rows that see nothing hold NaN or infinities."""
     ops, dt = _ops(), TYPES[op]
     g = torch.Generator().manual_seed(6)
-    m, docs = 200, [(0, 37), (50, 64), (64, 65), (70, 150), (150, 190)]
+    docs = [(0, 37), (50, 64), (64, 65), (70, 150), (150, 190)]
     lo, hi = [0] * m, [0] * m
     for a, b in docs:
         for i in range(a, b):
             lo[i], hi[i] = a, i + 1
-    q, k, v, do = (_normal(g, m, 128, dt=dt).to(cuda) for _ in range(4))
+    q, k, v, do = (_normal(g, m, heads * 64, dt=dt).to(cuda) for _ in range(4))
     off = torch.tensor([h == 0 for h in hi], device=cuda)
     lo, hi = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (lo, hi))
-    want = span_reference(q, k, v, lo, hi, 2, 2, 0.125, dout=do)
+    want = span_reference(q, k, v, lo, hi, heads, heads, 0.125, dout=do)
     for t in (q, k, v, do):
         t[off] = poison
-    out, lse = ops.attn_span(q, k, v, lo, hi, heads=2, scale=0.125)
+    out, lse = ops.attn_span(q, k, v, lo, hi, heads=heads, scale=0.125)
     check("out", out, want["out"])
     check("lse", lse, want["lse"])
-    check("step", ops.attn_span_step(q, k, v, lo, hi, heads=2, scale=0.125, max_keys=80), want["out"])
+    check("step", ops.attn_span_step(q, k, v, lo, hi, heads=heads, scale=0.125, max_keys=80), want["out"])
     if dt != torch.float16:
-        for name, x in zip(("dq", "dk", "dv"), ops.attn_span_grads(do, q, k, v, out, lse, lo, hi, heads=2, scale=0.125)):
+        for name, x in zip(("dq", "dk", "dv"), ops.attn_span_grads(do, q, k, v, out, lse, lo, hi, heads=heads, scale=0.125)):
             check(name, x, want[name])
 
 
 @pytest.mark.parametrize("op", ["bf16", "fp32"])
 @pytest.mark.parametrize("where", ["q", "k", "v", "dout"])
-def test_span_nan_reaches_its_own_document_only(cuda, op, where):
+@pytest.mark.parametrize("heads,m", [(2, 160), (64, 1100)])
+def test_span_nan_reaches_its_own_document_only(cuda, op, where, heads, m):
     ops, dt = _ops(), TYPES[op]
     g = torch.Generator().manual_seed(7)
-    lo, hi = _documents(160, 30, "document", 3, tail=0)
-    bad = next(i for i in range(60, 160) if hi[i] - lo[i] > 3)
+    lo, hi = _documents(m, 30, "document", 3, tail=0)
+    bad = next(i for i in range(60, m) if hi[i] - lo[i] > 3)
     mine = torch.tensor([a == lo[bad] for a in lo], device=cuda)
-    t = {n: _normal(g, 160, 128, dt=dt).to(cuda) for n in ("q", "k", "v", "dout")}
+    t = {n: _normal(g, m, heads * 64, dt=dt).to(cuda) for n in ("q", "k", "v", "dout")}
     lo, hi = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (lo, hi))
-    want = span_reference(t["q"], t["k"], t["v"], lo, hi, 2, 2, 0.125, dout=t["dout"])
+    want = span_reference(t["q"], t["k"], t["v"], lo, hi, heads, heads, 0.125, dout=t["dout"])
     t[where][bad] = float("nan")
-    out, lse = ops.attn_span(t["q"], t["k"], t["v"], lo, hi, heads=2, scale=0.125)
-    got = dict(zip(("dq", "dk", "dv"), ops.attn_span_grads(t["dout"], t["q"], t["k"], t["v"], out, lse, lo, hi, heads=2, scale=0.125)))
+    out, lse = ops.attn_span(t["q"], t["k"], t["v"], lo, hi, heads=heads, scale=0.125)
+    got = dict(zip(("dq", "dk", "dv"), ops.attn_span_grads(t["dout"], t["q"], t["k"], t["v"], out, lse, lo, hi, heads=heads, scale=0.125)))
     got.update(out=out, lse=lse)
     for name, x in got.items():
         check(name, x[~mine], (want[name][0][~mine], want[name][1][~mine]))
