@@ -141,10 +141,10 @@ __device__ __forceinline__ int64_t a_row_offset(const GemmParams& p, int r) {
                          : (int64_t)r * p.lda_b;
 }
 
-// Cross-entropy epilogues.  The product runs transposed like the STATS form: C rows = vocabulary entries, C columns =
-// hidden rows, so one hidden row's 64 logits of a wave tile sit in 16 registers of each of four lanes.
-// XSTAT: stats[vtile][row] = (max, sum exp(z - max)) over the entries of a 64-entry tile that exist, and with smoothing
-// their plain sum in zsum[vtile][row].
+// Cross-entropy epilogues.
+// XSTAT: the product runs transposed like the STATS form, C rows = vocabulary entries and C columns = hidden rows, so one
+// hidden row's 64 logits of a wave tile sit in 16 registers of each of four lanes: stats[vtile][row] = (max, sum exp(z -
+// max)) over the entries of a 64-entry tile that exist, and with smoothing their plain sum in zsum[vtile][row].
 template <int MT>
 __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
   const int fc = lane & 15, fq = lane >> 4;
@@ -152,113 +152,107 @@ __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)
   for (int ip = 0; ip < MT / 4; ++ip) {
     const int mb = m0 + 64 * ip;
     if (mb >= p.M) continue;
-    const bool whole = mb + 64 <= p.M;
+    if (mb + 64 > p.M) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = n0 + j * 16 + fc;
-      float mx = -INFINITY, zs = 0.f;
-#pragma unroll
-      for (int i = 4 * ip; i < 4 * ip + 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (!whole && m0 + i * 16 + 4 * fq + e >= p.M) acc[i][j][e] = -INFINITY;
-          mx = fmaxf(mx, acc[i][j][e]);
-        }
-      mx = groups4_max(mx);
-      const float mu = mx == -INFINITY ? 0.f : mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 4 * ip; i < 4 * ip + 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((acc[i][j][e] - mu) * 1.44269504088896341f);
-      sum = groups4_sum(sum);
-      if (p.x.zsum) {
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 4 * ip; i < 4 * ip + 4; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (whole || m0 + i * 16 + 4 * fq + e < p.M) zs += acc[i][j][e];
+            if (m0 + i * 16 + 4 * fq + e >= p.M) acc[i][j][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = n0 + j * 16 + fc;
+      float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[i][j][e]);
+      mx = groups4_max(mx);
+      const float mu2 = mx == -INFINITY ? 0.f : mx * 1.44269504088896341f;
+#pragma unroll
+      for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -mu2));
+      sum = groups4_sum(sum);
+      const int64_t at = (int64_t)((m0 >> 6) + ip) * p.N + row;
+      if (fq == 0 && row < p.N) p.stats[at] = make_float2(mx, sum);
+      if (p.x.zsum) {
+        float zs = 0.f;
+        if (mb + 64 > p.M) {
+#pragma unroll
+          for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zs += m0 + i * 16 + 4 * fq + e < p.M ? acc[i][j][e] : 0.f;
+        } else {
+#pragma unroll
+          for (int i = 4 * ip; i < 4 * ip + 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zs += acc[i][j][e];
+        }
         zs = groups4_sum(zs);
-      }
-      if (fq == 0 && row < p.N) {
-        const int64_t at = (int64_t)((m0 >> 6) + ip) * p.N + row;
-        p.stats[at] = make_float2(mx, sum);
-        if (p.x.zsum) p.x.zsum[at] = zs;
+        if (fq == 0 && row < p.N) p.x.zsum[at] = zs;
       }
     }
   }
 }
 
-// XGRAD: acc <- the part of d(logit) that differs from entry to entry, coef (exp(z - lse) - high [entry == label]), zero
-// where no row or entry is (the images are padded to whole k-tiles) - the constant -coef low is added in fp32 to the sums it
-// ends up in, where its rounding to 16 bits would add up.
-template <int MT>
-__device__ __forceinline__ void xgrad_values(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int lane, const float (&coef)[4],
-                                             const float (&lse2)[4], const int (&label)[4]) {
-  const int fq = lane >> 4;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        acc[i][j][e] = coef[j] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[j]));
-    if (__any(coef[j] == 0.f)) {                   // rows without a label: 0 whatever their logits are
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = coef[j] == 0.f ? 0.f : acc[i][j][e];
-    }
-    const int at = label[j] - m0;                  // few wave tiles hold the label of one of their columns
-    if (__any(at >= 0 && at < 16 * MT)) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at == 16 * i + 4 * fq + e) acc[i][j][e] -= coef[j] * p.x.high;
-    }
-  }
-  if (m0 + 16 * MT > p.M) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (m0 + 16 * i + 4 * fq + e >= p.M) acc[i][j][e] = 0.f;
-  }
-}
-// ... and its images: entry-major gt (rows contiguous) and, if asked for, row-major g
+// XGRAD: C rows = hidden rows, C columns = entries, so a lane holds four consecutive rows of one entry = 8 bytes of the
+// entry-major image gt.  d(logit) = coef (exp(z - lse) - high [entry == label]), zero where no row or entry is (the images
+// are padded to whole k-tiles); the constant -coef low of label smoothing is added in fp32 to the sums it ends up in, where
+// its rounding to 16 bits would add up.  Rows without a label have coef 0 and are 0 whatever their logits are.
+// rowv: the wave tile's rows as [coef | lse / ln 2 | label] of 16 MT each (LDS); null: from memory.
 template <typename OpT, int MT>
-__device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
+__device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane,
+                                               const float* rowv = nullptr) {
   const int fc = lane & 15, fq = lane >> 4;
   const XentEpilogue& x = p.x;
-  float coef[4], lse2[4];
-  int label[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = min(n0 + j * 16 + fc, x.rows_padded - 1);
-    coef[j] = x.coef[row];
-    lse2[j] = x.lse2[row];
-    label[j] = x.label[row] - x.first;
-  }
-  xgrad_values<MT>(p, acc, m0, lane, coef, lse2, label);
+  for (int i = 0; i < MT; ++i) {
+    const int mb = m0 + 16 * i + 4 * fq;
+    if (m0 + 16 * i >= x.rows_padded) continue;    // rows_padded is a multiple of 64
+    const float* at = rowv ? rowv + 16 * i + 4 * fq : x.coef + mb;
+    const int64_t step = rowv ? 16 * MT : x.lse2 - x.coef;
+    float coef[4], lse2[4];
+    VecIO<float, 4>::load(at, coef);
+    VecIO<float, 4>::load(at + step, lse2);
+    const int4 lab = *reinterpret_cast<const int4*>(rowv ? reinterpret_cast<const int32_t*>(at + 2 * step) : x.label + mb);
+    const int label[4] = {lab.x - x.first, lab.y - x.first, lab.z - x.first, lab.w - x.first};
+    bool hit = false, none = false;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = n0 + j * 16 + fc;
-    if (row >= x.rows_padded) continue;
+    for (int e = 0; e < 4; ++e) {
+      hit = hit || (unsigned)(label[e] - n0) < 64u;
+      none = none || coef[e] == 0.f;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int mb = m0 + i * 16 + 4 * fq;
-      if (mb >= x.piece_padded) continue;
-      OpT* outt = reinterpret_cast<OpT*>(x.gt) + (int64_t)mb * x.rows_padded + row;
-      float d[4];
+      for (int j = 0; j < 4; ++j)
+        acc[i][j][e] = coef[e] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[e]));
+    }
+    if (__any(hit)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        d[e] = acc[i][j][e];
-        OpTraits<OpT>::store(outt + (int64_t)e * x.rows_padded, d[e]);
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n0 + 16 * j + fc == label[e]) acc[i][j][e] -= coef[e] * x.high;
+    }
+    if (__any(none)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = coef[e] == 0.f ? 0.f : acc[i][j][e];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int entry = n0 + 16 * j + fc;
+      if (entry >= x.piece_padded) continue;
+      float d[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (entry >= p.N) d[0] = d[1] = d[2] = d[3] = 0.f;
+      VecIO<OpT, 4>::store(reinterpret_cast<OpT*>(x.gt) + (int64_t)entry * x.rows_padded + mb, d);
+      if (x.g) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (mb + e < p.M) OpTraits<OpT>::store(reinterpret_cast<OpT*>(x.g) + (int64_t)(mb + e) * x.piece_padded + entry, d[e]);
       }
-      if (x.g && row < p.N) VecIO<OpT, 4>::store(reinterpret_cast<OpT*>(x.g) + (int64_t)row * x.piece_padded + mb, d);
     }
   }
 }
@@ -740,8 +734,8 @@ static int launch_pipe(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + PBM - 1) / PBM;
-  p.ntn = (p.N + PBN - 1) / PBN;
+  p.ntm = (p.M + PBM - 1) / PBM;
+  p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + PBN - 1) / PBN;
   p.group_m = 2;                                 // tile order knob (L2 sharing of A panels vs Wt tiles); 1-4 measured best
   if (const char* e = getenv("NMTGAN_GEMM_GM")) p.group_m = atoi(e);
   if constexpr (EPI == NMTGAN_EPI_LINEAR) {
@@ -1078,7 +1072,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   // per-column epilogue values of the wave's 64 columns, LDS-DMA'd at the start of the tile's last k-step:
   // they ride the same in-order vmcnt stream as the tile DMAs and the epilogue needs no vector load (which
   // the compiler would wait vmcnt(0) for, draining the prefetch of the next tile)
-  constexpr int QEV = 2 * QSTAGE + 8 * 2048, QEVW = EPI == EPI_XGRAD ? 1024 : 512;
+  constexpr int QEV = 2 * QSTAGE + 8 * 2048, QEVW = EPI == EPI_XGRAD ? 1536 : 512;
   const float* ev = reinterpret_cast<const float*>(smem + QEV + wave * QEVW);
   const bool use_ev = (EPI == NMTGAN_EPI_LINEAR && p.bias != nullptr) || EPI == NMTGAN_EPI_CONVMAX;
   auto stage_ev = [&](int ord) {
@@ -1091,11 +1085,14 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     } else if constexpr (EPI == NMTGAN_EPI_CONVMAX) {
       glds4(p.scale + n, dst);
       glds4(p.shift + n, dst + 256);
-    } else if constexpr (EPI == EPI_XGRAD) {
-      const int r = min(tn * QBN + wc * 64 + lane, p.x.rows_padded - 1);
-      glds4(p.x.coef + r, dst);
-      glds4(p.x.lse2 + r, dst + 256);
-      glds4(p.x.label + r, dst + 512);
+    } else if constexpr (EPI == EPI_XGRAD) {       // the wave's 128 rows
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = min(tm * QBM + wr * 128 + 64 * k + lane, p.x.rows_padded - 1);
+        glds4(p.x.coef + r, dst + 256 * k);
+        glds4(p.x.lse2 + r, dst + 512 + 256 * k);
+        glds4(p.x.label + r, dst + 1024 + 256 * k);
+      }
     }
   };
 
@@ -1233,21 +1230,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     if constexpr (EPI == EPI_STATS) {
       epilogue_stats<8>(p, acc, m0, n0, lane);
     } else if constexpr (EPI == EPI_XGRAD) {
-      float coef[4], lse2[4];
-      int label[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        coef[j] = ev[j * 16 + fc];
-        lse2[j] = ev[64 + j * 16 + fc];
-        label[j] = __float_as_int(ev[128 + j * 16 + fc]) - p.x.first;
-      }
-      xgrad_values<8>(p, acc, m0, lane, coef, lse2, label);
-      if (n0 < p.x.rows_padded) {
-        GemmParams v{};                            // whole 64-column rows of gt; rows_padded and piece_padded bound them
-        v.M = p.x.piece_padded; v.N = p.x.rows_padded; v.wide_ok = 2; v.n_seg = 1;
-        v.out[0] = p.x.gt; v.ldo[0] = p.x.rows_padded; v.seg_scale[0] = 1.f;
-        epilogue_wide<OpT, 8>(v, acc, m0, n0, lane, scr, sizeof(OpT) == 4, 0, n0);
-      }
+      epilogue_xgrad<OpT, 8>(p, acc, m0, n0, lane, ev);
     } else if constexpr (KM) {
       GemmParams v{};
       v.M = p.M; v.N = p.N; v.n_seg = 1; v.out_f32[0] = 1; v.ldo[0] = p.N; v.seg_scale[0] = 1.f;
@@ -1275,7 +1258,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
 
 template <typename OpT, int EPI>
 static int launch_p8(GemmParams p, hipStream_t st) {
-  constexpr int smem = 2 * QSTAGE + 8 * 2048 + 8 * (EPI == EPI_XGRAD ? 1024 : 512);   // 128 KiB of staging + per-wave epilogue scratch + vectors
+  constexpr int smem = 2 * QSTAGE + 8 * 2048 + 8 * (EPI == EPI_XGRAD ? 1536 : 512);   // 128 KiB of staging + per-wave epilogue scratch + vectors
   static bool attr_done = false;
   if (!attr_done) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_p8_kernel<OpT, EPI>),
@@ -1283,12 +1266,12 @@ static int launch_p8(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + QBM - 1) / QBM;
-  p.ntn = (p.N + QBN - 1) / QBN;
+  p.ntm = (p.M + QBM - 1) / QBM;
+  p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + QBN - 1) / QBN;
   // tile groups of 2 row tiles (4 are as fast); the logits GEMM (rows = vocabulary) takes 8: an XCD then keeps 2 MiB
   // of the table in its L2 and sweeps the activations twice instead of eight times - same time, a third of the
   // fetches past the L2
-  p.group_m = EPI == EPI_STATS || EPI == EPI_XSTAT || EPI == EPI_XGRAD ? 8 : 2;
+  p.group_m = EPI == EPI_STATS || EPI == EPI_XSTAT ? 8 : 2;
   if (const char* e = getenv("NMTGAN_GEMM_GM")) p.group_m = atoi(e);
   if constexpr (EPI == NMTGAN_EPI_LINEAR) {
     const int es = sizeof(OpT);
@@ -1694,8 +1677,8 @@ static int launch_glds(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + BM - 1) / BM;
-  p.ntn = (p.N + BN - 1) / BN;
+  p.ntm = (p.M + BM - 1) / BM;
+  p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + BN - 1) / BN;
   const int slices = (EPI == NMTGAN_EPI_LINEAR && p.split_k > 1) ? p.split_k : 1;
   if (slices == 1) p.split_k = 0;
   hipLaunchKernelGGL((gemm_glds_kernel<OpT, EPI, BM, BN>), dim3(p.ntm * p.ntn, slices), dim3(64 * (BM / 64) * (BN / 64)),
@@ -1741,8 +1724,8 @@ static int launch_generic(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done = true;
   }
-  p.ntm = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.M) + GBM - 1) / GBM;
-  p.ntn = (p.N + GBN - 1) / GBN;
+  p.ntm = (p.M + GBM - 1) / GBM;
+  p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + GBN - 1) / GBN;
   hipLaunchKernelGGL((gemm_kernel<OpT, EPI>), dim3(p.ntm * p.ntn), dim3(256), 4 * GTILE, st, p);
   NMTGAN_CHECK_LAUNCH("gemm");
   return 0;
@@ -1936,15 +1919,15 @@ bool gemm_stats_supported(int op_dtype, int V, int K) {
   return V % 64 == 0 && V <= 65536 && (K * es) % BKB == 0 && (K * es) / BKB >= 4;   // <= 1024 vocabulary tiles
 }
 
-// z^T = W[entries,K] . H[rows,K]^T with one of the cross-entropy epilogues; the last tiles reach over the padding of the
-// gradient's images (both extents are at most a tile beyond the product's)
+// Logits with one of the cross-entropy epilogues, forward transposed (W[entries,K] . H[rows,K]^T), gradient as they are;
+// the last tiles reach over the padding of the gradient's images
 int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
                      int K, float2* stats, const XentEpilogue& x, hipStream_t st) {
   const int es = dtype_size(op_dtype);
   GemmParams p{};
-  p.A = (const char*)W; p.W = (const char*)H;
-  p.M = entries; p.N = rows; p.K = K;
-  p.lda_b = ldw * es; p.ldw_b = ldh * es; p.kbytes = K * es;
+  p.A = (const char*)(grad ? H : W); p.W = (const char*)(grad ? W : H);
+  p.M = grad ? rows : entries; p.N = grad ? entries : rows; p.K = K;
+  p.lda_b = (grad ? ldh : ldw) * es; p.ldw_b = (grad ? ldw : ldh) * es; p.kbytes = K * es;
   p.k_inner = 1; p.k_step = BKB; p.k_jump = BKB;
   p.stats = stats;
   p.x = x;
@@ -1953,9 +1936,7 @@ int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int en
   } else if (op_dtype == NMTGAN_BF16) {
     return dispatch<bf16_t, EPI_XGRAD>(p, st);
   } else {
-    // the fp32 form needs the row-major image too, which only the scalar epilogue writes
-    if (p.kbytes % BKB == 0) return launch_glds<float, EPI_XGRAD, 128, 128>(p, st);
-    return launch_generic<float, EPI_XGRAD>(p, st);
+    return dispatch<float, EPI_XGRAD>(p, st);
   }
   return 0;
 }

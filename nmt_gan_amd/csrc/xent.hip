@@ -35,12 +35,25 @@ __global__ __launch_bounds__(256) void xent_finish_kernel(const float2* stats, c
   const int r = min(blockIdx.x * 16 + rr, M - 1);
   const int t0 = (int)((int64_t)n_tiles * q / 16), t1 = (int)((int64_t)n_tiles * (q + 1) / 16);
   float m = -INFINITY, s = 0.f, z = 0.f;
-  for (int t = t0; t < t1; ++t) {
-    const float2 a = stats[(int64_t)t * M + r];
-    const float mn = fmaxf(m, a.x), mu = mn == -INFINITY ? 0.f : mn;
-    s = s * xexp(m - mu) + a.y * xexp(a.x - mu);
+  for (int t = t0; t < t1; t += 8) {                         // eight tiles in flight
+    float2 a[8];
+    float zs[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      a[k] = t + k < t1 ? stats[(int64_t)(t + k) * M + r] : make_float2(-INFINITY, 0.f);
+      zs[k] = zsum && t + k < t1 ? zsum[(int64_t)(t + k) * M + r] : 0.f;
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mn = fmaxf(mn, a[k].x);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    s *= xexp(m - mu);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s = fmaf(a[k].y, xexp(a[k].x - mu), s);
+      z += zs[k];
+    }
     m = mn;
-    if (zsum) z += zsum[(int64_t)t * M + r];
   }
   sm[rr][q] = m;
   ss[rr][q] = s;
@@ -88,13 +101,12 @@ __global__ __launch_bounds__(256) void xent_finish_kernel(const float2* stats, c
   }
 }
 
-// out[c][r] = in[r][c] for r < R, 0 for R <= r < Rp; rows whose label names no entry count as zeros (labels may be null)
+// out[c][r] = in[r][c] for r < R, 0 for R <= r < Rp, one 64 x 64 tile; with labels, rows without one count as zeros
 template <typename T>
-__global__ __launch_bounds__(256) void xent_transpose_kernel(const T* in, int64_t ld, int R, int C, T* out, int Rp,
-                                                             const int32_t* labels, int V) {
-  __shared__ T tile[64][66];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+__device__ __forceinline__ void transpose_tile(T (&tile)[64][66], const T* in, int64_t ld, int R, int C, T* out, int Rp, int r0,
+                                               int c0, const int32_t* labels, int V) {
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = r0 + ty + 4 * i, c = c0 + tx;
     T v = T(0);
@@ -102,66 +114,115 @@ __global__ __launch_bounds__(256) void xent_transpose_kernel(const T* in, int64_
     tile[ty + 4 * i][tx] = v;
   }
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int c = c0 + ty + 4 * i, r = r0 + tx;
     if (c < C && r < Rp) out[(int64_t)c * Rp + r] = tile[tx][ty + 4 * i];
   }
 }
-
-// per-row operands of the d(logits) epilogue, padded: coef = gradient of the row's loss (0 without a label), lse / ln 2, label
-__global__ __launch_bounds__(256) void xent_rows_kernel(const int32_t* labels, const float* grad_row, const float* lse, int M,
-                                                        int Mp, int V, float* coef, float* lse2, int32_t* label) {
-  const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r >= Mp) return;
-  const bool used = r < M && labels[r] >= 0 && labels[r] < V;
-  coef[r] = used ? (grad_row ? grad_row[r] : 1.f) : 0.f;
-  lse2[r] = r < M ? lse[r] * 1.44269504088896341f : 0.f;
-  label[r] = used ? labels[r] : -1;
+template <typename T>
+__global__ __launch_bounds__(256) void xent_transpose_kernel(const T* in, int64_t ld, int R, int C, T* out, int Rp) {
+  __shared__ T tile[64][66];
+  transpose_tile<T>(tile, in, ld, R, C, out, Rp, blockIdx.x * 64, blockIdx.y * 64, nullptr, 0);
 }
 
-// Column sums behind label smoothing, whose constant -coef_r low of every d(logit) is kept out of the 16-bit images:
-// dh_r -= coef_r low sum_j w_j, dw_j -= low sum_r coef_r h_r.  part[block][d] = sums over a block's rows (weighted if coef
-// is given), added in block order by xent_colsum_finish_kernel.
-constexpr int COLSUM_BLOCKS = 256;
+// Everything the gradient needs before its first product, in one launch by roles of workgroups:
+//   - per row, padded: coef = gradient of the row's loss (0 without a label), lse / ln 2, label
+//   - h^T, zero in rows without a label and in the padding
+//   - column sums behind label smoothing, whose constant -coef_r low of every d(logit) is kept out of the 16-bit images:
+//     dh_r -= coef_r low sum_j w_j, dw_j -= low sum_r coef_r h_r.  part[block][d], added in block order afterwards
+constexpr int SUM_W = 256, SUM_H = 32;
+struct XentPrep {
+  const void* h; const void* w; int64_t ldh, ldw;
+  const int32_t* labels; const float* grad_row; const float* lse;
+  float* coef; float* lse2; int32_t* label;
+  void* ht; float* part;
+  int M, Mp, V, d, n_rows, n_turn;                 // workgroups of the first two roles
+};
+__device__ __forceinline__ float row_coef(const XentPrep& p, int r) {
+  const bool used = p.labels[r] >= 0 && p.labels[r] < p.V;
+  return used ? (p.grad_row ? p.grad_row[r] : 1.f) : 0.f;
+}
 template <typename T>
-__global__ __launch_bounds__(256) void xent_colsum_kernel(const T* x, int64_t ld, int R, int C, const float* coef, float* part) {
+__global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
+  __shared__ T tile[64][66];
   __shared__ float red[4][64];
+  int b = blockIdx.x;
+  if (b < p.n_rows) {
+    const int r = b * 256 + threadIdx.x;
+    if (r >= p.Mp) return;
+    const bool used = r < p.M && p.labels[r] >= 0 && p.labels[r] < p.V;
+    p.coef[r] = r < p.M ? row_coef(p, r) : 0.f;
+    p.lse2[r] = r < p.M ? p.lse[r] * 1.44269504088896341f : 0.f;
+    p.label[r] = used ? p.labels[r] : -1;
+    return;
+  }
+  b -= p.n_rows;
+  if (b < p.n_turn) {
+    const int across = p.Mp / 64;
+    transpose_tile<T>(tile, (const T*)p.h, p.ldh, p.M, p.d, (T*)p.ht, p.Mp, b % across * 64, b / across * 64, p.labels, p.V);
+    return;
+  }
+  b -= p.n_turn;
+  constexpr int E = 16 / (int)sizeof(T);
+  const bool of_w = b < SUM_W;
+  const T* x = (const T*)(of_w ? p.w : p.h);
+  const int64_t ld = of_w ? p.ldw : p.ldh;
+  const int R = of_w ? p.V : p.M, blk = of_w ? b : b - SUM_W, blocks = of_w ? SUM_W : SUM_H;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int r0 = (int)((int64_t)R * blockIdx.x / COLSUM_BLOCKS), r1 = (int)((int64_t)R * (blockIdx.x + 1) / COLSUM_BLOCKS);
-  for (int c0 = 0; c0 < C; c0 += 512) {            // 64 lanes x 8 columns, four rows at a time
-    const int c = c0 + 8 * tx;
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < C)
-      for (int r = r0 + ty; r < r1; r += 4) {
-        const float f = coef ? coef[r] : 1.f;
-        if (f == 0.f) continue;
+  const int r0 = (int)((int64_t)R * blk / blocks), r1 = (int)((int64_t)R * (blk + 1) / blocks);
+  for (int c0 = 0; c0 < p.d; c0 += 64 * E) {       // 64 lanes x 16 bytes, four rows at a time
+    const int c = c0 + E * tx;
+    float s[E];
 #pragma unroll
-        for (int h = 0; h < 8; h += 16 / (int)sizeof(T)) {
-          if (c + h >= C) break;
-          float v[16 / (int)sizeof(T)];
-          VecIO<T, 16 / (int)sizeof(T)>::load(x + (int64_t)r * ld + c + h, v);
+    for (int e = 0; e < E; ++e) s[e] = 0.f;
+    if (c < p.d) {
+      constexpr int U = 4;
+      for (int r = r0 + ty; r < r1; r += 4 * U) {
+        float v[U][E], f[U];
 #pragma unroll
-          for (int e = 0; e < 16 / (int)sizeof(T); ++e) s[h + e] = fmaf(f, v[e], s[h + e]);
+        for (int u = 0; u < U; ++u) {
+          f[u] = r + 4 * u < r1 ? (of_w ? 1.f : row_coef(p, r + 4 * u)) : 0.f;
+          VecIO<T, E>::load(x + (int64_t)min(r + 4 * u, r1 - 1) * ld + c, v[u]);
         }
-      }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) s[e] += f[u] == 0.f ? 0.f : f[u] * v[u][e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
       __syncthreads();
       red[ty][tx] = s[e];
       __syncthreads();
-      if (ty == 0 && c + e < C) part[(int64_t)blockIdx.x * C + c + e] = (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
+      if (ty == 0 && c + e < p.d) p.part[(int64_t)b * p.d + c + e] = (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
     }
   }
 }
-__global__ __launch_bounds__(256) void xent_colsum_finish_kernel(const float* part, int C, float f, float* out) {
-  __shared__ float red[4][64];
+// wsum, hsum = -low times the sums of the parts, 16 threads per column
+__global__ __launch_bounds__(1024) void xent_sums_kernel(const float* part, int d, float f, float* wsum, float* hsum) {
+  __shared__ float red[16][64];
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, c = blockIdx.x * 64 + tx;
+  const bool of_w = blockIdx.y == 0;
+  const float* q = part + (of_w ? 0 : (int64_t)SUM_W * d);
   float s = 0.f;
-  if (c < C)
-    for (int k = ty; k < COLSUM_BLOCKS; k += 4) s += part[(int64_t)k * C + c];
+  if (c < d) {
+    if (of_w) {
+#pragma unroll
+      for (int k = 0; k < SUM_W / 16; ++k) s += q[(int64_t)(ty * (SUM_W / 16) + k) * d + c];
+    } else {
+#pragma unroll
+      for (int k = 0; k < SUM_H / 16; ++k) s += q[(int64_t)(ty * (SUM_H / 16) + k) * d + c];
+    }
+  }
   red[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && c < C) out[c] = f * ((red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]));
+  if (ty == 0 && c < d) {
+    float t = 0.f;
+    for (int k = 0; k < 16; ++k) t += red[k][tx];
+    (of_w ? wsum : hsum)[c] = f * t;
+  }
 }
 
 // dh = sum of the partials in order (+ the smoothing constant's part), rounded once
@@ -217,8 +278,9 @@ struct XentPlan {
   size_t bytes;
   float *coef, *lse2, *part, *colsum, *wsum, *hsum;
   int32_t* label;
-  void *g, *gt, *wt, *ht;
+  void *g, *gt, *wt, *ht, *splitk;
 };
+constexpr size_t SPLITK_BYTES = 8 << 20;
 // Pieces of the vocabulary: as few as keep a piece's d(logits) inside the 256 MB memory-side cache (the two products read
 // what the epilogue wrote).  Inside a piece the hidden gradient's product is cut along the entries into enough slices to
 // give every CU a tile.
@@ -230,8 +292,8 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   int64_t n = (a->V + fit - 1) / std::max<int64_t>(fit, 1);
   n = std::max<int64_t>(1, std::min<int64_t>(n, (a->V + 1023) / 1024));
   const int64_t want = (a->V + n - 1) / n, kt = std::max<int64_t>(4, (want + 63) / 64);
-  const int64_t tiles = (int64_t)((a->M + 255) / 256) * (f32 ? (a->d + 127) / 128 : (a->d + 255) / 256);
-  q.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
+  const int64_t tiles = (int64_t)((a->M + 255) / 256) * ((a->d + 255) / 256);
+  q.slices = f32 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
   q.kt_slice = (int)((kt + q.slices - 1) / q.slices);
   q.piece = q.slices * q.kt_slice * 64;
   q.n_pieces = (a->V + q.piece - 1) / q.piece;
@@ -244,10 +306,11 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.part = ar.get<float>((size_t)q.n_pieces * q.slices * a->M * a->d);
   q.colsum = q.wsum = q.hsum = nullptr;
   if (a->smoothing > 0.f) {
-    q.colsum = ar.get<float>((size_t)COLSUM_BLOCKS * a->d);
+    q.colsum = ar.get<float>((size_t)(SUM_W + SUM_H) * a->d);
     q.wsum = ar.get<float>(a->d);
     q.hsum = ar.get<float>(a->d);
   }
+  q.splitk = ar.take(SPLITK_BYTES);
   q.g = q.wt = nullptr;
   if (f32) {
     q.g = ar.take((size_t)a->M * q.piece * es);
@@ -301,23 +364,18 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
   XentPlan q;
   carve_xent(a, (char*)ws, ws_bytes, q);
   const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f;
-  hipLaunchKernelGGL(xent_rows_kernel, dim3((q.rows_padded + 255) / 256), dim3(256), 0, st, a->labels, grad_row, lse, a->M,
-                     q.rows_padded, a->V, q.coef, q.lse2, q.label);
-  NMTGAN_CHECK_LAUNCH("linear_xent_rows");
-  hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3(q.rows_padded / 64, (a->d + 63) / 64), dim3(256), 0, st, (const T*)a->h,
-                     a->ldh, a->M, a->d, (T*)q.ht, q.rows_padded, a->labels, a->V);
-  NMTGAN_CHECK_LAUNCH("linear_xent_transpose");
+  XentPrep pr{};
+  pr.h = a->h; pr.w = a->w; pr.ldh = a->ldh; pr.ldw = a->ldw;
+  pr.labels = a->labels; pr.grad_row = grad_row; pr.lse = lse;
+  pr.coef = q.coef; pr.lse2 = q.lse2; pr.label = q.label; pr.ht = q.ht; pr.part = q.colsum;
+  pr.M = a->M; pr.Mp = q.rows_padded; pr.V = a->V; pr.d = a->d;
+  pr.n_rows = (q.rows_padded + 255) / 256;
+  pr.n_turn = q.rows_padded / 64 * ((a->d + 63) / 64);
+  hipLaunchKernelGGL(xent_prep_kernel<T>, dim3(pr.n_rows + pr.n_turn + (low > 0.f ? SUM_W + SUM_H : 0)), dim3(256), 0, st, pr);
+  NMTGAN_CHECK_LAUNCH("linear_xent_prep");
   if (low > 0.f) {
-    hipLaunchKernelGGL(xent_colsum_kernel<T>, dim3(COLSUM_BLOCKS), dim3(256), 0, st, (const T*)a->w, a->ldw, a->V, a->d,
-                       (const float*)nullptr, q.colsum);
-    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
-    hipLaunchKernelGGL(xent_colsum_finish_kernel, dim3((a->d + 63) / 64), dim3(256), 0, st, q.colsum, a->d, -low, q.wsum);
-    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
-    hipLaunchKernelGGL(xent_colsum_kernel<T>, dim3(COLSUM_BLOCKS), dim3(256), 0, st, (const T*)a->h, a->ldh, a->M, a->d, q.coef,
-                       q.colsum);
-    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
-    hipLaunchKernelGGL(xent_colsum_finish_kernel, dim3((a->d + 63) / 64), dim3(256), 0, st, q.colsum, a->d, -low, q.hsum);
-    NMTGAN_CHECK_LAUNCH("linear_xent_colsum");
+    hipLaunchKernelGGL(xent_sums_kernel, dim3((a->d + 63) / 64, 2), dim3(1024), 0, st, q.colsum, a->d, -low, q.wsum, q.hsum);
+    NMTGAN_CHECK_LAUNCH("linear_xent_sums");
   }
   XentEpilogue x{};
   x.coef = q.coef; x.lse2 = q.lse2; x.label = q.label; x.g = q.g; x.gt = q.gt;
@@ -337,21 +395,17 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
       n_part += q.slices;
     } else {
       hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3(q.piece / 64, (a->d + 63) / 64), dim3(256), 0, st, w, a->ldw, n, a->d,
-                         (T*)q.wt, q.piece, (const int32_t*)nullptr, 0);
+                         (T*)q.wt, q.piece);
       NMTGAN_CHECK_LAUNCH("linear_xent_transpose");
-      nmtgan_gemm_args g[24];
-      for (int s = 0; s < q.slices; ++s) {
-        nmtgan_gemm_args& b = g[s];
-        b = nmtgan_gemm_args{};
-        b.op_dtype = a->dtype;
-        b.epilogue = NMTGAN_EPI_LINEAR;
-        b.A = (const T*)q.g + s * q.kt_slice * 64; b.lda = q.piece;
-        b.Wt = (const T*)q.wt + s * q.kt_slice * 64; b.ldw = q.piece;
-        b.M = a->M; b.N = a->d; b.K = q.kt_slice * 64;
-        b.n_seg = 1; b.out[0] = part + (int64_t)s * a->M * a->d; b.ldo[0] = a->d; b.out_f32[0] = 1; b.seg_scale[0] = 1.f;
-      }
-      NMTGAN_TRY(launch_gemm_group(g, q.slices, st));
-      n_part += q.slices;
+      nmtgan_gemm_args b{};
+      b.op_dtype = a->dtype;
+      b.epilogue = NMTGAN_EPI_LINEAR;
+      b.A = q.g; b.lda = q.piece; b.Wt = q.wt;
+      b.M = a->M; b.N = a->d; b.K = q.piece;
+      b.n_seg = 1; b.out[0] = part; b.ldo[0] = a->d; b.out_f32[0] = 1; b.seg_scale[0] = 1.f;
+      SplitKScope scope(q.splitk, SPLITK_BYTES);     // few tiles and a long k-loop: the library cuts it
+      NMTGAN_TRY(launch_gemm(&b, st));
+      n_part += 1;
     }
     nmtgan_gemm_args b{};
     b.op_dtype = a->dtype;
@@ -359,6 +413,7 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
     b.A = q.gt; b.lda = q.rows_padded; b.Wt = q.ht; b.bias = q.hsum;
     b.M = n; b.N = a->d; b.K = q.rows_padded;
     b.n_seg = 1; b.out[0] = (T*)dw + (int64_t)v0 * ld_dw; b.ldo[0] = ld_dw; b.out_f32[0] = es == 4; b.seg_scale[0] = 1.f;
+    SplitKScope scope(q.splitk, SPLITK_BYTES);
     NMTGAN_TRY(launch_gemm(&b, st));
   }
   hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, n_part,
