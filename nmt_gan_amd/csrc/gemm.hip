@@ -974,6 +974,9 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   // (256 bytes each), a fragment is two ds_read_b64_tr_b16 (4 k x 16 columns turned per 16 lanes), and column pair P of 16
   // sits at P ^ ((k & 3) | (k >> 1 & 4)): the 16 rows one read touches spread over all banks.
   constexpr bool KM = EPI == EPI_KPART;
+  // the cross-entropy forms' two wave groups meet for the epilogue and part again behind it: one barrier apart, the second
+  // group would wait at its last barrier through the first one's epilogue and the other way round
+  constexpr bool MEET = EPI == EPI_XSTAT || EPI == EPI_XGRAD || KM;
   const int nwg = p.ntm * p.ntn * (KM ? p.split_k : 1);
   const int G = gridDim.x;
   const int nkt = KM ? p.kt_slice : p.kbytes / BKB;      // >= 4 (launch guarantees it)
@@ -1222,6 +1225,8 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     for (int kt = 0; kt < nkt - 2; ++kt) kstep(M0{}, true);
     kstep(M1{}, has_next);
     kstep(M2{}, has_next);
+    if constexpr (MEET)
+      if (wr == 0) NMTGAN_BAR();                 // the second group's last barrier
     int tm, tn;
     const int slice = tile_of((int)blockIdx.x + t * G, tm, tn);
     const int m0 = tm * QBM + wr * 128, n0 = tn * QBN + wc * 64;
@@ -1250,6 +1255,8 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (MEET)
+      if (wr == 1) NMTGAN_BAR();                 // one barrier behind again
   }
   if (wr == 0) NMTGAN_BAR();                     // balance the barrier count of the two groups
 #undef NMTGAN_WAIT
