@@ -8,6 +8,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "common.h"
@@ -15,42 +16,67 @@
 
 namespace nmtgan {
 
-constexpr int LIST_MAX = 96, LIST_CHUNK = 16384, NORM_BLOCKS = 1024;
+constexpr int LIST_MAX = 160, LIST_CHUNK = 16384, NORM_BLOCKS = 1024;
 
-struct ListEntry { const void* g; void* out; int64_t n; int first_chunk; int16_t dtype, out_dtype; };
+// a tensor takes chunks [first_chunk, first_chunk of the next entry); tail = elements of its last one and the two dtypes
+struct ListEntry { const void* g; void* out; int first_chunk; unsigned tail; };
 struct ListParams { ListEntry e[LIST_MAX]; int n, n_chunks; };
+static_assert(sizeof(ListParams) + 64 <= 4096, "the list travels as kernel arguments (4 KB)");
+static inline unsigned pack_tail(int n, int dtype, int out_dtype) {
+  return (unsigned)n | (unsigned)dtype << 20 | (unsigned)out_dtype << 24;
+}
 
-// four consecutive elements; rows of a list may start at any element, so the vector types promise no more than that
-template <typename T> struct Four;
-template <> struct Four<float> {
-  typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
-  __device__ static __forceinline__ void load(const float* p, float (&x)[4]) {
-    const vec v = *reinterpret_cast<const vec*>(p);
-    x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; x[3] = v[3];
+// 16 bytes / four elements at any element of a tensor: the vector types promise no more than an element's alignment
+typedef unsigned u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T> struct Any {
+  using vec4 = std::conditional_t<sizeof(T) == 4, u32x4_at4, u32x4_at2>;
+  using vec2 = u32x2_at2;
+  static constexpr int E = 16 / (int)sizeof(T);
+  __device__ static __forceinline__ uint4 load16(const T* p) {
+    const vec4 v = *reinterpret_cast<const vec4*>(p);
+    return make_uint4(v[0], v[1], v[2], v[3]);
   }
-  __device__ static __forceinline__ void store(float* p, const float (&x)[4]) {
-    *reinterpret_cast<vec*>(p) = vec{x[0], x[1], x[2], x[3]};
+  __device__ static __forceinline__ void unpack(const uint4& r, float (&x)[E]) {
+    if constexpr (sizeof(T) == 2) {
+      unpack8<T>(r, x);
+    } else {
+      x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+    }
+  }
+  __device__ static __forceinline__ void load4(const T* p, float (&x)[4]) {
+    if constexpr (sizeof(T) == 2) {
+      const vec2 v = *reinterpret_cast<const vec2*>(p);
+      Pack16<T>::unpack2(v[0], x[0], x[1]);
+      Pack16<T>::unpack2(v[1], x[2], x[3]);
+    } else {
+      const vec4 v = *reinterpret_cast<const vec4*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[e]);
+    }
+  }
+  __device__ static __forceinline__ void store4(T* p, const float (&x)[4]) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<vec2*>(p) = vec2{Pack16<T>::pack2(x[0], x[1]), Pack16<T>::pack2(x[2], x[3])};
+    } else {
+      *reinterpret_cast<vec4*>(p) =
+          vec4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    }
   }
 };
-template <typename T> struct Four {
-  typedef unsigned vec __attribute__((ext_vector_type(2), aligned(2)));
-  __device__ static __forceinline__ void load(const T* p, float (&x)[4]) {
-    const vec v = *reinterpret_cast<const vec*>(p);
-    Pack16<T>::unpack2(v[0], x[0], x[1]);
-    Pack16<T>::unpack2(v[1], x[2], x[3]);
-  }
-  __device__ static __forceinline__ void store(T* p, const float (&x)[4]) {
-    *reinterpret_cast<vec*>(p) = vec{Pack16<T>::pack2(x[0], x[1]), Pack16<T>::pack2(x[2], x[3])};
-  }
-};
 
-__device__ __forceinline__ int entry_of(const ListParams& p, int chunk) {
+// entry of a chunk, the chunk's first element inside the tensor and its length
+__device__ __forceinline__ const ListEntry& chunk_of(const ListParams& p, int chunk, int64_t& off, int& n) {
   int a = 0, b = p.n - 1;                          // last entry whose first chunk is <= chunk
   while (a < b) {
     const int m = (a + b + 1) / 2;
     if (p.e[m].first_chunk <= chunk) a = m; else b = m - 1;
   }
-  return a;
+  const ListEntry& e = p.e[a];
+  off = (int64_t)(chunk - e.first_chunk) * LIST_CHUNK;
+  n = chunk + 1 == (a + 1 < p.n ? p.e[a + 1].first_chunk : p.n_chunks) ? (int)(e.tail & 0xfffff) : LIST_CHUNK;
+  return e;
 }
 
 __device__ __forceinline__ double block_sum_d(double v, double* red) {
@@ -64,30 +90,47 @@ __device__ __forceinline__ double block_sum_d(double v, double* red) {
 
 template <typename T>
 __device__ __forceinline__ double square_sum(const T* g, int n) {
-  double s = 0.0;
-  const int n4 = n / 4;
-  for (int i = threadIdx.x; i < n4; i += 256) {
-    float x[4];
-    Four<T>::load(g + 4 * i, x);
+  constexpr int E = Any<T>::E, U = 8;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  int i = 0;
+  for (; i + 256 * E * U <= n; i += 256 * E * U) {           // eight loads in flight
+    uint4 r[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = fma((double)x[e], (double)x[e], s);
+    for (int u = 0; u < U; ++u) r[u] = Any<T>::load16(g + i + (u * 256 + (int)threadIdx.x) * E);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[E];
+      Any<T>::unpack(r[u], x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e & 3] = fma((double)x[e], (double)x[e], s[e & 3]);
+    }
   }
-  for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) {
-    const double x = OpTraits<T>::load(g + i);
-    s = fma(x, x, s);
+  for (i += threadIdx.x * E; i < n; i += 256 * E) {
+    if (i + E <= n) {
+      float x[E];
+      Any<T>::unpack(Any<T>::load16(g + i), x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e & 3] = fma((double)x[e], (double)x[e], s[e & 3]);
+    } else {
+      for (int k = i; k < n; ++k) {
+        const double x = OpTraits<T>::load(g + k);
+        s[0] = fma(x, x, s[0]);
+      }
+    }
   }
-  return s;
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 __global__ __launch_bounds__(256) void norm_kernel(ListParams p, double* part) {
   __shared__ double red[4];
   double s = 0.0;
   for (int c = blockIdx.x; c < p.n_chunks; c += NORM_BLOCKS) {
-    const ListEntry& e = p.e[entry_of(p, c)];
-    const int64_t off = (int64_t)(c - e.first_chunk) * LIST_CHUNK;
-    const int n = (int)min((int64_t)LIST_CHUNK, e.n - off);
-    if (e.dtype == NMTGAN_F32) s += square_sum((const float*)e.g + off, n);
-    else if (e.dtype == NMTGAN_F16) s += square_sum((const f16_t*)e.g + off, n);
+    int64_t off;
+    int n;
+    const ListEntry& e = chunk_of(p, c, off, n);
+    const int dtype = e.tail >> 20 & 15;
+    if (dtype == NMTGAN_F32) s += square_sum((const float*)e.g + off, n);
+    else if (dtype == NMTGAN_F16) s += square_sum((const f16_t*)e.g + off, n);
     else s += square_sum((const bf16_t*)e.g + off, n);
   }
   s = block_sum_d(s, red);
@@ -108,15 +151,30 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const double* part, in
 
 template <typename T, typename O>
 __device__ __forceinline__ void scale_chunk(const T* g, O* out, int n, float f) {
-  const int n4 = n / 4;
-  for (int i = threadIdx.x; i < n4; i += 256) {
-    float x[4];
-    Four<T>::load(g + 4 * i, x);
+  constexpr int U = 8;
+  int i = 0;
+  for (; i + 1024 * U <= n; i += 1024 * U) {
+    float x[U][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] *= f;
-    Four<O>::store(out + 4 * i, x);
+    for (int u = 0; u < U; ++u) Any<T>::load4(g + i + (u * 256 + (int)threadIdx.x) * 4, x[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[u][e] *= f;
+      Any<O>::store4(out + i + (u * 256 + (int)threadIdx.x) * 4, x[u]);
+    }
   }
-  for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) OpTraits<O>::store(out + i, OpTraits<T>::load(g + i) * f);
+  for (i += threadIdx.x * 4; i < n; i += 1024) {
+    if (i + 4 <= n) {
+      float x[4];
+      Any<T>::load4(g + i, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] *= f;
+      Any<O>::store4(out + i, x);
+    } else {
+      for (int k = i; k < n; ++k) OpTraits<O>::store(out + k, OpTraits<T>::load(g + k) * f);
+    }
+  }
 }
 
 __global__ __launch_bounds__(256) void clip_kernel(ListParams p, const double* part, int n_part, float grad_scale,
@@ -127,16 +185,17 @@ __global__ __launch_bounds__(256) void clip_kernel(ListParams p, const double* p
   // a norm that is no finite number makes every output NaN, as tf.clip_by_global_norm does: the step is seen to be lost
   const float f = !(t < INFINITY) ? NAN : (t > (double)max_norm ? (float)((double)max_norm / t * (double)grad_scale) : grad_scale);
   for (int c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
-    const ListEntry& e = p.e[entry_of(p, c)];
+    int64_t off;
+    int n;
+    const ListEntry& e = chunk_of(p, c, off, n);
     if (f == 1.f && e.out == e.g) continue;          // nothing to change in place
-    const int64_t off = (int64_t)(c - e.first_chunk) * LIST_CHUNK;
-    const int n = (int)min((int64_t)LIST_CHUNK, e.n - off);
-    if (e.dtype == NMTGAN_F32) scale_chunk((const float*)e.g + off, (float*)e.out + off, n, f);
-    else if (e.dtype == NMTGAN_F16) {
-      if (e.out_dtype == NMTGAN_F32) scale_chunk((const f16_t*)e.g + off, (float*)e.out + off, n, f);
+    const int dtype = e.tail >> 20 & 15, out_dtype = e.tail >> 24 & 15;
+    if (dtype == NMTGAN_F32) scale_chunk((const float*)e.g + off, (float*)e.out + off, n, f);
+    else if (dtype == NMTGAN_F16) {
+      if (out_dtype == NMTGAN_F32) scale_chunk((const f16_t*)e.g + off, (float*)e.out + off, n, f);
       else scale_chunk((const f16_t*)e.g + off, (f16_t*)e.out + off, n, f);
     } else {
-      if (e.out_dtype == NMTGAN_F32) scale_chunk((const bf16_t*)e.g + off, (float*)e.out + off, n, f);
+      if (out_dtype == NMTGAN_F32) scale_chunk((const bf16_t*)e.g + off, (float*)e.out + off, n, f);
       else scale_chunk((const bf16_t*)e.g + off, (bf16_t*)e.out + off, n, f);
     }
   }
@@ -191,7 +250,7 @@ static int for_parts(const nmtgan_grad_ref* t, int n, F fn) {
     if (t[i].n == 0) continue;
     const int64_t c = (t[i].n + LIST_CHUNK - 1) / LIST_CHUNK;
     if (p.n == LIST_MAX || p.n_chunks + c > (1LL << 30)) NMTGAN_TRY(flush());
-    p.e[p.n++] = ListEntry{t[i].g, t[i].out, t[i].n, p.n_chunks, (int16_t)t[i].dtype, (int16_t)t[i].out_dtype};
+    p.e[p.n++] = ListEntry{t[i].g, t[i].out, p.n_chunks, pack_tail((int)(t[i].n - (c - 1) * LIST_CHUNK), t[i].dtype, t[i].out_dtype)};
     p.n_chunks += (int)c;
   }
   return flush();
