@@ -61,12 +61,11 @@ __global__ __launch_bounds__(256) void span_prep_kernel(SpanParams p) {
 }
 
 // ------------------------------------------------------------------------------------------ single tokens
-// One query row and one key head with up to GT of its query heads per workgroup, `splits` workgroups along the span.  A key
-// row is read once, as 16-byte chunks by LPK neighbouring lanes, so a wave reads 64 / LPK keys per instruction and STEP_U
-// such groups of K and of V are in flight while the previous ones are used.  Every lane group keeps a softmax of its own
-// (no exchange inside the loop but the LPK-lane sum of a dot product); groups, waves and splits are joined at the end in a
-// fixed order.  The arithmetic stays on the vector units: at 8 heads per key head it is what bounds the loop, at 4 or fewer
-// the reads are (48 rows, 8 heads over 2, spans of up to 16384 keys of 64 fp16: see the table of measurements).
+// One query row and one key head with its query heads per workgroup, `splits` workgroups along the span; waves and splits
+// are joined at the end in a fixed order.  Vector form (one query head per key head, and fp32 with up to GT): a key row is
+// read once, as 16-byte chunks by LPK neighbouring lanes, so a wave reads 64 / LPK keys per instruction and STEP_U such
+// groups of K and of V are in flight while the previous ones are used; every lane group keeps a softmax of its own (no
+// exchange inside the loop but the LPK-lane sum of a dot product).
 constexpr int STEP_U = 4;
 
 template <int LPK>
@@ -106,11 +105,54 @@ __device__ __forceinline__ void unpack_chunk(const uint4& r, float (&f)[16 / (in
   }
 }
 
+// one wave joins the four waves' parts of a head and hands them on: to the split's part, or as the result
+// (acc + w * stride = wave w's output of this head)
+template <typename T, int DP, typename B>
+__device__ __forceinline__ void step_finish(const SpanParams& p, const float* acc, int stride, const B& s_m, const B& s_l, int i,
+                                            int h, int t, int z, int splits, float* part, float* xs, int lane) {
+  const float mt = fmaxf(fmaxf(s_m[0][t], s_m[1][t]), fmaxf(s_m[2][t], s_m[3][t])), mu = mt == -INFINITY ? 0.f : mt;
+  float r[4], lt = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    r[k] = __builtin_amdgcn_exp2f(s_m[k][t] - mu);
+    lt += s_l[k][t] * r[k];
+  }
+  const int64_t at = (int64_t)i * p.heads + h;
+  float* mine = part + (at * splits + z) * (p.dh + 2);
+  float o[DP > 64 ? 2 : 1];
+  bool fine = lt < INFINITY;
+#pragma unroll
+  for (int u = 0; u < (DP > 64 ? 2 : 1); ++u) {
+    const int c = lane + 64 * u;
+    o[u] = c < p.dh ? (acc[c] * r[0] + acc[stride + c] * r[1]) + (acc[2 * stride + c] * r[2] + acc[3 * stride + c] * r[3]) : 0.f;
+    fine = fine && fmaf(o[u], 0.f, 0.f) == 0.f;
+  }
+  if (splits > 1) {
+#pragma unroll
+    for (int u = 0; u < (DP > 64 ? 2 : 1); ++u)
+      if (lane + 64 * u < p.dh) mine[lane + 64 * u] = o[u];
+    if (lane == 0) {
+      mine[p.dh] = mt;
+      mine[p.dh + 1] = lt;
+    }
+    return;
+  }
+  if (__any(!fine)) {                                        // (padding of a tile met an infinity): exactly, by itself
+    span_fwd_row<T>(p, i, h, xs, lane);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < (DP > 64 ? 2 : 1); ++u)
+    if (lane + 64 * u < p.dh)
+      OpTraits<T>::store((T*)p.out + (int64_t)i * p.ldo + h * p.dh + lane + 64 * u, lt == 0.f ? 0.f : o[u] / lt);
+  if (p.lse && lane == 0) p.lse[at] = lt == 0.f ? -INFINITY : mt * LN2 + logf(lt);
+}
+
 template <typename T, int DP, int GT, bool EXTRA>
 __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits, int groups, float* part) {
   constexpr int EPC = 16 / (int)sizeof(T), LPK = DP / EPC, KPW = 64 / LPK, KB = STEP_U * KPW;
   __shared__ float s_acc[4][GT][DP];
-  __shared__ float s_m[4][GT], s_l[4][GT];
+  __shared__ float s_m[4][GT], s_l[4][GT], s_xs[4][SPAN_MAX_DH];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, dh = p.dh, g = p.heads / p.kv_heads;
   const int i = blockIdx.x / splits, z = blockIdx.x % splits;
   const int kvh = blockIdx.y / groups, h0 = kvh * g + (blockIdx.y % groups) * GT, ng = min(GT, (kvh + 1) * g - h0);
@@ -130,7 +172,7 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
     unpack_chunk<T>(r, q[u]);
     m[u] = -INFINITY;
     l[u] = slope[u] = 0.f;
-    if (EXTRA && p.slopes && u < ng) slope[u] = p.slopes[h0 + u];
+    if (EXTRA && p.slopes && u < ng) slope[u] = p.slopes[h0 + u] * LOG2E;
 #pragma unroll
     for (int e = 0; e < EPC; ++e) {
       q[u][e] *= f;
@@ -138,7 +180,7 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
     }
   }
   const int pos = EXTRA ? pos_of(p, i) : 0;
-  const float inv_cap = EXTRA && p.cap > 0.f ? 1.f / p.cap : 0.f;
+  const float inv_cap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
 
   uint4 kr[STEP_U], vr[STEP_U];
   auto fetch = [&](int b) {
@@ -169,8 +211,11 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
 #pragma unroll
         for (int e = 0; e < EPC; ++e) d = fmaf(x[e], q[t][e], d);
         d = key_sum<LPK>(d);
-        float turn;
-        if constexpr (EXTRA) d = score2<T>(p, d, inv_cap, slope[t], pos, j, turn);
+        if constexpr (EXTRA) {
+          if (p.cap > 0.f) d = p.cap * LOG2E * span_tanh<T>(d * inv_cap);
+          else d *= p.scale * LOG2E;
+          if (p.slopes) d = fmaf(-slope[t], fabsf((float)(pos - j)), d);
+        }
         s[u][t] = j < j1 ? d : -INFINITY;
       }
     }
@@ -215,34 +260,152 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
     if (lane == 0) { s_m[w][t] = mt; s_l[w][t] = lt; }
   }
   __syncthreads();
-  for (int t = w; t < ng; t += 4) {                          // a wave per head joins the four
-    const float mt = fmaxf(fmaxf(s_m[0][t], s_m[1][t]), fmaxf(s_m[2][t], s_m[3][t])), mu = mt == -INFINITY ? 0.f : mt;
-    float r[4], lt = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      r[k] = __builtin_amdgcn_exp2f(s_m[k][t] - mu);
-      lt += s_l[k][t] * r[k];
-    }
-    const int64_t at = (int64_t)i * p.heads + h0 + t;
-    for (int k = lane; k < dh; k += 64) {
-      const float a = (s_acc[0][t][k] * r[0] + s_acc[1][t][k] * r[1]) + (s_acc[2][t][k] * r[2] + s_acc[3][t][k] * r[3]);
-      if (splits == 1) OpTraits<T>::store((T*)p.out + (int64_t)i * p.ldo + (h0 + t) * dh + k, lt == 0.f ? 0.f : a / lt);
-      else part[(at * splits + z) * (dh + 2) + k] = a;
-    }
-    if (lane == 0) {
-      if (splits > 1) {
-        part[(at * splits + z) * (dh + 2) + dh] = mt;
-        part[(at * splits + z) * (dh + 2) + dh + 1] = lt;
-      } else if (p.lse) {
-        p.lse[at] = lt == 0.f ? -INFINITY : mt * LN2 + logf(lt);
-      }
-    }
+  for (int t = w; t < ng; t += 4) step_finish<T, DP>(p, s_acc[0][t], GT * DP, s_m, s_l, i, h0 + t, t, z, splits, part, s_xs[w], lane);
+}
+
+// The same with the matrix cores, 16-bit types and 2 to 16 query heads per key head: the heads are the 16 columns of 16x16
+// products over tiles of 32 keys (S^T = K Q^T, out^T = V^T P^T, layouts as in span_tiles.h with four lanes a softmax row),
+// so the work per key does not grow with the heads.  Each wave walks every fourth tile of its split through LDS of its own.
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ f32x4_t mma16x16(const uint4& a, const uint4& b, f32x4_t c) {
+  if constexpr (__is_same(T, bf16_t)) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  } else {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
+}
+template <typename T, int DP, bool EXTRA>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void span_step_heads_kernel(SpanParams p, int splits, int groups, float* part) {
+  using G = Geo<T, DP>;
+  using D = Dma<T, DP>;
+  constexpr int NS = DP <= 64 ? 3 : 2, STAGE = 2 * D::BYTES, KS = DP / 32, DB = DP / 16;      // stages, k-steps, dh blocks
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ float s_m[4][16], s_l[4][16], xs[4][SPAN_MAX_DH];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int dh = p.dh, g = p.heads / p.kv_heads, col = lane & 15, q4 = lane >> 4;
+  const int i = blockIdx.x / splits, z = blockIdx.x % splits;
+  const int kvh = blockIdx.y / groups, h0 = kvh * g + (blockIdx.y % groups) * 16, ng = min(16, (kvh + 1) * g - h0);
+  int2 sp = span_of(p, i);
+  sp.x = __builtin_amdgcn_readfirstlane(sp.x);
+  sp.y = __builtin_amdgcn_readfirstlane(sp.y);
+  const int64_t len = sp.y - sp.x;
+  const int j0 = sp.x + (int)(len * z / splits), j1 = sp.x + (int)(len * (z + 1) / splits);
+  const T* K = (const T*)p.k + kvh * dh;
+  const T* V = (const T*)p.v + kvh * dh;
+  unsigned char* mine = smem + w * NS * STAGE;
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)mine);
+  D dk, dv;
+  dk.init(p.ldk, dh, lane);
+  dv.init(p.ldv, dh, lane);
+  const int nt = (j1 - j0 + 31) / 32;
+  auto issue = [&](int t, int buf) {
+    dk.issue(K, p.ldk, j0 + 32 * t, j1 - j0 - 32 * t, lds + buf * STAGE, lane);
+    dv.issue(V, p.ldv, j0 + 32 * t, j1 - j0 - 32 * t, lds + buf * STAGE + D::BYTES, lane);
+  };
+#pragma unroll
+  for (int k = 0; k < NS; ++k)
+    if (w + 4 * k < nt) issue(w + 4 * k, k);
+  uint4 own[KS];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const int c = 32 * k + 8 * q4;
+    own[k] = col < ng && c < dh ? *reinterpret_cast<const uint4*>((const T*)p.q + (int64_t)i * p.ldq + (h0 + col) * dh + c)
+                                : make_uint4(0, 0, 0, 0);
+  }
+  const float sc2 = p.scale * LOG2E;
+  const float slope2 = EXTRA && p.slopes && col < ng ? p.slopes[h0 + col] * LOG2E : 0.f;
+  const int pos = EXTRA ? pos_of(p, i) : 0;
+  const float cap2 = p.cap * LOG2E, inv2 = p.cap > 0.f ? p.scale / p.cap * 2.f * LOG2E : 0.f;
+  f32x4_t acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  int buf = 0;
+  for (int t = w; t < nt; t += 4) {
+    if (NS == 3 && t + 8 < nt) wait_dma<4 * D::NI>();
+    else if (t + 4 < nt) wait_dma<2 * D::NI>();
+    else wait_dma<0>();
+    const unsigned char* tk = mine + buf * STAGE;
+    const unsigned char* tv = tk + D::BYTES;
+    float s[8];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x4_t c = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        c = mma16x16<T>(*reinterpret_cast<const uint4*>(tk + G::swz(16 * kb + col, 4 * k + q4)), own[k], c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * kb + r] = c[r];
+    }
+    const int first = j0 + 32 * t + 4 * q4;                  // key of s[0]; s[4 kb + r] is key first + 16 kb + r
+    if (EXTRA && p.cap > 0.f) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        s[r] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * inv2)), -2.f * cap2, cap2);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] *= sc2;
+    }
+    if (EXTRA && p.slopes) {
+      const float away = (float)(pos - first);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(16 * (r >> 2) + (r & 3))), s[r]);
+    }
+    if (j0 + 32 * t + 32 > j1) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] = first + 16 * (r >> 2) + (r & 3) < j1 ? s[r] : -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    mx = groups4_max(mx);
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), c = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      l *= c;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[db][r] *= c;
+      m = mn;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(s[r] - mu);
+      l += s[r];
+    }
+    const uint4 pb = make_uint4(pack_pair<T>(s[0], s[1]), pack_pair<T>(s[2], s[3]), pack_pair<T>(s[4], s[5]), pack_pair<T>(s[6], s[7]));
+    const int row = 4 * q4 + (col >> 2);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int c = 16 * db + 4 * (lane & 3);
+      const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (lds_s16x4_p)(tv + G::swz(row, c >> 3) + 2 * (c & 7))));
+      const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (lds_s16x4_p)(tv + G::swz(row + 16, c >> 3) + 2 * (c & 7))));
+      acc[db] = mma16x16<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb, acc[db]);
+    }
+    if (t + 4 * NS < nt) {
+      wait_lds();
+      issue(t + 4 * NS, buf);
+    }
+    buf = buf + 1 == NS ? 0 : buf + 1;
+  }
+  l = groups4_sum(l);
+  if (lane < 16) { s_m[w][lane] = m; s_l[w][lane] = l; }
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+    *reinterpret_cast<float4*>(mine + (col * DP + 16 * db + 4 * q4) * 4) = make_float4(acc[db][0], acc[db][1], acc[db][2], acc[db][3]);
+  __syncthreads();
+  const float* out = reinterpret_cast<const float*>(smem);
+  for (int t = w; t < ng; t += 4) step_finish<T, DP>(p, out + t * DP, NS * STAGE / 4, s_m, s_l, i, h0 + t, t, z, splits, part, xs[w], lane);
 }
 
 // one wave per (row, head): the splits' parts, in order
 template <typename T>
 __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, int splits, const float* part) {
+  __shared__ float xs[4][SPAN_MAX_DH];
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= (int64_t)p.M * p.heads) return;
@@ -252,12 +415,29 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, int splits
   const float mz = lane < splits ? o[lane * (dh + 2) + dh] : -INFINITY, lz = lane < splits ? o[lane * (dh + 2) + dh + 1] : 0.f;
   const float m = wave_max(mz), mu = m == -INFINITY ? 0.f : m, rz = __builtin_amdgcn_exp2f(mz - mu);
   const float l = wave_sum(lz * rz);
-  for (int c0 = 0; c0 < dh; c0 += 64) {                      // every lane stays in the loop: it answers the exchange
-    const int c = min(c0 + lane, dh - 1);
-    float acc = 0.f;
-    for (int z = 0; z < splits; ++z) acc = fmaf(o[z * (dh + 2) + c], __shfl(rz, z, 64), acc);
-    if (c0 + lane < dh) OpTraits<T>::store((T*)p.out + (int64_t)i * p.ldo + h * dh + c, l == 0.f ? 0.f : acc / l);
+  float acc[2] = {0.f, 0.f};
+  bool fine = l < INFINITY;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {                              // every lane stays in the loop: it answers the exchange
+    if (64 * u >= dh) break;
+    const int c = min(64 * u + lane, dh - 1);
+    for (int z = 0; z < splits; z += 8) {                    // eight parts in flight
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = o[min(z + k, splits - 1) * (dh + 2) + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[u] = fmaf(z + k < splits ? v[k] : 0.f, __shfl(rz, min(z + k, 63), 64), acc[u]);
+    }
+    fine = fine && fmaf(acc[u], 0.f, 0.f) == 0.f;
   }
+  if (__any(!fine)) {
+    span_fwd_row<T>(p, i, h, xs[threadIdx.x >> 6], lane);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (64 * u + lane < dh)
+      OpTraits<T>::store((T*)p.out + (int64_t)i * p.ldo + h * dh + 64 * u + lane, l == 0.f ? 0.f : acc[u] / l);
   if (p.lse && lane == 0) p.lse[t] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
 }
 
@@ -328,12 +508,31 @@ static int launch_step(const SpanParams& p, int splits, float* part, hipStream_t
   return 0;
 }
 template <typename T, int DP>
+static int launch_step_heads(const SpanParams& p, int splits, float* part, hipStream_t st) {
+  constexpr size_t smem = (size_t)4 * (DP <= 64 ? 3 : 2) * 2 * Dma<T, DP>::BYTES;
+  const int groups = (p.heads / p.kv_heads + 15) / 16;
+  const dim3 grid((unsigned)(p.M * splits), p.kv_heads * groups);
+  if (p.cap > 0.f || p.slopes) {
+    NMTGAN_TRY(raise_lds(&span_step_heads_kernel<T, DP, true>, smem, "attn_span_step"));
+    hipLaunchKernelGGL((span_step_heads_kernel<T, DP, true>), grid, dim3(256), smem, st, p, splits, groups, part);
+  } else {
+    NMTGAN_TRY(raise_lds(&span_step_heads_kernel<T, DP, false>, smem, "attn_span_step"));
+    hipLaunchKernelGGL((span_step_heads_kernel<T, DP, false>), grid, dim3(256), smem, st, p, splits, groups, part);
+  }
+  NMTGAN_CHECK_LAUNCH("attn_span_step");
+  return 0;
+}
+template <typename T, int DP>
 static int choose_step(const SpanParams& p, int splits, float* part, hipStream_t st) {
   const int g = p.heads / p.kv_heads;
   if (g == 1) return launch_step<T, DP, 1>(p, splits, part, st);
-  if (g == 2) return launch_step<T, DP, 2>(p, splits, part, st);
-  if (g <= 4) return launch_step<T, DP, 4>(p, splits, part, st);
-  return launch_step<T, DP, 8>(p, splits, part, st);
+  if constexpr (sizeof(T) == 2) {
+    return launch_step_heads<T, DP>(p, splits, part, st);
+  } else {
+    if (g == 2) return launch_step<T, DP, 2>(p, splits, part, st);
+    if (g <= 4) return launch_step<T, DP, 4>(p, splits, part, st);
+    return launch_step<T, DP, 8>(p, splits, part, st);
+  }
 }
 int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, size_t ws_bytes, hipStream_t st) {
   prof::Scope prof_scope(prof::OTHER, st);
