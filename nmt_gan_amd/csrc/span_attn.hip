@@ -1,64 +1,7 @@
-// Span attention: preparation of the gradients, the form for single tokens, checks and launches (span_tiles.h has the formulas).
+// Span attention: the form for single tokens, checks and launches (span_tiles.h has the formulas).
 #include "span_tiles.h"
 
 namespace nmtgan {
-
-// What the gradient kernels need per row and per 32 rows: lse and delta_i = dout_i . out_i of every head (0 for rows that see
-// nothing, whatever their dout holds), the spans and their hull.  A workgroup takes 64 rows of one head, 8 lanes a row; the
-// first head's also write what all heads share.
-template <typename T>
-__global__ __launch_bounds__(256) void span_prep_kernel(SpanParams p) {
-  const int h = blockIdx.x % p.heads, b = blockIdx.x / p.heads, lane = threadIdx.x & 63, w = threadIdx.x >> 6, c8 = p.dh / 8;
-  float s[2], ls[2];
-  bool some[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int i = b * 64 + 32 * u + (threadIdx.x >> 3), ic = min(i, p.M - 1);
-    const T* o = (const T*)p.out + (int64_t)ic * p.ldo + h * p.dh;
-    const T* d = (const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh;
-    const int2 sp = span_of(p, ic);
-    some[u] = i < p.M && sp.y > sp.x;
-    ls[u] = i < p.M ? p.lse[(int64_t)ic * p.heads + h] : 0.f;
-    s[u] = 0.f;
-    for (int c = threadIdx.x & 7; c < c8; c += 8) {
-      float x[8], y[8];
-      VecIO<T, 8>::load(o + 8 * c, x);
-      VecIO<T, 8>::load(d + 8 * c, y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[u] = fmaf(x[e], y[e], s[u]);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int i = b * 64 + 32 * u + (threadIdx.x >> 3);
-    s[u] = dpp_add<0xB1>(s[u]);
-    s[u] = dpp_add<0x4E>(s[u]);
-    s[u] = dpp_add<0x141>(s[u]);
-    if ((threadIdx.x & 7) == 0 && b * 64 + 32 * u < p.M) {       // the block of 32 exists: its record is whole
-      float* at = delta_at(p, i, h);
-      at[-32] = ls[u] == -INFINITY ? 0.f : ls[u] * LOG2E;
-      at[0] = some[u] ? s[u] : 0.f;
-    }
-  }
-  if (h != 0 || w != 0) return;
-  const int i = b * 64 + lane;
-  int2 sp = make_int2(0, 0);
-  if (i < p.M) sp = span_of(p, i);
-  int4 hl = make_int4(sp.y > sp.x ? sp.x : 0x7fffffff, sp.y, sp.x, sp.y);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    hl.x = min(hl.x, __shfl_xor(hl.x, o, 64));
-    hl.y = max(hl.y, __shfl_xor(hl.y, o, 64));
-    hl.z = max(hl.z, __shfl_xor(hl.z, o, 64));
-    hl.w = min(hl.w, __shfl_xor(hl.w, o, 64));
-  }
-  if (b * 64 + (lane & 32) >= p.M) return;
-  const int64_t blk = 2 * b + (lane >> 5);
-  if ((lane & 31) == 0) p.hull[blk] = hl;
-  p.spans[blk * 64 + (lane & 31)] = sp.x;
-  p.spans[blk * 64 + 32 + (lane & 31)] = sp.y;
-  if (p.slopes) p.posr[blk * 64 + (lane & 31)] = i < p.M ? pos_of(p, i) : 0;
-}
 
 // ------------------------------------------------------------------------------------------ single tokens
 // One query row and one key head with its query heads per workgroup, `splits` workgroups along the span; waves and splits
@@ -595,10 +538,6 @@ int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
   p.dout = g->dout; p.ld_do = g->ld_dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
   p.ld_dq = g->ld_dq; p.ld_dk = g->ld_dk; p.ld_dv = g->ld_dv;
   if (p.M > 0) {
-    const int64_t prep = ((int64_t)p.M + 63) / 64 * p.heads;
-    NMTGAN_REQUIRE(prep < (1LL << 31), "attn_span_grads: too many rows");
-    NMTGAN_DISPATCH_GRAD(a->dtype, T, hipLaunchKernelGGL(span_prep_kernel<T>, dim3((unsigned)prep), dim3(256), 0, st, p));
-    NMTGAN_CHECK_LAUNCH("attn_span_prep");
     NMTGAN_TRY(span_dq_tiles(a->dtype, p, st));
   }
   return p.N > 0 ? span_dkv_tiles(a->dtype, p, st) : 0;

@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
   f32x16_t ak[G::DB], av[G::DB];
   clear(ak);
   clear(av);
-  const bool posr = EXTRA && p.slopes;
+  const bool posr = EXTRA && p.slopes, capped = EXTRA && p.cap > 0.f;
   constexpr int ND = 2 * D::NI + 2 + (EXTRA ? 1 : 0);        // transfers per tile (a record is one)
   auto issue = [&](int b, int h, int buf) {
     const unsigned dst = lds + buf * STAGE;
@@ -114,41 +114,39 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
       const bool whole = !solo && (entry & 1);
       f32x16_t s = score_block<T, DP>(tq, 0, kf, lane), turn;
       f32x16_t d = score_block<T, DP>(td, 0, vf, lane);
-      if constexpr (EXTRA) {
-        if (p.cap > 0.f) {
-          cap_scores<T, true>(s, turn, p.scale, p.cap);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[r] *= sc2;
-            turn[r] = 1.f;
-          }
-        }
-        if (posr) {
-          const float slope2 = p.slopes[h] * LOG2E;
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const int4 ps = *reinterpret_cast<const int4*>(spans + 64 + 8 * q4 + 4 * (lane >> 5));
-            s[4 * q4] = fmaf(-slope2, fabsf((float)(ps.x - j)), s[4 * q4]);
-            s[4 * q4 + 1] = fmaf(-slope2, fabsf((float)(ps.y - j)), s[4 * q4 + 1]);
-            s[4 * q4 + 2] = fmaf(-slope2, fabsf((float)(ps.z - j)), s[4 * q4 + 2]);
-            s[4 * q4 + 3] = fmaf(-slope2, fabsf((float)(ps.w - j)), s[4 * q4 + 3]);
-          }
-        }
-      }
+      if (capped) cap_scores<T, true>(s, turn, p.scale, p.cap, sizeof(T) == 2 ? p.cap * LOG2E : 0.f);     // (rec starts there)
+      const float slope2 = posr ? p.slopes[h] * LOG2E : 0.f;
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const int row = 8 * q4 + 4 * (lane >> 5);
         const float4 lse4 = *reinterpret_cast<const float4*>(rec + row), del4 = *reinterpret_cast<const float4*>(rec + 32 + row);
         const float ls[4] = {lse4.x, lse4.y, lse4.z, lse4.w}, de[4] = {del4.x, del4.y, del4.z, del4.w};
+        if (posr) {
+          const int4 ps = *reinterpret_cast<const int4*>(spans + 64 + row);
+          const int at[4] = {ps.x, ps.y, ps.z, ps.w};
+          if (!capped) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * q4 + e] *= sc2;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[4 * q4 + e] = fmaf(-slope2, fabsf((float)(at[e] - j)), s[4 * q4 + e] - ls[e]);
+        } else if (capped) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * q4 + e] -= ls[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fmaf(s[4 * q4 + e], sc2, -ls[e]);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * q4 + e;
-          const float pe = __builtin_amdgcn_exp2f(EXTRA ? s[r] - ls[e] : fmaf(s[r], sc2, -ls[e]));
-          float ds = pe * (d[r] - de[e]);
-          if constexpr (EXTRA) ds *= turn[r];
-          s[r] = pe;
-          d[r] = ds;
+          s[r] = __builtin_amdgcn_exp2f(s[r]);
+          d[r] = s[r] * (d[r] - de[e]);
+        }
+        if (capped) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[4 * q4 + e] *= turned<T>(turn[4 * q4 + e]);
         }
         if (!whole) {
           const int4 lo4 = *reinterpret_cast<const int4*>(spans + row), hi4 = *reinterpret_cast<const int4*>(spans + 32 + row);
@@ -173,7 +171,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     const unsigned long long off = __ballot(ok && !(all_finite(ak) && all_finite(av)));
     const unsigned again = (unsigned)off | (unsigned)(off >> 32);
     if (ok && !(again >> (lane & 31) & 1)) {
-      store_own<T, DP>((T*)p.dk + (int64_t)j * p.ld_dk + kvh * p.dh, ak, p.scale, p.dh, lane);
+      store_own<T, DP>((T*)p.dk + (int64_t)j * p.ld_dk + kvh * p.dh, ak, result_scale<T>(p), p.dh, lane);
       store_own<T, DP>((T*)p.dv + (int64_t)j * p.ld_dv + kvh * p.dh, av, 1.f, p.dh, lane);
     }
     float* xs = reinterpret_cast<float*>(mine);
@@ -202,7 +200,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     const int idx = tid + u * NT, row = idx / (DP / 4), col = idx % (DP / 4) * 4;
     const int64_t r = k0 + row;
     if (r >= p.N || col >= p.dh || bad[row]) continue;
-    const float x[4] = {tk[u].x * p.scale, tk[u].y * p.scale, tk[u].z * p.scale, tk[u].w * p.scale};
+    const float f = result_scale<T>(p), x[4] = {tk[u].x * f, tk[u].y * f, tk[u].z * f, tk[u].w * f};
     const float y[4] = {tv[u].x, tv[u].y, tv[u].z, tv[u].w};
     VecIO<T, 4>::store((T*)p.dk + r * p.ld_dk + kvh * p.dh + col, x);
     VecIO<T, 4>::store((T*)p.dv + r * p.ld_dv + kvh * p.dh + col, y);

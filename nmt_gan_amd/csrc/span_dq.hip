@@ -6,7 +6,7 @@
 namespace nmtgan {
 
 // dq.  delta of rows whose workgroup's spans fit in SHORT keys is summed from p dp in a first pass over the same tiles: there
-// p is large, and the rounding of `out` would show in it; long spans average it away and take delta from span_prep_kernel.
+// p is large, and the rounding of `out` would show in it; long spans average it away and take delta from dout . out.
 template <typename T, int DP, int KW, bool EXTRA>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_dq_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
@@ -14,7 +14,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   constexpr int REGION = 3 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // two K tiles and one V tile per wave
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_sum[KW][32], xs[KW][2][SPAN_MAX_DH];
-  __shared__ int bad[32], s_hull[KW];
+  __shared__ int bad[32], seen[32], s_hull[KW];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.x % p.heads, last = gridDim.x / p.heads - 1;
   const int kvh = h / (p.heads / p.kv_heads);
@@ -43,9 +43,17 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   uint4 own[G::STEPS], dout[G::STEPS];
   load_own<T, DP>((const T*)p.q + (int64_t)ic * p.ldq + h * p.dh, ok, p.dh, lane, own);
   load_own<T, DP>((const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh, ok, p.dh, lane, dout);
-  float* const at = delta_at(p, ic, h);
-  const float lse2 = at[-32], sc2 = p.scale * LOG2E;
-  float delta = at[0];
+  const float ls = ok ? p.lse[(int64_t)i * p.heads + h] : 0.f;
+  const float lse2 = ls == -INFINITY ? 0.f : ls * LOG2E, sc2 = p.scale * LOG2E;
+  const bool exact = sizeof(T) == 2 && nt * 32 <= SPAN_SHORT;     // (fp32 results carry no rounding to speak of)
+  float delta = 0.f;
+  if (!exact) {
+    uint4 o[G::STEPS];
+    load_own<T, DP>((const T*)p.out + (int64_t)ic * p.ldo + h * p.dh, ok, p.dh, lane, o);
+#pragma unroll
+    for (int s = 0; s < G::STEPS; ++s) delta += chunk_dot<T>(o[s], dout[s]);
+    delta = sp.y > sp.x ? both_halves_sum(delta) : 0.f;
+  }
   float slope2 = 0.f;
   int pos = 0;
   if constexpr (EXTRA) {
@@ -54,8 +62,55 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   f32x16_t acc[G::DB];
   clear(acc);
   const unsigned len = (unsigned)(sp.y - sp.x);
+  const bool capped = EXTRA && p.cap > 0.f;
+  struct Pairs { f32x16_t p, dp, t; };             // probabilities, dout . v, and what turned() takes
+  auto pairs = [&](const unsigned char* tk, int j0) -> Pairs {
+    f32x16_t s = score_block<T, DP>(tk, 0, own, lane), t = s;
+    const f32x16_t d = score_block<T, DP>(mine + 2 * D::BYTES, 0, dout, lane);
+    if (capped) {
+      cap_scores<T, true>(s, t, p.scale, p.cap, lse2);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc2, -lse2);
+    }
+    if (EXTRA && p.slopes) {
+      const float away = (float)(pos - (j0 + 4 * (lane >> 5)));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
+    return Pairs{s, d, t};
+  };
+  auto hide = [&](int j0, f32x16_t s) -> f32x16_t { // what lies outside the rows' spans counts as zero
+    if (j0 >= ws.all_lo && j0 + 32 <= ws.all_hi) return s;
+    const int at = j0 + 4 * (lane >> 5) - sp.x;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = (unsigned)(at + 8 * (r >> 2) + (r & 3)) < len ? s[r] : 0.f;
+    return s;
+  };
+  auto slopes_of = [&](int j0, const Pairs& q) -> f32x16_t {         // dr / scale
+    f32x16_t s = q.p;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= q.dp[r] - delta;
+    if (capped) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= turned<T>(q.t[r]);
+    }
+    return hide(j0, s);
+  };
+  auto sum_pairs = [&](int j0, const Pairs& q) -> float {
+    f32x16_t s = q.p;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= q.dp[r];
+    s = hide(j0, s);
+    float v = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v += s[r];
+    return v;
+  };
   float sum = 0.f;
-  auto walk = [&](auto FIRST) {                   // FIRST: sum p dp only
+  auto walk = [&](auto FIRST) __attribute__((always_inline)) {                   // FIRST: sum p dp only
     constexpr bool first_pass = decltype(FIRST)::value;
     if (t0 < nt) {
       issue_k(t0, 0);
@@ -68,48 +123,14 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
       if (t + dt < nt) wait_dma<D::NI>();         // the next K may still be under way
       else wait_dma<0>();
       const unsigned char* tk = mine + buf * D::BYTES;
-      f32x16_t s = score_block<T, DP>(tk, 0, own, lane), turn;
-      f32x16_t d = score_block<T, DP>(mine + 2 * D::BYTES, 0, dout, lane);
+      const Pairs q = pairs(tk, j0);
       if (t + dt < nt) {
         wait_lds();
         issue_v(t + dt);
       }
       if (__any(sp.x < j0 + 32 && sp.y > j0)) {
-        const int first = j0 + 4 * (lane >> 5);
-        if constexpr (EXTRA) {
-          if (p.cap > 0.f) {
-            cap_scores<T, true>(s, turn, p.scale, p.cap);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              s[r] *= sc2;
-              turn[r] = 1.f;
-            }
-          }
-          if (p.slopes) {
-            const float away = (float)(pos - first);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[r]);
-          }
-        }
-        const bool whole = j0 >= ws.all_lo && j0 + 32 <= ws.all_hi;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float pe = __builtin_amdgcn_exp2f(EXTRA ? s[r] - lse2 : fmaf(s[r], sc2, -lse2));
-          float ds = pe * (first_pass ? d[r] : d[r] - delta);
-          if (EXTRA && !first_pass) ds *= turn[r];
-          s[r] = ds;
-        }
-        if (!whole) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = (unsigned)(first - sp.x + 8 * (r >> 2) + (r & 3)) < len ? s[r] : 0.f;
-        }
-        if constexpr (first_pass) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sum += s[r];
-        } else {
-          accum_block<T, DP>(tk, 0, s, acc, lane);
-        }
+        if constexpr (first_pass) sum += sum_pairs(j0, q);
+        else accum_block<T, DP>(tk, 0, slopes_of(j0, q), acc, lane);
       }
       if (t + 2 * dt < nt) {
         wait_lds();
@@ -117,8 +138,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
       }
     }
   };
-  if (nt * 32 <= SPAN_SHORT) {
-    walk(std::integral_constant<bool, true>{});
+  auto sum_delta = [&]() __attribute__((always_inline)) {
     sum = both_halves_sum(sum);
     if (solo) {
       delta = sum;
@@ -129,23 +149,55 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
 #pragma unroll
       for (int k = 1; k < KW; ++k) delta += s_sum[k][lane & 31];
     }
-    if (ok && lane < 32 && (solo || w == 0)) at[0] = sp.y > sp.x ? delta : 0.f;
+    if (!(sp.y > sp.x)) delta = 0.f;
+  };
+  if (exact && nt <= dt) {                        // a tile per wave at most: it stays in registers
+    const int j0 = ws.lo + 32 * t0;
+    if (t0 < nt) {
+      issue_k(t0, 0);
+      issue_v(t0);
+    }
+    wait_dma<0>();
+    const Pairs q = pairs(mine, j0);              // (a wave without a tile multiplies what lies there, and drops it)
+    if (t0 < nt) sum = sum_pairs(j0, q);
+    sum_delta();
+    if (t0 < nt) accum_block<T, DP>(mine, 0, slopes_of(j0, q), acc, lane);
+  } else {
+    if (exact) {
+      walk(std::integral_constant<bool, true>{});
+      sum_delta();
+    }
+    walk(std::integral_constant<bool, false>{});
   }
-  walk(std::integral_constant<bool, false>{});
+  // what the dk/dv kernel reads of these rows: a record per head, and once for all heads the spans and their hull
+  if (lane < 32 && (solo || w == 0) && tile * 32 < p.M) {
+    float* const at = delta_at(p, i, h);
+    at[-32] = capped && sizeof(T) == 2 ? lse2 - p.cap * LOG2E : lse2;      // (where the capped score starts)
+    at[0] = delta;
+    if (h == 0) {
+      p.spans[(int64_t)tile * 64 + lane] = sp.x;
+      p.spans[(int64_t)tile * 64 + 32 + lane] = sp.y;
+      if (p.slopes) p.posr[(int64_t)tile * 64 + lane] = ok ? pos_of(p, i) : 0;
+      if (lane == 0) p.hull[tile] = make_int4(ws.lo, ws.hi, ws.all_lo, ws.all_hi);
+    }
+  }
   if (solo) {
     const bool some = sp.y > sp.x;
     const unsigned long long off = __ballot(some && !all_finite(acc));
     const unsigned again = (unsigned)off | (unsigned)(off >> 32);
     if (ok && !(again >> (lane & 31) & 1)) {
       if (!some) clear(acc);
-      store_own<T, DP>((T*)p.dq + (int64_t)i * p.ld_dq + h * p.dh, acc, p.scale, p.dh, lane);
+      store_own<T, DP>((T*)p.dq + (int64_t)i * p.ld_dq + h * p.dh, acc, result_scale<T>(p), p.dh, lane);
     }
     __threadfence_block();
     for (unsigned left = again; left; left &= left - 1)
       span_dq_row<T>(p, tile * 32 + __builtin_ctz(left), h, xs[w][0], xs[w][1], lane);
     return;
   }
-  if (tid < 32) bad[tid] = 0;
+  if (tid < 32) {
+    bad[tid] = 0;
+    seen[tid] = sp.y > sp.x;
+  }
   join_write<DP>(reinterpret_cast<float*>(mine), acc, 1.f, lane);
   __syncthreads();
   float4 tot[JN];
@@ -154,8 +206,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
     const int idx = tid + u * NT, row = idx / (DP / 4), c4 = idx % (DP / 4), r = tile * 32 + row;
     tot[u] = join_read<DP, KW>(reinterpret_cast<const float*>(smem), REGION / 4, row, c4);
     if (r >= p.M) continue;
-    const int2 span = span_of(p, r);
-    if (span.y <= span.x) tot[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!seen[row]) tot[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     else if (!finite4(tot[u])) bad[row] = 1;
   }
   __threadfence_block();                          // delta is read again by rows that are done one by one
@@ -164,7 +215,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   for (int u = 0; u < JN; ++u) {
     const int idx = tid + u * NT, row = idx / (DP / 4), col = idx % (DP / 4) * 4, r = tile * 32 + row;
     if (r >= p.M || col >= p.dh || bad[row]) continue;
-    const float x[4] = {tot[u].x * p.scale, tot[u].y * p.scale, tot[u].z * p.scale, tot[u].w * p.scale};
+    const float f = result_scale<T>(p), x[4] = {tot[u].x * f, tot[u].y * f, tot[u].z * f, tot[u].w * f};
     VecIO<T, 4>::store((T*)p.dq + (int64_t)r * p.ld_dq + h * p.dh + col, x);
   }
   for (int row = w; row < 32; row += KW)

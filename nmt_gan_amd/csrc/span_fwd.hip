@@ -12,7 +12,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
   constexpr int REGION = 2 * D::BYTES > 32 * DP * 4 ? 2 * D::BYTES : 32 * DP * 4, NT = 64 * KW, JN = 32 * DP / 4 / NT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_m[KW][32], s_l[KW][32], xs[KW][SPAN_MAX_DH];
-  __shared__ int bad[32], s_hull[KW];
+  __shared__ int bad[32], seen[32], s_hull[KW];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.x % p.heads, last = gridDim.x / p.heads - 1;
   const int kvh = h / (p.heads / p.kv_heads);
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
       const int first = j0 + 4 * (lane >> 5);
       if constexpr (EXTRA) {
         if (p.cap > 0.f) {
-          cap_scores<T, false>(s, s, p.scale, p.cap);
+          cap_scores<T, false>(s, s, p.scale, p.cap, 0.f);
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] *= sc2;
@@ -134,7 +134,10 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
     return;
   }
   if (lane < 32) { s_m[w][lane] = m; s_l[w][lane] = l; }
-  if (tid < 32) bad[tid] = 0;
+  if (tid < 32) {
+    bad[tid] = 0;
+    seen[tid] = sp.y > sp.x;
+  }
   __syncthreads();
   float mt = s_m[0][lane & 31];
 #pragma unroll
@@ -156,8 +159,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
     sum[u] = join_read<DP, KW>(reinterpret_cast<const float*>(smem), REGION / 4, row, c4);
     inv[u] = 0.f;
     if (r >= p.M) continue;
-    const int2 span = span_of(p, r);
-    if (span.y > span.x) {
+    if (seen[row]) {
       inv[u] = lr == 0.f ? 0.f : 1.f / lr;
       if (!(finite4(sum[u]) && lr < INFINITY)) bad[row] = 1;
     } else {

@@ -317,6 +317,23 @@ __device__ __forceinline__ void load_own(const T* row, bool ok, int dh, int lane
     own[s] = ok && c < dh ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
   }
 }
+template <typename T>
+__device__ __forceinline__ float chunk_dot(const uint4& a, const uint4& b) {
+  float s = 0.f;
+  if constexpr (sizeof(T) == 2) {
+    float x[8], y[8];
+    unpack8<T>(a, x);
+    unpack8<T>(b, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+  } else {
+    s = __uint_as_float(a.x) * __uint_as_float(b.x);
+    s = fmaf(__uint_as_float(a.y), __uint_as_float(b.y), s);
+    s = fmaf(__uint_as_float(a.z), __uint_as_float(b.z), s);
+    s = fmaf(__uint_as_float(a.w), __uint_as_float(b.w), s);
+  }
+  return s;
+}
 // transposed accumulators of the wave's own rows -> memory
 template <typename T, int DP>
 __device__ __forceinline__ void store_own(T* row, const f32x16_t (&acc)[Geo<T, DP>::DB], float f, int dh, int lane) {
@@ -377,17 +394,23 @@ __device__ __forceinline__ float score2(const SpanParams& p, float dot, float in
 }
 
 struct WaveSpan { int lo, hi, all_lo, all_hi; };   // hull of a wave's spans; keys all of its rows see
+template <int CTRL, bool MAX>
+__device__ __forceinline__ int dpp_minmax(int v) {
+  const int o = __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false);
+  return MAX ? max(v, o) : min(v, o);
+}
+template <bool MAX>
+__device__ __forceinline__ int rows_minmax(int v) { // over 32 lanes (both halves hold the same rows)
+  v = dpp_minmax<0xB1, MAX>(v);
+  v = dpp_minmax<0x4E, MAX>(v);
+  v = dpp_minmax<0x141, MAX>(v);
+  v = dpp_minmax<0x140, MAX>(v);
+  const u32x2_t a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane(MAX ? max((int)a[0], (int)a[1]) : min((int)a[0], (int)a[1]));
+}
 __device__ __forceinline__ WaveSpan wave_span(int2 sp) {
-  int a = sp.y > sp.x ? sp.x : 0x7fffffff, b = sp.y, c = sp.x, d = sp.y;
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    a = min(a, __shfl_xor(a, o, 64));
-    b = max(b, __shfl_xor(b, o, 64));
-    c = max(c, __shfl_xor(c, o, 64));
-    d = min(d, __shfl_xor(d, o, 64));
-  }
-  return WaveSpan{__builtin_amdgcn_readfirstlane(a), __builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(c),
-                  __builtin_amdgcn_readfirstlane(d)};
+  return WaveSpan{rows_minmax<false>(sp.y > sp.x ? sp.x : 0x7fffffff), rows_minmax<true>(sp.y), rows_minmax<true>(sp.x),
+                  rows_minmax<false>(sp.y)};
 }
 constexpr int SPAN_SHORT = 256;
 // whether the spans of none of KW consecutive blocks of 32 rows reach over more than SPAN_SHORT keys
@@ -468,29 +491,34 @@ template <typename T, int DP> struct Dma {
   }
 };
 
-// tanh and distance terms of a score block in place, in units of log 2: s = raw products -> scores (s, d hold 16 rows of
-// the tile at 8 (r >> 2) + (r & 3) from `first`); turn = 1 - t^2 where wanted
-template <typename T, bool TURN>
-__device__ __forceinline__ void cap_scores(f32x16_t& s, f32x16_t& turn, float scale, float cap) {
+// The tanh of a score block in place, in units of log 2: s = raw products -> capped scores minus `base`; BACK: t carries
+// what (1 - t^2) is made of, see turned() - for the 16-bit types t = 1 - 2 d with d = 1 / (1 + exp(2 r / cap)), whose
+// 1 - t^2 = 4 d (1 - d) leaves its 4 to the scale of the result
+template <typename T, bool BACK>
+__device__ __forceinline__ void cap_scores(f32x16_t& s, f32x16_t& t, float scale, float cap, float base) {
+  const float c2 = cap * LOG2E;
   if constexpr (sizeof(T) == 4) {
-    const float inv = scale / cap, c2 = cap * LOG2E;
+    const float inv = scale / cap;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float t = tanhf(s[r] * inv);
-      s[r] = c2 * t;
-      if constexpr (TURN) turn[r] = fmaf(-t, t, 1.f);
+      const float v = tanhf(s[r] * inv);
+      s[r] = fmaf(c2, v, -base);
+      if constexpr (BACK) t[r] = v;
     }
   } else {
-    // t = 1 - 2 d, d = 1 / (1 + exp(2 r / cap)); 1 - t^2 = 4 d (1 - d)
-    const float a = scale / cap * 2.f * LOG2E, c2 = cap * LOG2E, c4 = -2.f * c2;
+    const float a = scale / cap * 2.f * LOG2E, c4 = -2.f * c2, c0 = c2 - base;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float d = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * a));
-      s[r] = fmaf(d, c4, c2);
-      if constexpr (TURN) turn[r] = 4.f * fmaf(-d, d, d);
+      s[r] = fmaf(d, c4, c0);
+      if constexpr (BACK) t[r] = d;
     }
   }
 }
+template <typename T>
+__device__ __forceinline__ float turned(float t) { return sizeof(T) == 4 ? fmaf(-t, t, 1.f) : fmaf(-t, t, t); }
+template <typename T>
+__device__ __forceinline__ float result_scale(const SpanParams& p) { return p.cap > 0.f && sizeof(T) == 2 ? 4.f * p.scale : p.scale; }
 
 // sums the KW waves' transposed accumulators (32 own rows x DP, each wave's in LDS at region w) and hands the result to
 // put(row, col, x[4]) in whole rows; bad[row] is set where a sum is not finite
