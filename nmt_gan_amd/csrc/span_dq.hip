@@ -1,14 +1,16 @@
 // Span attention, gradient of the queries on tiles (span_tiles.h has the formulas and the layout).
-#include <type_traits>
-
 #include "span_tiles.h"
 
 namespace nmtgan {
 
-// dq.  delta of rows whose workgroup's spans fit in SHORT keys is summed from p dp in a first pass over the same tiles: there
-// p is large, and the rounding of `out` would show in it; long spans average it away and take delta from dout . out.
+// dq.  delta = dout . out carries the rounding of a 16-bit `out`, which shows where a row has few keys that count; the sum
+// of p dp over the walk does not.  So the walk runs with the former and corrects at the end: with c = p (1 - t^2),
+//   dq / scale = sum c (dp - delta) k = sum c (dp - delta16) k + (delta16 - delta) sum c k,
+// the second sum riding on the same turned K fragments.  The dk/dv kernel gets the corrected delta.  (16384 rows of long
+// documents, 8 heads of 64, capped and biased, bf16: 126 us, 111 without the correction and with 1.5 times the error that
+// rounding q, k, v and out alone leaves in dq and dk; taking every span twice instead: 190 us.)
 template <typename T, int DP, int KW, bool EXTRA>
-__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_dq_split_kernel(SpanParams p) {
+__global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dq_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
   constexpr int REGION = 3 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // two K tiles and one V tile per wave
@@ -45,9 +47,8 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   load_own<T, DP>((const T*)p.dout + (int64_t)ic * p.ld_do + h * p.dh, ok, p.dh, lane, dout);
   const float ls = ok ? p.lse[(int64_t)i * p.heads + h] : 0.f;
   const float lse2 = ls == -INFINITY ? 0.f : ls * LOG2E, sc2 = p.scale * LOG2E;
-  const bool exact = sizeof(T) == 2 && nt * 32 <= SPAN_SHORT;     // (fp32 results carry no rounding to speak of)
   float delta = 0.f;
-  if (!exact) {
+  {
     uint4 o[G::STEPS];
     load_own<T, DP>((const T*)p.out + (int64_t)ic * p.ldo + h * p.dh, ok, p.dh, lane, o);
 #pragma unroll
@@ -59,90 +60,76 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
   if constexpr (EXTRA) {
     if (p.slopes) { slope2 = p.slopes[h] * LOG2E; pos = pos_of(p, ic); }
   }
-  f32x16_t acc[G::DB];
+  constexpr bool FIX = sizeof(T) == 2;
+  f32x16_t acc[G::DB], ck[FIX ? G::DB : 1];
   clear(acc);
+  clear(ck);
   const unsigned len = (unsigned)(sp.y - sp.x);
   const bool capped = EXTRA && p.cap > 0.f;
-  struct Pairs { f32x16_t p, dp, t; };             // probabilities, dout . v, and what turned() takes
-  auto pairs = [&](const unsigned char* tk, int j0) -> Pairs {
-    f32x16_t s = score_block<T, DP>(tk, 0, own, lane), t = s;
-    const f32x16_t d = score_block<T, DP>(mine + 2 * D::BYTES, 0, dout, lane);
-    if (capped) {
-      cap_scores<T, true>(s, t, p.scale, p.cap, lse2);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc2, -lse2);
-    }
-    if (EXTRA && p.slopes) {
-      const float away = (float)(pos - (j0 + 4 * (lane >> 5)));
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[r]);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
-    return Pairs{s, d, t};
-  };
-  auto hide = [&](int j0, f32x16_t s) -> f32x16_t { // what lies outside the rows' spans counts as zero
-    if (j0 >= ws.all_lo && j0 + 32 <= ws.all_hi) return s;
-    const int at = j0 + 4 * (lane >> 5) - sp.x;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = (unsigned)(at + 8 * (r >> 2) + (r & 3)) < len ? s[r] : 0.f;
-    return s;
-  };
-  auto slopes_of = [&](int j0, const Pairs& q) -> f32x16_t {         // dr / scale
-    f32x16_t s = q.p;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= q.dp[r] - delta;
-    if (capped) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= turned<T>(q.t[r]);
-    }
-    return hide(j0, s);
-  };
-  auto sum_pairs = [&](int j0, const Pairs& q) -> float {
-    f32x16_t s = q.p;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= q.dp[r];
-    s = hide(j0, s);
-    float v = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) v += s[r];
-    return v;
-  };
   float sum = 0.f;
-  auto walk = [&](auto FIRST) __attribute__((always_inline)) {                   // FIRST: sum p dp only
-    constexpr bool first_pass = decltype(FIRST)::value;
-    if (t0 < nt) {
-      issue_k(t0, 0);
-      issue_v(t0);
+  if (t0 < nt) {
+    issue_k(t0, 0);
+    issue_v(t0);
+  }
+  if (t0 + dt < nt) issue_k(t0 + dt, 1);
+  int buf = 0;
+  for (int t = t0; t < nt; t += dt, buf ^= 1) {
+    const int j0 = ws.lo + 32 * t;
+    if (t + dt < nt) wait_dma<D::NI>();           // the next K may still be under way
+    else wait_dma<0>();
+    const unsigned char* tk = mine + buf * D::BYTES;
+    f32x16_t s = score_block<T, DP>(tk, 0, own, lane), turn = s;
+    f32x16_t d = score_block<T, DP>(mine + 2 * D::BYTES, 0, dout, lane);
+    if (t + dt < nt) {
+      wait_lds();
+      issue_v(t + dt);
     }
-    if (t0 + dt < nt) issue_k(t0 + dt, 1);
-    int buf = 0;
-    for (int t = t0; t < nt; t += dt, buf ^= 1) {
-      const int j0 = ws.lo + 32 * t;
-      if (t + dt < nt) wait_dma<D::NI>();         // the next K may still be under way
-      else wait_dma<0>();
-      const unsigned char* tk = mine + buf * D::BYTES;
-      const Pairs q = pairs(tk, j0);
-      if (t + dt < nt) {
-        wait_lds();
-        issue_v(t + dt);
+    if (__any(sp.x < j0 + 32 && sp.y > j0)) {
+      if (capped) {
+        cap_scores<T, true>(s, turn, p.scale, p.cap, lse2);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc2, -lse2);
       }
-      if (__any(sp.x < j0 + 32 && sp.y > j0)) {
-        if constexpr (first_pass) sum += sum_pairs(j0, q);
-        else accum_block<T, DP>(tk, 0, slopes_of(j0, q), acc, lane);
+      const int first = j0 + 4 * (lane >> 5);
+      if (EXTRA && p.slopes) {
+        const float away = (float)(pos - first);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope2, fabsf(away - (float)(8 * (r >> 2) + (r & 3))), s[r]);
       }
-      if (t + 2 * dt < nt) {
-        wait_lds();
-        issue_k(t + 2 * dt, buf);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
+      if (!(j0 >= ws.all_lo && j0 + 32 <= ws.all_hi)) {      // what lies outside the rows' spans counts as zero
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool on = (unsigned)(first - sp.x + 8 * (r >> 2) + (r & 3)) < len;
+          s[r] = on ? s[r] : 0.f;
+          d[r] = on ? d[r] : 0.f;
+        }
       }
+      if constexpr (FIX) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum = fmaf(s[r], d[r], sum);
+      }
+      if (capped) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= turned<T>(turn[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) d[r] = s[r] * (d[r] - delta);
+      if constexpr (FIX) accum_two<T, DP>(tk, d, s, acc, ck, lane);
+      else accum_block<T, DP>(tk, 0, d, acc, lane);
     }
-  };
-  auto sum_delta = [&]() __attribute__((always_inline)) {
+    if (t + 2 * dt < nt) {
+      wait_lds();
+      issue_k(t + 2 * dt, buf);
+    }
+  }
+  if constexpr (FIX) {
+    const float given = delta;
     sum = both_halves_sum(sum);
-    if (solo) {
-      delta = sum;
-    } else {
+    delta = sum;
+    if (!solo) {
       if (lane < 32) s_sum[w][lane] = sum;
       __syncthreads();
       delta = s_sum[0][lane & 31];
@@ -150,24 +137,11 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 3 : 1) void span_d
       for (int k = 1; k < KW; ++k) delta += s_sum[k][lane & 31];
     }
     if (!(sp.y > sp.x)) delta = 0.f;
-  };
-  if (exact && nt <= dt) {                        // a tile per wave at most: it stays in registers
-    const int j0 = ws.lo + 32 * t0;
-    if (t0 < nt) {
-      issue_k(t0, 0);
-      issue_v(t0);
-    }
-    wait_dma<0>();
-    const Pairs q = pairs(mine, j0);              // (a wave without a tile multiplies what lies there, and drops it)
-    if (t0 < nt) sum = sum_pairs(j0, q);
-    sum_delta();
-    if (t0 < nt) accum_block<T, DP>(mine, 0, slopes_of(j0, q), acc, lane);
-  } else {
-    if (exact) {
-      walk(std::integral_constant<bool, true>{});
-      sum_delta();
-    }
-    walk(std::integral_constant<bool, false>{});
+    const float off = given - delta;
+#pragma unroll
+    for (int db = 0; db < G::DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] = fmaf(off, ck[db][r], acc[db][r]);
   }
   // what the dk/dv kernel reads of these rows: a record per head, and once for all heads the spans and their hull
   if (lane < 32 && (solo || w == 0) && tile * 32 < p.M) {

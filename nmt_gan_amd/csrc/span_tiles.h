@@ -271,6 +271,16 @@ __device__ __forceinline__ unsigned pack_pair(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{a, b}), f16x2_t));
   }
 }
+// A operand of 16 tile rows turned: rows row .. + 3 and row + 8 .. + 11 of 16 columns around `col`
+template <typename T, int DP>
+__device__ __forceinline__ uint4 turned_rows(const unsigned char* tile, int row, int col) {
+  using G = Geo<T, DP>;
+  const uint2 u = __builtin_bit_cast(
+      uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_p)(tile + G::swz(row, col >> 3) + 2 * (col & 7))));
+  const uint2 v = __builtin_bit_cast(
+      uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_p)(tile + G::swz(row + 8, col >> 3) + 2 * (col & 7))));
+  return make_uint4(u.x, u.y, v.x, v.y);
+}
 // acc^T[dh][own] += (tile^T)[dh][rows 32 kb ..] . x, x = a score block's registers
 template <typename T, int DP>
 __device__ __forceinline__ void accum_block(const unsigned char* tile, int kb, const f32x16_t& x, f32x16_t (&acc)[Geo<T, DP>::DB],
@@ -284,15 +294,8 @@ __device__ __forceinline__ void accum_block(const unsigned char* tile, int kb, c
                                  pack_pair<T>(x[8 * t + 4], x[8 * t + 5]), pack_pair<T>(x[8 * t + 6], x[8 * t + 7]));
       const int row = 32 * kb + 16 * t + 4 * hl + ((lane & 15) >> 2);
 #pragma unroll
-      for (int db = 0; db < G::DB; ++db) {
-        const int col = 32 * db + (lane & 16) + 4 * (lane & 3);
-        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4_p)(tile + G::swz(row, col >> 3) + 2 * (col & 7)));
-        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4_p)(tile + G::swz(row + 8, col >> 3) + 2 * (col & 7)));
-        const uint2 u = __builtin_bit_cast(uint2, lo), v = __builtin_bit_cast(uint2, hi);
-        acc[db] = mfma16<T>(make_uint4(u.x, u.y, v.x, v.y), b, acc[db]);
-      }
+      for (int db = 0; db < G::DB; ++db)
+        acc[db] = mfma16<T>(turned_rows<T, DP>(tile, row, 32 * db + (lane & 16) + 4 * (lane & 3)), b, acc[db]);
     }
   } else {
 #pragma unroll
@@ -308,6 +311,26 @@ __device__ __forceinline__ void accum_block(const unsigned char* tile, int kb, c
   }
 }
 
+// two accumulations over the same rows of a tile (16-bit types): the turned fragments serve both
+template <typename T, int DP>
+__device__ __forceinline__ void accum_two(const unsigned char* tile, const f32x16_t& x, const f32x16_t& y,
+                                          f32x16_t (&accx)[Geo<T, DP>::DB], f32x16_t (&accy)[Geo<T, DP>::DB], int lane) {
+  using G = Geo<T, DP>;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint4 bx = make_uint4(pack_pair<T>(x[8 * t], x[8 * t + 1]), pack_pair<T>(x[8 * t + 2], x[8 * t + 3]),
+                                pack_pair<T>(x[8 * t + 4], x[8 * t + 5]), pack_pair<T>(x[8 * t + 6], x[8 * t + 7]));
+    const uint4 by = make_uint4(pack_pair<T>(y[8 * t], y[8 * t + 1]), pack_pair<T>(y[8 * t + 2], y[8 * t + 3]),
+                                pack_pair<T>(y[8 * t + 4], y[8 * t + 5]), pack_pair<T>(y[8 * t + 6], y[8 * t + 7]));
+    const int row = 16 * t + 4 * (lane >> 5) + ((lane & 15) >> 2);
+#pragma unroll
+    for (int db = 0; db < G::DB; ++db) {
+      const uint4 a = turned_rows<T, DP>(tile, row, 32 * db + (lane & 16) + 4 * (lane & 3));
+      accx[db] = mfma16<T>(a, bx, accx[db]);
+      accy[db] = mfma16<T>(a, by, accy[db]);
+    }
+  }
+}
 // own row as the B operand of score_block
 template <typename T, int DP>
 __device__ __forceinline__ void load_own(const T* row, bool ok, int dh, int lane, uint4 (&own)[Geo<T, DP>::STEPS]) {
