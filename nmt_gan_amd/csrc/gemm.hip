@@ -199,10 +199,9 @@ __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)
 }
 
 // XGRAD: C rows = hidden rows, C columns = entries, so a lane holds four consecutive rows of one entry = 8 bytes of the
-// entry-major image gt.  d(logit) = coef (exp(z - lse) - high [entry == label]), zero where no row or entry is (the images
-// are padded to whole k-tiles); the constant -coef low of label smoothing is added in fp32 to the sums it ends up in, where
-// its rounding to 16 bits would add up.  Rows without a label have coef 0 and are 0 whatever their logits are.
-// rowv: the wave tile's rows as [coef | lse / ln 2 | label] of 16 MT each (LDS); null: from memory.
+// entry-major image gt.  y = factor (exp(z - lse) - high [entry == label]), zero where no row or entry is (the images are
+// padded to whole k-tiles); factor = 1 / high.  Rows without a label have factor 0 and are 0 whatever their logits are.
+// rowv: the wave tile's rows as [factor | lse / ln 2 | label] of 16 MT each (LDS); null: from memory.
 template <typename OpT, int MT>
 __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane,
                                                const float* rowv = nullptr) {
@@ -212,10 +211,10 @@ __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)
   for (int i = 0; i < MT; ++i) {
     const int mb = m0 + 16 * i + 4 * fq;
     if (m0 + 16 * i >= x.rows_padded) continue;    // rows_padded is a multiple of 64
-    const float* at = rowv ? rowv + 16 * i + 4 * fq : x.coef + mb;
-    const int64_t step = rowv ? 16 * MT : x.lse2 - x.coef;
-    float coef[4], lse2[4];
-    VecIO<float, 4>::load(at, coef);
+    const float* at = rowv ? rowv + 16 * i + 4 * fq : x.factor + mb;
+    const int64_t step = rowv ? 16 * MT : x.lse2 - x.factor;
+    float factor[4], lse2[4];
+    VecIO<float, 4>::load(at, factor);
     VecIO<float, 4>::load(at + step, lse2);
     const int4 lab = *reinterpret_cast<const int4*>(rowv ? reinterpret_cast<const int32_t*>(at + 2 * step) : x.label + mb);
     const int label[4] = {lab.x - x.first, lab.y - x.first, lab.z - x.first, lab.w - x.first};
@@ -223,23 +222,23 @@ __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       hit = hit || (unsigned)(label[e] - n0) < 64u;
-      none = none || coef[e] == 0.f;
+      none = none || factor[e] == 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        acc[i][j][e] = coef[e] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[e]));
+        acc[i][j][e] = factor[e] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[e]));
     }
     if (__any(hit)) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n0 + 16 * j + fc == label[e]) acc[i][j][e] -= coef[e] * x.high;
+          if (n0 + 16 * j + fc == label[e]) acc[i][j][e] -= factor[e] * x.high;
     }
     if (__any(none)) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = coef[e] == 0.f ? 0.f : acc[i][j][e];
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = factor[e] == 0.f ? 0.f : acc[i][j][e];
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1092,7 +1091,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int r = min(tm * QBM + wr * 128 + 64 * k + lane, p.x.rows_padded - 1);
-        glds4(p.x.coef + r, dst + 256 * k);
+        glds4(p.x.factor + r, dst + 256 * k);
         glds4(p.x.lse2 + r, dst + 512 + 256 * k);
         glds4(p.x.label + r, dst + 1024 + 256 * k);
       }

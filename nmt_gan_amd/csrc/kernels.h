@@ -9,8 +9,8 @@ namespace nmtgan {
 // vocabulary the product covers, the images of d(logits) are padded with zeros to whole k-tiles
 struct XentEpilogue {
   float* zsum;                                   // forward, label smoothing only
-  // per hidden row, [rows_padded] each, 16-byte aligned: gradient of its loss (0 without a label), lse / ln 2, label (-1)
-  const float* coef; const float* lse2; const int32_t* label;
+  // per hidden row, [rows_padded] each, 16-byte aligned: 1 / high (0 without a gradient), lse / ln 2, label (-1)
+  const float* factor; const float* lse2; const int32_t* label;
   void* g; void* gt;                             // [rows][piece_padded] (may be null), [piece_padded][rows_padded]
   int first, piece_padded, rows_padded;
   float high;

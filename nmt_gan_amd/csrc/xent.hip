@@ -8,10 +8,13 @@
 // Forward: one product on the matrix cores whose epilogue leaves (max, sum exp) per 64 entries and row (gemm.hip), joined
 // in tile order by xent_finish_kernel, which also forms the label's own logit from the operands.
 // Gradient, per piece of the vocabulary: the product again (2 M V d operations are cheaper at d <= 1024 than 8 bytes of
-// fp32 logit written and read), its epilogue writes dz in the operand type, entry-major; two products with that image give
-// the piece's rows of dw (K = rows) and partials of dh (K = entries, both operands turned on their way out of LDS).  dz is
-// rounded once to the operand type - the matrix cores take no more - like every activation gradient of this library; lse,
-// loss and all sums are fp32.
+// fp32 logit written and read), its epilogue writes the image y = p / high - [j = label] in the operand type, entry-major;
+// two products with it give the piece's rows of dw = high y^T (g h) + ... (K = rows) and partials of dh = g high (y w) + ...
+// (K = entries, both operands turned on their way out of LDS).  y and g h are rounded once to the operand type - the matrix
+// cores take no more - like every activation gradient of this library; lse, loss and all sums are fp32.  Neither g nor high
+// is in y: where all rows weigh the same, g high is one number in every row, and its rounding would add up over them
+// (8192 rows of 1 / 8192 over 30000 entries, smoothing 0.1: error of dh and dw 0.0035 of their size with it).  The label's
+// -1 is exact.
 #include <math.h>
 
 #include <algorithm>
@@ -101,17 +104,13 @@ __global__ __launch_bounds__(256) void xent_finish_kernel(const float2* stats, c
   }
 }
 
-// out[c][r] = in[r][c] for r < R, 0 for R <= r < Rp, one 64 x 64 tile; with labels, rows without one count as zeros
-template <typename T>
-__device__ __forceinline__ void transpose_tile(T (&tile)[64][66], const T* in, int64_t ld, int R, int C, T* out, int Rp, int r0,
-                                               int c0, const int32_t* labels, int V) {
+// out[c][r] = row(r, c), a function that is 0 outside the input, for r < Rp and c < C: one 64 x 64 tile
+template <typename T, typename Row>
+__device__ __forceinline__ void transpose_tile(T (&tile)[64][66], Row row, int C, T* out, int Rp, int r0, int c0) {
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int r = r0 + ty + 4 * i, c = c0 + tx;
-    T v = T(0);
-    if (r < R && c < C && (!labels || (labels[r] >= 0 && labels[r] < V))) v = in[(int64_t)r * ld + c];
-    tile[ty + 4 * i][tx] = v;
+    tile[ty + 4 * i][tx] = row(r0 + ty + 4 * i, c0 + tx);
   }
   __syncthreads();
 #pragma unroll
@@ -123,20 +122,23 @@ __device__ __forceinline__ void transpose_tile(T (&tile)[64][66], const T* in, i
 template <typename T>
 __global__ __launch_bounds__(256) void xent_transpose_kernel(const T* in, int64_t ld, int R, int C, T* out, int Rp) {
   __shared__ T tile[64][66];
-  transpose_tile<T>(tile, in, ld, R, C, out, Rp, blockIdx.x * 64, blockIdx.y * 64, nullptr, 0);
+  transpose_tile<T>(tile, [&](int r, int c) { return r < R && c < C ? in[(int64_t)r * ld + c] : T(0); }, C, out, Rp,
+                    blockIdx.x * 64, blockIdx.y * 64);
 }
 
 // Everything the gradient needs before its first product, in one launch by roles of workgroups:
-//   - per row, padded: coef = gradient of the row's loss (0 without a label), lse / ln 2, label
-//   - h^T, zero in rows without a label and in the padding
+//   - per row, padded: coef = gradient of the row's loss (0 without a label), factor = 1 / unit (0 where coef is), lse / ln 2,
+//     label.  unit = high, or 1 where the smoothing leaves high = 0
+//   - (coef h)^T, zero in rows without a label and in the padding
 //   - column sums behind label smoothing, whose constant -coef_r low of every d(logit) is kept out of the 16-bit images:
 //     dh_r -= coef_r low sum_j w_j, dw_j -= low sum_r coef_r h_r.  part[block][d], added in block order afterwards
 constexpr int SUM_W = 256, SUM_H = 32;
 struct XentPrep {
   const void* h; const void* w; int64_t ldh, ldw;
   const int32_t* labels; const float* grad_row; const float* lse;
-  float* coef; float* lse2; int32_t* label;
+  float* coef; float* factor; float* lse2; int32_t* label;
   void* ht; float* part;
+  float inv_unit;
   int M, Mp, V, d, n_rows, n_turn;                 // workgroups of the first two roles
 };
 __device__ __forceinline__ float row_coef(const XentPrep& p, int r) {
@@ -152,7 +154,9 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
     const int r = b * 256 + threadIdx.x;
     if (r >= p.Mp) return;
     const bool used = r < p.M && p.labels[r] >= 0 && p.labels[r] < p.V;
-    p.coef[r] = r < p.M ? row_coef(p, r) : 0.f;
+    const float coef = r < p.M ? row_coef(p, r) : 0.f;
+    p.coef[r] = coef;
+    p.factor[r] = coef == 0.f ? 0.f : p.inv_unit;
     p.lse2[r] = r < p.M ? p.lse[r] * 1.44269504088896341f : 0.f;
     p.label[r] = used ? p.labels[r] : -1;
     return;
@@ -160,7 +164,13 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
   b -= p.n_rows;
   if (b < p.n_turn) {
     const int across = p.Mp / 64;
-    transpose_tile<T>(tile, (const T*)p.h, p.ldh, p.M, p.d, (T*)p.ht, p.Mp, b % across * 64, b / across * 64, p.labels, p.V);
+    auto row = [&](int r, int c) {
+      const float g = r < p.M ? row_coef(p, r) : 0.f;
+      T v = T(0);
+      if (g != 0.f && c < p.d) OpTraits<T>::store(&v, g * OpTraits<T>::load((const T*)p.h + (int64_t)r * p.ldh + c));
+      return v;
+    };
+    transpose_tile<T>(tile, row, p.d, (T*)p.ht, p.Mp, b % across * 64, b / across * 64);
     return;
   }
   b -= p.n_turn;
@@ -200,8 +210,8 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
     }
   }
 }
-// wsum, hsum = -low times the sums of the parts, 16 threads per column
-__global__ __launch_bounds__(1024) void xent_sums_kernel(const float* part, int d, float f, float* wsum, float* hsum) {
+// wsum = fw sum of w's parts, hsum = fh sum of h's, 16 threads per column
+__global__ __launch_bounds__(1024) void xent_sums_kernel(const float* part, int d, float fw, float fh, float* wsum, float* hsum) {
   __shared__ float red[16][64];
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, c = blockIdx.x * 64 + tx;
   const bool of_w = blockIdx.y == 0;
@@ -221,14 +231,14 @@ __global__ __launch_bounds__(1024) void xent_sums_kernel(const float* part, int 
   if (ty == 0 && c < d) {
     float t = 0.f;
     for (int k = 0; k < 16; ++k) t += red[k][tx];
-    (of_w ? wsum : hsum)[c] = f * t;
+    (of_w ? wsum : hsum)[c] = (of_w ? fw : fh) * t;
   }
 }
 
-// dh = sum of the partials in order (+ the smoothing constant's part), rounded once
+// dh = coef (unit times the sum of the partials in order + the smoothing constant's part), rounded once
 template <typename T>
 __global__ __launch_bounds__(256) void xent_dh_kernel(const float* part, int n_part, int M, int d, const float* coef,
-                                                      const float* wsum, T* dh, int64_t ld) {
+                                                      float unit, const float* wsum, T* dh, int64_t ld) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = (int64_t)M * d;      // d % 4 == 0
   if (i >= n) return;
   const int64_t r = i / d;
@@ -243,8 +253,7 @@ __global__ __launch_bounds__(256) void xent_dh_kernel(const float* part, int n_p
   const float f = coef[r];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (wsum) s[e] = fmaf(f, wsum[c + e], s[e]);
-    if (f == 0.f) s[e] = 0.f;
+    s[e] = f == 0.f ? 0.f : f * fmaf(unit, s[e], wsum ? wsum[c + e] : 0.f);
   }
   VecIO<T, 4>::store(dh + r * ld + c, s);
 }
@@ -276,7 +285,7 @@ static int pad64(int n) { return (n + 63) / 64 * 64; }
 struct XentPlan {
   int rows_padded, piece, n_pieces, slices, kt_slice;        // a piece = slices of kt_slice k-tiles of 64 entries
   size_t bytes;
-  float *coef, *lse2, *part, *colsum, *wsum, *hsum;
+  float *coef, *factor, *lse2, *part, *colsum, *wsum, *hsum;
   int32_t* label;
   void *g, *gt, *wt, *ht, *splitk;
 };
@@ -299,6 +308,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.n_pieces = (a->V + q.piece - 1) / q.piece;
   Arena ar(base, cap);
   q.coef = ar.get<float>(q.rows_padded);
+  q.factor = ar.get<float>(q.rows_padded);
   q.lse2 = ar.get<float>(q.rows_padded);
   q.label = ar.get<int32_t>(q.rows_padded);
   q.gt = ar.take((size_t)q.piece * q.rows_padded * es);
@@ -363,25 +373,27 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
   }
   XentPlan q;
   carve_xent(a, (char*)ws, ws_bytes, q);
-  const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f;
+  const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f, high = 1.f - a->smoothing - low;
+  const float unit = high != 0.f ? high : 1.f;
   XentPrep pr{};
   pr.h = a->h; pr.w = a->w; pr.ldh = a->ldh; pr.ldw = a->ldw;
   pr.labels = a->labels; pr.grad_row = grad_row; pr.lse = lse;
-  pr.coef = q.coef; pr.lse2 = q.lse2; pr.label = q.label; pr.ht = q.ht; pr.part = q.colsum;
+  pr.coef = q.coef; pr.factor = q.factor; pr.inv_unit = 1.f / unit; pr.lse2 = q.lse2; pr.label = q.label; pr.ht = q.ht; pr.part = q.colsum;
   pr.M = a->M; pr.Mp = q.rows_padded; pr.V = a->V; pr.d = a->d;
   pr.n_rows = (q.rows_padded + 255) / 256;
   pr.n_turn = q.rows_padded / 64 * ((a->d + 63) / 64);
   hipLaunchKernelGGL(xent_prep_kernel<T>, dim3(pr.n_rows + pr.n_turn + (low > 0.f ? SUM_W + SUM_H : 0)), dim3(256), 0, st, pr);
   NMTGAN_CHECK_LAUNCH("linear_xent_prep");
   if (low > 0.f) {
-    hipLaunchKernelGGL(xent_sums_kernel, dim3((a->d + 63) / 64, 2), dim3(1024), 0, st, q.colsum, a->d, -low, q.wsum, q.hsum);
+    hipLaunchKernelGGL(xent_sums_kernel, dim3((a->d + 63) / 64, 2), dim3(1024), 0, st, q.colsum, a->d, -low,
+                       -low / unit, q.wsum, q.hsum);
     NMTGAN_CHECK_LAUNCH("linear_xent_sums");
   }
   XentEpilogue x{};
-  x.coef = q.coef; x.lse2 = q.lse2; x.label = q.label; x.g = q.g; x.gt = q.gt;
+  x.factor = q.factor; x.lse2 = q.lse2; x.label = q.label; x.g = q.g; x.gt = q.gt;
   x.rows_padded = q.rows_padded;
   x.piece_padded = q.piece;
-  x.high = 1.f - a->smoothing - low;
+  x.high = high;
   int n_part = 0;
   for (int v0 = 0; v0 < a->V; v0 += q.piece) {
     const int n = std::min(q.piece, a->V - v0);
@@ -412,12 +424,12 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
     b.epilogue = NMTGAN_EPI_LINEAR;
     b.A = q.gt; b.lda = q.rows_padded; b.Wt = q.ht; b.bias = q.hsum;
     b.M = n; b.N = a->d; b.K = q.rows_padded;
-    b.n_seg = 1; b.out[0] = (T*)dw + (int64_t)v0 * ld_dw; b.ldo[0] = ld_dw; b.out_f32[0] = es == 4; b.seg_scale[0] = 1.f;
+    b.n_seg = 1; b.out[0] = (T*)dw + (int64_t)v0 * ld_dw; b.ldo[0] = ld_dw; b.out_f32[0] = es == 4; b.seg_scale[0] = unit;
     SplitKScope scope(q.splitk, SPLITK_BYTES);
     NMTGAN_TRY(launch_gemm(&b, st));
   }
   hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, n_part,
-                     a->M, a->d, q.coef, q.wsum, (T*)dh, ld_dh);
+                     a->M, a->d, q.coef, unit, q.wsum, (T*)dh, ld_dh);
   NMTGAN_CHECK_LAUNCH("linear_xent_dh");
   return 0;
 }

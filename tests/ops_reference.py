@@ -117,15 +117,17 @@ def xent_reference(h, w, labels, smoothing=0.0, grad_row=None):
     dz = torch.where((g != 0)[:, None], (P - wanted) * g[:, None], torch.zeros_like(z))
     e_dz = torch.where((g != 0)[:, None], (P * (e_z + e_lse[:, None] + 8 * E * (2 + far[:, None])) + 4 * E * wanted) * g[:, None].abs(),
                        torch.zeros_like(z))
-    # on its way into a product the entry-dependent part g p (g (p - 1 + smoothing) at the label) is rounded once; the
-    # constant part of label smoothing is summed apart in fp32
+    # on its way into the products the entry-dependent part, p / high - [label], is rounded once: g high u |p / high - [label]|
+    # <= g u (p + [label]) as |high| <= 1; the constant part of label smoothing is summed apart in fp32
     label_part = torch.zeros_like(z)
     label_part[torch.arange(h.shape[0], device=h.device), labels.clamp(0, v - 1).long()] = 1.0
-    e_dz = e_dz + u * ((P + label_part) * g[:, None].abs() * (g != 0)[:, None] + e_dz).nan_to_num(0.0)
+    e_img = u * ((P + label_part) * g[:, None].abs() * (g != 0)[:, None] + e_dz).nan_to_num(0.0)
+    e_dz = e_dz + e_img
     rows = float(h.shape[0])
     dh, dw = dz @ W, dz.t() @ H
     e_dh = e_dz @ W.abs() + (v + 8) * E * (dz.abs() @ W.abs())
-    e_dw = e_dz.t() @ H.abs() + (rows + 64) * E * (dz.abs().t() @ H.abs())
+    # dw's other factor is g h, rounded once too: u |g h| per term of the same size, (1 + u) for the two roundings together
+    e_dw = (e_dz + (1 + u) * e_img).t() @ H.abs() + (rows + 64) * E * (dz.abs().t() @ H.abs())
     res["dh"] = (dh, e_dh + HALF[dt] * (dh.abs() + e_dh) + 1e-30)
     res["dw"] = (dw, e_dw + HALF[dt] * (dw.abs() + e_dw) + 1e-30)
     return res
