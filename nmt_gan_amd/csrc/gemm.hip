@@ -198,58 +198,66 @@ __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)
   }
 }
 
-// XGRAD: C rows = hidden rows, C columns = entries, so a lane holds four consecutive rows of one entry = 8 bytes of the
-// entry-major image gt.  y = factor (exp(z - lse) - high [entry == label]), zero where no row or entry is (the images are
-// padded to whole k-tiles); factor = 1 / high.  Rows without a label have factor 0 and are 0 whatever their logits are.
+// XGRAD: C rows = hidden rows, C columns = entries.  y = factor (exp(z - lse) - high [entry == label]), zero where no row or
+// entry is (the images are padded to whole k-tiles); factor = 1 / high.  Rows without a label have factor 0 and are 0
+// whatever their logits are.  A lane holds four consecutive rows of one entry, 8 bytes of the entry-major image gt; with
+// WIDE the staging has put rows 8 q + 4 a + e of each 32 where 16 a + 4 q + e would be, so that a lane's two blocks join to
+// 16 bytes (3200 rows over 32000 entries, d = 512: 155 us, 183 with 8-byte stores).
 // rowv: the wave tile's rows as [factor | lse / ln 2 | label] of 16 MT each (LDS); null: from memory.
-template <typename OpT, int MT>
+template <typename OpT, int MT, bool WIDE = false>
 __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane,
                                                const float* rowv = nullptr) {
+  constexpr int NB = WIDE ? 2 : 1;               // blocks of four rows that a store takes
   const int fc = lane & 15, fq = lane >> 4;
   const XentEpilogue& x = p.x;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int mb = m0 + 16 * i + 4 * fq;
-    if (m0 + 16 * i >= x.rows_padded) continue;    // rows_padded is a multiple of 64
-    const float* at = rowv ? rowv + 16 * i + 4 * fq : x.factor + mb;
-    const int64_t step = rowv ? 16 * MT : x.lse2 - x.factor;
-    float factor[4], lse2[4];
-    VecIO<float, 4>::load(at, factor);
-    VecIO<float, 4>::load(at + step, lse2);
-    const int4 lab = *reinterpret_cast<const int4*>(rowv ? reinterpret_cast<const int32_t*>(at + 2 * step) : x.label + mb);
-    const int label[4] = {lab.x - x.first, lab.y - x.first, lab.z - x.first, lab.w - x.first};
-    bool hit = false, none = false;
+  for (int ib = 0; ib < MT; ib += NB) {
+    if (m0 + 16 * ib >= x.rows_padded) continue;   // rows_padded is a multiple of 64
+    const int first = 16 * ib + 4 * NB * fq, mb = m0 + first;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      hit = hit || (unsigned)(label[e] - n0) < 64u;
-      none = none || factor[e] == 0.f;
+    for (int i = ib; i < ib + NB; ++i) {
+      const int mr = first + 4 * (i - ib);
+      const float* at = rowv ? rowv + mr : x.factor + m0 + mr;
+      const int64_t step = rowv ? 16 * MT : x.lse2 - x.factor;
+      float factor[4], lse2[4];
+      VecIO<float, 4>::load(at, factor);
+      VecIO<float, 4>::load(at + step, lse2);
+      const int4 lab = *reinterpret_cast<const int4*>(rowv ? reinterpret_cast<const int32_t*>(at + 2 * step) : x.label + m0 + mr);
+      const int label[4] = {lab.x - x.first, lab.y - x.first, lab.z - x.first, lab.w - x.first};
+      bool hit = false, none = false;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc[i][j][e] = factor[e] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[e]));
-    }
-    if (__any(hit)) {
+      for (int e = 0; e < 4; ++e) {
+        hit = hit || (unsigned)(label[e] - n0) < 64u;
+        none = none || factor[e] == 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
+          acc[i][j][e] = factor[e] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[e]));
+      }
+      if (__any(hit)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n0 + 16 * j + fc == label[e]) acc[i][j][e] -= factor[e] * x.high;
-    }
-    if (__any(none)) {
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+          for (int e = 0; e < 4; ++e)
+            if (n0 + 16 * j + fc == label[e]) acc[i][j][e] -= factor[e] * x.high;
+      }
+      if (__any(none)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = factor[e] == 0.f ? 0.f : acc[i][j][e];
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = factor[e] == 0.f ? 0.f : acc[i][j][e];
+      }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int entry = n0 + 16 * j + fc;
       if (entry >= x.piece_padded) continue;
-      float d[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (entry >= p.N) d[0] = d[1] = d[2] = d[3] = 0.f;
-      VecIO<OpT, 4>::store(reinterpret_cast<OpT*>(x.gt) + (int64_t)entry * x.rows_padded + mb, d);
+      float d[4 * NB];
+#pragma unroll
+      for (int e = 0; e < 4 * NB; ++e) d[e] = entry < p.N ? acc[ib + e / 4][j][e & 3] : 0.f;
+      VecIO<OpT, 4 * NB>::store(reinterpret_cast<OpT*>(x.gt) + (int64_t)entry * x.rows_padded + mb, d);
       if (x.g) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4 * NB; ++e)
           if (mb + e < p.M) OpTraits<OpT>::store(reinterpret_cast<OpT*>(x.g) + (int64_t)(mb + e) * x.piece_padded + entry, d[e]);
       }
     }
@@ -1025,7 +1033,8 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
       const int rho = 8 * (wave + 8 * j) + (lane >> 3);
       const int lc = (lane & 7) ^ ((rho >> 1) & 7);
       if constexpr (u < 2) {
-        const int row = tm * QBM + (rho >> 6) * 128 + u * 64 + (rho & 63);
+        const int in = EPI == EPI_XGRAD ? (rho & 35) | ((rho & 12) << 1) | ((rho & 16) >> 2) : rho & 63;   // see its epilogue
+        const int row = tm * QBM + (rho >> 6) * 128 + u * 64 + in;
         src[u][j] = p.A + a_row_offset(p, min(row, p.M - 1)) + lc * 16;
       } else {
         const int col = tn * QBN + (rho >> 5) * 64 + (u - 2) * 32 + (rho & 31);
@@ -1234,7 +1243,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
     if constexpr (EPI == EPI_STATS) {
       epilogue_stats<8>(p, acc, m0, n0, lane);
     } else if constexpr (EPI == EPI_XGRAD) {
-      epilogue_xgrad<OpT, 8>(p, acc, m0, n0, lane, ev);
+      epilogue_xgrad<OpT, 8, true>(p, acc, m0, n0, lane, ev);
     } else if constexpr (KM) {
       GemmParams v{};
       v.M = p.M; v.N = p.N; v.n_seg = 1; v.out_f32[0] = 1; v.ldo[0] = p.N; v.seg_scale[0] = 1.f;
