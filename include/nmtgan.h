@@ -616,7 +616,8 @@ int nmtgan_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
  *   loss[i] = -sum_j q_j log softmax(h_i w^T)_j (label outside [0, V): 0),  lse[i] = log sum_j exp(h_i . w_j)
  * nmtgan_linear_xent_grads: bf16 or fp32; grad_row[i] = d(objective)/d(loss[i]) (NULL: 1; a mean over n rows is 1/n), lse of
  * the forward call; dh [M][d], dw [V][d] in `dtype` are overwritten.  Rows without a label have dh = 0 and add nothing to dw.
- * d(logits) is formed one piece of the vocabulary at a time in the workspace, rounded once to `dtype`.
+ * d(logits) is formed one piece of the vocabulary at a time in the workspace (about 224 MB at most, plus fp32 partial sums of
+ * dh), in bf16 rounded once to it where M V d > 2e8.  Outputs overlap neither each other nor an input.
  * d*esize a multiple of 16 bytes, rows 16-byte aligned, workspace 256-byte aligned. */
 typedef struct {
   int dtype;

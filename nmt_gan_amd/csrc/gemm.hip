@@ -198,9 +198,10 @@ __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)
   }
 }
 
-// XGRAD: C rows = hidden rows, C columns = entries.  y = factor (exp(z - lse) - high [entry == label]), zero where no row or
-// entry is (the images are padded to whole k-tiles); factor = 1 / high.  Rows without a label have factor 0 and are 0
-// whatever their logits are.  A lane holds four consecutive rows of one entry, 8 bytes of the entry-major image gt; with
+// XGRAD: C rows = hidden rows, C columns = entries.  y = factor (exp(z - lse) - high [entry == label] - low), zero where no
+// row or entry is (the image is padded); factor = 1 / high and low is left to the caller in the 16-bit types, whose image is
+// entry-major and rounded; fp32 has it row-major, with factor 1.  Rows without a label have factor 0 and are 0 whatever their
+// logits are.  A lane holds four consecutive rows of one entry, 8 bytes of the entry-major image; with
 // WIDE the staging has put rows 8 q + 4 a + e of each 32 where 16 a + 4 q + e would be, so that a lane's two blocks join to
 // 16 bytes (3200 rows over 32000 entries, d = 512: 155 us, 183 with 8-byte stores).
 // rowv: the wave tile's rows as [factor | lse / ln 2 | label] of 16 MT each (LDS); null: from memory.
@@ -230,8 +231,10 @@ __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)
         hit = hit || (unsigned)(label[e] - n0) < 64u;
         none = none || factor[e] == 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
           acc[i][j][e] = factor[e] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], 1.44269504088896341f, -lse2[e]));
+          if constexpr (sizeof(OpT) == 4) acc[i][j][e] -= x.low;
+        }
       }
       if (__any(hit)) {
 #pragma unroll
@@ -254,11 +257,12 @@ __device__ __forceinline__ void epilogue_xgrad(const GemmParams& p, f32x4 (&acc)
       float d[4 * NB];
 #pragma unroll
       for (int e = 0; e < 4 * NB; ++e) d[e] = entry < p.N ? acc[ib + e / 4][j][e & 3] : 0.f;
-      VecIO<OpT, 4 * NB>::store(reinterpret_cast<OpT*>(x.gt) + (int64_t)entry * x.rows_padded + mb, d);
-      if (x.g) {
+      if constexpr (sizeof(OpT) == 2) {
+        VecIO<OpT, 4 * NB>::store(reinterpret_cast<OpT*>(x.y) + (int64_t)entry * x.rows_padded + mb, d);
+      } else {
 #pragma unroll
         for (int e = 0; e < 4 * NB; ++e)
-          if (mb + e < p.M) OpTraits<OpT>::store(reinterpret_cast<OpT*>(x.g) + (int64_t)(mb + e) * x.piece_padded + entry, d[e]);
+          if (mb + e < p.M) OpTraits<OpT>::store(reinterpret_cast<OpT*>(x.y) + (int64_t)(mb + e) * x.piece_padded + entry, d[e]);
       }
     }
   }

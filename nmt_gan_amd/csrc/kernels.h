@@ -11,9 +11,9 @@ struct XentEpilogue {
   float* zsum;                                   // forward, label smoothing only
   // per hidden row, [rows_padded] each, 16-byte aligned: 1 / high (0 without a gradient), lse / ln 2, label (-1)
   const float* factor; const float* lse2; const int32_t* label;
-  void* g; void* gt;                             // [rows][piece_padded] (may be null), [piece_padded][rows_padded]
+  void* y;                                       // 16-bit types [piece_padded][rows_padded], fp32 [rows][piece_padded]
   int first, piece_padded, rows_padded;
-  float high;
+  float high, low;
 };
 int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
                      int K, float2* stats, const XentEpilogue& x, hipStream_t st);
@@ -61,6 +61,22 @@ size_t attn_span_step_workspace(int M, int heads, int kv_heads, int dh, int max_
 int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, size_t ws_bytes, hipStream_t st);
 size_t attn_span_grads_workspace(int M, int heads);
 int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g, void* ws, size_t ws_bytes, hipStream_t st);
+// the direct form of the cross entropy (xent_direct.hip) on entries first .. first + V - 1 of V_all.  Vp = V padded to 8
+// entries; stats and zsum per 32 entries and row
+struct XentDirect {
+  const void* h; const void* w; int64_t ldh, ldw;
+  const int32_t* labels;
+  int M, V, Vp, d, first, V_all;
+  float2* stats; float* zsum;                      // forward
+  const float* lse; const float* grad_row;         // gradient
+  float low, high;
+  float* coef; float* y; float* part;              // [M], [M][Vp], [slices][M][d] or null: dh itself
+  int slices;
+  void* dh; void* dw; int64_t ld_dh, ld_dw;
+  int n_dh;
+};
+int launch_xent_direct_z(int dtype, bool grad, const XentDirect& p, hipStream_t st);
+int launch_xent_direct_grads(int dtype, XentDirect p, hipStream_t st);
 size_t linear_xent_workspace(const nmtgan_xent_args* a, bool grads);
 int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void* ws, size_t ws_bytes, hipStream_t st);
 int launch_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh,

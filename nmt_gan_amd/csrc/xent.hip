@@ -120,13 +120,6 @@ __device__ __forceinline__ void transpose_tile(T (&tile)[64][66], Row row, int C
     if (c < C && r < Rp) out[(int64_t)c * Rp + r] = tile[tx][ty + 4 * i];
   }
 }
-template <typename T>
-__global__ __launch_bounds__(256) void xent_transpose_kernel(const T* in, int64_t ld, int R, int C, T* out, int Rp) {
-  __shared__ T tile[64][66];
-  transpose_tile<T>(tile, [&](int r, int c) { return r < R && c < C ? in[(int64_t)r * ld + c] : T(0); }, C, out, Rp,
-                    blockIdx.x * 64, blockIdx.y * 64);
-}
-
 // Everything the gradient needs before its first product, in one launch by roles of workgroups:
 //   - per row, padded: coef = gradient of the row's loss (0 without a label), factor = 1 / unit (0 where coef is), lse / ln 2,
 //     label.  unit = high, or 1 where the smoothing leaves high = 0
@@ -288,22 +281,25 @@ struct XentPlan {
   size_t bytes;
   float *coef, *factor, *lse2, *part, *colsum, *wsum, *hsum;
   int32_t* label;
-  void *g, *gt, *wt, *ht, *splitk;
+  void *y, *ht, *splitk;
 };
 constexpr size_t SPLITK_BYTES = 8 << 20;
 // Pieces of the vocabulary: as few as keep a piece's d(logits) inside the 256 MB memory-side cache (the two products read
-// what the epilogue wrote).  Inside a piece the hidden gradient's product is cut along the entries into enough slices to
-// give every CU a tile.
+// what the epilogue wrote).
+constexpr int64_t PIECE_BYTES = 224LL << 20;
+static int64_t pieces_of(const nmtgan_xent_args* a, int64_t entry_bytes) {
+  const int64_t fit = std::max<int64_t>(PIECE_BYTES / entry_bytes, 1);
+  return std::max<int64_t>(1, std::min<int64_t>((a->V + fit - 1) / fit, (a->V + 1023) / 1024));
+}
+// 16-bit products.  Inside a piece the hidden gradient's product is cut along the entries into enough slices to give every
+// CU a tile.
 static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPlan& q) {
   const int es = dtype_size(a->dtype);
-  const bool f32 = a->dtype == NMTGAN_F32;
   q.rows_padded = pad64(a->M);
-  const int64_t fit = (224LL << 20) / ((f32 ? 2LL : 1LL) * es * q.rows_padded);
-  int64_t n = (a->V + fit - 1) / std::max<int64_t>(fit, 1);
-  n = std::max<int64_t>(1, std::min<int64_t>(n, (a->V + 1023) / 1024));
+  const int64_t n = pieces_of(a, (int64_t)es * q.rows_padded);
   const int64_t want = (a->V + n - 1) / n, kt = std::max<int64_t>(4, (want + 63) / 64);
   const int64_t tiles = (int64_t)((a->M + 255) / 256) * ((a->d + 255) / 256);
-  q.slices = f32 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
+  q.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
   q.kt_slice = (int)((kt + q.slices - 1) / q.slices);
   q.piece = q.slices * q.kt_slice * 64;
   q.n_pieces = (a->V + q.piece - 1) / q.piece;
@@ -312,7 +308,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.factor = ar.get<float>(q.rows_padded);
   q.lse2 = ar.get<float>(q.rows_padded);
   q.label = ar.get<int32_t>(q.rows_padded);
-  q.gt = ar.take((size_t)q.piece * q.rows_padded * es);
+  q.y = ar.take((size_t)q.piece * q.rows_padded * es);
   q.ht = ar.take((size_t)a->d * q.rows_padded * es);
   q.part = ar.get<float>((size_t)q.n_pieces * q.slices * a->M * a->d);
   q.colsum = q.wsum = q.hsum = nullptr;
@@ -322,18 +318,79 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
     q.hsum = ar.get<float>(a->d);
   }
   q.splitk = ar.take(SPLITK_BYTES);
-  q.g = q.wt = nullptr;
-  if (f32) {
-    q.g = ar.take((size_t)a->M * q.piece * es);
-    q.wt = ar.take((size_t)a->d * q.piece * es);
+  q.bytes = ar.off;
+}
+// The direct form (xent_direct.hip) against this file's products on the library's tiles, by M V d:
+//   logits in fp32 up to 1e9 (50 x 9000 x 256: 18 us against 40, 900 x 9000 x 128: 52 against 45, 450 x 9000 x 512: 113
+//   against 73), in 16 bits never (50 x 9000 x 256: 19 against 15);
+//   gradient's products in fp32 always (97 x 509 x 64, with the logits: 17 us against 70, 900 x 9000 x 512: 515 against
+//   1362, 3200 x 32000 x 512: 5.9 ms against 6.6), in 16 bits up to 2e8 (50 x 9000 x 256: 39 against 59, 200 x 4000 x 256:
+//   48 against 49, 400 x 4000 x 256: 71 against 54).
+static int64_t xent_work(const nmtgan_xent_args* a) { return (int64_t)a->M * a->V * a->d; }
+static bool direct_logits(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 && xent_work(a) <= 1000000000; }
+static bool direct_grads(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 || xent_work(a) <= 200000000; }
+struct DirectPlan {
+  XentDirect p;
+  int piece, n_pieces;
+  size_t bytes;
+  float *part, *factor, *lse2;                   // the latter two and label for logits on the library's tiles only
+  int32_t* label;
+};
+static float xent_low(const nmtgan_xent_args* a) { return a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f; }
+static XentDirect direct_params(const nmtgan_xent_args* a) {
+  XentDirect p{};
+  p.h = a->h; p.w = a->w; p.ldh = a->ldh; p.ldw = a->ldw;
+  p.labels = a->labels;
+  p.M = a->M; p.V = a->V; p.Vp = (a->V + 7) / 8 * 8; p.d = a->d;
+  p.V_all = a->V;
+  p.low = xent_low(a);
+  p.high = 1.f - a->smoothing - p.low;
+  return p;
+}
+// Pieces as above; the hidden gradient's entries cut into slices of 1024 entries at least (16 waves share one), no more than
+// give every CU a workgroup
+static void carve_direct(const nmtgan_xent_args* a, char* base, size_t cap, DirectPlan& q) {
+  q.p = direct_params(a);
+  const int64_t n = pieces_of(a, 4LL * a->M);
+  q.piece = (int)((a->V + 8 * n - 1) / (8 * n) * 8);
+  q.n_pieces = (a->V + q.piece - 1) / q.piece;
+  const int64_t tiles = (int64_t)((a->M + 31) / 32) * ((a->d + 31) / 32);
+  q.p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(q.piece / 1024, 256 / tiles));
+  const int parts = q.n_pieces * q.p.slices;
+  Arena ar(base, cap);
+  q.p.coef = ar.get<float>(pad64(a->M));
+  q.p.y = ar.get<float>((size_t)a->M * q.piece);
+  q.part = parts > 1 ? ar.get<float>((size_t)parts * a->M * a->d) : nullptr;
+  q.factor = q.lse2 = nullptr;
+  q.label = nullptr;
+  if (!direct_logits(a) && a->dtype == NMTGAN_F32) {
+    q.factor = ar.get<float>(pad64(a->M));
+    q.lse2 = ar.get<float>(pad64(a->M));
+    q.label = ar.get<int32_t>(pad64(a->M));
   }
   q.bytes = ar.off;
+}
+// forward: statistics per 64 entries (32 in the direct form) and row
+static size_t carve_forward(const nmtgan_xent_args* a, char* base, size_t cap, int& tiles, float2*& stats, float*& zsum) {
+  const int per = direct_logits(a) ? 32 : 64;
+  tiles = (a->V + per - 1) / per;
+  Arena ar(base, cap);
+  stats = ar.get<float2>((size_t)tiles * a->M);
+  zsum = a->smoothing > 0.f ? ar.get<float>((size_t)tiles * a->M) : nullptr;
+  return ar.off;
 }
 size_t linear_xent_workspace(const nmtgan_xent_args* a, bool grads) {
   if (!a || a->M <= 0 || a->V <= 0 || a->d <= 0 || !valid_op_dtype(a->dtype)) return 0;
   if (!grads) {
-    const size_t n = (size_t)((a->V + 63) / 64) * a->M;
-    return align_up(n * sizeof(float2), 256) + (a->smoothing > 0.f ? n * sizeof(float) : 0);
+    int tiles;
+    float2* stats;
+    float* zsum;
+    return carve_forward(a, nullptr, 0, tiles, stats, zsum);
+  }
+  if (direct_grads(a)) {
+    DirectPlan q;
+    carve_direct(a, nullptr, 0, q);
+    return q.bytes;
   }
   XentPlan q;
   carve_xent(a, nullptr, 0, q);
@@ -348,12 +405,19 @@ int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void*
   const size_t need = linear_xent_workspace(a, false);
   NMTGAN_REQUIRE(ws && ws_bytes >= need && (uintptr_t)ws % 256 == 0, "linear_xent: workspace of %zu bytes (256-byte aligned) needed, %zu given",
                  need, ws_bytes);
-  const int tiles = (a->V + 63) / 64;
-  float2* stats = (float2*)ws;
+  int tiles;
+  float2* stats;
   XentEpilogue x{};
-  if (a->smoothing > 0.f) x.zsum = (float*)((char*)ws + align_up((size_t)tiles * a->M * sizeof(float2), 256));
-  NMTGAN_TRY(launch_gemm_xent(a->dtype, false, a->w, a->ldw, a->V, a->h, a->ldh, a->M, a->d, stats, x, st));
-  const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f, high = 1.f - a->smoothing - low;
+  carve_forward(a, (char*)ws, ws_bytes, tiles, stats, x.zsum);
+  if (direct_logits(a)) {
+    XentDirect p = direct_params(a);
+    p.stats = stats;
+    p.zsum = x.zsum;
+    NMTGAN_TRY(launch_xent_direct_z(a->dtype, false, p, st));
+  } else {
+    NMTGAN_TRY(launch_gemm_xent(a->dtype, false, a->w, a->ldw, a->V, a->h, a->ldh, a->M, a->d, stats, x, st));
+  }
+  const float low = xent_low(a), high = 1.f - a->smoothing - low;
   NMTGAN_DISPATCH_OP(a->dtype, T,
                      hipLaunchKernelGGL(xent_finish_kernel<T>, dim3((a->M + 15) / 16), dim3(256), 0, st, stats, x.zsum, tiles,
                                         (const T*)a->h, a->ldh, (const T*)a->w, a->ldw, a->labels, a->M, a->V, a->d, low, high,
@@ -363,18 +427,58 @@ int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void*
 }
 
 template <typename T>
-static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh, void* dw,
-                        int64_t ld_dw, void* ws, size_t ws_bytes, hipStream_t st) {
-  constexpr int es = sizeof(T);
-  if (a->M == 0) {
-    hipLaunchKernelGGL(xent_zero_rows_kernel<T>, dim3((unsigned)(((int64_t)a->V * a->d + 255) / 256)), dim3(256), 0, st, (T*)dw,
-                       ld_dw, a->V, a->d);
-    NMTGAN_CHECK_LAUNCH("linear_xent_zero");
-    return 0;
+static int direct_grads_t(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh, void* dw,
+                          int64_t ld_dw, void* ws, size_t ws_bytes, hipStream_t st) {
+  DirectPlan q;
+  carve_direct(a, (char*)ws, ws_bytes, q);
+  XentDirect& p = q.p;
+  p.lse = lse; p.grad_row = grad_row;
+  p.dh = dh; p.ld_dh = ld_dh; p.ld_dw = ld_dw;
+  if (q.factor) {
+    XentPrep pr{};
+    pr.labels = a->labels; pr.grad_row = grad_row; pr.lse = lse;
+    pr.coef = p.coef; pr.factor = q.factor; pr.lse2 = q.lse2; pr.label = q.label;
+    pr.inv_unit = 1.f;
+    pr.M = a->M; pr.Mp = pad64(a->M); pr.V = a->V;
+    pr.n_rows = (pr.Mp + 255) / 256;
+    hipLaunchKernelGGL(xent_prep_kernel<T>, dim3(pr.n_rows), dim3(256), 0, st, pr);
+    NMTGAN_CHECK_LAUNCH("linear_xent_prep");
   }
+  int parts = 0;
+  for (int v0 = 0; v0 < a->V; v0 += q.piece, parts += p.slices) {
+    p.first = v0;
+    p.V = std::min(q.piece, a->V - v0);
+    p.Vp = (p.V + 7) / 8 * 8;
+    p.w = (const T*)a->w + (int64_t)v0 * a->ldw;
+    p.dw = (T*)dw + (int64_t)v0 * ld_dw;
+    p.part = q.part ? q.part + (int64_t)parts * a->M * a->d : nullptr;
+    if (q.factor) {
+      XentEpilogue x{};
+      x.factor = q.factor; x.lse2 = q.lse2; x.label = q.label; x.y = p.y;
+      x.rows_padded = pad64(a->M);
+      x.piece_padded = p.Vp;
+      x.first = v0;
+      x.high = p.high;
+      x.low = p.low;
+      NMTGAN_TRY(launch_gemm_xent(a->dtype, true, p.w, a->ldw, p.V, a->h, a->ldh, a->M, a->d, nullptr, x, st));
+    } else {
+      NMTGAN_TRY(launch_xent_direct_z(a->dtype, true, p, st));
+    }
+    NMTGAN_TRY(launch_xent_direct_grads(a->dtype, p, st));
+  }
+  if (q.part) {
+    hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part,
+                       parts, a->M, a->d, p.coef, 1.f, nullptr, (T*)dh, ld_dh);
+    NMTGAN_CHECK_LAUNCH("linear_xent_dh");
+  }
+  return 0;
+}
+static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh, void* dw,
+                         int64_t ld_dw, void* ws, size_t ws_bytes, hipStream_t st) {
+  using T = bf16_t;
   XentPlan q;
   carve_xent(a, (char*)ws, ws_bytes, q);
-  const float low = a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f, high = 1.f - a->smoothing - low;
+  const float low = xent_low(a), high = 1.f - a->smoothing - low;
   const float unit = high != 0.f ? high : 1.f;
   XentPrep pr{};
   pr.h = a->h; pr.w = a->w; pr.ldh = a->ldh; pr.ldw = a->ldw;
@@ -391,7 +495,7 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
     NMTGAN_CHECK_LAUNCH("linear_xent_sums");
   }
   XentEpilogue x{};
-  x.factor = q.factor; x.lse2 = q.lse2; x.label = q.label; x.g = q.g; x.gt = q.gt;
+  x.factor = q.factor; x.lse2 = q.lse2; x.label = q.label; x.y = q.y;
   x.rows_padded = q.rows_padded;
   x.piece_padded = q.piece;
   x.high = high;
@@ -402,30 +506,15 @@ static int xent_grads_t(const nmtgan_xent_args* a, const float* lse, const float
     const T* w = (const T*)a->w + (int64_t)v0 * a->ldw;
     NMTGAN_TRY(launch_gemm_xent(a->dtype, true, w, a->ldw, n, a->h, a->ldh, a->M, a->d, nullptr, x, st));
     float* part = q.part + (int64_t)n_part * a->M * a->d;
-    if constexpr (es == 2) {
-      NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.gt, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice, part,
-                                    st));
-      n_part += q.slices;
-    } else {
-      hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3(q.piece / 64, (a->d + 63) / 64), dim3(256), 0, st, w, a->ldw, n, a->d,
-                         (T*)q.wt, q.piece);
-      NMTGAN_CHECK_LAUNCH("linear_xent_transpose");
-      nmtgan_gemm_args b{};
-      b.op_dtype = a->dtype;
-      b.epilogue = NMTGAN_EPI_LINEAR;
-      b.A = q.g; b.lda = q.piece; b.Wt = q.wt;
-      b.M = a->M; b.N = a->d; b.K = q.piece;
-      b.n_seg = 1; b.out[0] = part; b.ldo[0] = a->d; b.out_f32[0] = 1; b.seg_scale[0] = 1.f;
-      SplitKScope scope(q.splitk, SPLITK_BYTES);     // few tiles and a long k-loop: the library cuts it
-      NMTGAN_TRY(launch_gemm(&b, st));
-      n_part += 1;
-    }
+    NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.y, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice, part,
+                                  st));
+    n_part += q.slices;
     nmtgan_gemm_args b{};
     b.op_dtype = a->dtype;
     b.epilogue = NMTGAN_EPI_LINEAR;
-    b.A = q.gt; b.lda = q.rows_padded; b.Wt = q.ht; b.bias = q.hsum;
+    b.A = q.y; b.lda = q.rows_padded; b.Wt = q.ht; b.bias = q.hsum;
     b.M = n; b.N = a->d; b.K = q.rows_padded;
-    b.n_seg = 1; b.out[0] = (T*)dw + (int64_t)v0 * ld_dw; b.ldo[0] = ld_dw; b.out_f32[0] = es == 4; b.seg_scale[0] = unit;
+    b.n_seg = 1; b.out[0] = (T*)dw + (int64_t)v0 * ld_dw; b.ldo[0] = ld_dw; b.seg_scale[0] = unit;
     SplitKScope scope(q.splitk, SPLITK_BYTES);
     NMTGAN_TRY(launch_gemm(&b, st));
   }
@@ -446,8 +535,16 @@ int launch_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const 
   const size_t need = linear_xent_workspace(a, true);
   NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 256 == 0),
                  "linear_xent_grads: workspace of %zu bytes (256-byte aligned) needed, %zu given", need, ws_bytes);
-  if (a->dtype == NMTGAN_BF16) return xent_grads_t<bf16_t>(a, lse, grad_row, dh, ld_dh, dw, ld_dw, ws, ws_bytes, st);
-  return xent_grads_t<float>(a, lse, grad_row, dh, ld_dh, dw, ld_dw, ws, ws_bytes, st);
+  if (a->M == 0) {
+    NMTGAN_DISPATCH_OP(a->dtype, T,
+                       hipLaunchKernelGGL(xent_zero_rows_kernel<T>, dim3((unsigned)(((int64_t)a->V * a->d + 255) / 256)), dim3(256),
+                                          0, st, (T*)dw, ld_dw, a->V, a->d));
+    NMTGAN_CHECK_LAUNCH("linear_xent_zero");
+    return 0;
+  }
+  if (!direct_grads(a)) return xent_grads_16(a, lse, grad_row, dh, ld_dh, dw, ld_dw, ws, ws_bytes, st);
+  if (a->dtype == NMTGAN_BF16) return direct_grads_t<bf16_t>(a, lse, grad_row, dh, ld_dh, dw, ld_dw, ws, ws_bytes, st);
+  return direct_grads_t<float>(a, lse, grad_row, dh, ld_dh, dw, ld_dw, ws, ws_bytes, st);
 }
 
 }  // namespace nmtgan

@@ -1,0 +1,219 @@
+// Softmax cross entropy of hidden rows against a vocabulary table (formulas: xent.hip), the direct form: few launches and
+// 32 x 32 wave tiles, operands read from the caches in the layout they have and multiplied in fp32 (v_mfma_f32_32x32x2:
+// exact products of 16-bit operands, no rounding of d(logits)).  For little work, which on 256 x 256 tiles is launches, layout
+// changes and tiles that fill a few of the 256 CUs, and for fp32 gradients:
+//   forward: z^T by tiles with (max, sum exp) per row and 32 entries, then the finish kernel
+//   gradient: z again and y = dz / g [M][V] in fp32, then dh and dw side by side in one launch
+// Bound by the rate at which the caches answer: 8 flop per byte loaded, 54 TFLOP/s of the matrix cores' 154 at 3200 rows x
+// 32000 entries x 512; at 97 x 509 x 64 by the launches (17 us for both kernels, called back to back).
+// Which k goes into which slot of a product is free as long as both operands agree: lane half hl takes k = 8 s + 4 hl + t
+// in product t of step s, so that an operand with its k dimension in memory order is read by 16 bytes.
+#include "common.h"
+#include "kernels.h"
+
+namespace nmtgan {
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool ok, float (&o)[4]) {
+  if (ok) VecIO<T, 4>::load(p, o);
+  else o[0] = o[1] = o[2] = o[3] = 0.f;
+}
+__device__ __forceinline__ f32x16_t mul4(const float (&a)[4], const float (&b)[4], f32x16_t c) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f32x16_t zero16() {
+  f32x16_t c;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) c[r] = 0.f;
+  return c;
+}
+__device__ __forceinline__ float halves_sum(float v) { return v + __shfl_xor(v, 32); }
+
+// z^T: C rows = 32 entries, C columns = 32 hidden rows, so that a lane has 16 logits of one row.  grid: (groups of four
+// entry tiles, row tiles); a wave takes one tile.  GRAD: y = dz / g into y[M][Vp] (zero behind V and in rows
+// without a gradient), the rows' g into coef.
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void xent_direct_z_kernel(XentDirect p) {
+  const int lane = threadIdx.x & 63, hl = lane >> 5, tile = blockIdx.x * 4 + (threadIdx.x >> 6), e0 = tile * 32;
+  const int row = blockIdx.y * 32 + (lane & 31), rc = min(row, p.M - 1);
+  const int label = p.labels[rc];
+  const bool used = label >= 0 && label < p.V_all;
+  float coef = 0.f;
+  if constexpr (GRAD) {
+    coef = used ? (p.grad_row ? p.grad_row[rc] : 1.f) : 0.f;
+    if (tile == 0 && hl == 0 && row < p.M) p.coef[row] = coef;
+  }
+  if (e0 >= p.Vp) return;
+  const T* a = (const T*)p.w + (int64_t)min(e0 + (lane & 31), p.V - 1) * p.ldw + 4 * hl;
+  const T* b = (const T*)p.h + (int64_t)rc * p.ldh + 4 * hl;
+  f32x16_t z = zero16();
+  constexpr int U = 8;
+  for (int k = 0; k < p.d; k += 8 * U) {           // d is a multiple of 4
+    float x[U][4], y[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool ok = k + 8 * u + 4 * hl < p.d;
+      load4<T>(a + k + 8 * u, ok, x[u]);
+      load4<T>(b + k + 8 * u, ok, y[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) z = mul4(x[u], y[u], z);
+  }
+  if constexpr (GRAD) {
+    if (row >= p.M) return;
+    const float lse2 = p.lse[row] * 1.44269504088896341f;
+    float* out = p.y + (int64_t)row * p.Vp + e0 + 4 * hl;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int e = e0 + 8 * g + 4 * hl;
+      if (e >= p.Vp) continue;
+      float o[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float q = p.first + e + t == label ? p.high + p.low : p.low;
+        o[t] = __builtin_amdgcn_exp2f(fmaf(z[4 * g + t], 1.44269504088896341f, -lse2)) - q;
+        if (coef == 0.f || e + t >= p.V) o[t] = 0.f;
+      }
+      VecIO<float, 4>::store(out + 8 * g, o);
+    }
+  } else {
+    const int left = p.V - e0 - 4 * hl;            // entries of the lane: 8 (r / 4) + r % 4 < left
+    float mx = -INFINITY, zs = 0.f, s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const bool on = 8 * (r >> 2) + (r & 3) < left;
+      zs += on ? z[r] : 0.f;
+      z[r] = on ? z[r] : -INFINITY;
+      mx = fmaxf(mx, z[r]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mu2 = mx == -INFINITY ? 0.f : mx * 1.44269504088896341f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(z[r], 1.44269504088896341f, -mu2));
+    s = halves_sum(s);
+    zs = halves_sum(zs);
+    if (hl == 0 && row < p.M) {
+      p.stats[(int64_t)tile * p.M + row] = make_float2(mx, s);
+      if (p.zsum) p.zsum[(int64_t)tile * p.M + row] = zs;
+    }
+  }
+}
+
+// dh = g (y w) by the first n_dh workgroups, one slice of the entries of a 32 x 32 tile each, which 16 waves divide; dw =
+// y^T (g h) by the others, four tiles each, four waves dividing a tile's rows.  Waves are joined in order through LDS, one
+// element per thread; of several slices each leaves its part.  Loads go to clamped addresses and are selected afterwards:
+// under a condition each, they would not be in flight together.
+template <typename T>
+__global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
+  __shared__ float part[16][1024];
+  const int lane = threadIdx.x & 63, hl = lane >> 5, w = threadIdx.x >> 6;
+  f32x16_t c = zero16();
+  const int across = (p.d + 31) / 32;
+  const int reg = threadIdx.x >> 6, sub = 8 * (reg >> 2) + 4 * hl + (reg & 3);      // the element joined by this thread
+  if ((int)blockIdx.x < p.n_dh) {
+    const int slice = blockIdx.x % p.slices, tile = blockIdx.x / p.slices, share = slice * 16 + w, shares = 16 * p.slices;
+    const int r0 = tile / across * 32, c0 = tile % across * 32, col = c0 + (lane & 31);
+    const float* a = p.y + (int64_t)min(r0 + (lane & 31), p.M - 1) * p.Vp + 4 * hl;
+    const T* b = (const T*)p.w + min(col, p.d - 1);
+    const int n = p.Vp / 8, s1 = (int)((int64_t)n * (share + 1) / shares);
+    constexpr int U = 4;
+    for (int s = (int)((int64_t)n * share / shares); s < s1; s += U) {
+      float x[U][4], y[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = min(s + u, s1 - 1);
+        VecIO<float, 4>::load(a + 8 * at, x[u]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) y[u][t] = OpTraits<T>::load(b + (int64_t)min(8 * at + 4 * hl + t, p.V - 1) * p.ldw);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {              // entries behind the table count as zero: y is zero there, w is not read
+          const bool ok = s + u < s1 && 8 * (s + u) + 4 * hl + t < p.V;
+          x[u][t] = ok ? x[u][t] : 0.f;
+          y[u][t] = ok ? y[u][t] : 0.f;
+        }
+        c = mul4(x[u], y[u], c);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[r];
+    __syncthreads();
+    const int row = r0 + sub;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += part[k][threadIdx.x];
+    if (row < p.M && col < p.d) {
+      const float g = p.coef[row];
+      if (p.part) p.part[((int64_t)slice * p.M + row) * p.d + col] = s;
+      else OpTraits<T>::store((T*)p.dh + (int64_t)row * p.ld_dh + col, g == 0.f ? 0.f : g * s);
+    }
+    return;
+  }
+  const int tiles = (p.V + 31) / 32 * across, first = (blockIdx.x - p.n_dh) * 4;
+  {
+    const int tile = first + (w >> 2);
+    if (tile < tiles) {
+      const int e = tile / across * 32 + (lane & 31), col = tile % across * 32 + (lane & 31);
+      const float* a = p.y + min(e, p.V - 1);
+      const T* b = (const T*)p.h + min(col, p.d - 1);
+      const int n = (p.M + 7) / 8, s1 = n * ((w & 3) + 1) / 4;
+      constexpr int U = 2;
+      for (int s = n * (w & 3) / 4; s < s1; s += U) {
+        float x[U][4], y[U][4], g[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int r = min(8 * (s + u) + 4 * hl + t, p.M - 1);
+            x[u][t] = a[(int64_t)r * p.Vp];
+            y[u][t] = OpTraits<T>::load(b + (int64_t)r * p.ldh);
+            g[u][t] = p.coef[r];
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {            // rows without a gradient count as zero, whatever they hold
+            const bool ok = s + u < s1 && 8 * (s + u) + 4 * hl + t < p.M && g[u][t] != 0.f;
+            x[u][t] = ok ? x[u][t] : 0.f;
+            y[u][t] = ok ? g[u][t] * y[u][t] : 0.f;
+          }
+          c = mul4(x[u], y[u], c);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[r];
+  __syncthreads();
+  for (int q = 0; q < 4; ++q) {
+    const int tile = first + q, e = tile / across * 32 + sub, col = tile % across * 32 + (lane & 31);
+    if (tile >= tiles || e >= p.V || col >= p.d) continue;
+    const float s = (part[4 * q][threadIdx.x] + part[4 * q + 1][threadIdx.x]) + (part[4 * q + 2][threadIdx.x] + part[4 * q + 3][threadIdx.x]);
+    OpTraits<T>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, s);
+  }
+}
+
+int launch_xent_direct_z(int dtype, bool grad, const XentDirect& p, hipStream_t st) {
+  const dim3 grid((p.Vp + 127) / 128, (p.M + 31) / 32);
+  NMTGAN_DISPATCH_OP(dtype, T, {
+    if (grad) hipLaunchKernelGGL((xent_direct_z_kernel<T, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((xent_direct_z_kernel<T, false>), grid, dim3(256), 0, st, p);
+  });
+  NMTGAN_CHECK_LAUNCH("linear_xent_direct");
+  return 0;
+}
+int launch_xent_direct_grads(int dtype, XentDirect p, hipStream_t st) {
+  const int across = (p.d + 31) / 32;
+  p.n_dh = (p.M + 31) / 32 * across * p.slices;
+  const int64_t grid = p.n_dh + ((int64_t)(p.V + 31) / 32 * across + 3) / 4;
+  NMTGAN_REQUIRE(grid < (1LL << 31), "linear_xent_grads: too many tiles");
+  NMTGAN_DISPATCH_OP(dtype, T, hipLaunchKernelGGL(xent_direct_grads_kernel<T>, dim3((unsigned)grid), dim3(1024), 0, st, p));
+  NMTGAN_CHECK_LAUNCH("linear_xent_direct_grads");
+  return 0;
+}
+
+}  // namespace nmtgan

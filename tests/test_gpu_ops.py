@@ -301,6 +301,21 @@ def test_xent_many_pieces(cuda, op):
     _xent_case(cuda, _ops(), TYPES[op], 3001, 30011 if op == "bf16" else 18013, 128, 0.1, True, seed=2)
 
 
+@pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,v,d", [(700, 2600, 136), (700, 2600, 256), (601, 7003, 256), (2500, 6001, 256), (3001, 30011, 64)])
+def test_xent_more_work(cuda, op, m, v, d):
+    """Sizes on both sides of the choices between the products' forms, their tiles and one or several pieces."""
+    h, w, labels, gr, got = _xent_case(cuda, _ops(), TYPES[op], m, v, d, 0.1, True, seed=m, strided=True)
+    if op == "fp16":
+        return
+    ops, off = _ops(), (labels < 0) | (labels >= v)
+    h[off] = float("nan")
+    loss, lse = ops.linear_xent(h, w, labels, smoothing=0.1)
+    dh, dw = ops.linear_xent_grads(h, w, labels, lse, gr, smoothing=0.1)
+    for x, y in ((loss, got["loss"]), (lse[~off], got["lse"][~off]), (dh, got["dh"]), (dw, got["dw"])):
+        assert torch.equal(x, y)                     # rows without a label count nowhere, and sums have one order
+
+
 @pytest.mark.parametrize("op", ["bf16", "fp32"])
 def test_xent_strided_and_large_logits(cuda, op):
     _xent_case(cuda, _ops(), TYPES[op], 150, 700, 256, 0.1, True, seed=3, strided=True)
