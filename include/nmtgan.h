@@ -592,7 +592,7 @@ typedef struct {
   const void* k; int64_t ldk;
   const void* v; int64_t ldv;
   const int32_t* lo; const int32_t* hi;      /* [M] */
-  const int32_t* pos;                        /* [M] place of row i among the keys (for slopes); NULL: hi[i] - 1 */
+  const int32_t* pos;                        /* [M] place of row i among the keys (for slopes), within +-2^30; NULL: hi[i] - 1 */
   const float* slopes;                       /* [heads] or NULL */
   float scale, cap;                          /* cap <= 0 is refused unless exactly 0 = no cap */
   void* out; int64_t ldo;
@@ -616,8 +616,9 @@ int nmtgan_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
  *   loss[i] = -sum_j q_j log softmax(h_i w^T)_j (label outside [0, V): 0),  lse[i] = log sum_j exp(h_i . w_j)
  * nmtgan_linear_xent_grads: bf16 or fp32; grad_row[i] = d(objective)/d(loss[i]) (NULL: 1; a mean over n rows is 1/n), lse of
  * the forward call; dh [M][d], dw [V][d] in `dtype` are overwritten.  Rows without a label have dh = 0 and add nothing to dw.
- * d(logits) is formed one piece of the vocabulary at a time in the workspace (about 224 MB at most, plus fp32 partial sums of
- * dh), in bf16 rounded once to it where M V d > 2e8.  Outputs overlap neither each other nor an input.
+ * d(logits) is formed one piece of the vocabulary at a time in the workspace (about 224 MB or 256 entries, plus fp32 partial
+ * sums), in bf16 rounded once to it where M V d > 2e8.  Outputs overlap neither each other nor an input.  Gradients take at
+ * most 2^22 rows.
  * d*esize a multiple of 16 bytes, rows 16-byte aligned, workspace 256-byte aligned. */
 typedef struct {
   int dtype;

@@ -78,6 +78,7 @@ struct GemmParams {
   XentEpilogue x;
   // EPI_KPART (K-major operands, split_k slices of kt_slice k-tiles each): last k row and last 8-column chunk of A and W
   int kt_slice, ka_last, kw_last, m_last, n_last;
+  bool split_add;                                  // EPI_KPART adds to the parts
 };
 constexpr int EPI_STATS = 100;                  // internal: never a value of nmtgan_gemm_args.epilogue
 constexpr int EPI_XSTAT = 102, EPI_XGRAD = 103; // internal: vocabulary cross entropy, forward and d(logits)
@@ -1252,6 +1253,18 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
       GemmParams v{};
       v.M = p.M; v.N = p.N; v.n_seg = 1; v.out_f32[0] = 1; v.ldo[0] = p.N; v.seg_scale[0] = 1.f;
       v.out[0] = p.split_part + (int64_t)slice * p.M * p.N;
+      if (p.split_add) {
+        const float* had = reinterpret_cast<const float*>(v.out[0]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int m = m0 + 16 * i + 4 * fq + e, n = n0 + 16 * j + fc;
+              if (m < p.M && n < p.N) acc[i][j][e] += had[(int64_t)m * p.N + n];
+            }
+      }
       if (p.wide_ok && n0 < p.N) epilogue_wide<OpT, 8>(v, acc, m0, n0, lane, scr, true, 0, n0);
       else if (!p.wide_ok) epilogue<OpT, NMTGAN_EPI_LINEAR, 8>(v, acc, m0, n0, lane);
     } else if (wide) {
@@ -1960,11 +1973,11 @@ int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int en
   return 0;
 }
 
-// part[z][M][N] (fp32) = sum over k rows [64 z kt_slice, 64 (z + 1) kt_slice) of A[k][m] W[k][n], 16-bit operands; rows of A
-// from ka on and of W from kw on are not read, and one of the two holds zeros where the other ends.  lda, ldw in elements
+// part[z][M][N] (fp32; `add`: +=) = sum over k rows [64 z kt_slice, 64 (z + 1) kt_slice) of A[k][m] W[k][n], 16-bit
+// operands; rows of A from ka on and of W from kw on are not read, and one of the two holds zeros where the other ends.  lda, ldw in elements
 // (multiples of 8, at least M resp. N rounded up to 8); both matrices below 4 GiB.
 int launch_gemm_kmajor(int op_dtype, const void* A, int64_t lda, int ka, const void* W, int64_t ldw, int kw, int M, int N,
-                       int slices, int kt_slice, float* part, hipStream_t st) {
+                       int slices, int kt_slice, float* part, bool add, hipStream_t st) {
   NMTGAN_REQUIRE(op_dtype == NMTGAN_BF16, "gemm_kmajor: bf16 operands");
   NMTGAN_REQUIRE(A && W && part && M > 0 && N > 0 && ka > 0 && kw > 0 && slices > 0 && kt_slice >= 4 && lda % 8 == 0 && ldw % 8 == 0 &&
                      lda >= (M + 7) / 8 * 8 && ldw >= (N + 7) / 8 * 8 && (int64_t)ka * lda < (1LL << 31) && (int64_t)kw * ldw < (1LL << 31),
@@ -1973,7 +1986,7 @@ int launch_gemm_kmajor(int op_dtype, const void* A, int64_t lda, int ka, const v
   p.A = (const char*)A; p.W = (const char*)W;
   p.M = M; p.N = N;
   p.lda_b = lda * 2; p.ldw_b = ldw * 2;
-  p.split_k = slices; p.split_part = part; p.kt_slice = kt_slice;
+  p.split_k = slices; p.split_part = part; p.split_add = add; p.kt_slice = kt_slice;
   p.ka_last = ka - 1; p.kw_last = kw - 1;
   p.m_last = (M + 7) / 8 * 8 - 8; p.n_last = (N + 7) / 8 * 8 - 8;
   return launch_p8<bf16_t, EPI_KPART>(p, st);

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256) void clip_kernel(ListParams p, const double* p
   __shared__ double red[4];
   const double t = total_norm(part, n_part, grad_scale, red);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)t;
-  // a norm that is no finite number makes every output NaN, as tf.clip_by_global_norm does: the step is seen to be lost
+  // a norm that is no finite number makes every output NaN: the step is seen to be lost
   const float f = !(t < INFINITY) ? NAN : (t > (double)max_norm ? (float)((double)max_norm / t * (double)grad_scale) : grad_scale);
   for (int c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
     int64_t off;

@@ -18,7 +18,7 @@ struct XentEpilogue {
 int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
                      int K, float2* stats, const XentEpilogue& x, hipStream_t st);
 int launch_gemm_kmajor(int op_dtype, const void* A, int64_t lda, int ka, const void* W, int64_t ldw, int kw, int M, int N,
-                       int slices, int kt_slice, float* part, hipStream_t st);
+                       int slices, int kt_slice, float* part, bool add, hipStream_t st);
 int launch_gemm(const nmtgan_gemm_args* a, hipStream_t st);
 // n independent problems of one epilogue kind (CONVMAX - with or without the additive term - or LINEAR with one fp32 or
 // op-dtype output) in one persistent launch per 24 problems; min_tiles > 0 leaves problems of at least that many 256x128 tiles to
@@ -70,8 +70,9 @@ struct XentDirect {
   float2* stats; float* zsum;                      // forward
   const float* lse; const float* grad_row;         // gradient
   float low, high;
-  float* coef; float* y; float* part;              // [M], [M][Vp], [slices][M][d] or null: dh itself
-  int slices;
+  float* coef; float* y;                           // [M], [M][Vp]
+  float* part; int slices; bool add;               // [slices][M][d] (added to?) or null: dh itself
+  float* part_w; int row_slices, waves;            // [row_slices][V][d] or null: dw itself; waves per tile of dw, 4 or 16
   void* dh; void* dw; int64_t ld_dh, ld_dw;
   int n_dh;
 };

@@ -391,7 +391,8 @@ static bool rows_ok(const void* ptr, int64_t ld, int64_t width, int es) {
 static int fill_span(const nmtgan_span_args* a, SpanParams& p, const char* what) {
   NMTGAN_REQUIRE(a != nullptr, "%s: null args", what);
   NMTGAN_REQUIRE(valid_op_dtype(a->dtype), "%s: bad dtype %d", what, a->dtype);
-  NMTGAN_REQUIRE(a->M >= 0 && a->N >= 0, "%s: bad shape M=%d N=%d", what, a->M, a->N);
+  constexpr int MOST = INT32_MAX - 65536;         // indexes run over the end of the last tile
+  NMTGAN_REQUIRE(a->M >= 0 && a->N >= 0 && a->M <= MOST && a->N <= MOST, "%s: bad shape M=%d N=%d", what, a->M, a->N);
   NMTGAN_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads <= 4096,
                  "%s: heads=%d must be a multiple of kv_heads=%d, at most 4096", what, a->heads, a->kv_heads);
   NMTGAN_REQUIRE(a->dh > 0 && a->dh % 8 == 0 && a->dh <= SPAN_MAX_DH, "%s: head width %d must be a multiple of 8, at most %d",
@@ -487,7 +488,7 @@ int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, siz
   NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0),
                  "attn_span_step: workspace of %zu bytes needed, %zu given", need, ws_bytes);
   const int splits = span_splits(p.M, p.kv_heads, max_keys);
-  NMTGAN_REQUIRE((int64_t)p.M * splits < (1LL << 31), "attn_span_step: too many rows");
+  NMTGAN_REQUIRE((int64_t)p.M * splits < (1LL << 31) && ((int64_t)p.M * p.heads + 3) / 4 < (1LL << 31), "attn_span_step: too many rows");
   NMTGAN_DISPATCH_OP(a->dtype, T, {
     if (p.dh <= 32) NMTGAN_TRY((choose_step<T, 32>(p, splits, (float*)ws, st)));
     else if (p.dh <= 64) NMTGAN_TRY((choose_step<T, 64>(p, splits, (float*)ws, st)));

@@ -7,7 +7,7 @@
 //   dp = dout_i . v_j   delta_i = dout_i . out_i   dr = p (dp - delta_i) (1 - t^2) scale
 //   dq_i = sum_j dr k_j    dk_j = sum_i dr q_i    dv_j = sum_i p dout_i   (sums over the heads that share a key head too)
 //
-// The tile kernels (span_fwd.hip, span_grad.hip) multiply whole tiles on the matrix cores and give the pairs outside the
+// The tile kernels (span_fwd.hip, span_dq.hip, span_dkv.hip) multiply whole tiles on the matrix cores and give the pairs outside the
 // spans the weight zero.  A NaN or an infinity in such a row would still come through (0 x NaN), so a wave that ends with
 // a value that is not finite does those rows again with the row functions below: one row by one wave in plain fp32
 // arithmetic over visible (row, key) pairs only.

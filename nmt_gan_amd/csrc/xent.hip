@@ -229,7 +229,8 @@ __global__ __launch_bounds__(1024) void xent_sums_kernel(const float* part, int 
   }
 }
 
-// dh = coef (unit times the sum of the partials in order + the smoothing constant's part), rounded once
+// dh = coef (unit times the sum of the partials in order + the smoothing constant's part), rounded once; without coef the
+// plain sum
 template <typename T>
 __global__ __launch_bounds__(256) void xent_dh_kernel(const float* part, int n_part, int M, int d, const float* coef,
                                                       float unit, const float* wsum, T* dh, int64_t ld) {
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(256) void xent_dh_kernel(const float* part, int n_p
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += v[e];
   }
-  const float f = coef[r];
+  const float f = coef ? coef[r] : 1.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     s[e] = f == 0.f ? 0.f : f * fmaf(unit, s[e], wsum ? wsum[c + e] : 0.f);
@@ -262,7 +263,12 @@ __global__ __launch_bounds__(256) void xent_zero_rows_kernel(T* out, int64_t ld,
 static int check_xent(const nmtgan_xent_args* a, const char* what) {
   NMTGAN_REQUIRE(a != nullptr, "%s: null args", what);
   NMTGAN_REQUIRE(valid_op_dtype(a->dtype), "%s: bad dtype %d", what, a->dtype);
-  NMTGAN_REQUIRE(a->M >= 0 && a->V > 0 && a->d > 0, "%s: bad shape M=%d V=%d d=%d", what, a->M, a->V, a->d);
+  constexpr int MOST = INT32_MAX - 65536;         // indexes run over the end of the last tile
+  NMTGAN_REQUIRE(a->M >= 0 && a->V > 0 && a->d > 0 && a->M <= MOST && a->V <= MOST, "%s: bad shape M=%d V=%d d=%d", what, a->M,
+                 a->V, a->d);
+  NMTGAN_REQUIRE((int64_t)((a->M + 127) / 128) * ((a->V + 127) / 128) < (1LL << 31), "%s: more than 2^31 tiles of 128 x 128 logits",
+                 what);
+  NMTGAN_REQUIRE(a->ldw <= 1 << 20 && a->ldh <= 1 << 20, "%s: rows further than 2^20 elements apart", what);
   const int es = dtype_size(a->dtype);
   NMTGAN_REQUIRE((int64_t)a->d * es % 16 == 0, "%s: d*esize must be a multiple of 16 bytes (d=%d)", what, a->d);
   NMTGAN_REQUIRE(a->smoothing >= 0.f && a->smoothing < 1.f && (a->smoothing == 0.f || a->V > 1),
@@ -289,14 +295,14 @@ constexpr size_t SPLITK_BYTES = 8 << 20;
 constexpr int64_t PIECE_BYTES = 224LL << 20;
 static int64_t pieces_of(const nmtgan_xent_args* a, int64_t entry_bytes) {
   const int64_t fit = std::max<int64_t>(PIECE_BYTES / entry_bytes, 1);
-  return std::max<int64_t>(1, std::min<int64_t>((a->V + fit - 1) / fit, (a->V + 1023) / 1024));
+  return std::max<int64_t>(1, std::min<int64_t>((a->V + fit - 1) / fit, (a->V + 255) / 256));
 }
 // 16-bit products.  Inside a piece the hidden gradient's product is cut along the entries into enough slices to give every
 // CU a tile.
 static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPlan& q) {
   const int es = dtype_size(a->dtype);
   q.rows_padded = pad64(a->M);
-  const int64_t n = pieces_of(a, (int64_t)es * q.rows_padded);
+  const int64_t n = std::max<int64_t>(pieces_of(a, (int64_t)es * q.rows_padded), (a->V * a->ldw + (1LL << 30) - 1) >> 30);   // (32-bit offsets)
   const int64_t want = (a->V + n - 1) / n, kt = std::max<int64_t>(4, (want + 63) / 64);
   const int64_t tiles = (int64_t)((a->M + 255) / 256) * ((a->d + 255) / 256);
   q.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
@@ -310,7 +316,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.label = ar.get<int32_t>(q.rows_padded);
   q.y = ar.take((size_t)q.piece * q.rows_padded * es);
   q.ht = ar.take((size_t)a->d * q.rows_padded * es);
-  q.part = ar.get<float>((size_t)q.n_pieces * q.slices * a->M * a->d);
+  q.part = ar.get<float>((size_t)q.slices * a->M * a->d);
   q.colsum = q.wsum = q.hsum = nullptr;
   if (a->smoothing > 0.f) {
     q.colsum = ar.get<float>((size_t)(SUM_W + SUM_H) * a->d);
@@ -333,7 +339,7 @@ struct DirectPlan {
   XentDirect p;
   int piece, n_pieces;
   size_t bytes;
-  float *part, *factor, *lse2;                   // the latter two and label for logits on the library's tiles only
+  float *factor, *lse2;                          // these and label for logits on the library's tiles only
   int32_t* label;
 };
 static float xent_low(const nmtgan_xent_args* a) { return a->smoothing > 0.f ? a->smoothing / (float)(a->V - 1) : 0.f; }
@@ -347,8 +353,8 @@ static XentDirect direct_params(const nmtgan_xent_args* a) {
   p.high = 1.f - a->smoothing - p.low;
   return p;
 }
-// Pieces as above; the hidden gradient's entries cut into slices of 1024 entries at least (16 waves share one), no more than
-// give every CU a workgroup
+// Pieces as above; dh's entries cut into slices of 1024 at least (16 waves share one) and dw's rows into slices of 2048 at
+// least, no more than give every CU a workgroup
 static void carve_direct(const nmtgan_xent_args* a, char* base, size_t cap, DirectPlan& q) {
   q.p = direct_params(a);
   const int64_t n = pieces_of(a, 4LL * a->M);
@@ -356,11 +362,14 @@ static void carve_direct(const nmtgan_xent_args* a, char* base, size_t cap, Dire
   q.n_pieces = (a->V + q.piece - 1) / q.piece;
   const int64_t tiles = (int64_t)((a->M + 31) / 32) * ((a->d + 31) / 32);
   q.p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(q.piece / 1024, 256 / tiles));
-  const int parts = q.n_pieces * q.p.slices;
+  const int64_t tiles_w = (int64_t)((q.piece + 31) / 32) * ((a->d + 31) / 32);
+  q.p.waves = tiles_w < 1024 ? 16 : 4;
+  q.p.row_slices = (int)std::max<int64_t>(1, std::min<int64_t>(a->M / 2048, 256 * 16 / (tiles_w * q.p.waves)));
   Arena ar(base, cap);
   q.p.coef = ar.get<float>(pad64(a->M));
   q.p.y = ar.get<float>((size_t)a->M * q.piece);
-  q.part = parts > 1 ? ar.get<float>((size_t)parts * a->M * a->d) : nullptr;
+  q.p.part = q.n_pieces > 1 || q.p.slices > 1 ? ar.get<float>((size_t)q.p.slices * a->M * a->d) : nullptr;
+  q.p.part_w = q.p.row_slices > 1 ? ar.get<float>((size_t)q.p.row_slices * q.piece * a->d) : nullptr;
   q.factor = q.lse2 = nullptr;
   q.label = nullptr;
   if (!direct_logits(a) && a->dtype == NMTGAN_F32) {
@@ -444,14 +453,19 @@ static int direct_grads_t(const nmtgan_xent_args* a, const float* lse, const flo
     hipLaunchKernelGGL(xent_prep_kernel<T>, dim3(pr.n_rows), dim3(256), 0, st, pr);
     NMTGAN_CHECK_LAUNCH("linear_xent_prep");
   }
-  int parts = 0;
-  for (int v0 = 0; v0 < a->V; v0 += q.piece, parts += p.slices) {
+  auto sum = [&](const float* part, int n, int rows, const float* coef, T* out, int64_t ld) -> int {
+    hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)rows * a->d / 4 + 255) / 256)), dim3(256), 0, st, part, n,
+                       rows, a->d, coef, 1.f, nullptr, out, ld);
+    NMTGAN_CHECK_LAUNCH("linear_xent_sum");
+    return 0;
+  };
+  for (int v0 = 0; v0 < a->V; v0 += q.piece) {
     p.first = v0;
     p.V = std::min(q.piece, a->V - v0);
     p.Vp = (p.V + 7) / 8 * 8;
     p.w = (const T*)a->w + (int64_t)v0 * a->ldw;
     p.dw = (T*)dw + (int64_t)v0 * ld_dw;
-    p.part = q.part ? q.part + (int64_t)parts * a->M * a->d : nullptr;
+    p.add = v0 > 0;
     if (q.factor) {
       XentEpilogue x{};
       x.factor = q.factor; x.lse2 = q.lse2; x.label = q.label; x.y = p.y;
@@ -465,12 +479,9 @@ static int direct_grads_t(const nmtgan_xent_args* a, const float* lse, const flo
       NMTGAN_TRY(launch_xent_direct_z(a->dtype, true, p, st));
     }
     NMTGAN_TRY(launch_xent_direct_grads(a->dtype, p, st));
+    if (p.part_w) NMTGAN_TRY(sum(p.part_w, p.row_slices, p.V, nullptr, (T*)p.dw, ld_dw));
   }
-  if (q.part) {
-    hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part,
-                       parts, a->M, a->d, p.coef, 1.f, nullptr, (T*)dh, ld_dh);
-    NMTGAN_CHECK_LAUNCH("linear_xent_dh");
-  }
+  if (p.part) NMTGAN_TRY(sum(p.part, p.slices, a->M, p.coef, (T*)dh, ld_dh));
   return 0;
 }
 static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const float* grad_row, void* dh, int64_t ld_dh, void* dw,
@@ -499,16 +510,13 @@ static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const floa
   x.rows_padded = q.rows_padded;
   x.piece_padded = q.piece;
   x.high = high;
-  int n_part = 0;
   for (int v0 = 0; v0 < a->V; v0 += q.piece) {
     const int n = std::min(q.piece, a->V - v0);
     x.first = v0;
     const T* w = (const T*)a->w + (int64_t)v0 * a->ldw;
     NMTGAN_TRY(launch_gemm_xent(a->dtype, true, w, a->ldw, n, a->h, a->ldh, a->M, a->d, nullptr, x, st));
-    float* part = q.part + (int64_t)n_part * a->M * a->d;
-    NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.y, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice, part,
-                                  st));
-    n_part += q.slices;
+    NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.y, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice, q.part,
+                                  v0 > 0, st));
     nmtgan_gemm_args b{};
     b.op_dtype = a->dtype;
     b.epilogue = NMTGAN_EPI_LINEAR;
@@ -518,7 +526,7 @@ static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const floa
     SplitKScope scope(q.splitk, SPLITK_BYTES);
     NMTGAN_TRY(launch_gemm(&b, st));
   }
-  hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, n_part,
+  hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, q.slices,
                      a->M, a->d, q.coef, unit, q.wsum, (T*)dh, ld_dh);
   NMTGAN_CHECK_LAUNCH("linear_xent_dh");
   return 0;
@@ -532,6 +540,7 @@ int launch_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const 
   NMTGAN_REQUIRE(dw && (uintptr_t)dw % 16 == 0 && ld_dw >= a->d && ld_dw * es % 16 == 0, "linear_xent_grads: bad dw");
   NMTGAN_REQUIRE(a->M == 0 || (lse && dh && (uintptr_t)dh % 16 == 0 && ld_dh >= a->d && ld_dh * es % 16 == 0),
                  "linear_xent_grads: null lse or bad dh");
+  NMTGAN_REQUIRE(a->M <= 1 << 22, "linear_xent_grads: more than 2^22 rows (a column of d(logits) would outgrow its piece)");
   const size_t need = linear_xent_workspace(a, true);
   NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 256 == 0),
                  "linear_xent_grads: workspace of %zu bytes (256-byte aligned) needed, %zu given", need, ws_bytes);

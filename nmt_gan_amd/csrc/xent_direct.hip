@@ -31,13 +31,14 @@ __device__ __forceinline__ f32x16_t zero16() {
 }
 __device__ __forceinline__ float halves_sum(float v) { return v + __shfl_xor(v, 32); }
 
-// z^T: C rows = 32 entries, C columns = 32 hidden rows, so that a lane has 16 logits of one row.  grid: (groups of four
-// entry tiles, row tiles); a wave takes one tile.  GRAD: y = dz / g into y[M][Vp] (zero behind V and in rows
+// z^T: C rows = 32 entries, C columns = 32 hidden rows, so that a lane has 16 logits of one row.  A workgroup takes four
+// entry tiles of a row tile, a wave each.  GRAD: y = dz / g into y[M][Vp] (zero behind V and in rows
 // without a gradient), the rows' g into coef.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void xent_direct_z_kernel(XentDirect p) {
-  const int lane = threadIdx.x & 63, hl = lane >> 5, tile = blockIdx.x * 4 + (threadIdx.x >> 6), e0 = tile * 32;
-  const int row = blockIdx.y * 32 + (lane & 31), rc = min(row, p.M - 1);
+  const int across = (p.Vp + 127) / 128;
+  const int lane = threadIdx.x & 63, hl = lane >> 5, tile = blockIdx.x % across * 4 + (threadIdx.x >> 6), e0 = tile * 32;
+  const int row = blockIdx.x / across * 32 + (lane & 31), rc = min(row, p.M - 1);
   const int label = p.labels[rc];
   const bool used = label >= 0 && label < p.V_all;
   float coef = 0.f;
@@ -102,8 +103,8 @@ __global__ __launch_bounds__(256) void xent_direct_z_kernel(XentDirect p) {
 }
 
 // dh = g (y w) by the first n_dh workgroups, one slice of the entries of a 32 x 32 tile each, which 16 waves divide; dw =
-// y^T (g h) by the others, four tiles each, four waves dividing a tile's rows.  Waves are joined in order through LDS, one
-// element per thread; of several slices each leaves its part.  Loads go to clamped addresses and are selected afterwards:
+// y^T (g h) by the others, one slice of the rows of one tile or of four, which 16 or four waves divide.  Waves are joined in
+// order through LDS, one element per thread; of several slices each leaves its part.  Loads go to clamped addresses and are selected afterwards:
 // under a condition each, they would not be in flight together.
 template <typename T>
 __global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
@@ -148,21 +149,23 @@ __global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
     for (int k = 0; k < 16; ++k) s += part[k][threadIdx.x];
     if (row < p.M && col < p.d) {
       const float g = p.coef[row];
-      if (p.part) p.part[((int64_t)slice * p.M + row) * p.d + col] = s;
+      float* at = p.part + ((int64_t)slice * p.M + row) * p.d + col;
+      if (p.part) *at = p.add ? *at + s : s;
       else OpTraits<T>::store((T*)p.dh + (int64_t)row * p.ld_dh + col, g == 0.f ? 0.f : g * s);
     }
     return;
   }
-  const int tiles = (p.V + 31) / 32 * across, first = (blockIdx.x - p.n_dh) * 4;
+  const int per = p.waves, held = 16 / per, b = blockIdx.x - p.n_dh, slice = b % p.row_slices;
+  const int tiles = (p.V + 31) / 32 * across, first = b / p.row_slices * held;
   {
-    const int tile = first + (w >> 2);
+    const int tile = first + w / per, share = slice * per + w % per, shares = per * p.row_slices;
     if (tile < tiles) {
       const int e = tile / across * 32 + (lane & 31), col = tile % across * 32 + (lane & 31);
       const float* a = p.y + min(e, p.V - 1);
       const T* b = (const T*)p.h + min(col, p.d - 1);
-      const int n = (p.M + 7) / 8, s1 = n * ((w & 3) + 1) / 4;
+      const int n = (p.M + 7) / 8, s1 = (int)((int64_t)n * (share + 1) / shares);
       constexpr int U = 2;
-      for (int s = n * (w & 3) / 4; s < s1; s += U) {
+      for (int s = (int)((int64_t)n * share / shares); s < s1; s += U) {
         float x[U][4], y[U][4], g[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -189,16 +192,20 @@ __global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[r];
   __syncthreads();
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < held; ++q) {
     const int tile = first + q, e = tile / across * 32 + sub, col = tile % across * 32 + (lane & 31);
     if (tile >= tiles || e >= p.V || col >= p.d) continue;
-    const float s = (part[4 * q][threadIdx.x] + part[4 * q + 1][threadIdx.x]) + (part[4 * q + 2][threadIdx.x] + part[4 * q + 3][threadIdx.x]);
-    OpTraits<T>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, s);
+    float s = 0.f;
+    for (int k = q * per; k < (q + 1) * per; ++k) s += part[k][threadIdx.x];
+    if (p.part_w) p.part_w[((int64_t)slice * p.V + e) * p.d + col] = s;
+    else OpTraits<T>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, s);
   }
 }
 
 int launch_xent_direct_z(int dtype, bool grad, const XentDirect& p, hipStream_t st) {
-  const dim3 grid((p.Vp + 127) / 128, (p.M + 31) / 32);
+  const int64_t blocks = (int64_t)((p.Vp + 127) / 128) * ((p.M + 31) / 32);
+  NMTGAN_REQUIRE(blocks < (1LL << 31), "linear_xent: too many tiles");
+  const dim3 grid((unsigned)blocks);
   NMTGAN_DISPATCH_OP(dtype, T, {
     if (grad) hipLaunchKernelGGL((xent_direct_z_kernel<T, true>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((xent_direct_z_kernel<T, false>), grid, dim3(256), 0, st, p);
@@ -209,7 +216,8 @@ int launch_xent_direct_z(int dtype, bool grad, const XentDirect& p, hipStream_t 
 int launch_xent_direct_grads(int dtype, XentDirect p, hipStream_t st) {
   const int across = (p.d + 31) / 32;
   p.n_dh = (p.M + 31) / 32 * across * p.slices;
-  const int64_t grid = p.n_dh + ((int64_t)(p.V + 31) / 32 * across + 3) / 4;
+  const int64_t tiles = (int64_t)(p.V + 31) / 32 * across, held = 16 / p.waves;
+  const int64_t grid = p.n_dh + (tiles + held - 1) / held * p.row_slices;
   NMTGAN_REQUIRE(grid < (1LL << 31), "linear_xent_grads: too many tiles");
   NMTGAN_DISPATCH_OP(dtype, T, hipLaunchKernelGGL(xent_direct_grads_kernel<T>, dim3((unsigned)grid), dim3(1024), 0, st, p));
   NMTGAN_CHECK_LAUNCH("linear_xent_direct_grads");

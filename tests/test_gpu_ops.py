@@ -302,7 +302,8 @@ def test_xent_many_pieces(cuda, op):
 
 
 @pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("m,v,d", [(700, 2600, 136), (700, 2600, 256), (601, 7003, 256), (2500, 6001, 256), (3001, 30011, 64)])
+@pytest.mark.parametrize("m,v,d", [(700, 2600, 136), (700, 2600, 256), (601, 7003, 256), (2500, 6001, 256), (3001, 30011, 64),
+                                   (9001, 70, 40), (70001, 2100, 64)])
 def test_xent_more_work(cuda, op, m, v, d):
     """Sizes on both sides of the choices between the products' forms, their tiles and one or several pieces."""
     h, w, labels, gr, got = _xent_case(cuda, _ops(), TYPES[op], m, v, d, 0.1, True, seed=m, strided=True)
@@ -314,6 +315,12 @@ def test_xent_more_work(cuda, op, m, v, d):
     dh, dw = ops.linear_xent_grads(h, w, labels, lse, gr, smoothing=0.1)
     for x, y in ((loss, got["loss"]), (lse[~off], got["lse"][~off]), (dh, got["dh"]), (dw, got["dw"])):
         assert torch.equal(x, y)                     # rows without a label count nowhere, and sums have one order
+
+
+@pytest.mark.parametrize("op", ["bf16", "fp32"])
+def test_xent_two_million_rows(cuda, op):
+    """More row tiles than a grid's second dimension would hold."""
+    _xent_case(cuda, _ops(), TYPES[op], 2100003, 9, 8, 0.1, True, seed=8)
 
 
 @pytest.mark.parametrize("op", ["bf16", "fp32"])

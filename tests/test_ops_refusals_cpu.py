@@ -23,7 +23,7 @@ def _refused(rc, part):
 
 
 @pytest.mark.parametrize("kw,part", [
-    (dict(dtype=7), "dtype"), (dict(M=-1), "shape"), (dict(N=-1), "shape"), (dict(heads=0), "heads"), (dict(kv_heads=0), "heads"),
+    (dict(dtype=7), "dtype"), (dict(M=-1), "shape"), (dict(N=-1), "shape"), (dict(M=2**31 - 65000), "shape"), (dict(N=2**31 - 1), "shape"), (dict(heads=0), "heads"), (dict(kv_heads=0), "heads"),
     (dict(heads=3), "heads"), (dict(dh=0), "head width"), (dict(dh=60), "head width"), (dict(dh=136), "head width"),
     (dict(scale=float("inf")), "finite"), (dict(cap=-1.0), "cap"), (dict(cap=float("nan")), "cap"), (dict(q=None), "null"),
     (dict(lo=None), "null"), (dict(hi=None), "null"), (dict(out=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"),
@@ -72,7 +72,8 @@ def _xent(**kw):
 @pytest.mark.parametrize("kw,part", [
     (dict(dtype=3), "dtype"), (dict(M=-1), "shape"), (dict(V=0), "shape"), (dict(d=0), "shape"), (dict(d=62), "16 bytes"),
     (dict(smoothing=1.0), "smoothing"), (dict(smoothing=-0.1), "smoothing"), (dict(smoothing=0.1, V=1), "smoothing"), (dict(h=None), "null"),
-    (dict(labels=None), "null"), (dict(w=None), "null"), (dict(w=P + 4), "16-byte"), (dict(ldw=60), "16-byte"), (dict(ldh=65), "16-byte")])
+    (dict(labels=None), "null"), (dict(w=None), "null"), (dict(w=P + 4), "16-byte"), (dict(ldw=60), "16-byte"), (dict(ldh=65), "16-byte"),
+    (dict(M=2**31 - 1), "shape"), (dict(V=2**31 - 1), "shape"), (dict(M=2**30, V=2**30), "tiles"), (dict(ldw=2**21), "apart"), (dict(ldh=2**21), "apart")])
 def test_xent_refusals(kw, part):
     _refused(L.lib.nmtgan_linear_xent(C.byref(_xent(**kw)), P, P, P, 1 << 30, None), part)
     _refused(L.lib.nmtgan_linear_xent_grads(C.byref(_xent(**kw)), P, None, P, 64, P, 64, P, 1 << 30, None), part)
@@ -87,6 +88,7 @@ def test_xent_other_refusals():
     _refused(L.lib.nmtgan_linear_xent_grads(C.byref(_xent()), P, None, P, 60, P, 64, P, 1 << 30, None), "dh")
     _refused(L.lib.nmtgan_linear_xent_grads(C.byref(_xent()), P, None, P, 64, None, 64, P, 1 << 30, None), "dw")
     _refused(L.lib.nmtgan_linear_xent_grads(C.byref(_xent()), P, None, P, 64, P, 64, P, 8, None), "workspace")
+    _refused(L.lib.nmtgan_linear_xent_grads(C.byref(_xent(M=2**22 + 1)), P, None, P, 64, P, 64, P, 1 << 40, None), "2^22 rows")
 
 
 def _list(*refs):
