@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include <algorithm>
+#include <atomic>
 #include <vector>
 
 #include "common.h"
@@ -736,15 +737,21 @@ static inline int persistent_grid(int nwg) {
   return nwg < cus ? nwg : cus;
 }
 
+static uint64_t device_bit() {
+  int d = 0;
+  (void)hipGetDevice(&d);
+  return 1ull << (d & 63);
+}
 template <typename OpT, int EPI>
 static int launch_pipe(GemmParams p, hipStream_t st) {
   constexpr int smem = 3 * PSTAGE + PNW * 2048;  // 3 stages + per-wave epilogue scratch = 160 KiB
-  static bool attr_done = false;
-  if (!attr_done) {
+  static std::atomic<uint64_t> attr_done{0};     // a bit per device
+  const uint64_t device = device_bit();
+  if (!(attr_done & device)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_pipe_kernel<OpT, EPI>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
-    attr_done = true;
+    attr_done |= device;
   }
   p.ntm = (p.M + PBM - 1) / PBM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + PBN - 1) / PBN;
@@ -932,12 +939,13 @@ __global__ __launch_bounds__(512) void gemm_group_kernel(GroupParams gp) {
 template <typename OpT, int EPI>
 static int launch_group(const GroupParams& gp, hipStream_t st) {
   constexpr int smem = 3 * PSTAGE;
-  static bool attr_done = false;
-  if (!attr_done) {
+  static std::atomic<uint64_t> attr_done{0};     // a bit per device
+  const uint64_t device = device_bit();
+  if (!(attr_done & device)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_group_kernel<OpT, EPI>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
-    attr_done = true;
+    attr_done |= device;
   }
   hipLaunchKernelGGL((gemm_group_kernel<OpT, EPI>), dim3(persistent_grid(gp.n_tiles)), dim3(512), smem, st, gp);
   NMTGAN_CHECK_LAUNCH("gemm_group");
@@ -1291,12 +1299,13 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
 template <typename OpT, int EPI>
 static int launch_p8(GemmParams p, hipStream_t st) {
   constexpr int smem = 2 * QSTAGE + 8 * 2048 + 8 * (EPI == EPI_XGRAD ? 1536 : 512);   // 128 KiB of staging + per-wave epilogue scratch + vectors
-  static bool attr_done = false;
-  if (!attr_done) {
+  static std::atomic<uint64_t> attr_done{0};     // a bit per device
+  const uint64_t device = device_bit();
+  if (!(attr_done & device)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_p8_kernel<OpT, EPI>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
-    attr_done = true;
+    attr_done |= device;
   }
   p.ntm = (p.M + QBM - 1) / QBM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + QBN - 1) / QBN;
@@ -1702,12 +1711,13 @@ __global__ __launch_bounds__(256, 2) void gemm_kernel(GemmParams p) {
 template <typename OpT, int EPI, int BM, int BN>
 static int launch_glds(GemmParams p, hipStream_t st) {
   constexpr int smem = 2 * (BM + BN) * BKB;
-  static bool attr_done = false;
-  if (!attr_done) {
+  static std::atomic<uint64_t> attr_done{0};     // a bit per device
+  const uint64_t device = device_bit();
+  if (!(attr_done & device)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_glds_kernel<OpT, EPI, BM, BN>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
-    attr_done = true;
+    attr_done |= device;
   }
   p.ntm = (p.M + BM - 1) / BM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + BN - 1) / BN;
@@ -1749,12 +1759,13 @@ static int choose_split_k(const GemmParams& p, int nkt) {
 
 template <typename OpT, int EPI>
 static int launch_generic(GemmParams p, hipStream_t st) {
-  static bool attr_done = false;
-  if (!attr_done) {
+  static std::atomic<uint64_t> attr_done{0};     // a bit per device
+  const uint64_t device = device_bit();
+  if (!(attr_done & device)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<OpT, EPI>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, 4 * GTILE) != hipSuccess)
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
-    attr_done = true;
+    attr_done |= device;
   }
   p.ntm = (p.M + GBM - 1) / GBM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + GBN - 1) / GBN;
@@ -1767,12 +1778,13 @@ template <typename OpT, int BM, int NW>
 static int launch_ln(GemmParams p, hipStream_t st) {
   // four stages of (BM + 512) rows x 64 bytes; the epilogue's scratch and statistics live in the stage buffer it keeps free
   constexpr int smem = 4 * (BM + LBN) * LKB;
-  static bool attr_done = false;
-  if (!attr_done) {
+  static std::atomic<uint64_t> attr_done{0};     // a bit per device
+  const uint64_t device = device_bit();
+  if (!(attr_done & device)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_ln_kernel<OpT, BM, NW>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
-    attr_done = true;
+    attr_done |= device;
   }
   p.ntm = (p.M + BM - 1) / BM;
   p.ntn = 1;
