@@ -283,7 +283,8 @@ static int check_xent(const nmtgan_xent_args* a, const char* what) {
 static int pad64(int n) { return (n + 63) / 64 * 64; }
 
 struct XentPlan {
-  int rows_padded, piece, n_pieces, slices, kt_slice;        // a piece = slices of kt_slice k-tiles of 64 entries
+  int rows_padded, piece, slices, kt_slice;        // a piece = slices of kt_slice k-tiles of 64 entries
+  int sets;                                        // sets of dh's partial sums that the pieces take in turn
   size_t bytes;
   float *coef, *factor, *lse2, *part, *colsum, *wsum, *hsum;
   int32_t* label;
@@ -297,6 +298,9 @@ static int64_t pieces_of(const nmtgan_xent_args* a, int64_t entry_bytes) {
   const int64_t fit = std::max<int64_t>(PIECE_BYTES / entry_bytes, 1);
   return std::max<int64_t>(1, std::min<int64_t>((a->V + fit - 1) / fit, (a->V + 255) / 256));
 }
+// Partial sums of dh are kept apart by pieces up to a gigabyte (of 288) and added to behind it: 8000 rows over 50257 entries,
+// d = 1024, 262 MB of them: the product writes them in 174 us a piece and adds to them in 217.
+constexpr int64_t SETS_BYTES = 1LL << 30;
 // 16-bit products.  Inside a piece the hidden gradient's product is cut along the entries into enough slices to give every
 // CU a tile.
 static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPlan& q) {
@@ -308,7 +312,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(24, 256 / tiles), kt / 4));
   q.kt_slice = (int)((kt + q.slices - 1) / q.slices);
   q.piece = q.slices * q.kt_slice * 64;
-  q.n_pieces = (a->V + q.piece - 1) / q.piece;
+  q.sets = (int)std::max<int64_t>(1, std::min<int64_t>((a->V + q.piece - 1) / q.piece, SETS_BYTES / (4LL * q.slices * a->M * a->d)));
   Arena ar(base, cap);
   q.coef = ar.get<float>(q.rows_padded);
   q.factor = ar.get<float>(q.rows_padded);
@@ -316,7 +320,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.label = ar.get<int32_t>(q.rows_padded);
   q.y = ar.take((size_t)q.piece * q.rows_padded * es);
   q.ht = ar.take((size_t)a->d * q.rows_padded * es);
-  q.part = ar.get<float>((size_t)q.slices * a->M * a->d);
+  q.part = ar.get<float>((size_t)q.sets * q.slices * a->M * a->d);
   q.colsum = q.wsum = q.hsum = nullptr;
   if (a->smoothing > 0.f) {
     q.colsum = ar.get<float>((size_t)(SUM_W + SUM_H) * a->d);
@@ -510,13 +514,14 @@ static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const floa
   x.rows_padded = q.rows_padded;
   x.piece_padded = q.piece;
   x.high = high;
-  for (int v0 = 0; v0 < a->V; v0 += q.piece) {
+  int used = 0;
+  for (int v0 = 0; v0 < a->V; v0 += q.piece, ++used) {
     const int n = std::min(q.piece, a->V - v0);
     x.first = v0;
     const T* w = (const T*)a->w + (int64_t)v0 * a->ldw;
     NMTGAN_TRY(launch_gemm_xent(a->dtype, true, w, a->ldw, n, a->h, a->ldh, a->M, a->d, nullptr, x, st));
-    NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.y, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice, q.part,
-                                  v0 > 0, st));
+    NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.y, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice,
+                                  q.part + (int64_t)(used % q.sets) * q.slices * a->M * a->d, used >= q.sets, st));
     nmtgan_gemm_args b{};
     b.op_dtype = a->dtype;
     b.epilogue = NMTGAN_EPI_LINEAR;
@@ -526,7 +531,7 @@ static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const floa
     SplitKScope scope(q.splitk, SPLITK_BYTES);
     NMTGAN_TRY(launch_gemm(&b, st));
   }
-  hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, q.slices,
+  hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)a->M * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part, q.sets * q.slices,
                      a->M, a->d, q.coef, unit, q.wsum, (T*)dh, ld_dh);
   NMTGAN_CHECK_LAUNCH("linear_xent_dh");
   return 0;

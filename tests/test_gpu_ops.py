@@ -317,6 +317,11 @@ def test_xent_more_work(cuda, op, m, v, d):
         assert torch.equal(x, y)                     # rows without a label count nowhere, and sums have one order
 
 
+def test_xent_partial_sums_of_pieces(cuda):
+    """More partial sums of dh than are kept apart: the second piece adds to the first one's."""
+    _xent_case(cuda, _ops(), torch.bfloat16, 262145, 700, 512, 0.1, True, seed=9)
+
+
 @pytest.mark.parametrize("op", ["bf16", "fp32"])
 def test_xent_two_million_rows(cuda, op):
     """More row tiles than a grid's second dimension would hold."""
