@@ -72,7 +72,7 @@ struct XentDirect {
   float low, high;
   float* coef; float* y;                           // [M], [M][Vp]
   float* part; int slices; bool add;               // [slices][M][d] (added to?) or null: dh itself
-  float* part_w; int row_slices, waves;            // [row_slices][V][d] or null: dw itself; waves per tile of dw, 4 or 16
+  float* part_w; int row_slices, waves;            // [row_slices][V][d] or null: dw itself; waves per tile of dw: 1, 4, 16
   void* dh; void* dw; int64_t ld_dh, ld_dw;
   int n_dh;
 };

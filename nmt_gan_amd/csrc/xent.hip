@@ -367,7 +367,7 @@ static void carve_direct(const nmtgan_xent_args* a, char* base, size_t cap, Dire
   const int64_t tiles = (int64_t)((a->M + 31) / 32) * ((a->d + 31) / 32);
   q.p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(q.piece / 1024, 256 / tiles));
   const int64_t tiles_w = (int64_t)((q.piece + 31) / 32) * ((a->d + 31) / 32);
-  q.p.waves = tiles_w < 1024 ? 16 : 4;
+  q.p.waves = tiles_w < 1024 ? 16 : (a->M > 64 ? 4 : 1);        // (1: at most eight steps)
   q.p.row_slices = (int)std::max<int64_t>(1, std::min<int64_t>(a->M / 2048, 256 * 16 / (tiles_w * q.p.waves)));
   Arena ar(base, cap);
   q.p.coef = ar.get<float>(pad64(a->M));

@@ -1,6 +1,6 @@
 // Softmax cross entropy of hidden rows against a vocabulary table (formulas: xent.hip), the direct form: few launches and
-// 32 x 32 wave tiles, operands read from the caches in the layout they have and multiplied in fp32 (v_mfma_f32_32x32x2:
-// exact products of 16-bit operands, no rounding of d(logits)).  For little work, which on 256 x 256 tiles is launches, layout
+// 32 x 32 wave tiles, operands read from the caches in the layout they have and multiplied in fp32 (v_mfma_f32_32x32x2,
+// no rounding of d(logits); logits of 16-bit operands on their own matrix instructions).  For little work, which on 256 x 256 tiles is launches, layout
 // changes and tiles that fill a few of the 256 CUs, and for fp32 gradients:
 //   forward: z^T by tiles with (max, sum exp) per row and 32 entries, then the finish kernel
 //   gradient: z again and y = dz / g [M][V] in fp32, then dh and dw side by side in one launch
@@ -13,10 +13,17 @@
 
 namespace nmtgan {
 
+// products of two operands' 16-byte chunks, one per lane half
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool ok, float (&o)[4]) {
-  if (ok) VecIO<T, 4>::load(p, o);
-  else o[0] = o[1] = o[2] = o[3] = 0.f;
+__device__ __forceinline__ f32x16_t mul_chunk(const uint4& a, const uint4& b, f32x16_t c) {
+  if constexpr (sizeof(T) == 2) {
+    return mfma16<T>(a, b, c);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  }
 }
 __device__ __forceinline__ f32x16_t mul4(const float (&a)[4], const float (&b)[4], f32x16_t c) {
 #pragma unroll
@@ -47,20 +54,31 @@ __global__ __launch_bounds__(256) void xent_direct_z_kernel(XentDirect p) {
     if (tile == 0 && hl == 0 && row < p.M) p.coef[row] = coef;
   }
   if (e0 >= p.Vp) return;
-  const T* a = (const T*)p.w + (int64_t)min(e0 + (lane & 31), p.V - 1) * p.ldw + 4 * hl;
-  const T* b = (const T*)p.h + (int64_t)rc * p.ldh + 4 * hl;
+  const T* a = (const T*)p.w + (int64_t)min(e0 + (lane & 31), p.V - 1) * p.ldw;
+  const T* b = (const T*)p.h + (int64_t)rc * p.ldh;
   f32x16_t z = zero16();
-  constexpr int U = 8;
-  for (int k = 0; k < p.d; k += 8 * U) {           // d is a multiple of 4
-    float x[U][4], y[U][4];
+  constexpr int U = 8, E = 16 / (int)sizeof(T);    // a batch of 16 E k, the next one under way while it is multiplied
+  uint4 x[U], y[U];
+  auto fetch = [&](int k) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool ok = k + 8 * u + 4 * hl < p.d;
-      load4<T>(a + k + 8 * u, ok, x[u]);
-      load4<T>(b + k + 8 * u, ok, y[u]);
+      const int at = min(k + E * (2 * u + hl), p.d - E);
+      x[u] = *reinterpret_cast<const uint4*>(a + at);
+      y[u] = *reinterpret_cast<const uint4*>(b + at);
     }
+  };
+  fetch(0);
+  for (int k = 0; k < p.d; k += 2 * E * U) {
+    uint4 f[U], g[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) z = mul4(x[u], y[u], z);
+    for (int u = 0; u < U; ++u) {
+      const bool ok = k + E * (2 * u + hl) < p.d;
+      f[u] = ok ? x[u] : make_uint4(0, 0, 0, 0);
+      g[u] = ok ? y[u] : make_uint4(0, 0, 0, 0);
+    }
+    if (k + 2 * E * U < p.d) fetch(k + 2 * E * U);
+#pragma unroll
+    for (int u = 0; u < U; ++u) z = mul_chunk<T>(f[u], g[u], z);
   }
   if constexpr (GRAD) {
     if (row >= p.M) return;
@@ -103,7 +121,7 @@ __global__ __launch_bounds__(256) void xent_direct_z_kernel(XentDirect p) {
 }
 
 // dh = g (y w) by the first n_dh workgroups, one slice of the entries of a 32 x 32 tile each, which 16 waves divide; dw =
-// y^T (g h) by the others, one slice of the rows of one tile or of four, which 16 or four waves divide.  Waves are joined in
+// y^T (g h) by the others, one slice of the rows of 1, 4 or 16 tiles, which 16, 4 or 1 waves divide.  Waves are joined in
 // order through LDS, one element per thread; of several slices each leaves its part.  Loads go to clamped addresses and are selected afterwards:
 // under a condition each, they would not be in flight together.
 template <typename T>
@@ -188,6 +206,16 @@ __global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
         }
       }
     }
+  }
+  if (per == 1) {                                  // nothing to join
+    const int tile = first + w, col = tile % across * 32 + (lane & 31);
+    if (tile >= tiles || col >= p.d) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int e = tile / across * 32 + 8 * (r >> 2) + 4 * hl + (r & 3);
+      if (e < p.V) OpTraits<T>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, c[r]);
+    }
+    return;
   }
 #pragma unroll
   for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[r];
