@@ -331,14 +331,14 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.bytes = ar.off;
 }
 // The direct form (xent_direct.hip) against this file's products on the library's tiles, by M V d:
-//   logits in fp32 up to 1e9 (50 x 9000 x 256: 18 us against 40, 900 x 9000 x 128: 52 against 45, 450 x 9000 x 512: 113
-//   against 73), in 16 bits never (50 x 9000 x 256: 19 against 15);
-//   gradient's products in fp32 always (97 x 509 x 64, with the logits: 17 us against 70, 900 x 9000 x 512: 515 against
-//   1362, 3200 x 32000 x 512: 5.9 ms against 6.6), in 16 bits up to 2e8 (50 x 9000 x 256: 39 against 59, 200 x 4000 x 256:
-//   48 against 49, 400 x 4000 x 256: 71 against 54).
+//   logits in fp32 up to 1e9 (50 x 9000 x 256: 16 us against 39, 900 x 9000 x 128: 42 against 43), in 16 bits never (8 x
+//   32000 x 512: 20 against 19);
+//   gradient's products in fp32 always (97 x 509 x 64, with the logits: 17 us against 70, 900 x 9000 x 512: 456 against
+//   1362, 3200 x 32000 x 512: 4.7 ms against 6.6), in 16 bits up to 3e8 (8 x 32000 x 512: 58 against 105, 900 x 1000 x 256: 37
+//   against 55, 200 x 4000 x 256: 47 against 49, 400 x 4000 x 256: 68 against 54).
 static int64_t xent_work(const nmtgan_xent_args* a) { return (int64_t)a->M * a->V * a->d; }
 static bool direct_logits(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 && xent_work(a) <= 1000000000; }
-static bool direct_grads(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 || xent_work(a) <= 200000000; }
+static bool direct_grads(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 || xent_work(a) <= 300000000; }
 struct DirectPlan {
   XentDirect p;
   int piece, n_pieces;

@@ -302,7 +302,7 @@ def test_xent_many_pieces(cuda, op):
 
 
 @pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("m,v,d", [(700, 2600, 136), (700, 2600, 256), (601, 7003, 256), (2500, 6001, 256), (3001, 30011, 64),
+@pytest.mark.parametrize("m,v,d", [(700, 3600, 136), (700, 2600, 256), (601, 7003, 256), (2500, 6001, 256), (3001, 30011, 64),
                                    (9001, 70, 40), (70001, 2100, 64)])
 def test_xent_more_work(cuda, op, m, v, d):
     """Sizes on both sides of the choices between the products' forms, their tiles and one or several pieces."""
