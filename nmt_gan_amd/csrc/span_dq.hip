@@ -6,9 +6,9 @@ namespace nmtgan {
 // dq.  delta = dout . out carries the rounding of a 16-bit `out`, which shows where a row has few keys that count; the sum
 // of p dp over the walk does not.  So the walk runs with the former and corrects at the end: with c = p (1 - t^2),
 //   dq / scale = sum c (dp - delta) k = sum c (dp - delta16) k + (delta16 - delta) sum c k,
-// the second sum riding on the same turned K fragments.  The dk/dv kernel gets the corrected delta.  (16384 rows of long
-// documents, 8 heads of 64, capped and biased, bf16: 126 us, 111 without the correction and with 1.5 times the error that
-// rounding q, k, v and out alone leaves in dq and dk; taking every span twice instead: 190 us.)
+// the second sum riding on the same turned K fragments.  The dk/dv kernel gets the corrected delta.  (8192 rows of documents up to
+// 3626 long, 8 heads of 64, capped and biased, bf16: 127 us, 111 without the correction and with 1.5 times the error that
+// rounding the results alone leaves in dq and dk; taking every span twice instead: 190 us.)
 template <typename T, int DP, int KW, bool EXTRA>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dq_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
