@@ -146,7 +146,9 @@ __device__ __forceinline__ int64_t a_row_offset(const GemmParams& p, int r) {
 // Cross-entropy epilogues.
 // XSTAT: the product runs transposed like the STATS form, C rows = vocabulary entries and C columns = hidden rows, so one
 // hidden row's 64 logits of a wave tile sit in 16 registers of each of four lanes: stats[vtile][row] = (max, sum exp(z -
-// max)) over the entries of a 64-entry tile that exist, and with smoothing their plain sum in zsum[vtile][row].
+// max)) over the entries of a 64-entry tile that exist, and with smoothing their plain sum in zsum[vtile][row].  The epilogue
+// (an exponential per logit) is not covered by the next tile's products: 3200 rows x 32000 entries x 512 157 us (668 TFLOP/s; 6 %
+// of it the sums), 8000 x 50257 x 1024 790 us (1042).
 template <int MT>
 __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
   const int fc = lane & 15, fq = lane >> 4;

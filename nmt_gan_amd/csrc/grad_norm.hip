@@ -4,7 +4,8 @@
 // NORM_BLOCKS workgroups take in turn.  Squares are summed in fp64 - no gradient of a finite type overflows or vanishes -
 // and every sum has a fixed order, so a norm has the same bits in every run.  Two passes over the data with one
 // dependency between them: the second pass' workgroups each add the NORM_BLOCKS partial sums again (8 KiB out of L2)
-// instead of waiting for a third launch.
+// instead of waiting for a third launch.  Bound by memory: the 195 tensors and 93 million entries of a six-block generator
+// with its tables (16 bits, two launches of each kernel): norm 55 us, clip into an fp32 buffer 106 us = 5.3 TB/s.
 #include <math.h>
 
 #include <algorithm>

@@ -9,6 +9,7 @@ namespace nmtgan {
 // read once, as 16-byte chunks by LPK neighbouring lanes, so a wave reads 64 / LPK keys per instruction and STEP_U such
 // groups of K and of V are in flight while the previous ones are used; every lane group keeps a softmax of its own (no
 // exchange inside the loop but the LPK-lane sum of a dot product).
+// Bound by the rate at which K and V come; where heads share a key, by the arithmetic per key (hence the matrix form below).  One row over 300 keys, 8 heads: 5.6 us, a launch and two dependent loads.
 constexpr int STEP_U = 4;
 
 template <int LPK>
@@ -209,6 +210,8 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
 // The same with the matrix cores, 16-bit types and 2 to 16 query heads per key head: the heads are the 16 columns of 16x16
 // products over tiles of 32 keys (S^T = K Q^T, out^T = V^T P^T, layouts as in span_tiles.h with four lanes a softmax row),
 // so the work per key does not grow with the heads.  Each wave walks every fourth tile of its split through LDS of its own.
+// 48 rows over 522499 keys together (up to 16384 each), 8 heads of 64 over 2, capped, fp16: 53 us = 5.07 TB/s, the rate of a
+// large copy here; the vector form took 82 us.
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 template <typename T>
 __device__ __forceinline__ f32x4_t mma16x16(const uint4& a, const uint4& b, f32x4_t c) {
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void span_step_heads_kernel(
   for (int t = w; t < ng; t += 4) step_finish<T, DP>(p, out + t * DP, NS * STAGE / 4, s_m, s_l, i, h0 + t, t, z, splits, part, xs[w], lane);
 }
 
-// one wave per (row, head): the splits' parts, in order
+// one wave per (row, head): the splits' parts, in order (48 rows x 8 heads x 11 parts: 4.8 us, a launch's latency)
 template <typename T>
 __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, int splits, const float* part) {
   __shared__ float xs[4][SPAN_MAX_DH];

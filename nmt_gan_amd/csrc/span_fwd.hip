@@ -3,6 +3,12 @@
 
 namespace nmtgan {
 
+// One pass over the keys with the running maximum and sum of the softmax.  Bound by vector arithmetic (an exponential, with a
+// cap a second one and a reciprocal, per score) and, where one long document holds most of the work, by its last rows:
+//   8192 rows of documents up to 3626 long, 8 heads of 64, capped and biased, bf16: 99 us (60 % of the vector units' time)
+//   5000 rows of prompts up to 2390 long, 8 heads of 128 over 2 key heads, fp16: 47 us, 1.4 waves a SIMD on average of the 2
+//     that fit; eight waves a workgroup instead of four: 63 us (and 90 and 8.8 us for the two other cases)
+//   2048 rows of sentences up to 50 long, 8 heads of 64, bf16: 7.5 us, most of it launch and first loads
 template <typename T, int DP, int KW, bool EXTRA>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_fwd_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;

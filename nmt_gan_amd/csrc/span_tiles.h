@@ -451,10 +451,11 @@ __device__ __forceinline__ bool group_is_short(const SpanParams& p, int first, i
 
 // ------------------------------------------------------------------------------------------ split form
 // The KW waves of a workgroup share their own 32 rows and take every KW-th 32-row tile of the other side, each into LDS of
-// its own by DMA ahead of its use - no barrier inside the walk - and are joined at the end.  Where a launch has workgroups
-// enough without that (more than SPAN_FEW blocks of 32 rows) and the spans of KW neighbouring blocks are short, one
-// workgroup takes all KW, a wave each ("solo"), and the others leave: sentences of at most 50 tokens would give each of
-// four waves less than a tile.
+// its own by DMA ahead of its use - no barrier inside the walk - and are joined at the end (against four row blocks per
+// workgroup that share every tile: long documents 161 against 185 us forward when both existed).  Where a launch has
+// workgroups enough without that (more than SPAN_FEW blocks of 32 rows times heads) and the spans of KW neighbouring blocks
+// are short, one workgroup takes all KW, a wave each ("solo"), and the others leave: sentences of at most 50 tokens would
+// give each of four waves less than a tile (32768 rows of them, forward: 39 us, 67 with four row blocks sharing tiles).
 // Scalar base + one 32-bit lane offset per swizzle period; chunks behind dh and rows behind the last repeat a valid one
 // (they meet zeros of the own rows or weights of zero).
 // a pointer / offset that is the same in every lane, in scalar registers
@@ -579,7 +580,8 @@ static inline int raise_lds(F* kernel, size_t bytes, const char* what) {
                      hipSuccess, "%s: cannot raise the dynamic LDS limit", what);
   return 0;
 }
-// Blocks of 32 rows (times heads) from which waves may walk alone: two workgroups of four waves on every SIMD.
+// Blocks of 32 rows (times heads) from which waves may walk alone: two workgroups of four waves on every SIMD.  Below it the
+// chip is not full either way, and four waves a block finish sooner.
 constexpr int64_t SPAN_FEW = 2048;
 
 int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st);
