@@ -115,3 +115,18 @@ def test_norm_other_refusals():
     _refused(L.lib.nmtgan_global_norm(None, 3, 1.0, P, P, 1 << 20, None), "null")
     _refused(L.lib.nmtgan_global_norm(a, -1, 1.0, P, P, 1 << 20, None), "null")
     assert L.lib.nmtgan_global_norm_workspace_bytes(200) >= 3 * 1024 * 8
+
+
+def test_tensor_calls_refuse_what_is_not_on_a_gpu():
+    import torch
+
+    from nmt_gan_amd import ops
+    q, i = torch.zeros(4, 64), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda x: ops.attn_span(x, q, q, i, i, heads=1), lambda x: ops.attn_span_step(x, q, q, i, i, heads=1, max_keys=4),
+                 lambda x: ops.attn_span_grads(q, x, q, q, q, q[:, 0], i, i, heads=1), lambda x: ops.linear_xent(x, q, i),
+                 lambda x: ops.linear_xent_grads(x, q, i, q[:, 0]), lambda x: ops.global_norm([x]), lambda x: ops.clip_global_norm([x], 1.0)):
+        for x in (q, None, q.numpy(), q.double()):
+            with pytest.raises(ValueError):
+                call(x)
+    with pytest.raises(ValueError):
+        ops.clip_global_norm([q], None)
