@@ -1,11 +1,11 @@
 // Global gradient norm and clipping over a list of tensors:
 //   norm = sqrt(sum over all entries of (grad_scale g)^2)      out = g grad_scale min(1, max_norm / norm)
 // The list travels in the kernel arguments (LIST_MAX tensors per launch), cut into chunks of LIST_CHUNK elements that
-// NORM_BLOCKS workgroups take in turn.  Squares are summed in fp64 - no gradient of a finite type overflows or vanishes -
+// up to NORM_BLOCKS workgroups take in turn.  Squares are summed in fp64 - no gradient of a finite type overflows or vanishes -
 // and every sum has a fixed order, so a norm has the same bits in every run.  Two passes over the data with one
-// dependency between them: the second pass' workgroups each add the NORM_BLOCKS partial sums again (8 KiB out of L2)
+// dependency between them: the second pass' workgroups each add the partial sums again (8 KiB out of L2 at most)
 // instead of waiting for a third launch.  Bound by memory: the 195 tensors and 93 million entries of a six-block generator
-// with its tables (16 bits, two launches of each kernel): norm 55 us, clip into an fp32 buffer 106 us = 5.3 TB/s.
+// with its tables (16 bits, two launches of each kernel): norm 52 us, clip into an fp32 buffer 102 us = 5.5 TB/s.
 #include <math.h>
 
 #include <algorithm>
@@ -69,10 +69,12 @@ template <typename T> struct Any {
 
 // entry of a chunk, the chunk's first element inside the tensor and its length
 __device__ __forceinline__ const ListEntry& chunk_of(const ListParams& p, int chunk, int64_t& off, int& n) {
-  int a = 0, b = p.n - 1;                          // last entry whose first chunk is <= chunk
-  while (a < b) {
-    const int m = (a + b + 1) / 2;
-    if (p.e[m].first_chunk <= chunk) a = m; else b = m - 1;
+  // last entry whose first chunk is <= chunk: all entries at once, a search by halves waits for a load at every step
+  int a = -1;
+#pragma unroll
+  for (int u = 0; u < (LIST_MAX + 63) / 64; ++u) {
+    const int i = 64 * u + (threadIdx.x & 63);
+    a += __popcll(__ballot(i < p.n && p.e[min(i, LIST_MAX - 1)].first_chunk <= chunk));
   }
   const ListEntry& e = p.e[a];
   off = (int64_t)(chunk - e.first_chunk) * LIST_CHUNK;
@@ -125,7 +127,7 @@ __device__ __forceinline__ double square_sum(const T* g, int n) {
 __global__ __launch_bounds__(256) void norm_kernel(ListParams p, double* part) {
   __shared__ double red[4];
   double s = 0.0;
-  for (int c = blockIdx.x; c < p.n_chunks; c += NORM_BLOCKS) {
+  for (int c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
     int64_t off;
     int n;
     const ListEntry& e = chunk_of(p, c, off, n);
@@ -270,10 +272,11 @@ static int sum_squares(const nmtgan_grad_ref* t, int n, void* ws, size_t ws_byte
   NMTGAN_REQUIRE(ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0, "%s: workspace of %zu bytes needed, %zu given", what, need,
                  ws_bytes);
   *n_part = 0;
-  return for_parts(t, n, [&](const ListParams& p, int k) -> int {
-    hipLaunchKernelGGL(norm_kernel, dim3(NORM_BLOCKS), dim3(256), 0, st, p, (double*)ws + (int64_t)k * NORM_BLOCKS);
+  return for_parts(t, n, [&](const ListParams& p, int) -> int {
+    const int grid = std::min(p.n_chunks, NORM_BLOCKS);
+    hipLaunchKernelGGL(norm_kernel, dim3(grid), dim3(256), 0, st, p, (double*)ws + *n_part);
     NMTGAN_CHECK_LAUNCH("global_norm");
-    *n_part = (k + 1) * NORM_BLOCKS;
+    *n_part += grid;
     return 0;
   });
 }
