@@ -147,7 +147,7 @@ __device__ __forceinline__ int64_t a_row_offset(const GemmParams& p, int r) {
 // XSTAT: the product runs transposed like the STATS form, C rows = vocabulary entries and C columns = hidden rows, so one
 // hidden row's 64 logits of a wave tile sit in 16 registers of each of four lanes: stats[vtile][row] = (max, sum exp(z -
 // max)) over the entries of a 64-entry tile that exist, and with smoothing their plain sum in zsum[vtile][row].  The epilogue
-// (an exponential per logit) is not covered by the next tile's products: 3200 rows x 32000 entries x 512 157 us (668 TFLOP/s; 6 %
+// (an exponential per logit) is not covered by the next tile's products: 3200 rows x 32000 entries x 512 148 us (709 TFLOP/s; 6 %
 // of it the sums), 8000 x 50257 x 1024 790 us (1042).
 template <int MT>
 __device__ __forceinline__ void epilogue_xstat(const GemmParams& p, f32x4 (&acc)[MT][4], int m0, int n0, int lane) {
@@ -1856,6 +1856,16 @@ static bool prefer_p8_linear(int64_t M, int N, int nkt) {
   const int64_t rounds_pipe = (rt * ((N + 127) / 128) + cus - 1) / cus, rounds_p8 = (rt * ((N + 255) / 256) + cus - 1) / cus;
   return (double)rounds_p8 * (13.3 + 1.21 * nkt) < (double)rounds_pipe * (5.7 + 0.854 * nkt);
 }
+// XSTAT epilogue, 16-bit operands: the same model with its own fit - V x rows x K measured on 256x128 / 256x256 tiles in us:
+// 32000 x 3200 x 512 148 / 157, 32000 x 1601 x 512 73 / 79, 50257 x 8000 x 1024 829 / 790
+static bool prefer_p8_xstat(int64_t M, int N, int nkt) {
+  const int mode = p8_mode();
+  if (mode == 0 || nkt < 4) return false;
+  if (mode == 2) return true;
+  const int64_t cus = persistent_grid(1 << 30), rt = (M + 255) / 256;
+  const int64_t rounds_pipe = (rt * ((N + 127) / 128) + cus - 1) / cus, rounds_p8 = (rt * ((N + 255) / 256) + cus - 1) / cus;
+  return (double)rounds_p8 * (11.4 + 1.26 * nkt) < (double)rounds_pipe * (5.1 + 0.737 * nkt);
+}
 // LINEAR epilogue over plain rows, 16-bit operands: a problem that fills the CUs r times with 256x256 tiles and then
 // leaves a last round mostly empty (N = 512, M = 49152: 384 tiles on 256 CUs) is cut by rows - the first m1 rows are
 // r FULL rounds of the 256x256 kernel, the remainder goes back through the kernel choice on its own (usually one round
@@ -1927,6 +1937,10 @@ static int dispatch(const GemmParams& p, hipStream_t st) {
         return dispatch<OpT, EPI>(b, st);
       }
     }
+  }
+  if constexpr (EPI == EPI_XSTAT && sizeof(OpT) == 2) {
+    if (pipe_ok && ov < 0 && tiles256 >= 16)
+      return prefer_p8_xstat(p.M, p.N, nkt) ? launch_p8<OpT, EPI>(p, st) : launch_pipe<OpT, EPI>(p, st);
   }
   if (pipe_ok && (modelled ? prefer_p8_linear(p.M, p.N, nkt) : prefer_p8(p.M, p.N, nkt))) return launch_p8<OpT, EPI>(p, st);
   static const int pipe_min_tiles = [] { const char* e = getenv("NMTGAN_PIPE_MIN_TILES"); return e && atoi(e) > 0 ? atoi(e) : 16; }();
