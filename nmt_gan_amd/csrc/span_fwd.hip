@@ -75,7 +75,8 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
       const int first = j0 + 4 * (lane >> 5);
       if constexpr (EXTRA) {
         if (p.cap > 0.f) {
-          cap_scores<T, false>(s, s, p.scale, p.cap, 0.f);
+          if (sizeof(T) == 2 && ws.hi - ws.lo <= SPAN_SHORT) cap_scores_fine(s, p.scale, p.cap);
+          else cap_scores<T, false>(s, s, p.scale, p.cap, 0.f);
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] *= sc2;

@@ -539,6 +539,17 @@ __device__ __forceinline__ void cap_scores(f32x16_t& s, f32x16_t& t, float scale
     }
   }
 }
+// The same without `back`, to 2^-22 relative: the exponential's form is off by cap 2^-23 absolute, which shows in the lse of a
+// few small scores.  tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 - ... below 1/4
+__device__ __forceinline__ void cap_scores_fine(f32x16_t& s, float scale, float cap) {
+  const float inv = scale / cap, c2 = cap * LOG2E;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float x = s[r] * inv, y = x * x;
+    const float small = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
+    s[r] = c2 * (fabsf(x) < 0.25f ? small : span_tanh<bf16_t>(x));
+  }
+}
 template <typename T>
 __device__ __forceinline__ float turned(float t) { return sizeof(T) == 4 ? fmaf(-t, t, 1.f) : fmaf(-t, t, t); }
 template <typename T>
