@@ -221,6 +221,31 @@ def test_span_step(cuda, op, rows, cache, heads, kv_heads, dh, cap, bias):
     check("rows form", ops.attn_span(q, k, v, lo, hi, **how)[0], want)
 
 
+@pytest.mark.parametrize("op,heads,kv_heads", [("bf16", 8, 2), ("fp16", 2, 2), ("fp32", 4, 1)])
+def test_span_step_captured_and_replayed(cuda, op, heads, kv_heads):
+    """Tokens over growing caches by replays of one graph, with eager calls between."""
+    ops, dt = _ops(), TYPES[op]
+    g = torch.Generator().manual_seed(heads)
+    rows, cache, dh = 3, 3000, 64
+    q = _normal(g, rows, heads * dh, dt=dt).to(cuda)
+    k, v = (_normal(g, rows * cache, kv_heads * dh, dt=dt).to(cuda) for _ in range(2))
+    lo = torch.arange(rows, dtype=torch.int32, device=cuda) * cache
+    hi = lo.clone()
+    how = dict(heads=heads, kv_heads=kv_heads, scale=0.125, cap=20.0, max_keys=cache)
+    ops.attn_span_step(q, k, v, lo, hi, **how)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.attn_span_step(q, k, v, lo, hi, **how)
+    for n in (0, 1, 33, 600, 3000):
+        hi.copy_(lo + n)
+        q.copy_(_normal(g, rows, heads * dh, dt=dt))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.attn_span_step(q, k, v, lo, hi, **how)), n
+        check("replay", out, span_reference(q, k, v, lo, hi, heads, kv_heads, 0.125, 20.0)["out"])
+
+
 def test_span_offsets_beyond_32_bits(cuda):
     """A key buffer of more than 2^32 bytes and 2^31 elements, spans at its end."""
     ops = _ops()
@@ -320,6 +345,13 @@ def test_xent_more_work(cuda, op, m, v, d):
 def test_xent_partial_sums_of_pieces(cuda):
     """More partial sums of dh than are kept apart: the second piece adds to the first one's."""
     _xent_case(cuda, _ops(), torch.bfloat16, 262145, 700, 512, 0.1, True, seed=9)
+
+
+@pytest.mark.parametrize("op", ["bf16", "fp32"])
+@pytest.mark.parametrize("m,v,d,smoothing", [(300, 2, 64, 0.5), (300, 2, 64, 0.9), (300, 3, 64, 2 / 3), (300000, 3, 512, 0.9)])
+def test_xent_smoothing_beyond_the_uniform_distribution(cuda, op, m, v, d, smoothing):
+    """The label's own weight 1 - smoothing at or below the others'."""
+    _xent_case(cuda, _ops(), TYPES[op], m, v, d, smoothing, True, seed=10)
 
 
 @pytest.mark.parametrize("op", ["bf16", "fp32"])
