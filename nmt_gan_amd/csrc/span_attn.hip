@@ -512,8 +512,9 @@ static size_t carve_span_grads(int M, int heads, char* base, SpanParams* p) {
     p->hull = (int4*)(base + a);
     p->spans = (int*)(base + a + b);
     p->posr = (int*)(base + a + b + c);
+    p->chunk = (int2*)(base + a + b + 2 * c);
   }
-  return a + b + 2 * c;
+  return a + b + 2 * c + (nb > LIST_STEP ? align_up((nb + LIST_STEP - 1) / LIST_STEP * sizeof(int2), 256) : 0);
 }
 size_t attn_span_grads_workspace(int M, int heads) { return M > 0 && heads > 0 ? carve_span_grads(M, heads, nullptr, nullptr) : 0; }
 int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g, void* ws, size_t ws_bytes, hipStream_t st) {

@@ -10,7 +10,34 @@ namespace nmtgan {
 // Vector arithmetic bounds it where scores are capped and biased (three transcendentals a score): 8192 rows of documents up to
 // 3626 long, 8 heads of 64, bf16: 135 us (13 % of the matrix cores' time at the clock it ran at); with the row records read
 // where they are used, behind branches of their own, 158 us.  Sentences of at most 50, 2048 rows: 8.8 us.
-constexpr int LIST_STEP = 1024, SOLO_BLOCKS = 12;
+constexpr int SOLO_BLOCKS = 12;
+
+// hulls of whole chunks of LIST_STEP row blocks, where there are several: a key block passes over the chunks that it does not
+// meet (524288 rows of sentences up to 50: both gradients 2.8 ms, 5.4 without)
+__global__ __launch_bounds__(256) void span_chunk_kernel(SpanParams p, int nb) {
+  __shared__ int lo[4], hi[4];
+  int a = 0x7fffffff, b = 0;
+#pragma unroll
+  for (int u = 0; u < LIST_STEP / 256; ++u) {
+    const int at = blockIdx.x * LIST_STEP + 256 * u + threadIdx.x;
+    const int4 hl = at < nb ? p.hull[at] : make_int4(0, 0, 0, 0);
+    if (hl.y > hl.x) { a = min(a, hl.x); b = max(b, hl.y); }
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    a = min(a, __shfl_xor(a, m));
+    b = max(b, __shfl_xor(b, m));
+  }
+  if ((threadIdx.x & 63) == 0) { lo[threadIdx.x >> 6] = a; hi[threadIdx.x >> 6] = b; }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    p.chunk[blockIdx.x] = make_int2(min(min(lo[0], lo[1]), min(lo[2], lo[3])), max(max(hi[0], hi[1]), max(hi[2], hi[3])));
+}
+__device__ __forceinline__ bool chunk_meets(const SpanParams& p, int chunk, int a, int b) {
+  if (!p.chunk) return true;
+  const int2 c = p.chunk[chunk];
+  return c.x < b && c.y > a;
+}
 
 // appends the blocks of [from, from + LIST_STEP) whose hull meets keys [a, b), in order; returns how many.  All waves call it.
 template <int KW>
@@ -59,11 +86,17 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
   const int kvh = blockIdx.x % p.kv_heads, g = p.heads / p.kv_heads;
   const int nb = (p.M + 31) / 32;
   int k0 = blockIdx.x / p.kv_heads * 32;
-  int n_solo = -1;                                 // entries of the one list of a solo workgroup
-  if (p.solo && nb <= LIST_STEP) {
+  int n_solo = -1, begin = 0;                      // entries of the one list of a solo workgroup, its chunk's first block
+  if (p.solo) {
     const int first = k0 / (32 * KW) * (32 * KW);
-    n_solo = list_blocks<KW>(p, 0, nb, first, first + 32 * KW, list, count, w, lane);
-    if (n_solo * g > SOLO_BLOCKS) {
+    int met = 0;
+    for (int c = 0; c * LIST_STEP < nb; ++c)
+      if (chunk_meets(p, c, first, first + 32 * KW)) {
+        begin = c * LIST_STEP;
+        ++met;
+      }
+    if (met <= 1) n_solo = list_blocks<KW>(p, begin, nb, first, first + 32 * KW, list, count, w, lane);
+    if (met > 1 || n_solo * g > SOLO_BLOCKS) {
       n_solo = -1;
     } else {
       const int group = first / (32 * KW);        // (not always its first: workgroups go round the shader engines by index)
@@ -98,7 +131,8 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     if constexpr (EXTRA) dma4(lane * 4, (posr ? p.posr : p.spans) + (int64_t)b * 64, dst + 2 * D::BYTES + 512);
   };
 
-  for (int from = 0; from < nb; from += LIST_STEP) {
+  for (int from = solo ? begin : 0; from < nb; from += LIST_STEP) {
+    if (!solo && !chunk_meets(p, from / LIST_STEP, k0, k0 + 32)) continue;
     const int n = solo ? n_solo : list_blocks<KW>(p, from, nb, k0, k0 + 32, list, count, w, lane), total = n * g;
     struct Place { int nth, h; };                  // of a pair: its place in the list, its head
     auto move = [&](Place& at, int by) {
@@ -183,6 +217,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
         issue_at(ahead, buf);
       }
     }
+    if (solo) break;
   }
   if (solo) {
     const unsigned long long off = __ballot(ok && !(all_finite(ak) && all_finite(av)));
@@ -234,6 +269,13 @@ static int launch_dkv(SpanParams p, hipStream_t st) {
   const int64_t grid = ((int64_t)p.N + 32 * KW - 1) / (32 * KW) * KW * p.kv_heads;
   NMTGAN_REQUIRE(grid < (1LL << 31), "attn_span_dkv: too many rows");
   p.solo = grid > SPAN_FEW;
+  const int nb = (p.M + 31) / 32;
+  if (nb > LIST_STEP) {
+    hipLaunchKernelGGL(span_chunk_kernel, dim3((nb + LIST_STEP - 1) / LIST_STEP), dim3(256), 0, st, p, nb);
+    NMTGAN_CHECK_LAUNCH("attn_span_chunks");
+  } else {
+    p.chunk = nullptr;
+  }
   if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
     NMTGAN_TRY(raise_lds(&span_dkv_split_kernel<T, DP, KW, true>, smem, "attn_span_dkv"));
     hipLaunchKernelGGL((span_dkv_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);

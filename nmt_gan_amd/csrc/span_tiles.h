@@ -40,6 +40,7 @@ struct SpanParams {
   // per head and 32 rows: [lse / ln 2 x 32][delta x 32]; per 32 rows: [lo x 32][hi x 32] and [pos x 32][unused x 32]
   float* rec; int* spans; int* posr;
   int4* hull;                                    // [ceil(M / 32)] of 32 rows: keys seen by any row [x, y), by every row [z, w)
+  int2* chunk;                                   // of LIST_STEP row blocks: keys seen by any; null where they are one chunk
 };
 
 __device__ __forceinline__ float span_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
@@ -594,6 +595,8 @@ static inline int raise_lds(F* kernel, size_t bytes, const char* what) {
 // Blocks of 32 rows (times heads) from which waves may walk alone: two workgroups of four waves on every SIMD.  Below it the
 // chip is not full either way, and four waves a block finish sooner.
 constexpr int64_t SPAN_FEW = 2048;
+// Row blocks whose hulls the dk/dv kernel looks through at a time
+constexpr int LIST_STEP = 1024;
 
 int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st);
 int span_dq_tiles(int dtype, const SpanParams& p, hipStream_t st);

@@ -92,6 +92,34 @@ def test_span_many_blocks(cuda, op, heads, kv_heads, dh, longest, kind, cap, bia
 
 
 @pytest.mark.parametrize("op", ["bf16", "fp32"])
+@pytest.mark.parametrize("heads,kv_heads,crossing", [(1, 1, 50), (2, 2, 50), (4, 2, 700)])
+def test_span_more_row_blocks_than_one_list(cuda, op, heads, kv_heads, crossing):
+    """40000 rows of short documents and one of `crossing` rows over row 32768; checked where the lists begin and end."""
+    ops, dt, dh, n = _ops(), TYPES[op], 64, 40000
+    rng, starts = random.Random(heads), [0]
+    while starts[-1] < n:
+        at = starts[-1]
+        if at < 32768 - crossing // 2 <= at + 50:
+            starts += [32768 - crossing // 2, 32768 - crossing // 2 + crossing]
+        else:
+            starts.append(min(n, at + rng.randint(1, 50)))
+    lo = [a for a, b in zip(starts, starts[1:]) for _ in range(a, b)]
+    lo, hi = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (lo, range(1, n + 1)))
+    g = torch.Generator().manual_seed(heads)
+    q, dout = (_normal(g, n, heads * dh, dt=dt).to(cuda) for _ in range(2))
+    k, v = (_normal(g, n, kv_heads * dh, dt=dt).to(cuda) for _ in range(2))
+    how = dict(heads=heads, kv_heads=kv_heads, scale=dh ** -0.5)
+    out, lse = ops.attn_span(q, k, v, lo, hi, **how)
+    got = dict(zip(("dq", "dk", "dv"), ops.attn_span_grads(dout, q, k, v, out, lse, lo, hi, **how)), out=out, lse=lse)
+    for near in (0, 32768 - 900, n - 900):
+        a = max(x for x in starts if x <= near)
+        b = min(x for x in starts if x >= min(a + 1500, n))
+        want = span_reference(q[a:b], k[a:b], v[a:b], lo[a:b] - a, hi[a:b] - a, heads, kv_heads, dh ** -0.5, dout=dout[a:b])
+        for name, x in got.items():
+            check("%s from row %d" % (name, a), x[a:b], want[name])
+
+
+@pytest.mark.parametrize("op", ["bf16", "fp32"])
 @pytest.mark.parametrize("m,n", [(1, 1), (1, 200), (200, 1), (3, 0), (0, 5), (77, 500), (500, 77), (1025, 1300)])
 def test_span_shapes_and_cross_attention(cuda, op, m, n):
     """Query rows over another buffer: random spans, some empty, some reaching outside (cut), in no order."""
