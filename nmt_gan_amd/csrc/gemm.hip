@@ -77,13 +77,15 @@ struct GemmParams {
   const float* add; const int32_t* add_blk; int add_rows; int add_row0;
   // cross-entropy epilogues (xent.hip)
   XentEpilogue x;
-  // EPI_KPART (K-major operands, split_k slices of kt_slice k-tiles each): last k row and last 8-column chunk of A and W
+  // EPI_KPART, EPI_KSLICE: split_k slices of kt_slice k-tiles each; EPI_KPART (K-major operands): last k row and last
+  // 8-column chunk of A and W
   int kt_slice, ka_last, kw_last, m_last, n_last;
   bool split_add;                                  // EPI_KPART adds to the parts
 };
 constexpr int EPI_STATS = 100;                  // internal: never a value of nmtgan_gemm_args.epilogue
 constexpr int EPI_XSTAT = 102, EPI_XGRAD = 103; // internal: vocabulary cross entropy, forward and d(logits)
 constexpr int EPI_KPART = 104;                  // internal: fp32 partials of A[K][M]^T . W[K][N], both operands K-major
+constexpr int EPI_KSLICE = 105;                 // internal: fp32 partials of A[M][K] . W[N][K]^T
 constexpr int EPI_CONVADD = 101;                // internal: CONVMAX + additive term, chosen when nmtgan_gemm_args.add is set
 
 // acc[I0 + i][J0 + j] += A-fragment i x B-fragment j for one k-half of a k-tile (MT x NT 16x16 tiles).  Consecutive
@@ -755,7 +757,7 @@ static int launch_pipe(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done |= device;
   }
-  p.ntm = (p.M + PBM - 1) / PBM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.rows_padded : p.M) + PBM - 1) / PBM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + PBN - 1) / PBN;
   p.group_m = 2;                                 // tile order knob (L2 sharing of A panels vs Wt tiles); 1-4 measured best
   if (const char* e = getenv("NMTGAN_GEMM_GM")) p.group_m = atoi(e);
@@ -995,20 +997,20 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
   // KM (EPI_KPART): both operands are K-major, A[K][M] and W[K][N].  A staging unit then holds 64 k rows of its 128 columns
   // (256 bytes each), a fragment is two ds_read_b64_tr_b16 (4 k x 16 columns turned per 16 lanes), and column pair P of 16
   // sits at P ^ ((k & 3) | (k >> 1 & 4)): the 16 rows one read touches spread over all banks.
-  constexpr bool KM = EPI == EPI_KPART;
+  constexpr bool KM = EPI == EPI_KPART, SLICED = KM || EPI == EPI_KSLICE;
   // the cross-entropy forms' two wave groups meet for the epilogue and part again behind it: one barrier apart, the second
   // group would wait at its last barrier through the first one's epilogue and the other way round
-  constexpr bool MEET = EPI == EPI_XSTAT || EPI == EPI_XGRAD || KM;
-  const int nwg = p.ntm * p.ntn * (KM ? p.split_k : 1);
+  constexpr bool MEET = EPI == EPI_XSTAT || EPI == EPI_XGRAD || SLICED;
+  const int nwg = p.ntm * p.ntn * (SLICED ? p.split_k : 1);
   const int G = gridDim.x;
-  const int nkt = KM ? p.kt_slice : p.kbytes / BKB;      // >= 4 (launch guarantees it)
+  const int nkt = SLICED ? p.kt_slice : p.kbytes / BKB;      // >= 4 (launch guarantees it)
   const int my_tiles = (nwg - (int)blockIdx.x + G - 1) / G;
 
   auto tile_of = [&](int L, int& tm, int& tn) {
     const int xcd = L & 7, q = nwg >> 3, r = nwg & 7;
     int idx = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (L >> 3);
     int slice = 0;
-    if constexpr (KM) {
+    if constexpr (SLICED) {
       slice = idx / (p.ntm * p.ntn);
       idx -= slice * (p.ntm * p.ntn);
     }
@@ -1050,10 +1052,10 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
       if constexpr (u < 2) {
         const int in = EPI == EPI_XGRAD ? (rho & 35) | ((rho & 12) << 1) | ((rho & 16) >> 2) : rho & 63;   // see its epilogue
         const int row = tm * QBM + (rho >> 6) * 128 + u * 64 + in;
-        src[u][j] = p.A + a_row_offset(p, min(row, p.M - 1)) + lc * 16;
+        src[u][j] = p.A + a_row_offset(p, min(row, p.M - 1)) + lc * 16 + (SLICED ? (int64_t)slice * nkt * BKB : 0);
       } else {
         const int col = tn * QBN + (rho >> 5) * 64 + (u - 2) * 32 + (rho & 31);
-        src[u][j] = p.W + (int64_t)min(col, p.N - 1) * p.ldw_b + lc * 16;
+        src[u][j] = p.W + (int64_t)min(col, p.N - 1) * p.ldw_b + lc * 16 + (SLICED ? (int64_t)slice * nkt * BKB : 0);
       }
     }
   };
@@ -1259,7 +1261,7 @@ __global__ __launch_bounds__(512) void gemm_p8_kernel(GemmParams p) {
       epilogue_stats<8>(p, acc, m0, n0, lane);
     } else if constexpr (EPI == EPI_XGRAD) {
       epilogue_xgrad<OpT, 8, true>(p, acc, m0, n0, lane, ev);
-    } else if constexpr (KM) {
+    } else if constexpr (SLICED) {
       GemmParams v{};
       v.M = p.M; v.N = p.N; v.n_seg = 1; v.out_f32[0] = 1; v.ldo[0] = p.N; v.seg_scale[0] = 1.f;
       v.out[0] = p.split_part + (int64_t)slice * p.M * p.N;
@@ -1309,7 +1311,7 @@ static int launch_p8(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done |= device;
   }
-  p.ntm = (p.M + QBM - 1) / QBM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.rows_padded : p.M) + QBM - 1) / QBM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + QBN - 1) / QBN;
   // tile groups of 2 row tiles (4 are as fast); the logits GEMM (rows = vocabulary) takes 8: an XCD then keeps 2 MiB
   // of the table in its L2 and sweeps the activations twice instead of eight times - same time, a third of the
@@ -1326,8 +1328,9 @@ static int launch_p8(GemmParams p, hipStream_t st) {
     p.wide_ok = ok ? 2 : 0;
     if (const char* e = getenv("NMTGAN_GEMM_WIDE")) p.wide_ok = p.wide_ok ? atoi(e) : 0;
   }
-  if constexpr (EPI == EPI_KPART) p.wide_ok = p.N % 64 == 0;
-  const int nwg = p.ntm * p.ntn * (EPI == EPI_KPART ? p.split_k : 1);
+  constexpr bool sliced = EPI == EPI_KPART || EPI == EPI_KSLICE;
+  if constexpr (sliced) p.wide_ok = p.N % 64 == 0;
+  const int nwg = p.ntm * p.ntn * (sliced ? p.split_k : 1);
   const int grid = persistent_grid(nwg);
   hipLaunchKernelGGL((gemm_p8_kernel<OpT, EPI>), dim3(grid), dim3(512), smem, st, p);
   NMTGAN_CHECK_LAUNCH("gemm_p8");
@@ -1721,7 +1724,7 @@ static int launch_glds(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done |= device;
   }
-  p.ntm = (p.M + BM - 1) / BM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.rows_padded : p.M) + BM - 1) / BM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + BN - 1) / BN;
   const int slices = (EPI == NMTGAN_EPI_LINEAR && p.split_k > 1) ? p.split_k : 1;
   if (slices == 1) p.split_k = 0;
@@ -1769,7 +1772,7 @@ static int launch_generic(GemmParams p, hipStream_t st) {
       NMTGAN_FAIL(-3, "gemm: cannot raise dynamic LDS limit");
     attr_done |= device;
   }
-  p.ntm = (p.M + GBM - 1) / GBM;
+  p.ntm = ((EPI == EPI_XGRAD ? p.x.rows_padded : p.M) + GBM - 1) / GBM;
   p.ntn = ((EPI == EPI_XGRAD ? p.x.piece_padded : p.N) + GBN - 1) / GBN;
   hipLaunchKernelGGL((gemm_kernel<OpT, EPI>), dim3(p.ntm * p.ntn), dim3(256), 4 * GTILE, st, p);
   NMTGAN_CHECK_LAUNCH("gemm");
@@ -1856,15 +1859,16 @@ static bool prefer_p8_linear(int64_t M, int N, int nkt) {
   const int64_t rounds_pipe = (rt * ((N + 127) / 128) + cus - 1) / cus, rounds_p8 = (rt * ((N + 255) / 256) + cus - 1) / cus;
   return (double)rounds_p8 * (13.3 + 1.21 * nkt) < (double)rounds_pipe * (5.7 + 0.854 * nkt);
 }
-// XSTAT epilogue, 16-bit operands: the same model with its own fit - V x rows x K measured on 256x128 / 256x256 tiles in us:
-// 32000 x 3200 x 512 148 / 157, 32000 x 1601 x 512 73 / 79, 50257 x 8000 x 1024 829 / 790
-static bool prefer_p8_xstat(int64_t M, int N, int nkt) {
+// Cross-entropy epilogues, 16-bit operands: the same model with fits of their own - V x rows x K measured on 256x128 /
+// 256x256 tiles in us, logits: 32000 x 3200 x 512 148 / 157, 32000 x 1601 x 512 73 / 79, 50257 x 8000 x 1024 829 / 790;
+// d(logits): 32000 x 3200 x 512 193 / 155, 12565 x 8000 x 1024 273 / 219
+static bool prefer_p8_xent(int64_t M, int N, int nkt, bool grad) {
   const int mode = p8_mode();
   if (mode == 0 || nkt < 4) return false;
   if (mode == 2) return true;
   const int64_t cus = persistent_grid(1 << 30), rt = (M + 255) / 256;
   const int64_t rounds_pipe = (rt * ((N + 127) / 128) + cus - 1) / cus, rounds_p8 = (rt * ((N + 255) / 256) + cus - 1) / cus;
-  return (double)rounds_p8 * (11.4 + 1.26 * nkt) < (double)rounds_pipe * (5.1 + 0.737 * nkt);
+  return (double)rounds_p8 * (11.4 + 1.26 * nkt) < (double)rounds_pipe * (grad ? 8.6 + 0.775 * nkt : 5.1 + 0.737 * nkt);
 }
 // LINEAR epilogue over plain rows, 16-bit operands: a problem that fills the CUs r times with 256x256 tiles and then
 // leaves a last round mostly empty (N = 512, M = 49152: 384 tiles on 256 CUs) is cut by rows - the first m1 rows are
@@ -1938,9 +1942,9 @@ static int dispatch(const GemmParams& p, hipStream_t st) {
       }
     }
   }
-  if constexpr (EPI == EPI_XSTAT && sizeof(OpT) == 2) {
+  if constexpr ((EPI == EPI_XSTAT || EPI == EPI_XGRAD) && sizeof(OpT) == 2) {
     if (pipe_ok && ov < 0 && tiles256 >= 16)
-      return prefer_p8_xstat(p.M, p.N, nkt) ? launch_p8<OpT, EPI>(p, st) : launch_pipe<OpT, EPI>(p, st);
+      return prefer_p8_xent(p.M, p.N, nkt, EPI == EPI_XGRAD) ? launch_p8<OpT, EPI>(p, st) : launch_pipe<OpT, EPI>(p, st);
   }
   if (pipe_ok && (modelled ? prefer_p8_linear(p.M, p.N, nkt) : prefer_p8(p.M, p.N, nkt))) return launch_p8<OpT, EPI>(p, st);
   static const int pipe_min_tiles = [] { const char* e = getenv("NMTGAN_PIPE_MIN_TILES"); return e && atoi(e) > 0 ? atoi(e) : 16; }();
@@ -1999,6 +2003,23 @@ int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int en
     return dispatch<float, EPI_XGRAD>(p, st);
   }
   return 0;
+}
+
+// part[z][M][N] (fp32) = sum over k in [64 z kt_slice, 64 (z + 1) kt_slice) of A[m][k] W[n][k], 16-bit operands with
+// 64 slices kt_slice elements a row at least; ld in elements, a multiple of 8
+int launch_gemm_kslice(int op_dtype, const void* A, int64_t lda, const void* W, int64_t ldw, int M, int N, int slices, int kt_slice,
+                       float* part, hipStream_t st) {
+  const int64_t k = 64LL * slices * kt_slice;
+  NMTGAN_REQUIRE(op_dtype == NMTGAN_BF16, "gemm_kslice: bf16 operands");
+  NMTGAN_REQUIRE(A && W && part && M > 0 && N > 0 && slices > 0 && kt_slice >= 4 && lda % 8 == 0 && ldw % 8 == 0 && lda >= k && ldw >= k,
+                 "gemm_kslice: bad arguments");
+  GemmParams p{};
+  p.A = (const char*)A; p.W = (const char*)W;
+  p.M = M; p.N = N;
+  p.lda_b = lda * 2; p.ldw_b = ldw * 2;
+  p.k_inner = 1; p.k_step = BKB; p.k_jump = BKB;
+  p.split_k = slices; p.split_part = part; p.kt_slice = kt_slice;
+  return launch_p8<bf16_t, EPI_KSLICE>(p, st);
 }
 
 // part[z][M][N] (fp32; `add`: +=) = sum over k rows [64 z kt_slice, 64 (z + 1) kt_slice) of A[k][m] W[k][n], 16-bit

@@ -17,6 +17,8 @@ struct XentEpilogue {
 };
 int launch_gemm_xent(int op_dtype, bool grad, const void* W, int64_t ldw, int entries, const void* H, int64_t ldh, int rows,
                      int K, float2* stats, const XentEpilogue& x, hipStream_t st);
+int launch_gemm_kslice(int op_dtype, const void* A, int64_t lda, const void* W, int64_t ldw, int M, int N, int slices, int kt_slice,
+                       float* part, hipStream_t st);
 int launch_gemm_kmajor(int op_dtype, const void* A, int64_t lda, int ka, const void* W, int64_t ldw, int kw, int M, int N,
                        int slices, int kt_slice, float* part, bool add, hipStream_t st);
 int launch_gemm(const nmtgan_gemm_args* a, hipStream_t st);

@@ -127,8 +127,8 @@ __device__ __forceinline__ void transpose_tile(T (&tile)[64][66], Row row, int C
 //   - (coef h)^T, zero in rows without a label and in the padding
 //   - column sums behind label smoothing, whose constant -coef_r low of every d(logit) is kept out of the 16-bit images:
 //     dh_r -= coef_r low sum_j w_j, dw_j -= low sum_r coef_r h_r.  part[block][d], added in block order afterwards
-// (3200 rows, 32000 entries, d = 512: 17.7 us for 36 MB)
-constexpr int SUM_W = 256, SUM_H = 32;
+// (3200 rows, 32000 entries, d = 512: 14 us for 36 MB)
+constexpr int SUM_W = 256, SUM_H = 128;
 struct XentPrep {
   const void* h; const void* w; int64_t ldh, ldw;
   const int32_t* labels; const float* grad_row; const float* lse;
@@ -286,9 +286,10 @@ static int pad64(int n) { return (n + 63) / 64 * 64; }
 
 struct XentPlan {
   int rows_padded, piece, slices, kt_slice;        // a piece = slices of kt_slice k-tiles of 64 entries
+  int row_slices, kt_rows;                         // dw's k-loop: slices of kt_rows k-tiles of 64 rows
   int sets;                                        // sets of dh's partial sums that the pieces take in turn
   size_t bytes;
-  float *coef, *factor, *lse2, *part, *colsum, *wsum, *hsum;
+  float *coef, *factor, *lse2, *part, *part_w, *colsum, *wsum, *hsum;
   int32_t* label;
   void *y, *ht, *splitk;
 };
@@ -315,6 +316,15 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.kt_slice = (int)((kt + q.slices - 1) / q.slices);
   q.piece = q.slices * q.kt_slice * 64;
   q.sets = (int)std::max<int64_t>(1, std::min<int64_t>((a->V + q.piece - 1) / q.piece, SETS_BYTES / (4LL * q.slices * a->M * a->d)));
+  // dw of a piece with few tiles and many rows: the rows are cut too (65536 rows over 32000 entries, d = 512: 109 us and 20 for
+  // the sum a piece, 849 without).  Strides of a multiple of 2 KiB are avoided: rows of the
+  // images would fall on a few memory channels.
+  const int64_t tiles_w = (int64_t)((q.piece + 255) / 256) * ((a->d + 255) / 256);
+  q.kt_rows = q.rows_padded / 64;
+  q.row_slices = tiles_w < 192 ? (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / tiles_w, 15), q.kt_rows / 16)) : 1;
+  q.kt_rows = (q.kt_rows + q.row_slices - 1) / q.row_slices;
+  while (q.row_slices * q.kt_rows % 16 == 0) ++q.kt_rows;
+  q.rows_padded = 64 * q.row_slices * q.kt_rows;
   Arena ar(base, cap);
   q.coef = ar.get<float>(q.rows_padded);
   q.factor = ar.get<float>(q.rows_padded);
@@ -323,6 +333,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.y = ar.take((size_t)q.piece * q.rows_padded * es);
   q.ht = ar.take((size_t)a->d * q.rows_padded * es);
   q.part = ar.get<float>((size_t)q.sets * q.slices * a->M * a->d);
+  q.part_w = q.row_slices > 1 ? ar.get<float>((size_t)q.row_slices * q.piece * a->d) : nullptr;
   q.colsum = q.wsum = q.hsum = nullptr;
   if (a->smoothing > 0.f) {
     q.colsum = ar.get<float>((size_t)(SUM_W + SUM_H) * a->d);
@@ -508,7 +519,7 @@ static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const floa
   NMTGAN_CHECK_LAUNCH("linear_xent_prep");
   if (low > 0.f) {
     hipLaunchKernelGGL(xent_sums_kernel, dim3((a->d + 63) / 64, 2), dim3(1024), 0, st, q.colsum, a->d, -low,
-                       -low / unit, q.wsum, q.hsum);
+                       q.part_w ? -low : -low / unit, q.wsum, q.hsum);
     NMTGAN_CHECK_LAUNCH("linear_xent_sums");
   }
   XentEpilogue x{};
@@ -524,6 +535,13 @@ static int xent_grads_16(const nmtgan_xent_args* a, const float* lse, const floa
     NMTGAN_TRY(launch_gemm_xent(a->dtype, true, w, a->ldw, n, a->h, a->ldh, a->M, a->d, nullptr, x, st));
     NMTGAN_TRY(launch_gemm_kmajor(a->dtype, q.y, q.rows_padded, q.piece, w, a->ldw, n, a->M, a->d, q.slices, q.kt_slice,
                                   q.part + (int64_t)(used % q.sets) * q.slices * a->M * a->d, used >= q.sets, st));
+    if (q.part_w) {
+      NMTGAN_TRY(launch_gemm_kslice(a->dtype, q.y, q.rows_padded, q.ht, q.rows_padded, n, a->d, q.row_slices, q.kt_rows, q.part_w, st));
+      hipLaunchKernelGGL(xent_dh_kernel<T>, dim3((unsigned)(((int64_t)n * a->d / 4 + 255) / 256)), dim3(256), 0, st, q.part_w,
+                         q.row_slices, n, a->d, nullptr, unit, q.hsum, (T*)dw + (int64_t)v0 * ld_dw, ld_dw);
+      NMTGAN_CHECK_LAUNCH("linear_xent_dw");
+      continue;
+    }
     nmtgan_gemm_args b{};
     b.op_dtype = a->dtype;
     b.epilogue = NMTGAN_EPI_LINEAR;
