@@ -75,6 +75,7 @@ struct XentDirect {
   float* coef; float* y;                           // [M], [M][Vp]
   float* part; int slices; bool add;               // [slices][M][d] (added to?) or null: dh itself
   float* part_w; int row_slices, waves;            // [row_slices][V][d] or null: dw itself; waves per tile of dw: 1, 4, 16
+  int cols;                                        // columns per lane, 1 or 2
   void* dh; void* dw; int64_t ld_dh, ld_dw;
   int n_dh;
 };

@@ -321,7 +321,7 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   // images would fall on a few memory channels.
   const int64_t tiles_w = (int64_t)((q.piece + 255) / 256) * ((a->d + 255) / 256);
   q.kt_rows = q.rows_padded / 64;
-  q.row_slices = tiles_w < 192 ? (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / tiles_w, 15), q.kt_rows / 16)) : 1;
+  q.row_slices = tiles_w < 192 ? (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / tiles_w, 15), q.kt_rows / 6)) : 1;
   q.kt_rows = (q.kt_rows + q.row_slices - 1) / q.row_slices;
   while (q.row_slices * q.kt_rows % 16 == 0) ++q.kt_rows;
   q.rows_padded = 64 * q.row_slices * q.kt_rows;
@@ -346,9 +346,9 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
 // The direct form (xent_direct.hip) against this file's products on the library's tiles, by M V d:
 //   logits in fp32 up to 1e9 (50 x 9000 x 256: 16 us against 39, 900 x 9000 x 128: 42 against 43), in 16 bits never (8 x
 //   32000 x 512: 20 against 19);
-//   gradient's products in fp32 always (97 x 509 x 64, with the logits: 17 us against 70, 900 x 9000 x 512: 456 against
-//   1362, 3200 x 32000 x 512: 4.7 ms against 6.6), in 16 bits up to 3e8 (8 x 32000 x 512: 58 against 105, 900 x 1000 x 256: 37
-//   against 55, 200 x 4000 x 256: 47 against 49, 400 x 4000 x 256: 68 against 54).
+//   gradient's products in fp32 always (97 x 509 x 64, with the logits: 13 us against 70, 900 x 9000 x 512: 480 against 1362,
+//   3200 x 32000 x 512: 4.7 ms against 6.6), in 16 bits up to 3e8 (8 x 32000 x 512: 57 us against 105, 900 x 1000 x 256: 36
+//   against 55, 200 x 4000 x 256: 42 against 49, 400 x 4000 x 256: 68 against 54).
 static int64_t xent_work(const nmtgan_xent_args* a) { return (int64_t)a->M * a->V * a->d; }
 static bool direct_logits(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 && xent_work(a) <= 1000000000; }
 static bool direct_grads(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 || xent_work(a) <= 300000000; }
@@ -377,9 +377,10 @@ static void carve_direct(const nmtgan_xent_args* a, char* base, size_t cap, Dire
   const int64_t n = pieces_of(a, 4LL * a->M);
   q.piece = (int)((a->V + 8 * n - 1) / (8 * n) * 8);
   q.n_pieces = (a->V + q.piece - 1) / q.piece;
-  const int64_t tiles = (int64_t)((a->M + 31) / 32) * ((a->d + 31) / 32);
+  const int64_t down = (a->M + 31) / 32, down_w = (q.piece + 31) / 32;
+  q.p.cols = (down + down_w) * ((a->d + 63) / 64) >= 512 ? 2 : 1;
+  const int64_t across = (a->d + 32 * q.p.cols - 1) / (32 * q.p.cols), tiles = down * across, tiles_w = down_w * across;
   q.p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(q.piece / 1024, 256 / tiles));
-  const int64_t tiles_w = (int64_t)((q.piece + 31) / 32) * ((a->d + 31) / 32);
   q.p.waves = tiles_w < 1024 ? 16 : (a->M > 64 ? 4 : 1);        // (1: at most eight steps)
   q.p.row_slices = (int)std::max<int64_t>(1, std::min<int64_t>(a->M / 2048, 256 * 16 / (tiles_w * q.p.waves)));
   Arena ar(base, cap);

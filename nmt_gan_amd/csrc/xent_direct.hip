@@ -4,10 +4,10 @@
 // changes and tiles that fill a few of the 256 CUs, and for fp32 gradients:
 //   forward: z^T by tiles with (max, sum exp) per row and 32 entries, then the finish kernel
 //   gradient: z again and y = dz / g [M][V] in fp32, then dh and dw side by side in one launch
-// Bound by the rate at which the caches answer: 8 flop per byte loaded, 54 TFLOP/s of the fp32 matrix cores' 154 in the
-// gradient of 3200 rows over 32000 entries, d = 512 (4.7 ms); of few rows by w and dw in memory: 8 rows over 32000 entries, d =
-// 512, bf16, 12 us for the logits (2.8 TB/s) and 41 us for both products (1.6 TB/s: two-byte accesses); of little work by the
-// launches: 17 us for the gradient's two at 97 x 509 x 64, called back to back.
+// Bound by the rate at which the caches answer: 8 to 11 flop per byte loaded, 44 TFLOP/s of the fp32 matrix cores' 154 in the
+// products of 3200 rows over 32000 entries, d = 512; of few rows by w and dw in memory: 8 rows over 32000 entries, d = 512,
+// bf16, 11 us for the logits (3 TB/s) and 36 us for both products (1.8 TB/s); of little work by the launches: 13 us for the
+// gradient's two at 97 x 509 x 64, called back to back.
 // Which k goes into which slot of a product is free as long as both operands agree: lane half hl takes k = 8 s + 4 hl + t
 // in product t of step s, so that an operand with its k dimension in memory order is read by 16 bytes.
 #include "common.h"
@@ -26,11 +26,6 @@ __device__ __forceinline__ f32x16_t mul_chunk(const uint4& a, const uint4& b, f3
     c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
   }
-}
-__device__ __forceinline__ f32x16_t mul4(const float (&a)[4], const float (&b)[4], f32x16_t c) {
-#pragma unroll
-  for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
-  return c;
 }
 __device__ __forceinline__ f32x16_t zero16() {
   f32x16_t c;
@@ -122,113 +117,150 @@ __global__ __launch_bounds__(256) void xent_direct_z_kernel(XentDirect p) {
   }
 }
 
-// dh = g (y w) by the first n_dh workgroups, one slice of the entries of a 32 x 32 tile each, which 16 waves divide; dw =
-// y^T (g h) by the others, one slice of the rows of 1, 4 or 16 tiles, which 16, 4 or 1 waves divide.  Waves are joined in
-// order through LDS, one element per thread; of several slices each leaves its part.  Loads go to clamped addresses and are selected afterwards:
-// under a condition each, they would not be in flight together.
-template <typename T>
+// dh = g (y w) by the first n_dh workgroups, one slice of the entries of a tile of 32 rows x 32 NC columns each, which 16 waves
+// divide; dw = y^T (g h) by the others, one slice of the rows of 1, 4 or 16 tiles of 32 entries x 32 NC columns, which 16, 4 or 1
+// waves divide.  A lane has NC neighbouring columns: 2 make rows come and go in whole cache lines and use a value of y twice (1
+// row over 31989 entries, d = 768, bf16: 46 us against 61), 1 fills more CUs where tiles are few (97 x 509 x 64, fp32: 7 us
+// against 10).  Waves are joined in order through LDS, one element per thread; of several slices each leaves
+// its part.  Loads go to clamped addresses and are selected afterwards: under a condition each, they would not be in flight
+// together.
+template <typename T, int NC>
 __global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
   __shared__ float part[16][1024];
   const int lane = threadIdx.x & 63, hl = lane >> 5, w = threadIdx.x >> 6;
-  f32x16_t c = zero16();
-  const int across = (p.d + 31) / 32;
+  f32x16_t c[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) c[k] = zero16();
+  constexpr int WIDE = 32 * NC;
+  const int across = (p.d + WIDE - 1) / WIDE;
   const int reg = threadIdx.x >> 6, sub = 8 * (reg >> 2) + 4 * hl + (reg & 3);      // the element joined by this thread
+  auto put = [&](int half) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[half][r];
+    __syncthreads();
+  };
   if ((int)blockIdx.x < p.n_dh) {
     const int slice = blockIdx.x % p.slices, tile = blockIdx.x / p.slices, share = slice * 16 + w, shares = 16 * p.slices;
-    const int r0 = tile / across * 32, c0 = tile % across * 32, col = c0 + (lane & 31);
+    const int r0 = tile / across * 32, col = tile % across * WIDE + NC * (lane & 31);
     const float* a = p.y + (int64_t)min(r0 + (lane & 31), p.M - 1) * p.Vp + 4 * hl;
-    const T* b = (const T*)p.w + min(col, p.d - 1);
+    const T* b = (const T*)p.w + min(col, p.d - NC);
     const int n = p.Vp / 8, s1 = (int)((int64_t)n * (share + 1) / shares);
     constexpr int U = 4;
     for (int s = (int)((int64_t)n * share / shares); s < s1; s += U) {
-      float x[U][4], y[U][4];
+      float x[U][4], y[U][4][NC];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = min(s + u, s1 - 1);
         VecIO<float, 4>::load(a + 8 * at, x[u]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) y[u][t] = OpTraits<T>::load(b + (int64_t)min(8 * at + 4 * hl + t, p.V - 1) * p.ldw);
+        for (int t = 0; t < 4; ++t) VecIO<T, NC>::load(b + (int64_t)min(8 * at + 4 * hl + t, p.V - 1) * p.ldw, y[u][t]);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {              // entries behind the table count as zero: y is zero there, w is not read
           const bool ok = s + u < s1 && 8 * (s + u) + 4 * hl + t < p.V;
-          x[u][t] = ok ? x[u][t] : 0.f;
-          y[u][t] = ok ? y[u][t] : 0.f;
+          const float f = ok ? x[u][t] : 0.f;
+#pragma unroll
+          for (int k = 0; k < NC; ++k) c[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, ok ? y[u][t][k] : 0.f, c[k], 0, 0, 0);
         }
-        c = mul4(x[u], y[u], c);
-      }
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[r];
-    __syncthreads();
     const int row = r0 + sub;
-    float s = 0.f;
+    float s[NC];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += part[k][threadIdx.x];
+    for (int half = 0; half < NC; ++half) {
+      put(half);
+      s[half] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s[half] += part[k][threadIdx.x];
+      __syncthreads();
+    }
     if (row < p.M && col < p.d) {
       const float g = p.coef[row];
       float* at = p.part + ((int64_t)slice * p.M + row) * p.d + col;
-      if (p.part) *at = p.add ? *at + s : s;
-      else OpTraits<T>::store((T*)p.dh + (int64_t)row * p.ld_dh + col, g == 0.f ? 0.f : g * s);
+      if (p.part) {
+        if (p.add) {
+          float had[NC];
+          VecIO<float, NC>::load(at, had);
+#pragma unroll
+          for (int k = 0; k < NC; ++k) s[k] += had[k];
+        }
+        VecIO<float, NC>::store(at, s);
+      } else {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) s[k] = g == 0.f ? 0.f : g * s[k];
+        VecIO<T, NC>::store((T*)p.dh + (int64_t)row * p.ld_dh + col, s);
+      }
     }
     return;
   }
   const int per = p.waves, held = 16 / per, b = blockIdx.x - p.n_dh, slice = b % p.row_slices;
   const int tiles = (p.V + 31) / 32 * across, first = b / p.row_slices * held;
+  auto store = [&](int e, int col, const float (&o)[NC]) {
+    if (e >= p.V || col >= p.d) return;
+    if (p.part_w) VecIO<float, NC>::store(p.part_w + ((int64_t)slice * p.V + e) * p.d + col, o);
+    else VecIO<T, NC>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, o);
+  };
   {
     const int tile = first + w / per, share = slice * per + w % per, shares = per * p.row_slices;
     if (tile < tiles) {
-      const int e = tile / across * 32 + (lane & 31), col = tile % across * 32 + (lane & 31);
+      const int e = tile / across * 32 + (lane & 31), col = tile % across * WIDE + NC * (lane & 31);
       const float* a = p.y + min(e, p.V - 1);
-      const T* b = (const T*)p.h + min(col, p.d - 1);
+      const T* b = (const T*)p.h + min(col, p.d - NC);
       const int n = (p.M + 7) / 8, s1 = (int)((int64_t)n * (share + 1) / shares);
       constexpr int U = 2;
       for (int s = (int)((int64_t)n * share / shares); s < s1; s += U) {
-        float x[U][4], y[U][4], g[U][4];
+        float x[U][4], y[U][4][NC], g[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const int r = min(8 * (s + u) + 4 * hl + t, p.M - 1);
             x[u][t] = a[(int64_t)r * p.Vp];
-            y[u][t] = OpTraits<T>::load(b + (int64_t)r * p.ldh);
+            VecIO<T, NC>::load(b + (int64_t)r * p.ldh, y[u][t]);
             g[u][t] = p.coef[r];
           }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int t = 0; t < 4; ++t) {            // rows without a gradient count as zero, whatever they hold
             const bool ok = s + u < s1 && 8 * (s + u) + 4 * hl + t < p.M && g[u][t] != 0.f;
-            x[u][t] = ok ? x[u][t] : 0.f;
-            y[u][t] = ok ? g[u][t] * y[u][t] : 0.f;
+            const float f = ok ? x[u][t] : 0.f;
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+              c[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, ok ? g[u][t] * y[u][t][k] : 0.f, c[k], 0, 0, 0);
           }
-          c = mul4(x[u], y[u], c);
-        }
       }
     }
   }
   if (per == 1) {                                  // nothing to join
-    const int tile = first + w, col = tile % across * 32 + (lane & 31);
-    if (tile >= tiles || col >= p.d) return;
+    const int tile = first + w;
+    if (tile >= tiles) return;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int e = tile / across * 32 + 8 * (r >> 2) + 4 * hl + (r & 3);
-      if (e < p.V) OpTraits<T>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, c[r]);
+      float o[NC];
+#pragma unroll
+      for (int k = 0; k < NC; ++k) o[k] = c[k][r];
+      store(tile / across * 32 + 8 * (r >> 2) + 4 * hl + (r & 3), tile % across * WIDE + NC * (lane & 31), o);
     }
     return;
   }
+  float s[4][NC];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) part[w][r * 64 + lane] = c[r];
-  __syncthreads();
-  for (int q = 0; q < held; ++q) {
-    const int tile = first + q, e = tile / across * 32 + sub, col = tile % across * 32 + (lane & 31);
-    if (tile >= tiles || e >= p.V || col >= p.d) continue;
-    float s = 0.f;
-    for (int k = q * per; k < (q + 1) * per; ++k) s += part[k][threadIdx.x];
-    if (p.part_w) p.part_w[((int64_t)slice * p.V + e) * p.d + col] = s;
-    else OpTraits<T>::store((T*)p.dw + (int64_t)e * p.ld_dw + col, s);
+  for (int half = 0; half < NC; ++half) {
+    put(half);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s[q][half] = 0.f;
+      if (q < held)
+        for (int k = q * per; k < (q + 1) * per; ++k) s[q][half] += part[k][threadIdx.x];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int tile = first + q;
+    if (q < held && tile < tiles) store(tile / across * 32 + sub, tile % across * WIDE + NC * (lane & 31), s[q]);
   }
 }
 
@@ -244,12 +276,15 @@ int launch_xent_direct_z(int dtype, bool grad, const XentDirect& p, hipStream_t 
   return 0;
 }
 int launch_xent_direct_grads(int dtype, XentDirect p, hipStream_t st) {
-  const int across = (p.d + 31) / 32;
+  const int across = (p.d + 32 * p.cols - 1) / (32 * p.cols);
   p.n_dh = (p.M + 31) / 32 * across * p.slices;
   const int64_t tiles = (int64_t)(p.V + 31) / 32 * across, held = 16 / p.waves;
   const int64_t grid = p.n_dh + (tiles + held - 1) / held * p.row_slices;
   NMTGAN_REQUIRE(grid < (1LL << 31), "linear_xent_grads: too many tiles");
-  NMTGAN_DISPATCH_OP(dtype, T, hipLaunchKernelGGL(xent_direct_grads_kernel<T>, dim3((unsigned)grid), dim3(1024), 0, st, p));
+  NMTGAN_DISPATCH_OP(dtype, T, {
+    if (p.cols == 2) hipLaunchKernelGGL((xent_direct_grads_kernel<T, 2>), dim3((unsigned)grid), dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((xent_direct_grads_kernel<T, 1>), dim3((unsigned)grid), dim3(1024), 0, st, p);
+  });
   NMTGAN_CHECK_LAUNCH("linear_xent_direct_grads");
   return 0;
 }
