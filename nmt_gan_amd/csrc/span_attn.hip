@@ -92,9 +92,10 @@ __device__ __forceinline__ void step_finish(const SpanParams& p, const float* ac
   if (p.lse && lane == 0) p.lse[at] = lt == 0.f ? -INFINITY : mt * LN2 + logf(lt);
 }
 
-template <typename T, int DP, int GT, bool EXTRA>
+template <typename T, int DP, int GT, int FORM>
 __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits, int groups, float* part) {
   constexpr int EPC = 16 / (int)sizeof(T), LPK = DP / EPC, KPW = 64 / LPK, KB = STEP_U * KPW;
+  constexpr bool EXTRA = FORM != SPAN_PLAIN, LIBRARY = library_tanh<T, FORM>;
   __shared__ float s_acc[4][GT][DP];
   __shared__ float s_m[4][GT], s_l[4][GT], s_xs[4][SPAN_MAX_DH];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, dh = p.dh, g = p.heads / p.kv_heads;
@@ -124,7 +125,8 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
     }
   }
   const int pos = EXTRA ? pos_of(p, i) : 0;
-  const float inv_cap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
+  const float inv_cap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f, cap2 = p.cap * LOG2E;
+  const float border = len <= SPAN_SHORT ? SMALL_TANH : 0.f;    // see cap_scores_fine
 
   uint4 kr[STEP_U], vr[STEP_U];
   auto fetch = [&](int b) {
@@ -156,7 +158,7 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
         for (int e = 0; e < EPC; ++e) d = fmaf(x[e], q[t][e], d);
         d = key_sum<LPK>(d);
         if constexpr (EXTRA) {
-          if (p.cap > 0.f) d = p.cap * LOG2E * span_tanh<T>(d * inv_cap);
+          if (p.cap > 0.f) d = cap_score<LIBRARY>(d * inv_cap, cap2, border);
           else d *= p.scale * LOG2E;
           if (p.slopes) d = fmaf(-slope[t], fabsf((float)(pos - j)), d);
         }
@@ -223,10 +225,11 @@ __device__ __forceinline__ f32x4_t mma16x16(const uint4& a, const uint4& b, f32x
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
 }
-template <typename T, int DP, bool EXTRA>
+template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void span_step_heads_kernel(SpanParams p, int splits, int groups, float* part) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
+  constexpr bool EXTRA = FORM != SPAN_PLAIN, LIBRARY = library_tanh<T, FORM>;
   constexpr int NS = DP <= 64 ? 3 : 2, STAGE = 2 * D::BYTES, KS = DP / 32, DB = DP / 16;      // stages, k-steps, dh blocks
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_m[4][16], s_l[4][16], xs[4][SPAN_MAX_DH];
@@ -264,7 +267,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void span_step_heads_kernel(
   const float sc2 = p.scale * LOG2E;
   const float slope2 = EXTRA && p.slopes && col < ng ? p.slopes[h0 + col] * LOG2E : 0.f;
   const int pos = EXTRA ? pos_of(p, i) : 0;
-  const float cap2 = p.cap * LOG2E, inv2 = p.cap > 0.f ? p.scale / p.cap * 2.f * LOG2E : 0.f;
+  const float cap2 = p.cap * LOG2E, inv_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
+  const float inv2 = inv_cap * 2.f * LOG2E;
+  const bool fine = LIBRARY || (int)len <= SPAN_SHORT;       // see cap_scores_fine
   f32x4_t acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -287,10 +292,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void span_step_heads_kernel(
       for (int r = 0; r < 4; ++r) s[4 * kb + r] = c[r];
     }
     const int first = j0 + 32 * t + 4 * q4;                  // key of s[0]; s[4 kb + r] is key first + 16 kb + r
-    if (EXTRA && p.cap > 0.f) {
+    if (EXTRA && p.cap > 0.f && !fine) {
 #pragma unroll
       for (int r = 0; r < 8; ++r)
         s[r] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * inv2)), -2.f * cap2, cap2);
+    } else if (EXTRA && p.cap > 0.f) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] = cap_score<LIBRARY>(s[r] * inv_cap, cap2, SMALL_TANH);
     } else {
 #pragma unroll
       for (int r = 0; r < 8; ++r) s[r] *= sc2;
@@ -447,27 +455,24 @@ template <typename T, int DP, int GT>
 static int launch_step(const SpanParams& p, int splits, float* part, hipStream_t st) {
   const int groups = (p.heads / p.kv_heads + GT - 1) / GT;
   const dim3 grid((unsigned)(p.M * splits), p.kv_heads * groups);
-  if (p.cap > 0.f || p.slopes)
-    hipLaunchKernelGGL((span_step_kernel<T, DP, GT, true>), grid, dim3(256), 0, st, p, splits, groups, part);
-  else
-    hipLaunchKernelGGL((span_step_kernel<T, DP, GT, false>), grid, dim3(256), 0, st, p, splits, groups, part);
-  NMTGAN_CHECK_LAUNCH("attn_span_step");
-  return 0;
+  return with_form<T>(p, [&](auto form) -> int {
+    hipLaunchKernelGGL((span_step_kernel<T, DP, GT, decltype(form)::value>), grid, dim3(256), 0, st, p, splits, groups, part);
+    NMTGAN_CHECK_LAUNCH("attn_span_step");
+    return 0;
+  });
 }
 template <typename T, int DP>
 static int launch_step_heads(const SpanParams& p, int splits, float* part, hipStream_t st) {
   constexpr size_t smem = (size_t)4 * (DP <= 64 ? 3 : 2) * 2 * Dma<T, DP>::BYTES;
   const int groups = (p.heads / p.kv_heads + 15) / 16;
   const dim3 grid((unsigned)(p.M * splits), p.kv_heads * groups);
-  if (p.cap > 0.f || p.slopes) {
-    NMTGAN_TRY(raise_lds(&span_step_heads_kernel<T, DP, true>, smem, "attn_span_step"));
-    hipLaunchKernelGGL((span_step_heads_kernel<T, DP, true>), grid, dim3(256), smem, st, p, splits, groups, part);
-  } else {
-    NMTGAN_TRY(raise_lds(&span_step_heads_kernel<T, DP, false>, smem, "attn_span_step"));
-    hipLaunchKernelGGL((span_step_heads_kernel<T, DP, false>), grid, dim3(256), smem, st, p, splits, groups, part);
-  }
-  NMTGAN_CHECK_LAUNCH("attn_span_step");
-  return 0;
+  return with_form<T>(p, [&](auto form) -> int {
+    constexpr int FORM = decltype(form)::value;
+    NMTGAN_TRY(raise_lds(&span_step_heads_kernel<T, DP, FORM>, smem, "attn_span_step"));
+    hipLaunchKernelGGL((span_step_heads_kernel<T, DP, FORM>), grid, dim3(256), smem, st, p, splits, groups, part);
+    NMTGAN_CHECK_LAUNCH("attn_span_step");
+    return 0;
+  });
 }
 template <typename T, int DP>
 static int choose_step(const SpanParams& p, int splits, float* part, hipStream_t st) {

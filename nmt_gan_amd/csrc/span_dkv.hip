@@ -74,10 +74,11 @@ __device__ __forceinline__ int list_blocks(const SpanParams& p, int from, int nb
   return __builtin_amdgcn_readfirstlane(total);
 }
 
-template <typename T, int DP, int KW, bool EXTRA>
+template <typename T, int DP, int KW, int FORM>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dkv_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
+  constexpr bool EXTRA = FORM != SPAN_PLAIN, LIBRARY = library_tanh<T, FORM>;
   constexpr int STAGE = 2 * D::BYTES + 1024;      // Q, dO and the records of 32 rows
   constexpr int REGION = 2 * STAGE, NT = 64 * KW, JN = 32 * DP / 4 / NT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
       f32x16_t s = score_block<T, DP>(tq, 0, kf, lane), turn;
       f32x16_t d = score_block<T, DP>(td, 0, vf, lane);
       if (capped) {
-        cap_scores<T, true>(s, turn, p.scale, p.cap, sizeof(T) == 2 ? p.cap * LOG2E : 0.f);     // (rec starts there)
+        cap_scores<LIBRARY, true>(s, turn, p.scale, p.cap, LIBRARY ? 0.f : p.cap * LOG2E);     // (rec starts there)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] -= of(lse4[r >> 2], r & 3);
       } else {
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
       }
       if (capped) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) d[r] *= turned<T>(turn[r]);
+        for (int r = 0; r < 16; ++r) d[r] *= turned<LIBRARY>(turn[r]);
       }
       if (!whole) {
 #pragma unroll
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     const unsigned long long off = __ballot(ok && !(all_finite(ak) && all_finite(av)));
     const unsigned again = (unsigned)off | (unsigned)(off >> 32);
     if (ok && !(again >> (lane & 31) & 1)) {
-      store_own<T, DP>((T*)p.dk + (int64_t)j * p.ld_dk + kvh * p.dh, ak, result_scale<T>(p), p.dh, lane);
+      store_own<T, DP>((T*)p.dk + (int64_t)j * p.ld_dk + kvh * p.dh, ak, result_scale<LIBRARY>(p), p.dh, lane);
       store_own<T, DP>((T*)p.dv + (int64_t)j * p.ld_dv + kvh * p.dh, av, 1.f, p.dh, lane);
     }
     float* xs = reinterpret_cast<float*>(mine);
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     const int idx = tid + u * NT, row = idx / (DP / 4), col = idx % (DP / 4) * 4;
     const int64_t r = k0 + row;
     if (r >= p.N || col >= p.dh || bad[row]) continue;
-    const float f = result_scale<T>(p), x[4] = {tk[u].x * f, tk[u].y * f, tk[u].z * f, tk[u].w * f};
+    const float f = result_scale<LIBRARY>(p), x[4] = {tk[u].x * f, tk[u].y * f, tk[u].z * f, tk[u].w * f};
     const float y[4] = {tv[u].x, tv[u].y, tv[u].z, tv[u].w};
     VecIO<T, 4>::store((T*)p.dk + r * p.ld_dk + kvh * p.dh + col, x);
     VecIO<T, 4>::store((T*)p.dv + r * p.ld_dv + kvh * p.dh + col, y);
@@ -276,15 +277,13 @@ static int launch_dkv(SpanParams p, hipStream_t st) {
   } else {
     p.chunk = nullptr;
   }
-  if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
-    NMTGAN_TRY(raise_lds(&span_dkv_split_kernel<T, DP, KW, true>, smem, "attn_span_dkv"));
-    hipLaunchKernelGGL((span_dkv_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
-  } else {
-    NMTGAN_TRY(raise_lds(&span_dkv_split_kernel<T, DP, KW, false>, smem, "attn_span_dkv"));
-    hipLaunchKernelGGL((span_dkv_split_kernel<T, DP, KW, false>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
-  }
-  NMTGAN_CHECK_LAUNCH("attn_span_dkv");
-  return 0;
+  return with_form<T>(p, [&](auto form) -> int {
+    constexpr int FORM = decltype(form)::value;
+    NMTGAN_TRY(raise_lds(&span_dkv_split_kernel<T, DP, KW, FORM>, smem, "attn_span_dkv"));
+    hipLaunchKernelGGL((span_dkv_split_kernel<T, DP, KW, FORM>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+    NMTGAN_CHECK_LAUNCH("attn_span_dkv");
+    return 0;
+  });
 }
 int span_dkv_tiles(int dtype, const SpanParams& p, hipStream_t st) {
   NMTGAN_DISPATCH_GRAD(dtype, T, {

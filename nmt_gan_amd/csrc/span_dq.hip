@@ -9,10 +9,11 @@ namespace nmtgan {
 // the second sum riding on the same turned K fragments.  The dk/dv kernel gets the corrected delta.  (8192 rows of documents up to
 // 3626 long, 8 heads of 64, capped and biased, bf16: 127 us, 111 without the correction and with 1.5 times the error that
 // rounding the results alone leaves in dq and dk; taking every span twice instead: 190 us.)
-template <typename T, int DP, int KW, bool EXTRA>
+template <typename T, int DP, int KW, int FORM>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_dq_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
+  constexpr bool EXTRA = FORM != SPAN_PLAIN, LIBRARY = library_tanh<T, FORM>;
   constexpr int REGION = 3 * D::BYTES, NT = 64 * KW, JN = 32 * DP / 4 / NT;      // two K tiles and one V tile per wave
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ float s_sum[KW][32], xs[KW][2][SPAN_MAX_DH];
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     }
     if (__any(sp.x < j0 + 32 && sp.y > j0)) {
       if (capped) {
-        cap_scores<T, true>(s, turn, p.scale, p.cap, lse2);
+        cap_scores<LIBRARY, true>(s, turn, p.scale, p.cap, lse2);
       } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc2, -lse2);
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
       }
       if (capped) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= turned<T>(turn[r]);
+        for (int r = 0; r < 16; ++r) s[r] *= turned<LIBRARY>(turn[r]);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) d[r] = s[r] * (d[r] - delta);
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
   // what the dk/dv kernel reads of these rows: a record per head, and once for all heads the spans and their hull
   if (lane < 32 && (solo || w == 0) && tile * 32 < p.M) {
     float* const at = delta_at(p, i, h);
-    at[-32] = capped && sizeof(T) == 2 ? lse2 - p.cap * LOG2E : lse2;      // (where the capped score starts)
+    at[-32] = capped && !LIBRARY ? lse2 - p.cap * LOG2E : lse2;      // (where the capped score starts)
     at[0] = delta;
     if (h == 0) {
       p.spans[(int64_t)tile * 64 + lane] = sp.x;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
     const unsigned again = (unsigned)off | (unsigned)(off >> 32);
     if (ok && !(again >> (lane & 31) & 1)) {
       if (!some) clear(acc);
-      store_own<T, DP>((T*)p.dq + (int64_t)i * p.ld_dq + h * p.dh, acc, result_scale<T>(p), p.dh, lane);
+      store_own<T, DP>((T*)p.dq + (int64_t)i * p.ld_dq + h * p.dh, acc, result_scale<LIBRARY>(p), p.dh, lane);
     }
     __threadfence_block();
     for (unsigned left = again; left; left &= left - 1)
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 128 ? 2 : 1) void span_d
   for (int u = 0; u < JN; ++u) {
     const int idx = tid + u * NT, row = idx / (DP / 4), col = idx % (DP / 4) * 4, r = tile * 32 + row;
     if (r >= p.M || col >= p.dh || bad[row]) continue;
-    const float f = result_scale<T>(p), x[4] = {tot[u].x * f, tot[u].y * f, tot[u].z * f, tot[u].w * f};
+    const float f = result_scale<LIBRARY>(p), x[4] = {tot[u].x * f, tot[u].y * f, tot[u].z * f, tot[u].w * f};
     VecIO<T, 4>::store((T*)p.dq + (int64_t)r * p.ld_dq + h * p.dh + col, x);
   }
   for (int row = w; row < 32; row += KW)
@@ -203,15 +204,13 @@ static int launch_dq(SpanParams p, hipStream_t st) {
   const int64_t grid = ((int64_t)p.M + 32 * KW - 1) / (32 * KW) * KW * p.heads;
   NMTGAN_REQUIRE(grid < (1LL << 31), "attn_span_dq: too many rows");
   p.solo = grid > SPAN_FEW;
-  if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
-    NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, true>, smem, "attn_span_dq"));
-    hipLaunchKernelGGL((span_dq_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
-  } else {
-    NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, false>, smem, "attn_span_dq"));
-    hipLaunchKernelGGL((span_dq_split_kernel<T, DP, KW, false>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
-  }
-  NMTGAN_CHECK_LAUNCH("attn_span_dq");
-  return 0;
+  return with_form<T>(p, [&](auto form) -> int {
+    constexpr int FORM = decltype(form)::value;
+    NMTGAN_TRY(raise_lds(&span_dq_split_kernel<T, DP, KW, FORM>, smem, "attn_span_dq"));
+    hipLaunchKernelGGL((span_dq_split_kernel<T, DP, KW, FORM>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+    NMTGAN_CHECK_LAUNCH("attn_span_dq");
+    return 0;
+  });
 }
 int span_dq_tiles(int dtype, const SpanParams& p, hipStream_t st) {
   NMTGAN_DISPATCH_GRAD(dtype, T, {

@@ -9,10 +9,11 @@ namespace nmtgan {
 //   5000 rows of prompts up to 2390 long, 8 heads of 128 over 2 key heads, fp16: 47 us, 1.4 waves a SIMD on average of the 2
 //     that fit; eight waves a workgroup instead of four: 63 us (and 90 and 8.8 us for the two other cases)
 //   2048 rows of sentences up to 50 long, 8 heads of 64, bf16: 7.5 us, most of it launch and first loads
-template <typename T, int DP, int KW, bool EXTRA>
+template <typename T, int DP, int KW, int FORM>
 __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_fwd_split_kernel(SpanParams p) {
   using G = Geo<T, DP>;
   using D = Dma<T, DP>;
+  constexpr bool EXTRA = FORM != SPAN_PLAIN, LIBRARY = library_tanh<T, FORM>;
   // one K and one V tile per wave: the next K is under way during the softmax and the second product, the next V during
   // the first product and the softmax, and the small footprint buys waves to hide the rest behind
   constexpr int REGION = 2 * D::BYTES > 32 * DP * 4 ? 2 * D::BYTES : 32 * DP * 4, NT = 64 * KW, JN = 32 * DP / 4 / NT;
@@ -60,6 +61,7 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
   clear(acc);
   float m = -INFINITY, l = 0.f;
   const unsigned len = (unsigned)(sp.y - sp.x);
+  const bool few = len <= SPAN_SHORT && len > 0, any_few = !LIBRARY && __any(few);
 
   for (int t = t0; t < nt; t += dt) {
     const int j0 = ws.lo + 32 * t;
@@ -75,8 +77,8 @@ __global__ __launch_bounds__(64 * KW, DP * sizeof(T) <= 256 ? 2 : 1) void span_f
       const int first = j0 + 4 * (lane >> 5);
       if constexpr (EXTRA) {
         if (p.cap > 0.f) {
-          if (sizeof(T) == 2 && ws.hi - ws.lo <= SPAN_SHORT) cap_scores_fine(s, p.scale, p.cap);
-          else cap_scores<T, false>(s, s, p.scale, p.cap, 0.f);
+          if (any_few) cap_scores_fine(s, p.scale, p.cap, few);
+          else cap_scores<LIBRARY, false>(s, s, p.scale, p.cap, 0.f);
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] *= sc2;
@@ -196,15 +198,13 @@ static int launch_fwd(SpanParams p, hipStream_t st) {
   const int64_t grid = ((int64_t)p.M + 32 * KW - 1) / (32 * KW) * KW * p.heads;
   NMTGAN_REQUIRE(grid < (1LL << 31), "attn_span: too many rows");
   p.solo = grid > SPAN_FEW;
-  if (p.cap > 0.f || p.slopes || p.scale == 0.f) {
-    NMTGAN_TRY(raise_lds(&span_fwd_split_kernel<T, DP, KW, true>, smem, "attn_span"));
-    hipLaunchKernelGGL((span_fwd_split_kernel<T, DP, KW, true>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
-  } else {
-    NMTGAN_TRY(raise_lds(&span_fwd_split_kernel<T, DP, KW, false>, smem, "attn_span"));
-    hipLaunchKernelGGL((span_fwd_split_kernel<T, DP, KW, false>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
-  }
-  NMTGAN_CHECK_LAUNCH("attn_span");
-  return 0;
+  return with_form<T>(p, [&](auto form) -> int {
+    constexpr int FORM = decltype(form)::value;
+    NMTGAN_TRY(raise_lds(&span_fwd_split_kernel<T, DP, KW, FORM>, smem, "attn_span"));
+    hipLaunchKernelGGL((span_fwd_split_kernel<T, DP, KW, FORM>), dim3((unsigned)grid), dim3(64 * KW), smem, st, p);
+    NMTGAN_CHECK_LAUNCH("attn_span");
+    return 0;
+  });
 }
 int span_fwd_tiles(int dtype, const SpanParams& p, hipStream_t st) {
   NMTGAN_DISPATCH_OP(dtype, T, {

@@ -15,6 +15,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -397,24 +398,24 @@ __device__ __forceinline__ float both_halves_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// tanh to about 2^-23 absolute: exp2 and a reciprocal for the 16-bit types, the library function for fp32
-template <typename T>
-__device__ __forceinline__ float span_tanh(float x) {
-  if constexpr (sizeof(T) == 4) return tanhf(x);
-  else return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * LOG2E)));
+// What a launch's scores need.  EXTRA: a cap, a distance bias or the scale zero.  WIDE_CAP: with a cap above SPAN_WIDE, the 16-bit
+// types only: tanh as 1 - 2 / (1 + exp(2 x)) is off by 2^-23 to 2^-22 absolute, a score by cap times that - up to 2^-16 at 64,
+// far below the rounding of a probability to 16 bits, but 2^-3 at a cap of a million.  There, and in fp32, it is the library's tanh.
+enum SpanForm { SPAN_PLAIN, SPAN_EXTRA, SPAN_WIDE_CAP };
+constexpr float SPAN_WIDE = 64.f;
+template <typename T, int FORM> constexpr bool library_tanh = sizeof(T) == 4 || FORM == SPAN_WIDE_CAP;
+// tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 - ..., below 1/4
+__device__ __forceinline__ float small_tanh(float x) {
+  const float y = x * x;
+  return x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
 }
-// score of a raw product in units of log 2, and 1 - t^2
-template <typename T>
-__device__ __forceinline__ float score2(const SpanParams& p, float dot, float inv_cap, float slope, int pos, int j, float& turn) {
-  float r = dot * p.scale;
-  turn = 1.f;
-  if (p.cap > 0.f) {
-    const float t = span_tanh<T>(r * inv_cap);
-    r = p.cap * t;
-    turn = fmaf(-t, t, 1.f);
-  }
-  r -= slope * fabsf((float)(pos - j));
-  return r * LOG2E;
+constexpr float SMALL_TANH = 0.25f;
+// cap tanh x in units of log 2 (c2 = cap / ln 2).  By the series where |x| < border, SMALL_TANH or 0
+template <bool LIBRARY>
+__device__ __forceinline__ float cap_score(float x, float c2, float border) {
+  if constexpr (LIBRARY) return c2 * tanhf(x);
+  const float d = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * LOG2E)));
+  return fabsf(x) < border ? c2 * small_tanh(x) : fmaf(d, -2.f * c2, c2);
 }
 
 struct WaveSpan { int lo, hi, all_lo, all_hi; };   // hull of a wave's spans; keys all of its rows see
@@ -517,12 +518,12 @@ template <typename T, int DP> struct Dma {
 };
 
 // The tanh of a score block in place, in units of log 2: s = raw products -> capped scores minus `base`; BACK: t carries
-// what (1 - t^2) is made of, see turned() - for the 16-bit types t = 1 - 2 d with d = 1 / (1 + exp(2 r / cap)), whose
+// what (1 - t^2) is made of, see turned() - t itself from the library, else t = 1 - 2 d with d = 1 / (1 + exp(2 r / cap)), whose
 // 1 - t^2 = 4 d (1 - d) leaves its 4 to the scale of the result
-template <typename T, bool BACK>
+template <bool LIBRARY, bool BACK>
 __device__ __forceinline__ void cap_scores(f32x16_t& s, f32x16_t& t, float scale, float cap, float base) {
   const float c2 = cap * LOG2E;
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (LIBRARY) {
     const float inv = scale / cap;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -540,21 +541,24 @@ __device__ __forceinline__ void cap_scores(f32x16_t& s, f32x16_t& t, float scale
     }
   }
 }
-// The same without `back`, to 2^-22 relative: the exponential's form is off by cap 2^-23 absolute, which shows in the lse of a
-// few small scores.  tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 - ... below 1/4
-__device__ __forceinline__ void cap_scores_fine(f32x16_t& s, float scale, float cap) {
-  const float inv = scale / cap, c2 = cap * LOG2E;
+// The same of the 16-bit types, forward, where a row of the wave sees few keys (`fine`: this lane's does): the exponential's
+// error, cap 2^-23 or more absolute, shows in the lse of a few small scores, so those rows take the series for them.  It goes by
+// the row, not by its block: what a row is packed beside changes nothing in its scores.  Relative error of a score 2^-22 in the series,
+// up to 2^-20 in the exponential's form, just above 1/4.  (8192 rows of documents up to 3626 long, capped at 30: 1 % of the forward pass.)
+__device__ __forceinline__ void cap_scores_fine(f32x16_t& s, float scale, float cap, bool fine) {
+  const float inv = scale / cap, c2 = cap * LOG2E, a = scale / cap * 2.f * LOG2E;
+  const float border = fine ? SMALL_TANH : 0.f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const float x = s[r] * inv, y = x * x;
-    const float small = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
-    s[r] = c2 * (fabsf(x) < 0.25f ? small : span_tanh<bf16_t>(x));
+    const float x = s[r] * inv, d = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * a));
+    s[r] = fabsf(x) < border ? c2 * small_tanh(x) : fmaf(d, -2.f * c2, c2);
+    if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);       // (not all sixteen at once: registers)
   }
 }
-template <typename T>
-__device__ __forceinline__ float turned(float t) { return sizeof(T) == 4 ? fmaf(-t, t, 1.f) : fmaf(-t, t, t); }
-template <typename T>
-__device__ __forceinline__ float result_scale(const SpanParams& p) { return p.cap > 0.f && sizeof(T) == 2 ? 4.f * p.scale : p.scale; }
+template <bool LIBRARY>
+__device__ __forceinline__ float turned(float t) { return LIBRARY ? fmaf(-t, t, 1.f) : fmaf(-t, t, t); }
+template <bool LIBRARY>
+__device__ __forceinline__ float result_scale(const SpanParams& p) { return p.cap > 0.f && !LIBRARY ? 4.f * p.scale : p.scale; }
 
 // sums the KW waves' transposed accumulators (32 own rows x DP, each wave's in LDS at region w) and hands the result to
 // put(row, col, x[4]) in whole rows; bad[row] is set where a sum is not finite
@@ -591,6 +595,14 @@ static inline int raise_lds(F* kernel, size_t bytes, const char* what) {
   NMTGAN_REQUIRE(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
                      hipSuccess, "%s: cannot raise the dynamic LDS limit", what);
   return 0;
+}
+// f(form of these scores as a constant)
+template <typename T, typename F>
+static inline int with_form(const SpanParams& p, F f) {
+  if constexpr (sizeof(T) == 2)
+    if (p.cap > SPAN_WIDE) return f(std::integral_constant<int, SPAN_WIDE_CAP>{});
+  if (p.cap > 0.f || p.slopes || p.scale == 0.f) return f(std::integral_constant<int, SPAN_EXTRA>{});
+  return f(std::integral_constant<int, SPAN_PLAIN>{});
 }
 // Blocks of 32 rows (times heads) from which waves may walk alone: two workgroups of four waves on every SIMD.  Below it the
 // chip is not full either way, and four waves a block finish sooner.

@@ -1,0 +1,95 @@
+"""Scores of span attention where a form could lose them: wide caps, small capped scores of short spans, packed beside long ones."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ops_reference import E, TYPES, check, heads_of, span_reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _ops():
+    from nmt_gan_amd import ops
+    return ops
+
+
+def _normal(g, *shape, dt, times=1.0):
+    return (torch.randn(*shape, generator=g) * times).to(dt)
+
+
+def _whole(values, cuda):
+    return torch.tensor(values, dtype=torch.int32, device=cuda)
+
+
+def step_with_lse(q, k, v, lo, hi, heads, kv_heads, scale, cap=0.0, slopes=None, max_keys=1):
+    """nmtgan_attn_span_step with its lse, which the function of tensors does not hand out."""
+    from nmt_gan_amd import _lib as L
+    m, dh = q.shape[0], q.shape[1] // heads
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((m, heads), 7.0, device=q.device)
+    a = L.SpanArgs(dtype={torch.bfloat16: L.NMTGAN_BF16, torch.float16: L.NMTGAN_F16, torch.float32: L.NMTGAN_F32}[q.dtype], M=m,
+                   N=k.shape[0], heads=heads, kv_heads=kv_heads, dh=dh, q=q.data_ptr(), ldq=q.stride(0), k=k.data_ptr(), ldk=k.stride(0),
+                   v=v.data_ptr(), ldv=v.stride(0), lo=lo.data_ptr(), hi=hi.data_ptr(), slopes=None if slopes is None else slopes.data_ptr(),
+                   scale=scale, cap=cap, out=out.data_ptr(), ldo=out.stride(0), lse=lse.data_ptr())
+    need = L.lib.nmtgan_attn_span_step_workspace_bytes(m, heads, kv_heads, dh, max_keys)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    L.check(L.lib.nmtgan_attn_span_step(C.byref(a), max_keys, ws.data_ptr() if need else None, need, L.stream_ptr()), "step")
+    torch.cuda.synchronize()
+    return out, lse
+
+
+@pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(2, 2, 64), (4, 1, 32), (2, 1, 128)])
+@pytest.mark.parametrize("cap", [100.0, 3e4, 1e6, 1e30])
+def test_wide_caps(cuda, op, heads, kv_heads, dh, cap):
+    """A cap far above the scores changes next to nothing, and loses nothing.  A capped score is its product through a
+    hyperbolic tangent and a few products, relative errors of 8 E in all on top of (dh + 4) E of the sum's magnitude: the bounds
+    of the same scores without a cap, 1 + 8 / (dh + 4) <= 1.25 times.  (The cap itself moves a probability by s^3 / (3 cap^2) < 2 %.)"""
+    ops, dt = _ops(), TYPES[op]
+    g = torch.Generator().manual_seed(dh)
+    m = 300
+    q = _normal(g, m, heads * dh, dt=dt).to(cuda)
+    k, v = (_normal(g, m, kv_heads * dh, dt=dt).to(cuda) for _ in range(2))
+    dout = _normal(g, m, heads * dh, dt=dt, times=0.1).to(cuda)
+    lo, hi = _whole([0] * 40 + [i // 30 * 30 for i in range(40, m - 2)] + [0, 0], cuda), _whole(list(range(1, m - 1)) + [0, 0], cuda)
+    how = dict(heads=heads, kv_heads=kv_heads, scale=dh ** -0.5, cap=cap)
+    grads = None if dt == torch.float16 else dout
+    value = span_reference(q, k, v, lo, hi, heads, kv_heads, dh ** -0.5, cap, dout=grads)
+    bound = span_reference(q, k, v, lo, hi, heads, kv_heads, dh ** -0.5, dout=grads)
+    out, lse = ops.attn_span(q, k, v, lo, hi, **how)
+    got = {"out": out, "lse": lse}
+    if grads is not None:
+        got["dq"], got["dk"], got["dv"] = ops.attn_span_grads(dout, q, k, v, out, lse, lo, hi, **how)
+    for name, x in got.items():
+        check(name, x, (value[name][0], 1.25 * bound[name][1]))
+    for keys in (1, 5000):                                          # in one part, in several
+        out, lse = step_with_lse(q, k, v, lo, hi, heads, kv_heads, dh ** -0.5, cap, max_keys=keys)
+        check("step", out, (value["out"][0], 1.25 * bound["out"][1]))
+        check("step lse", lse, (value["lse"][0], 1.25 * bound["lse"][1]))
+
+
+@pytest.mark.parametrize("op", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (64, 64), (4, 1)])
+def test_small_capped_scores_beside_a_long_document(cuda, op, heads, kv_heads):
+    """Rows that see one key: lse is the score itself.  Its error: dh E of the sum's magnitude for the product, 12 E of the score
+    for the tangent (4 E), the scale, the cap and the passage through log 2.  It is the same bits wherever the row is packed."""
+    ops, dt, dh, cap = _ops(), TYPES[op], 64, 50.0
+    g = torch.Generator().manual_seed(heads)
+    m = 1100
+    q = _normal(g, m, heads * dh, dt=dt, times=0.2).to(cuda)
+    k, v = (_normal(g, m, kv_heads * dh, dt=dt, times=0.2).to(cuda) for _ in range(2))
+    # rows 0 .. 999 one causal document, of its rows every fifth one sees itself only; the rest see themselves only
+    alone = [i % 5 == 3 or i >= 1000 for i in range(m)]
+    lo, hi = _whole([i if a else 0 for i, a in enumerate(alone)], cuda), _whole([i + 1 for i in range(m)], cuda)
+    mine = torch.tensor(alone, device=cuda)
+    scores = dh ** -0.5 * heads_of(q, heads) * heads_of(k, kv_heads).repeat_interleave(heads // kv_heads, 0)
+    value = (cap * torch.tanh(scores.sum(-1) / cap)).transpose(0, 1)
+    bound = (dh + 16) * E * scores.abs().sum(-1).transpose(0, 1)
+    how = dict(heads=heads, kv_heads=kv_heads, scale=dh ** -0.5, cap=cap)
+    lse = ops.attn_span(q, k, v, lo, hi, **how)[1]
+    check("lse", lse[mine], (value[mine], bound[mine]))
+    by_itself = ops.attn_span(q, k, v, hi - 1, hi, **how)[1]
+    assert torch.equal(lse[mine], by_itself[mine])
+    for keys in (1, 5000):
+        check("step lse", step_with_lse(q, k, v, lo, hi, heads, kv_heads, dh ** -0.5, cap, max_keys=keys)[1][mine], (value[mine], bound[mine]))
