@@ -637,7 +637,8 @@ int nmtgan_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const 
  *   norm[0] = sqrt(sum (grad_scale g)^2)     out = g grad_scale min(1, max_norm / norm)
  * `tensors` is a HOST array read before the call returns; g and out are device pointers aligned to their element, out in
  * the gradient's type or fp32 (the update kernels read fp32), equal to g for clipping in place.  Squares are summed in
- * fp64.  A norm that is not finite makes every output NaN.  Outputs may overlap neither each other nor another gradient. */
+ * fp64.  A sum that is not finite there (a gradient was not) makes every output NaN; a norm too large for fp32 alone does not,
+ * norm[0] reads inf then.  Outputs may overlap neither each other nor another gradient. */
 typedef struct { const void* g; void* out; int64_t n; int dtype; int out_dtype; } nmtgan_grad_ref;
 size_t nmtgan_global_norm_workspace_bytes(int n_tensors);
 int nmtgan_global_norm(const nmtgan_grad_ref* tensors, int n_tensors, float grad_scale, float* norm, void* workspace,

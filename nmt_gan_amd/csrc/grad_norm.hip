@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const double* part, in
 }
 
 template <typename T, typename O>
-__device__ __forceinline__ void scale_chunk(const T* g, O* out, int n, float f) {
+__device__ __forceinline__ void scale_chunk(const T* g, O* out, int n, float pre, float f) {
   constexpr int U = 8;
   int i = 0;
   for (; i + 1024 * U <= n; i += 1024 * U) {
@@ -163,7 +163,7 @@ __device__ __forceinline__ void scale_chunk(const T* g, O* out, int n, float f) 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[u][e] *= f;
+      for (int e = 0; e < 4; ++e) x[u][e] = x[u][e] * pre * f;
       Any<O>::store4(out + i + (u * 256 + (int)threadIdx.x) * 4, x[u]);
     }
   }
@@ -172,10 +172,10 @@ __device__ __forceinline__ void scale_chunk(const T* g, O* out, int n, float f) 
       float x[4];
       Any<T>::load4(g + i, x);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= f;
+      for (int e = 0; e < 4; ++e) x[e] = x[e] * pre * f;
       Any<O>::store4(out + i, x);
     } else {
-      for (int k = i; k < n; ++k) OpTraits<O>::store(out + k, OpTraits<T>::load(g + k) * f);
+      for (int k = i; k < n; ++k) OpTraits<O>::store(out + k, OpTraits<T>::load(g + k) * pre * f);
     }
   }
 }
@@ -186,20 +186,23 @@ __global__ __launch_bounds__(256) void clip_kernel(ListParams p, const double* p
   const double t = total_norm(part, n_part, grad_scale, red);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)t;
   // a norm that is no finite number makes every output NaN: the step is seen to be lost
-  const float f = !(t < INFINITY) ? NAN : (t > (double)max_norm ? (float)((double)max_norm / t * (double)grad_scale) : grad_scale);
+  const double all = !(t < INFINITY) ? NAN : (t > (double)max_norm ? (double)max_norm / t * (double)grad_scale : (double)grad_scale);
+  // a factor below fp32's normal range, of a norm above 8e37 max_norm, goes in two: the values it makes are not that small
+  const bool tiny = fabs(all) < 0x1p-126;
+  const float pre = tiny ? 0x1p-126f : 1.f, f = (float)(tiny ? all * 0x1p126 : all);
   for (int c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
     int64_t off;
     int n;
     const ListEntry& e = chunk_of(p, c, off, n);
-    if (f == 1.f && e.out == e.g) continue;          // nothing to change in place
+    if (f == 1.f && !tiny && e.out == e.g) continue;          // nothing to change in place
     const int dtype = e.tail >> 20 & 15, out_dtype = e.tail >> 24 & 15;
-    if (dtype == NMTGAN_F32) scale_chunk((const float*)e.g + off, (float*)e.out + off, n, f);
+    if (dtype == NMTGAN_F32) scale_chunk((const float*)e.g + off, (float*)e.out + off, n, pre, f);
     else if (dtype == NMTGAN_F16) {
-      if (out_dtype == NMTGAN_F32) scale_chunk((const f16_t*)e.g + off, (float*)e.out + off, n, f);
-      else scale_chunk((const f16_t*)e.g + off, (f16_t*)e.out + off, n, f);
+      if (out_dtype == NMTGAN_F32) scale_chunk((const f16_t*)e.g + off, (float*)e.out + off, n, pre, f);
+      else scale_chunk((const f16_t*)e.g + off, (f16_t*)e.out + off, n, pre, f);
     } else {
-      if (out_dtype == NMTGAN_F32) scale_chunk((const bf16_t*)e.g + off, (float*)e.out + off, n, f);
-      else scale_chunk((const bf16_t*)e.g + off, (bf16_t*)e.out + off, n, f);
+      if (out_dtype == NMTGAN_F32) scale_chunk((const bf16_t*)e.g + off, (float*)e.out + off, n, pre, f);
+      else scale_chunk((const bf16_t*)e.g + off, (bf16_t*)e.out + off, n, pre, f);
     }
   }
 }

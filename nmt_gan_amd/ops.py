@@ -108,7 +108,7 @@ def global_norm(tensors, *, grad_scale=1.0):
 
 def clip_global_norm(tensors, max_norm, *, grad_scale=1.0):
     """Writes grad_scale g min(1, max_norm / norm) to the list's outputs and returns the norm (before clipping), a float32
-    scalar on the device.  A norm that is not finite makes every output NaN."""
+    scalar on the device.  A gradient that is not finite makes every output NaN."""
     if max_norm is None:
         raise ValueError("clip_global_norm: max_norm=None")
     t = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
