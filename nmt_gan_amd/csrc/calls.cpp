@@ -15,6 +15,7 @@
 #include <cmath>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/nmtgan.h"
 
@@ -32,6 +33,7 @@ struct Entry {
   decltype(&nmtgan_linear_xent_workspace_bytes) linear_xent_workspace_bytes;
   decltype(&nmtgan_linear_xent) linear_xent;
   decltype(&nmtgan_linear_xent_grads) linear_xent_grads;
+  decltype(&nmtgan_global_norm_workspace_bytes) global_norm_workspace_bytes;
   decltype(&nmtgan_global_norm) global_norm;
   decltype(&nmtgan_clip_global_norm) clip_global_norm;
 } entry;
@@ -289,24 +291,57 @@ PyObject* linear_xent_grads(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------------------------------------- global norm
-// (address of the list, its length, one of its tensors, workspace bytes, grad_scale, max_norm or None) -> norm
+int type_code(at::ScalarType s) { return s == at::kBFloat16 ? NMTGAN_BF16 : s == at::kHalf ? NMTGAN_F16 : s == at::kFloat ? NMTGAN_F32 : -1; }
+// The list of o[0] (gradients) and o[1] (where their clipped values go), two Python lists, as the entry points take it.  Made anew by every call: a tensor may have been given other memory, another size or type since the last one.
+Common refs_of(const char* what, PyObject* const* o, std::vector<nmtgan_grad_ref>& refs) {
+  if (!PyList_Check(o[0]) || !PyList_Check(o[1])) refuse(what, "lists of tensors are needed");
+  const Py_ssize_t count = PyList_GET_SIZE(o[0]);
+  if (count == 0) refuse(what, "no tensors");
+  if (PyList_GET_SIZE(o[1]) != count)
+    refuse(what, std::to_string(count) + " gradients, " + std::to_string(PyList_GET_SIZE(o[1])) + " outputs");
+  const Common c = common(what, "gradient", PyList_GET_ITEM(o[0], 0));
+  refs.resize(count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const Tensor& g = tensor(what, "every gradient", PyList_GET_ITEM(o[0], i));
+    const Tensor& to = tensor(what, "every output", PyList_GET_ITEM(o[1], i));
+    for (const Tensor* t : {&g, &to})
+      if (t->device() != c.device || type_code(t->scalar_type()) < 0 || !t->is_contiguous())
+        refuse(what, "tensor " + std::to_string(i) + " must be contiguous, floating and on " + c.device.str());
+    if (to.numel() != g.numel() || (to.scalar_type() != g.scalar_type() && to.scalar_type() != at::kFloat))
+      refuse(what, "output " + std::to_string(i) + " must have its gradient's size, and its type or float32");
+    refs[i] = {g.data_ptr(), to.data_ptr(), g.numel(), type_code(g.scalar_type()), type_code(to.scalar_type())};
+  }
+  return c;
+}
+// (gradients, outputs): checks only
+PyObject* check_list(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  need_args(n, 2);
+  std::vector<nmtgan_grad_ref> refs;
+  refs_of("TensorList", o, refs);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (gradients, outputs, grad_scale, max_norm or None) -> norm
 PyObject* global_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  need_args(n, 6);
-  const bool clip = o[5] != Py_None;
+  need_args(n, 4);
+  const bool clip = o[3] != Py_None;
   const char* what = clip ? "clip_global_norm" : "global_norm";
-  const Common c = common(what, "gradient", o[2]);
-  const auto* list = (const nmtgan_grad_ref*)PyLong_AsVoidPtr(o[0]);
-  const long count = integer(what, "length", o[1]), bytes = integer(what, "bytes", o[3]);
-  const double scale = number(what, "grad_scale", o[4]), most = clip ? number(what, "max_norm", o[5]) : 1.0;
+  std::vector<nmtgan_grad_ref> refs;
+  const Common c = refs_of(what, o, refs);
+  const nmtgan_grad_ref* list = refs.data();
+  const int count = (int)refs.size();
+  const size_t bytes = entry.global_norm_workspace_bytes(count);
+  const double scale = number(what, "grad_scale", o[2]), most = clip ? number(what, "max_norm", o[3]) : 1.0;
   if (!std::isfinite((float)scale)) refuse(what, "grad_scale=" + std::to_string(scale));
   if (!std::isfinite((float)most) || !((float)most > 0.f)) refuse(what, "max_norm=" + std::to_string(most));
   Tensor norm = fresh(c, {}, at::kFloat);
   const Tensor ws = scratch(c, bytes);
   float* to = (float*)norm.data_ptr();
   checked(c, run(c, [&](void* st) {
-            return clip ? entry.clip_global_norm(list, (int)count, (float)most, (float)scale, to, ws.data_ptr(), bytes, st)
-                        : entry.global_norm(list, (int)count, (float)scale, to, ws.data_ptr(), bytes, st);
+            return clip ? entry.clip_global_norm(list, count, (float)most, (float)scale, to, ws.data_ptr(), bytes, st)
+                        : entry.global_norm(list, count, (float)scale, to, ws.data_ptr(), bytes, st);
           }));
   return THPVariable_Wrap(std::move(norm));
   END_HANDLE_TH_ERRORS
@@ -330,6 +365,7 @@ PyObject* bind(PyObject*, PyObject* const* o, Py_ssize_t n) {
   set("nmtgan_linear_xent_workspace_bytes", entry.linear_xent_workspace_bytes);
   set("nmtgan_linear_xent", entry.linear_xent);
   set("nmtgan_linear_xent_grads", entry.linear_xent_grads);
+  set("nmtgan_global_norm_workspace_bytes", entry.global_norm_workspace_bytes);
   set("nmtgan_global_norm", entry.global_norm);
   set("nmtgan_clip_global_norm", entry.clip_global_norm);
   Py_RETURN_NONE;
@@ -343,6 +379,7 @@ PyMethodDef methods[] = {
     {"attn_span_grads", (PyCFunction)(void (*)())attn_span_grads, METH_FASTCALL, nullptr},
     {"linear_xent", (PyCFunction)(void (*)())linear_xent, METH_FASTCALL, nullptr},
     {"linear_xent_grads", (PyCFunction)(void (*)())linear_xent_grads, METH_FASTCALL, nullptr},
+    {"check_list", (PyCFunction)(void (*)())check_list, METH_FASTCALL, nullptr},
     {"global_norm", (PyCFunction)(void (*)())global_norm, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -11,9 +11,6 @@ from __future__ import annotations
 
 import ctypes as C
 
-import torch
-
-from . import _lib as L
 from ._lib import lib
 
 try:
@@ -24,8 +21,7 @@ except ImportError as e:
 _calls.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in (
     "nmtgan_attn_span", "nmtgan_attn_span_step", "nmtgan_attn_span_step_workspace_bytes", "nmtgan_attn_span_grads",
     "nmtgan_attn_span_grads_workspace_bytes", "nmtgan_linear_xent", "nmtgan_linear_xent_grads",
-    "nmtgan_linear_xent_workspace_bytes", "nmtgan_global_norm", "nmtgan_clip_global_norm")})
-_CODE = {torch.bfloat16: L.NMTGAN_BF16, torch.float16: L.NMTGAN_F16, torch.float32: L.NMTGAN_F32}
+    "nmtgan_linear_xent_workspace_bytes", "nmtgan_global_norm_workspace_bytes", "nmtgan_global_norm", "nmtgan_clip_global_norm")})
 
 
 # ---------------------------------------------------------------------------------------------- span attention
@@ -74,36 +70,26 @@ def split_flat(flat, tensors):
 class TensorList:
     """A list of contiguous gradient tensors (bfloat16, float16, float32, mixed) on one GPU, and where their clipped values
     go: `out` holds a tensor of the same size for each, of its type or float32; without it they are clipped in place.
-    Built once for buffers that live as long as the list, which keeps them alive."""
+    Built once for buffers that live as long as the list, which keeps them alive; every call looks at the tensors again, so one
+    that has been given other memory (t.data = ..., t.set_(...)) since is read and written there."""
 
     def __init__(self, grads, out=None):
-        grads = list(grads)
-        out = grads if out is None else list(out)
-        if not grads:
-            raise ValueError("TensorList: no tensors")
-        if len(out) != len(grads):
-            raise ValueError("TensorList: %d gradients, %d outputs" % (len(grads), len(out)))
-        first = grads[0]
-        if not isinstance(first, torch.Tensor) or not first.is_cuda or first.dtype not in _CODE:
-            raise ValueError("TensorList: bfloat16, float16 or float32 tensors on a GPU are needed")
-        self.device = first.device
-        self.grads, self.out = grads, out
-        self._refs = (L.GradRef * len(grads))()
-        for i, (g, o) in enumerate(zip(grads, out)):
-            for t in (g, o):
-                if t.device != self.device or t.dtype not in _CODE or not t.is_contiguous():
-                    raise ValueError("TensorList: tensor %d must be contiguous, floating and on %s" % (i, self.device))
-            if o.numel() != g.numel() or (o.dtype != g.dtype and o.dtype != torch.float32):
-                raise ValueError("TensorList: output %d must have its gradient's size, and its type or float32" % i)
-            r = self._refs[i]
-            r.g, r.out, r.n, r.dtype, r.out_dtype = g.data_ptr(), o.data_ptr(), g.numel(), _CODE[g.dtype], _CODE[o.dtype]
-        self._call = (C.addressof(self._refs), len(grads), first, lib.nmtgan_global_norm_workspace_bytes(len(grads)))
+        self.grads = list(grads)
+        self.out = self.grads if out is None else list(out)
+        _calls.check_list(self.grads, self.out)
+        self.device = self.grads[0].device
+
+
+def _lists(tensors):
+    if isinstance(tensors, TensorList):
+        return tensors.grads, tensors.out
+    grads = list(tensors)
+    return grads, grads
 
 
 def global_norm(tensors, *, grad_scale=1.0):
     """sqrt(sum (grad_scale g)^2) over a TensorList (or a list of tensors), as a float32 scalar on the device."""
-    t = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
-    return _calls.global_norm(*t._call, grad_scale, None)
+    return _calls.global_norm(*_lists(tensors), grad_scale, None)
 
 
 def clip_global_norm(tensors, max_norm, *, grad_scale=1.0):
@@ -111,5 +97,4 @@ def clip_global_norm(tensors, max_norm, *, grad_scale=1.0):
     scalar on the device.  A gradient that is not finite makes every output NaN."""
     if max_norm is None:
         raise ValueError("clip_global_norm: max_norm=None")
-    t = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
-    return _calls.global_norm(*t._call, grad_scale, max_norm)
+    return _calls.global_norm(*_lists(tensors), grad_scale, max_norm)

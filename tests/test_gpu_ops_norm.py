@@ -32,3 +32,33 @@ def test_clip_by_a_tiny_scale(cuda):
     norm = ops.clip_global_norm([g], 1.0, grad_scale=1e-40)
     assert bool(((g.double() - want).abs() <= want.abs() * 2.0 ** -22 + 2.0 ** -149).all())
     assert abs(float(norm) - 3e37 * scale) <= 3e37 * scale * 2.0 ** -20
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_a_list_follows_its_tensors(cuda, given):
+    """Tensors that get other memory, another size or another type behind the list are read and written where they are now."""
+    from nmt_gan_amd import ops
+    first = [torch.full((1000,), 3.0, device=cuda), torch.full((17,), 4.0, device=cuda)]
+    grads = [t.clone() for t in first]
+    out = [torch.zeros(1000, device=cuda), torch.zeros(17, device=cuda)] if given else None
+    tensors = ops.TensorList(grads, out=out)
+    before = [t.data for t in grads]                                # keeps the memory that the list was built on
+    ops.global_norm(tensors)
+    grads[0].data = torch.full((1000,), 30.0, device=cuda)
+    grads[1].set_(torch.full((17,), 40.0, device=cuda))
+    norm = ops.clip_global_norm(tensors, 1.0)
+    want = math.sqrt(1000 * 900.0 + 17 * 1600.0)
+    assert abs(float(norm) - want) <= want * 2.0 ** -23
+    for o, value in zip(out if given else grads, (30.0, 40.0)):
+        assert bool(((o.double() - value / want).abs() <= 2.0 ** -22 * value / want).all())
+    assert all(torch.equal(a, b) for a, b in zip(before, first))    # nothing was written there
+    grads[1].data = torch.ones(5, device=cuda)
+    if given:                                                       # its output no longer fits
+        with pytest.raises(ValueError):
+            ops.clip_global_norm(tensors, 1.0)
+    else:
+        grads[0].data = torch.full((9,), 2.0, dtype=torch.float16, device=cuda)
+        assert abs(float(ops.global_norm(tensors)) - math.sqrt(41.0)) <= 1e-6
+    grads[0].data = torch.ones(1000)
+    with pytest.raises(ValueError):
+        ops.global_norm(tensors)
