@@ -1,4 +1,5 @@
 // Span attention: the form for single tokens, checks and launches (span_tiles.h has the formulas).
+#include "regions.h"
 #include "span_tiles.h"
 
 namespace nmtgan {
@@ -429,11 +430,29 @@ static int fill_span(const nmtgan_span_args* a, SpanParams& p, const char* what)
   return 0;
 }
 
+// what every form reads
+static Region region(const char* name, const void* at, int64_t rows, int64_t ld, int64_t width, int es) {
+  return Region(name, at, rows, ld * es, width * es);
+}
+#define SPAN_INPUTS(a, wq, wk, es)                                                                            \
+  region("q", (a)->q, (a)->M, (a)->ldq, wq, es), region("k", (a)->k, (a)->N, (a)->ldk, wk, es),               \
+      region("v", (a)->v, (a)->N, (a)->ldv, wk, es), Region("lo", (a)->lo, 4LL * (a)->M),                     \
+      Region("hi", (a)->hi, 4LL * (a)->M), Region("pos", (a)->pos, 4LL * (a)->M), Region("slopes", (a)->slopes, 4LL * (a)->heads)
+// of the forward forms
+static int span_overlaps(const nmtgan_span_args* a, const void* ws, size_t ws_bytes, const char* what) {
+  const int es = dtype_size(a->dtype);
+  const int64_t wq = (int64_t)a->heads * a->dh, wk = (int64_t)a->kv_heads * a->dh;
+  return refuse_overlaps(what, {region("out", a->out, a->M, a->ldo, wq, es), Region("lse", a->lse, 4LL * a->M * a->heads),
+                                Region("workspace", ws, (int64_t)ws_bytes)},
+                         {SPAN_INPUTS(a, wq, wk, es)});
+}
+
 int launch_attn_span(const nmtgan_span_args* a, hipStream_t st) {
   prof::Scope prof_scope(prof::OTHER, st);
   SpanParams p;
   NMTGAN_TRY(fill_span(a, p, "attn_span"));
   if (p.M == 0) return 0;
+  NMTGAN_TRY(span_overlaps(a, nullptr, 0, "attn_span"));
   return span_fwd_tiles(a->dtype, p, st);
 }
 
@@ -497,6 +516,7 @@ int launch_attn_span_step(const nmtgan_span_args* a, int max_keys, void* ws, siz
                  "attn_span_step: workspace of %zu bytes needed, %zu given", need, ws_bytes);
   const int splits = span_splits(p.M, p.kv_heads, max_keys);
   NMTGAN_REQUIRE((int64_t)p.M * splits < (1LL << 31) && ((int64_t)p.M * p.heads + 3) / 4 < (1LL << 31), "attn_span_step: too many rows");
+  NMTGAN_TRY(span_overlaps(a, ws, need, "attn_span_step"));
   NMTGAN_DISPATCH_OP(a->dtype, T, {
     if (p.dh <= 32) NMTGAN_TRY((choose_step<T, 32>(p, splits, (float*)ws, st)));
     else if (p.dh <= 64) NMTGAN_TRY((choose_step<T, 64>(p, splits, (float*)ws, st)));
@@ -544,6 +564,11 @@ int launch_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
   const size_t need = attn_span_grads_workspace(p.M, p.heads);
   NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0),
                  "attn_span_grads: workspace of %zu bytes needed, %zu given", need, ws_bytes);
+  NMTGAN_TRY(refuse_overlaps("attn_span_grads",
+                             {region("dq", g->dq, p.M, g->ld_dq, wq, es), region("dk", g->dk, p.N, g->ld_dk, wk, es),
+                              region("dv", g->dv, p.N, g->ld_dv, wk, es), Region("workspace", ws, (int64_t)need)},
+                             {SPAN_INPUTS(a, wq, wk, es), region("out", a->out, p.M, a->ldo, wq, es),
+                              region("dout", g->dout, p.M, g->ld_dout, wq, es), Region("lse", a->lse, 4LL * p.M * p.heads)}));
   if (p.M > 0) carve_span_grads(p.M, p.heads, (char*)ws, &p);
   p.dout = g->dout; p.ld_do = g->ld_dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
   p.ld_dq = g->ld_dq; p.ld_dk = g->ld_dk; p.ld_dv = g->ld_dv;

@@ -23,6 +23,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "regions.h"
 
 namespace nmtgan {
 
@@ -432,6 +433,11 @@ int launch_linear_xent(const nmtgan_xent_args* a, float* loss, float* lse, void*
   const size_t need = linear_xent_workspace(a, false);
   NMTGAN_REQUIRE(ws && ws_bytes >= need && (uintptr_t)ws % 256 == 0, "linear_xent: workspace of %zu bytes (256-byte aligned) needed, %zu given",
                  need, ws_bytes);
+  const int es = dtype_size(a->dtype);
+  NMTGAN_TRY(refuse_overlaps("linear_xent",
+                             {Region("loss", loss, 4LL * a->M), Region("lse", lse, 4LL * a->M), Region("workspace", ws, (int64_t)need)},
+                             {Region("h", a->h, a->M, a->ldh * es, (int64_t)a->d * es), Region("w", a->w, a->V, a->ldw * es, (int64_t)a->d * es),
+                              Region("labels", a->labels, 4LL * a->M)}));
   int tiles;
   float2* stats;
   XentEpilogue x{};
@@ -570,6 +576,13 @@ int launch_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const 
   const size_t need = linear_xent_workspace(a, true);
   NMTGAN_REQUIRE(need == 0 || (ws && ws_bytes >= need && (uintptr_t)ws % 256 == 0),
                  "linear_xent_grads: workspace of %zu bytes (256-byte aligned) needed, %zu given", need, ws_bytes);
+  const int64_t width = (int64_t)a->d * es;
+  NMTGAN_TRY(refuse_overlaps("linear_xent_grads",
+                             {Region("dh", dh, a->M, ld_dh * es, width), Region("dw", dw, a->V, ld_dw * es, width),
+                              Region("workspace", ws, (int64_t)need)},
+                             {Region("h", a->h, a->M, a->ldh * es, width), Region("w", a->w, a->V, a->ldw * es, width),
+                              Region("labels", a->labels, 4LL * a->M), Region("lse", lse, 4LL * a->M),
+                              Region("grad_row", grad_row, 4LL * a->M)}));
   if (a->M == 0) {
     NMTGAN_DISPATCH_OP(a->dtype, T,
                        hipLaunchKernelGGL(xent_zero_rows_kernel<T>, dim3((unsigned)(((int64_t)a->V * a->d + 255) / 256)), dim3(256),
