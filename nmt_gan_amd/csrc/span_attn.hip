@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
   }
   const int pos = EXTRA ? pos_of(p, i) : 0;
   const float inv_cap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f, cap2 = p.cap * LOG2E;
-  const float border = len <= SPAN_SHORT ? SMALL_TANH : 0.f;    // see cap_scores_fine
+  const bool few = __builtin_amdgcn_readfirstlane((int)len) <= SPAN_SHORT;      // see cap_scores_fine
 
   uint4 kr[STEP_U], vr[STEP_U];
   auto fetch = [&](int b) {
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void span_step_kernel(SpanParams p, int splits
         for (int e = 0; e < EPC; ++e) d = fmaf(x[e], q[t][e], d);
         d = key_sum<LPK>(d);
         if constexpr (EXTRA) {
-          if (p.cap > 0.f) d = cap_score<LIBRARY>(d * inv_cap, cap2, border);
+          if (p.cap > 0.f) d = few ? cap_score<LIBRARY>(d * inv_cap, cap2, SMALL_TANH) : cap_score<LIBRARY>(d * inv_cap, cap2, 0.f);
           else d *= p.scale * LOG2E;
           if (p.slopes) d = fmaf(-slope[t], fabsf((float)(pos - j)), d);
         }
