@@ -154,6 +154,7 @@ Common span(const char* what, PyObject* const* o, nmtgan_span_args& a) {
   if (dh < 1 || dh % 8 || dh > 128) refuse(what, "the head width " + std::to_string(dh) + " must be a multiple of 8, at most 128");
   const double scale = number(what, "scale", o[7]), cap = number(what, "cap", o[8]);
   if (!std::isfinite((float)scale) || !std::isfinite((float)cap) || cap < 0) refuse(what, "scale and cap must be finite, cap >= 0");
+  if (cap != 0.0 && (float)cap == 0.f) refuse(what, "cap is below the least float32 number and would read as no cap");
   if (m > INT32_MAX || n > INT32_MAX || v.size(0) != n)
     refuse(what, "k has " + std::to_string(n) + " rows, v " + std::to_string(v.size(0)));
   a = {};

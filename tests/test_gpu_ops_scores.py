@@ -93,3 +93,20 @@ def test_small_capped_scores_beside_a_long_document(cuda, op, heads, kv_heads):
     assert torch.equal(lse[mine], by_itself[mine])
     for keys in (1, 5000):
         check("step lse", step_with_lse(q, k, v, lo, hi, heads, kv_heads, dh ** -0.5, cap, max_keys=keys)[1][mine], (value[mine], bound[mine]))
+
+
+def test_a_cap_that_float32_does_not_have_is_refused(cuda):
+    """Rounded to zero it would mean no cap; the least one that there is makes all scores equal."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (_normal(g, 50, 64, dt=torch.float32, times=4.0).to(cuda) for _ in range(3))
+    lo, hi = _whole([0] * 50, cuda), _whole(range(1, 51), cuda)
+    o, lse = ops.attn_span(q, k, v, lo, hi, heads=1)
+    for call in (lambda c: ops.attn_span(q, k, v, lo, hi, heads=1, cap=c), lambda c: ops.attn_span_step(q, k, v, lo, hi, heads=1, max_keys=50, cap=c),
+                 lambda c: ops.attn_span_grads(o, q, k, v, o, lse, lo, hi, heads=1, cap=c)):
+        with pytest.raises(ValueError, match="cap"):
+            call(1e-60)
+    out, lse = ops.attn_span(q, k, v, lo, hi, heads=1, cap=1e-36)
+    mean = v.double().cumsum(0) / hi.double()[:, None]
+    assert bool(((out.double() - mean).abs() <= 60 * E * v.double().abs().cumsum(0) / hi.double()[:, None]).all())
+    assert bool(((lse[:, 0].double() - hi.double().log()).abs() <= 8 * E * (1 + hi.double().log())).all())
