@@ -2,6 +2,7 @@
 boundary), as hand-written gfx950 HIP kernels behind a C ABI (include/nmtgan.h).
 
 Importing the package loads libnmtgan_hip.so and raises if it is missing: there is no fallback.
+_calls.so (ops.py) is loaded by the first call of an operator, and raises there.
 """
 from ._lib import lib, LIB_PATH, NmtGanError          # noqa: F401  (loads the HIP library)
 from .utils import AttrDict                            # noqa: F401

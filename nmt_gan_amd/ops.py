@@ -13,15 +13,30 @@ import ctypes as C
 
 from ._lib import lib
 
-try:
-    from . import _calls
-except ImportError as e:
-    raise ImportError("nmt_gan_amd/_calls.so is missing or does not fit this torch: make -C nmt_gan_amd/csrc") from e
+_ENTRIES = ("nmtgan_attn_span", "nmtgan_attn_span_step", "nmtgan_attn_span_step_workspace_bytes", "nmtgan_attn_span_grads",
+            "nmtgan_attn_span_grads_workspace_bytes", "nmtgan_linear_xent", "nmtgan_linear_xent_grads",
+            "nmtgan_linear_xent_workspace_bytes", "nmtgan_global_norm_workspace_bytes", "nmtgan_global_norm", "nmtgan_clip_global_norm")
 
-_calls.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in (
-    "nmtgan_attn_span", "nmtgan_attn_span_step", "nmtgan_attn_span_step_workspace_bytes", "nmtgan_attn_span_grads",
-    "nmtgan_attn_span_grads_workspace_bytes", "nmtgan_linear_xent", "nmtgan_linear_xent_grads",
-    "nmtgan_linear_xent_workspace_bytes", "nmtgan_global_norm_workspace_bytes", "nmtgan_global_norm", "nmtgan_clip_global_norm")})
+
+class _FirstUse:
+    """Stands for the compiled calls until one is made: they are built against one torch, and nothing else in the package needs
+    them.  There is no other path: without them a call raises."""
+
+    def __getattr__(self, name):
+        global _calls
+        if name.startswith("__"):
+            raise AttributeError(name)
+        import torch                                       # noqa: F401  (the library that _calls.so is linked against)
+        try:
+            from . import _calls as found
+        except ImportError as e:
+            raise ImportError("nmt_gan_amd/_calls.so is missing or does not fit this torch: make -C nmt_gan_amd/csrc") from e
+        found.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in _ENTRIES})
+        _calls = found
+        return getattr(found, name)
+
+
+_calls = _FirstUse()
 
 
 # ---------------------------------------------------------------------------------------------- span attention
