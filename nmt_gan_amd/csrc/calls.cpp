@@ -114,6 +114,10 @@ void* vector(const Common& c, const char* name, const Tensor& t, int64_t n, at::
 Tensor fresh(const Common& c, at::IntArrayRef shape, at::ScalarType type) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(c.device));
 }
+// a tensor of the caller's has been written: torch's version of it goes up, so that autograd sees a saved one that has changed
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // an output given by the caller, or a new one
 Tensor target(const Common& c, const char* name, PyObject* o, int64_t n, int64_t width) {
   if (o == Py_None) return fresh(c, {n, width}, c.type);
@@ -189,6 +193,7 @@ PyObject* attn_span(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const Rows ro = rows(c, "out", out, width);
   a.out = ro.at; a.ldo = ro.ld; a.lse = (float*)lse.data_ptr();
   checked(c, run(c, [&](void* st) { return entry.attn_span(&a, st); }));
+  written(out);
   return pair(std::move(out), std::move(lse));
   END_HANDLE_TH_ERRORS
 }
@@ -207,6 +212,7 @@ PyObject* attn_span_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const size_t bytes = entry.attn_span_step_workspace_bytes(a.M, a.heads, a.kv_heads, a.dh, (int)keys);
   if (bytes) ws = scratch(c, bytes);
   checked(c, run(c, [&](void* st) { return entry.attn_span_step(&a, (int)keys, bytes ? ws.data_ptr() : nullptr, bytes, st); }));
+  written(out);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -232,6 +238,7 @@ PyObject* attn_span_grads(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const size_t bytes = entry.attn_span_grads_workspace_bytes(a.M, a.heads);
   const Tensor ws = scratch(c, bytes);
   checked(c, run(c, [&](void* st) { return entry.attn_span_grads(&a, &g, ws.data_ptr(), bytes, st); }));
+  for (const Tensor* t : {&dq, &dk, &dv}) written(*t);
   THPObjectPtr x(THPVariable_Wrap(std::move(dq))), y(THPVariable_Wrap(std::move(dk))), z(THPVariable_Wrap(std::move(dv)));
   return x && y && z ? PyTuple_Pack(3, x.get(), y.get(), z.get()) : nullptr;
   END_HANDLE_TH_ERRORS
@@ -287,6 +294,8 @@ PyObject* linear_xent_grads(PyObject*, PyObject* const* o, Py_ssize_t n) {
   checked(c, run(c, [&](void* st) {
             return entry.linear_xent_grads(&a, lse, g, rh.at, rh.ld, rw.at, rw.ld, ws.data_ptr(), bytes, st);
           }));
+  written(dh);
+  written(dw);
   return pair(std::move(dh), std::move(dw));
   END_HANDLE_TH_ERRORS
 }
@@ -344,6 +353,7 @@ PyObject* global_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
             return clip ? entry.clip_global_norm(list, count, (float)most, (float)scale, to, ws.data_ptr(), bytes, st)
                         : entry.global_norm(list, count, (float)scale, to, ws.data_ptr(), bytes, st);
           }));
+  for (int i = 0; clip && i < count; ++i) written(THPVariable_Unpack(PyList_GET_ITEM(o[1], i)));
   return THPVariable_Wrap(std::move(norm));
   END_HANDLE_TH_ERRORS
 }
