@@ -584,9 +584,9 @@ int launch_linear_xent_grads(const nmtgan_xent_args* a, const float* lse, const 
                               Region("labels", a->labels, 4LL * a->M), Region("lse", lse, 4LL * a->M),
                               Region("grad_row", grad_row, 4LL * a->M)}));
   if (a->M == 0) {
-    NMTGAN_DISPATCH_OP(a->dtype, T,
-                       hipLaunchKernelGGL(xent_zero_rows_kernel<T>, dim3((unsigned)(((int64_t)a->V * a->d + 255) / 256)), dim3(256),
-                                          0, st, (T*)dw, ld_dw, a->V, a->d));
+    const dim3 grid((unsigned)(((int64_t)a->V * a->d + 255) / 256));
+    if (a->dtype == NMTGAN_F32) hipLaunchKernelGGL(xent_zero_rows_kernel<float>, grid, dim3(256), 0, st, (float*)dw, ld_dw, a->V, a->d);
+    else hipLaunchKernelGGL(xent_zero_rows_kernel<bf16_t>, grid, dim3(256), 0, st, (bf16_t*)dw, ld_dw, a->V, a->d);
     NMTGAN_CHECK_LAUNCH("linear_xent_zero");
     return 0;
   }

@@ -266,12 +266,12 @@ __global__ __launch_bounds__(1024) void xent_direct_grads_kernel(XentDirect p) {
 
 int launch_xent_direct_z(int dtype, bool grad, const XentDirect& p, hipStream_t st) {
   const int64_t blocks = (int64_t)((p.Vp + 127) / 128) * ((p.M + 31) / 32);
+  NMTGAN_REQUIRE(dtype == NMTGAN_F32 || (grad && dtype == NMTGAN_BF16), "linear_xent: no direct form of dtype %d", dtype);
   NMTGAN_REQUIRE(blocks < (1LL << 31), "linear_xent: too many tiles");
   const dim3 grid((unsigned)blocks);
-  NMTGAN_DISPATCH_OP(dtype, T, {
-    if (grad) hipLaunchKernelGGL((xent_direct_z_kernel<T, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((xent_direct_z_kernel<T, false>), grid, dim3(256), 0, st, p);
-  });
+  if (!grad) hipLaunchKernelGGL((xent_direct_z_kernel<float, false>), grid, dim3(256), 0, st, p);
+  else if (dtype == NMTGAN_F32) hipLaunchKernelGGL((xent_direct_z_kernel<float, true>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((xent_direct_z_kernel<bf16_t, true>), grid, dim3(256), 0, st, p);
   NMTGAN_CHECK_LAUNCH("linear_xent_direct");
   return 0;
 }
@@ -281,10 +281,14 @@ int launch_xent_direct_grads(int dtype, XentDirect p, hipStream_t st) {
   const int64_t tiles = (int64_t)(p.V + 31) / 32 * across, held = 16 / p.waves;
   const int64_t grid = p.n_dh + (tiles + held - 1) / held * p.row_slices;
   NMTGAN_REQUIRE(grid < (1LL << 31), "linear_xent_grads: too many tiles");
-  NMTGAN_DISPATCH_OP(dtype, T, {
+  NMTGAN_REQUIRE(dtype == NMTGAN_F32 || dtype == NMTGAN_BF16, "linear_xent_grads: no direct form of dtype %d", dtype);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
     if (p.cols == 2) hipLaunchKernelGGL((xent_direct_grads_kernel<T, 2>), dim3((unsigned)grid), dim3(1024), 0, st, p);
     else hipLaunchKernelGGL((xent_direct_grads_kernel<T, 1>), dim3((unsigned)grid), dim3(1024), 0, st, p);
-  });
+  };
+  if (dtype == NMTGAN_F32) launch(float{});
+  else launch(bf16_t{});
   NMTGAN_CHECK_LAUNCH("linear_xent_direct_grads");
   return 0;
 }
