@@ -617,7 +617,7 @@ int nmtgan_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
  * nmtgan_linear_xent_grads: bf16 or fp32; grad_row[i] = d(objective)/d(loss[i]) (NULL: 1; a mean over n rows is 1/n), lse of
  * the forward call; dh [M][d], dw [V][d] in `dtype` are overwritten.  Rows without a label have dh = 0 and add nothing to dw.
  * d(logits) is formed one piece of the vocabulary at a time in the workspace (about 224 MB or 256 entries, plus fp32 partial
- * sums), in bf16 rounded once to it where M V d > 3e8.  Outputs overlap neither each other nor an input.  Gradients take at
+ * sums), in bf16 rounded once to it where M V d > 3e8 and M > 32.  Outputs overlap neither each other nor an input.  Gradients take at
  * most 2^22 rows.
  * d*esize a multiple of 16 bytes, rows 16-byte aligned, workspace 256-byte aligned. */
 typedef struct {

@@ -344,15 +344,17 @@ static void carve_xent(const nmtgan_xent_args* a, char* base, size_t cap, XentPl
   q.splitk = ar.take(SPLITK_BYTES);
   q.bytes = ar.off;
 }
-// The direct form (xent_direct.hip) against this file's products on the library's tiles, by M V d:
+// The direct form (xent_direct.hip) against this file's products on the library's tiles, by M V d and rows:
 //   logits in fp32 up to 1e9 (50 x 9000 x 256: 16 us against 39, 900 x 9000 x 128: 42 against 43), in 16 bits never (8 x
 //   32000 x 512: 20 against 19);
 //   gradient's products in fp32 always (97 x 509 x 64, with the logits: 13 us against 70, 900 x 9000 x 512: 480 against 1362,
-//   3200 x 32000 x 512: 4.7 ms against 6.6), in 16 bits up to 3e8 (8 x 32000 x 512: 57 us against 105, 900 x 1000 x 256: 36
-//   against 55, 200 x 4000 x 256: 42 against 49, 400 x 4000 x 256: 68 against 54).
+//   3200 x 32000 x 512: 4.7 ms against 6.6), in 16 bits up to 3e8 (900 x 1000 x 256: 36 us against 55, 200 x 4000 x 256: 42
+//   against 49, 400 x 4000 x 256: 68 against 54) and up to one tile of 32 rows, where the table's bytes count and not the
+//   products (8 x 32000 x 512: 57 against 99, 8 x 50257 x 1024: 126 against 203, 32 x 50257 x 1024: 161 against 205, 32 x
+//   128256 x 1024: 390 against 485; 64 rows of these two: 278 against 209, 703 against 489).
 static int64_t xent_work(const nmtgan_xent_args* a) { return (int64_t)a->M * a->V * a->d; }
 static bool direct_logits(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 && xent_work(a) <= 1000000000; }
-static bool direct_grads(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 || xent_work(a) <= 300000000; }
+static bool direct_grads(const nmtgan_xent_args* a) { return a->dtype == NMTGAN_F32 || a->M <= 32 || xent_work(a) <= 300000000; }
 struct DirectPlan {
   XentDirect p;
   int piece, n_pieces;
