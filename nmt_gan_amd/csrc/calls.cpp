@@ -314,12 +314,15 @@ Common refs_of(const char* what, PyObject* const* o, std::vector<nmtgan_grad_ref
   for (Py_ssize_t i = 0; i < count; ++i) {
     const Tensor& g = tensor(what, "every gradient", PyList_GET_ITEM(o[0], i));
     const Tensor& to = tensor(what, "every output", PyList_GET_ITEM(o[1], i));
-    for (const Tensor* t : {&g, &to})
-      if (t->device() != c.device || type_code(t->scalar_type()) < 0 || !t->is_contiguous())
-        refuse(what, "tensor " + std::to_string(i) + " must be contiguous, floating and on " + c.device.str());
-    if (to.numel() != g.numel() || (to.scalar_type() != g.scalar_type() && to.scalar_type() != at::kFloat))
+    const bool other = !to.is_same(g);
+    const int type = type_code(g.scalar_type()), to_type = other ? type_code(to.scalar_type()) : type;
+    if (type < 0 || to_type < 0 || g.device() != c.device || !g.is_contiguous() || (other && (to.device() != c.device || !to.is_contiguous())))
+      refuse(what, "tensor " + std::to_string(i) + " must be contiguous, floating and on " + c.device.str());
+    const int64_t size = g.numel();
+    if (other && (to.numel() != size || (to_type != type && to_type != NMTGAN_F32)))
       refuse(what, "output " + std::to_string(i) + " must have its gradient's size, and its type or float32");
-    refs[i] = {g.data_ptr(), to.data_ptr(), g.numel(), type_code(g.scalar_type()), type_code(to.scalar_type())};
+    void* at = g.data_ptr();
+    refs[i] = {at, other ? to.data_ptr() : at, size, type, to_type};
   }
   return c;
 }

@@ -211,6 +211,8 @@ static int check_list(const nmtgan_grad_ref* t, int n, bool clip, const char* wh
   NMTGAN_REQUIRE(n >= 0 && (n == 0 || t), "%s: null list", what);
   struct Range { uintptr_t a, b; int tensor; };
   std::vector<Range> written, read;
+  written.reserve(clip ? n : 0);
+  read.reserve(clip ? n : 0);
   for (int i = 0; i < n; ++i) {
     NMTGAN_REQUIRE(t[i].n >= 0 && valid_op_dtype(t[i].dtype), "%s: tensor %d: bad size or dtype", what, i);
     NMTGAN_REQUIRE(t[i].n < (1LL << 40), "%s: tensor %d: too large", what, i);
