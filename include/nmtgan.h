@@ -577,7 +577,8 @@ int nmtgan_clip_values(float* w, int64_t n, float lo, float hi, void* w_op, int 
  * q/out [M][heads dh], k/v [N][kv_heads dh] in `dtype`, head-major inside a row, ld* elements from row to row; query head h
  * reads key head h / (heads / kv_heads).  A row with an empty span gets out = 0, lse = -inf and no gradient.  Rows outside
  * every span may hold anything, and a NaN or an infinity reaches exactly the rows that see it.
- * dh: a multiple of 8 up to 128; rows 16-byte aligned; inputs and outputs do not overlap.
+ * dh: a multiple of 8 up to 128; rows 16-byte aligned; an output over an input, another output or the workspace is refused
+ * (columns of one buffer side by side are not).
  * nmtgan_attn_span: prompts and training rows.  nmtgan_attn_span_step: few rows over long spans (single tokens): each
  *   span is cut along its keys.  max_keys is a hint for the cut - the longest span expected - and changes no value beyond
  *   the order of fp32 sums.
@@ -592,9 +593,10 @@ typedef struct {
   const void* k; int64_t ldk;
   const void* v; int64_t ldv;
   const int32_t* lo; const int32_t* hi;      /* [M] */
-  const int32_t* pos;                        /* [M] place of row i among the keys (for slopes), within +-2^30; NULL: hi[i] - 1 */
+  const int32_t* pos;                        /* [M] place of row i among the keys (for slopes); NULL: hi[i] - 1.  pos[i] - j
+                                              * has to fit 32 bits for every key j */
   const float* slopes;                       /* [heads] or NULL */
-  float scale, cap;                          /* cap <= 0 is refused unless exactly 0 = no cap */
+  float scale, cap;                          /* cap < 0 is refused, 0 = no cap */
   void* out; int64_t ldo;
   float* lse;                                /* [M][heads] natural log; NULL if not wanted (forward only) */
 } nmtgan_span_args;
@@ -617,8 +619,8 @@ int nmtgan_attn_span_grads(const nmtgan_span_args* a, const nmtgan_span_grads* g
  * nmtgan_linear_xent_grads: bf16 or fp32; grad_row[i] = d(objective)/d(loss[i]) (NULL: 1; a mean over n rows is 1/n), lse of
  * the forward call; dh [M][d], dw [V][d] in `dtype` are overwritten.  Rows without a label have dh = 0 and add nothing to dw.
  * d(logits) is formed one piece of the vocabulary at a time in the workspace (about 224 MB or 256 entries, plus fp32 partial
- * sums), in bf16 rounded once to it where M V d > 3e8 and M > 32.  Outputs overlap neither each other nor an input.  Gradients take at
- * most 2^22 rows.
+ * sums), in bf16 rounded once to it where M V d > 3e8 and M > 32.  An output over an input, another output or the workspace is
+ * refused.  Gradients take at most 2^22 rows.
  * d*esize a multiple of 16 bytes, rows 16-byte aligned, workspace 256-byte aligned. */
 typedef struct {
   int dtype;

@@ -10,7 +10,7 @@ namespace nmtgan {
 // read once, as 16-byte chunks by LPK neighbouring lanes, so a wave reads 64 / LPK keys per instruction and STEP_U such
 // groups of K and of V are in flight while the previous ones are used; every lane group keeps a softmax of its own (no
 // exchange inside the loop but the LPK-lane sum of a dot product).
-// Bound by the rate at which K and V come; where heads share a key, by the arithmetic per key (hence the matrix form below).  One row over 300 keys, 8 heads: 5.6 us, a launch and two dependent loads.
+// Bound by the rate at which K and V come; where heads share a key, by the arithmetic per key (hence the matrix form below).  One row over 256 keys, 8 heads: 5.5 us, a launch and two dependent loads.
 constexpr int STEP_U = 4;
 
 template <int LPK>
@@ -458,7 +458,9 @@ int launch_attn_span(const nmtgan_span_args* a, hipStream_t st) {
 
 // Workgroups along a span: enough to fill the chip four workgroups deep, none with less than 512 keys, and none but one
 // below 1024 keys - the second launch that joins them costs more than the walk.  max_keys is a hint (the cut is made of the
-// true length on the device), so a wrong one costs time only.
+// true length on the device), so a wrong one costs time only.  No more than 64, a lane each in the joining wave: one request
+// over 2^20 keys then reads at 5.4 TB/s with 8 key heads of 64, 3.5 with 2, and at 2.5 to 2.8 with one (64 or 128 wide), which
+// leaves three of four CUs without work; four requests of 2^18 keys with one key head of 128: 5.1.
 static int span_splits(int M, int kv_heads, int max_keys) {
   if (max_keys <= 1024) return 1;
   const int64_t groups = std::max<int64_t>(1, (int64_t)M * kv_heads);

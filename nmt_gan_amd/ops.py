@@ -1,10 +1,11 @@
 """Operators of teacher-forced training, prompts and single tokens as functions of torch tensors over the C ABI
 (include/nmtgan.h: nmtgan_attn_span*, nmtgan_linear_xent*, nmtgan_*global_norm).
 
-Every function checks its arguments on the host (ValueError), allocates outputs and scratch through torch's caching
-allocator and enqueues on the current stream of the tensors' device without synchronising; inside a graph capture the
-scratch belongs to the graph's pool.  Tensors made on another stream are the caller's to order, as with any kernel.
-There is no autograd: gradients are explicit calls, as everywhere in this package.  (The checks and calls themselves are
+Every function checks its arguments on the host (ValueError; NmtGanError with the library's message for what the library
+refuses, outputs that lie over an input among it), allocates outputs and scratch through torch's caching allocator and enqueues on
+the current stream of the tensors' device without synchronising; inside a graph capture the scratch belongs to the graph's pool.  Tensors made on another stream are the caller's to order, as with any kernel.
+There is no autograd: gradients are explicit calls, as everywhere in this package, inputs that require gradients are taken as
+they are, and torch's version of every tensor that a call writes goes up.  (The checks and calls themselves are
 compiled: csrc/calls.cpp.)
 """
 from __future__ import annotations
@@ -43,8 +44,8 @@ _calls = _FirstUse()
 def attn_span(q, k, v, lo, hi, *, heads, kv_heads=None, scale=1.0, cap=0.0, slopes=None, pos=None, out=None):
     """(out [M, heads dh], lse [M, heads] fp32) of q [M, heads dh] over k, v [N, kv_heads dh]; row i sees keys lo[i] <= j < hi[i].
 
-    score = scale q.k, with cap > 0 cap tanh(score / cap), minus slopes[h] |pos[i] - j| (pos: hi - 1 unless given).  A row
-    that sees nothing gets 0 and -inf.  For many rows (training, prompts); attn_span_step is the form for single tokens.
+    score = scale q.k, with cap > 0 cap tanh(score / cap), minus slopes[h] |pos[i] - j| (pos: hi - 1 unless given; pos[i] - j has to
+    fit 32 bits).  A row that sees nothing gets 0 and -inf.  For many rows (training, prompts); attn_span_step is the form for single tokens.
     """
     return _calls.attn_span(q, k, v, lo, hi, heads, kv_heads, scale, cap, slopes, pos, out)
 
