@@ -302,7 +302,8 @@ PyObject* linear_xent_grads(PyObject*, PyObject* const* o, Py_ssize_t n) {
 
 // ---------------------------------------------------------------------------------------------- global norm
 int type_code(at::ScalarType s) { return s == at::kBFloat16 ? NMTGAN_BF16 : s == at::kHalf ? NMTGAN_F16 : s == at::kFloat ? NMTGAN_F32 : -1; }
-// The list of o[0] (gradients) and o[1] (where their clipped values go), two Python lists, as the entry points take it.  Made anew by every call: a tensor may have been given other memory, another size or type since the last one.
+// The list of o[0] (gradients) and o[1] (where their clipped values go), two Python lists, as the entry points take it.  Made
+// anew by every call: a tensor may have been given other memory, another size or type since the last one.
 Common refs_of(const char* what, PyObject* const* o, std::vector<nmtgan_grad_ref>& refs) {
   if (!PyList_Check(o[0]) || !PyList_Check(o[1])) refuse(what, "lists of tensors are needed");
   const Py_ssize_t count = PyList_GET_SIZE(o[0]);

@@ -10,7 +10,8 @@ namespace nmtgan {
 // read once, as 16-byte chunks by LPK neighbouring lanes, so a wave reads 64 / LPK keys per instruction and STEP_U such
 // groups of K and of V are in flight while the previous ones are used; every lane group keeps a softmax of its own (no
 // exchange inside the loop but the LPK-lane sum of a dot product).
-// Bound by the rate at which K and V come; where heads share a key, by the arithmetic per key (hence the matrix form below).  One row over 256 keys, 8 heads: 5.5 us, a launch and two dependent loads.
+// Bound by the rate at which K and V come; where heads share a key, by the arithmetic per key (hence the matrix form below).  One
+// row over 256 keys, 8 heads: 5.5 us, a launch and two dependent loads.
 constexpr int STEP_U = 4;
 
 template <int LPK>
